@@ -447,6 +447,166 @@ STG_API stg_status stg_htdemucs_spec(stg_engine* engine, const float* d_x, int32
 STG_API stg_status stg_htdemucs_ispec(stg_engine* engine, const float* d_spec, int32_t n_channels,
                                       int32_t n_frames, int64_t length, float* d_y, void* stream);
 
+/* ---- layers of the network between the halves -------------------------------------------- */
+
+/* The reference runs its networks through ggml (src/htdemucs.cpp:322-416, src/roformer.cpp:
+ * 90-214, src/tfc_tdf.cpp:98-350); here the network is the caller's (stg_separate_network).
+ * These are layers such a network is made of and that a callback enqueues between stg_front
+ * and stg_back: rotary positions (RoFormer's attention), group norm with an activation
+ * (HTDemucs, TFC-TDF), the gated projection (feed-forward layers), the latter two with their
+ * backward passes for fine-tuning, and RoFormer's mask head, which writes the layout stg_back reads.
+ *
+ * All are asynchronous on `stream`, allocate nothing, keep nothing between calls and may be
+ * captured into a CUDA graph. Scratch is the caller's: a *_workspace function gives the bytes
+ * for a configuration; d_workspace (256-byte aligned) is used only while the call's kernels
+ * run, so calls that can overlap on the GPU, captured graphs among them, need one each. The
+ * same inputs give the same bits (no floating-point atomics). Every buffer belongs to the
+ * engine's device; the caller's current device is left as it was. Strides count elements and
+ * are at least 0; outputs must not overlap each other or the inputs except where said. Zero
+ * sizes are allowed: what they leave empty is not touched. Statuses: STG_INVALID_ARGUMENT for
+ * NULL buffers, sizes and strides that make no sense, pointers that are not aligned to their
+ * element, and a workspace that is too small; STG_UNSUPPORTED for sizes past the stated limits. */
+
+/* Element types. Arithmetic is in float whatever the type; results are rounded once. */
+enum { STG_F32 = 0, STG_F16 = 1, STG_BF16 = 2 };
+/* Activations: z, max(z, 0), z sigmoid(z), z (1 + erf(z / sqrt 2)) / 2, sigmoid(z). ReLU's
+ * derivative at 0 is 0. */
+enum { STG_ACT_NONE = 0, STG_ACT_RELU = 1, STG_ACT_SILU = 2, STG_ACT_GELU = 3, STG_ACT_SIGMOID = 4 };
+
+/* Rotary positions (ggml's rope_ext at src/roformer.cpp:101-139). The first rotary_dim
+ * elements of each head are rotary_dim / 2 pairs, (2i, 2i + 1) interleaved (layout 0) or
+ * (i, i + rotary_dim / 2) in halves (layout 1). Pair i of a token at position p turns by the
+ * angle p f_i and is scaled by m; the head's other elements are copied. f_i = base^(-2i/rotary_dim),
+ * m = 1, and for longer contexts than a model was trained on (factor s >= 1):
+ *   scaling 1 linear   f_i / s
+ *   scaling 2 NTK      base s^(rotary_dim / (rotary_dim - 2)) in place of base
+ *   scaling 3 YaRN     (1 - g_i) f_i + g_i f_i / s and m = 0.1 ln(s) + 1, where g_i rises from 0 to 1
+ *                      between i = max(floor(j(beta_fast)), 0) and min(ceil(j(beta_slow)), rotary_dim / 2 - 1)
+ *                      (at least 0.001 apart), j(r) = rotary_dim ln(original_length / (2 pi r)) / (2 ln base)
+ * Angles are reduced in double, so far positions keep their phase. */
+typedef struct {
+    uint32_t size;
+    int32_t dtype;
+    int32_t layout;            /* 0 interleaved, 1 halves */
+    int32_t inverse;           /* 1: turn by -p f_i, still scaled by m: the gradient of the call without it */
+    int64_t batch, tokens;
+    int32_t head_dim;          /* 1..65536 */
+    int32_t rotary_dim;        /* even, 0 = head_dim; at most 512 */
+    int32_t scaling;           /* 0 none, 1 linear, 2 NTK, 3 YaRN */
+    int32_t offset;            /* without d_positions, token t is at offset + t */
+    double base;               /* > 0, not 1; 0 = 10000 */
+    double factor;             /* s */
+    double original_length;    /* YaRN; > 0 */
+    double beta_fast, beta_slow;   /* YaRN, beta_fast > beta_slow > 0; both 0 = 32 and 1 */
+    double magnitude;          /* m; 0 = the scaling's own */
+} stg_rotary_config;
+/* One tensor [batch][tokens][heads][head_dim] with element stride 1 inside a head. d_y may be
+ * d_x with the same strides (in place). A stride of 0 in y is refused unless its size is 1. */
+typedef struct {
+    const void* d_x;
+    void* d_y;
+    int64_t heads;
+    int64_t x_batch, x_token, x_head;   /* strides */
+    int64_t y_batch, y_token, y_head;
+} stg_rotary_tensor;
+/* The frequencies f_i [rotary_dim / 2] and m of a configuration. Host only. */
+STG_API stg_status stg_rotary_frequencies(const stg_rotary_config* config, double* frequencies,
+                                          double* magnitude);
+/* One launch over one or two tensors (queries and keys; their head counts may differ).
+ * d_positions: int32 [tokens] with position_batch_stride 0, or [batch] rows of them that many
+ * elements apart, or NULL. */
+STG_API stg_status stg_rotary(stg_engine* engine, const stg_rotary_config* config,
+                              const stg_rotary_tensor* tensors, int32_t n_tensors,
+                              const int32_t* d_positions, int64_t position_batch_stride, void* stream);
+
+/* Group norm with an activation, channels last: x, y [batch][positions][channels], channel
+ * stride 1. Per batch item and group of channels / groups neighbouring channels, mean and
+ * biased variance over positions and channels; y = act((x - mean) rstd gamma + beta),
+ * rstd = 1 / sqrt(var + eps). groups == channels is instance norm, groups == 1 the norm of
+ * HTDemucs' residual branches (src/htdemucs.cpp:66-260). */
+typedef struct {
+    uint32_t size;
+    int32_t dtype;             /* x, y and their gradients */
+    int32_t param_dtype;       /* gamma, beta and their gradients: dtype or STG_F32 */
+    int32_t activation;
+    int64_t batch;             /* at most 65535 */
+    int64_t positions;         /* positions * channels at most 2^40 */
+    int32_t channels;          /* 1..8192 */
+    int32_t groups;            /* divides channels */
+    int64_t x_batch, x_position;   /* strides of x */
+    int64_t y_batch, y_position;   /* strides of y; of dy in the backward pass */
+    int64_t dx_batch, dx_position; /* strides of dx (backward pass only) */
+    double eps;                /* >= 0 */
+} stg_group_norm_config;
+/* backward: 0 the bytes of stg_group_norm's workspace, 1 of stg_group_norm_backward's. Host only. */
+STG_API stg_status stg_group_norm_workspace(const stg_group_norm_config* config, int32_t backward,
+                                            size_t* bytes);
+/* d_gamma / d_beta NULL: 1 and 0. d_mean / d_rstd float [batch][groups], or NULL when no
+ * backward pass will need them; an item without positions leaves its statistics unwritten.
+ * y may be x with the same strides. */
+STG_API stg_status stg_group_norm(stg_engine* engine, const stg_group_norm_config* config,
+                                  const void* d_x, const void* d_gamma, const void* d_beta, void* d_y,
+                                  float* d_mean, float* d_rstd, void* d_workspace, size_t workspace_bytes,
+                                  void* stream);
+/* Gradients of stg_group_norm from dy (strides of y), x and the forward pass's statistics:
+ * dx, and dgamma / dbeta [channels], summed over batch and positions. Any of the three may be
+ * NULL. dx may be x or dy with the same strides. */
+STG_API stg_status stg_group_norm_backward(stg_engine* engine, const stg_group_norm_config* config,
+                                           const void* d_dy, const void* d_x, const void* d_gamma,
+                                           const void* d_beta, const float* d_mean, const float* d_rstd,
+                                           void* d_dx, void* d_dgamma, void* d_dbeta, void* d_workspace,
+                                           size_t workspace_bytes, void* stream);
+
+/* The gated projection of a feed-forward layer: y = act(x Wg^T + bg) (x Wu^T + bu), both
+ * products, the activation and the product of the two in one kernel, so that neither
+ * projection is written out. x [rows][features], Wg and Wu [width][features], bg and bu
+ * [width] or NULL, y [rows][width], the innermost stride 1. f16 and bf16 run on the tensor
+ * cores with float accumulators; f32 in float on the CUDA cores, without tf32. */
+typedef struct {
+    uint32_t size;
+    int32_t dtype;
+    int32_t activation;
+    int32_t features;          /* at least 1 */
+    int32_t width;             /* at least 1 */
+    int64_t rows;              /* rows, width and features below 2^31 each; rows 0 allowed */
+    int64_t x_row, wg_row, wu_row, y_row;   /* row strides; y_row is dy's in the backward pass */
+    int64_t dx_row, dwg_row, dwu_row;       /* row strides of the gradients (backward pass only) */
+} stg_gated_config;
+/* backward: 0 the bytes of stg_gated's workspace, 1 of stg_gated_backward's. Host only. */
+STG_API stg_status stg_gated_workspace(const stg_gated_config* config, int32_t backward, size_t* bytes);
+STG_API stg_status stg_gated(stg_engine* engine, const stg_gated_config* config, const void* d_x,
+                             const void* d_wg, const void* d_wu, const void* d_bg, const void* d_bu,
+                             void* d_y, void* d_workspace, size_t workspace_bytes, void* stream);
+/* Gradients from dy and the forward pass's inputs (the projections are computed again): dx,
+ * dWg, dWu, dbg, dbu in the layouts of what they are the gradients of. Any may be NULL. The
+ * projections' own gradients pass between the products in `dtype`. With rows 0 the weights'
+ * gradients are zeros. */
+STG_API stg_status stg_gated_backward(stg_engine* engine, const stg_gated_config* config, const void* d_dy,
+                                      const void* d_x, const void* d_wg, const void* d_wu, const void* d_bg,
+                                      const void* d_bu, void* d_dx, void* d_dwg, void* d_dwu, void* d_dbg,
+                                      void* d_dbu, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* The last layer of RoFormer's mask estimators (src/roformer.cpp:190-214) over a batch of
+ * chunks, every stem and band in one launch: per chunk, stem s and band b of the plan,
+ * v = h Wv^T + bv and g = h Wg^T + bg, mask = v sigmoid(g) (torch's GLU), written as float in the
+ * plan's mask layout, ready for stg_back or stg_separate. h [n_chunks][S][n_bands][T][hidden];
+ * weight [S][2 sum_b din_b][hidden], band after band, a band's din_b value rows before its
+ * din_b gate rows; bias [S][2 sum_b din_b] or NULL; all contiguous. din_b as in the mask layout. */
+typedef struct {
+    uint32_t size;
+    int32_t dtype;             /* h, weight and bias */
+    int32_t hidden;            /* at least 1 */
+    int32_t n_chunks;
+} stg_mask_head_config;
+/* S, n_bands, T and sum_b din_b of a RoFormer plan: the sizes of the mask head's buffers. */
+STG_API stg_status stg_mask_head_sizes(const stg_plan* plan, int32_t* stems, int32_t* bands,
+                                       int32_t* frames, int64_t* columns);
+STG_API stg_status stg_mask_head_workspace(const stg_plan* plan, const stg_mask_head_config* config,
+                                           size_t* bytes);
+STG_API stg_status stg_mask_head(stg_plan* plan, const stg_mask_head_config* config, const void* d_hidden,
+                                 const void* d_weight, const void* d_bias, float* d_masks,
+                                 void* d_workspace, size_t workspace_bytes, void* stream);
+
 /* ---- a separation that allocates no device memory ---------------------------------------- */
 
 /* No counterpart in the reference: the reference runs this path on the host.

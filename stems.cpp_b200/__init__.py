@@ -100,6 +100,36 @@ class NetworkInfo(C.Structure):
                 ("net_out_floats_per_chunk", C.c_int64)]
 
 
+class RotaryConfig(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("dtype", C.c_int32), ("layout", C.c_int32), ("inverse", C.c_int32),
+                ("batch", C.c_int64), ("tokens", C.c_int64), ("head_dim", C.c_int32), ("rotary_dim", C.c_int32),
+                ("scaling", C.c_int32), ("offset", C.c_int32), ("base", C.c_double), ("factor", C.c_double),
+                ("original_length", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double),
+                ("magnitude", C.c_double)]
+
+
+class RotaryTensor(C.Structure):
+    _fields_ = [("d_x", C.c_void_p), ("d_y", C.c_void_p)] + [(k, C.c_int64) for k in (
+        "heads", "x_batch", "x_token", "x_head", "y_batch", "y_token", "y_head")]
+
+
+class GroupNormConfig(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("activation", C.c_int32),
+                ("batch", C.c_int64), ("positions", C.c_int64), ("channels", C.c_int32), ("groups", C.c_int32),
+                ("x_batch", C.c_int64), ("x_position", C.c_int64), ("y_batch", C.c_int64), ("y_position", C.c_int64),
+                ("dx_batch", C.c_int64), ("dx_position", C.c_int64), ("eps", C.c_double)]
+
+
+class GatedConfig(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("dtype", C.c_int32), ("activation", C.c_int32), ("features", C.c_int32),
+                ("width", C.c_int32)] + [(k, C.c_int64) for k in (
+                    "rows", "x_row", "wg_row", "wu_row", "y_row", "dx_row", "dwg_row", "dwu_row")]
+
+
+class MaskHeadConfig(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("dtype", C.c_int32), ("hidden", C.c_int32), ("n_chunks", C.c_int32)]
+
+
 NETWORK_FN = C.CFUNCTYPE(C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p)
 
 
@@ -162,6 +192,20 @@ _SIGNATURES = {
     "stg_htdemucs_spec": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p]),
     "stg_htdemucs_ispec": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_void_p,
                                        C.c_void_p]),
+    "stg_rotary_frequencies": (C.c_int32, [C.POINTER(RotaryConfig), C.POINTER(C.c_double), C.POINTER(C.c_double)]),
+    "stg_rotary": (C.c_int32, [C.c_void_p, C.POINTER(RotaryConfig), C.POINTER(RotaryTensor), C.c_int32, C.c_void_p,
+                               C.c_int64, C.c_void_p]),
+    "stg_group_norm_workspace": (C.c_int32, [C.POINTER(GroupNormConfig), C.c_int32, C.POINTER(C.c_size_t)]),
+    "stg_group_norm": (C.c_int32, [C.c_void_p, C.POINTER(GroupNormConfig)] + [C.c_void_p] * 7 + [C.c_size_t, C.c_void_p]),
+    "stg_group_norm_backward": (C.c_int32, [C.c_void_p, C.POINTER(GroupNormConfig)] + [C.c_void_p] * 10 +
+                                [C.c_size_t, C.c_void_p]),
+    "stg_gated_workspace": (C.c_int32, [C.POINTER(GatedConfig), C.c_int32, C.POINTER(C.c_size_t)]),
+    "stg_gated": (C.c_int32, [C.c_void_p, C.POINTER(GatedConfig)] + [C.c_void_p] * 7 + [C.c_size_t, C.c_void_p]),
+    "stg_gated_backward": (C.c_int32, [C.c_void_p, C.POINTER(GatedConfig)] + [C.c_void_p] * 12 +
+                           [C.c_size_t, C.c_void_p]),
+    "stg_mask_head_sizes": (C.c_int32, [C.c_void_p, _I32P, _I32P, _I32P, C.POINTER(C.c_int64)]),
+    "stg_mask_head_workspace": (C.c_int32, [C.c_void_p, C.POINTER(MaskHeadConfig), C.POINTER(C.c_size_t)]),
+    "stg_mask_head": (C.c_int32, [C.c_void_p, C.POINTER(MaskHeadConfig)] + [C.c_void_p] * 5 + [C.c_size_t, C.c_void_p]),
     "stg_separate_roformer_noalloc": (C.c_int32, [C.c_int, C.POINTER(RoFormerConfig), C.c_int64, C.c_void_p,
                                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]),
 }
@@ -224,6 +268,81 @@ def _stream_of(stream, *tensors):
             import torch
             return torch.cuda.current_stream(t.device).cuda_stream
     return None
+
+
+# ---- the network's layers: tensors, not pointers ---------------------------------------------
+_DTYPES = {}
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "sigmoid": 4}
+_LAYOUTS = {"interleaved": 0, "half": 1}
+_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+
+def _choice(table, key, what):
+    try:
+        return table[key]
+    except (KeyError, TypeError):
+        raise StemsError(1, f"{what} must be one of {', '.join(table)}") from None
+
+
+def _layer_tensor(t, what, device, dtype=None, shape=None):
+    """A layer's tensor argument, checked; its dtype code."""
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    if not hasattr(t, "data_ptr"):
+        raise StemsError(1, f"{what}: expected a tensor")
+    if t.dtype not in _DTYPES:
+        raise StemsError(1, f"{what}: dtype must be float32, float16 or bfloat16")
+    if dtype is not None and t.dtype != dtype:
+        raise StemsError(1, f"{what}: expected dtype {dtype}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise StemsError(1, f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_cuda or t.get_device() != device:
+        raise StemsError(1, f"{what}: expected a tensor on the engine's device cuda:{device}")
+    return _DTYPES[t.dtype]
+
+
+def _inner(t, what):
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise StemsError(1, f"{what}: the last dimension must have stride 1")
+    return t
+
+
+def _run(shape, strides, alone):
+    """(count, stride) of dimensions that are one run of equally spaced items; stride None when
+    they are not, `alone` when there is at most one item."""
+    count, step = 1, None
+    for n, s in zip(reversed(shape), reversed(strides)):
+        if n != 1 and count and n:
+            if step is not None and s != step * count:
+                return count, None
+            step = s if step is None else step
+        count *= n
+    return count, alone if step is None or not count else step
+
+
+def _empty(shape, dtype, device, stream):
+    """A new tensor from the pool of the stream the kernels run on: its memory's earlier users
+    are then ahead of them in that stream."""
+    import torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
+    s = torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
+    with torch.cuda.stream(s):
+        return torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, scaling="none", factor=1.0, original_length=0.0, beta_fast=0.0,
+                       beta_slow=0.0, magnitude=0.0):
+    """(radians per position [rotary_dim / 2] as float64, the factor on the rotated values) of
+    Engine.rotary's angles. Needs no GPU."""
+    cfg = RotaryConfig(C.sizeof(RotaryConfig), 0, 0, 0, 1, 1, rotary_dim, rotary_dim, _choice(_SCALINGS, scaling, "scaling"),
+                       0, base, factor, original_length, beta_fast, beta_slow, magnitude)
+    f, m = np.zeros(max(1, rotary_dim // 2), np.float64), C.c_double()
+    rc = lib().stg_rotary_frequencies(C.byref(cfg), f.ctypes.data_as(C.POINTER(C.c_double)), C.byref(m))
+    if rc != 0:
+        raise StemsError(rc, "rotary_frequencies")
+    return f, m.value
 
 
 def separate_multi_host(plans, mix, mask, out=None):
@@ -385,6 +504,209 @@ class Engine:
                                              _stream_of(stream, spec)), "htdemucs_ispec")
         return y
 
+    # -- layers of the network between the halves --------------------------------------------
+    def rotary(self, q, k=None, positions=None, offset=0, rotary_dim=0, layout="interleaved", base=10000.0,
+               scaling="none", factor=1.0, original_length=0.0, beta_fast=0.0, beta_slow=0.0, magnitude=0.0,
+               inverse=False, out=None, out_k=None, stream=None):
+        """Rotary positions (stg_rotary) of q, and of k in the same launch, [batch][tokens][heads]
+        [head_dim] with any strides outside the heads; the rotated q, or (q, k). positions: int32
+        [tokens] or [batch][tokens], else token t is at offset + t. out / out_k may be q / k
+        themselves. inverse=True is the gradient: rotary(dy, ..., inverse=True) of the same
+        arguments gives dx."""
+        dev = self.device
+        code = _layer_tensor(q, "q", dev)
+        if q.dim() != 4:
+            raise StemsError(1, "q: expected [batch][tokens][heads][head_dim]")
+        b, t, _, d = q.shape
+        pairs = [(_inner(q, "q"), out)]
+        if k is not None:
+            _layer_tensor(k, "k", dev, q.dtype)
+            if k.dim() != 4 or k.shape[0] != b or k.shape[1] != t or k.shape[3] != d:
+                raise StemsError(1, "k: expected q's batch, tokens and head_dim")
+            pairs.append((_inner(k, "k"), out_k))
+        pos, pos_stride = None, 0
+        if positions is not None:
+            if not hasattr(positions, "data_ptr") or str(positions.dtype) != "torch.int32":
+                raise StemsError(1, "positions: expected an int32 tensor")
+            if not positions.is_cuda or positions.get_device() != dev:
+                raise StemsError(1, f"positions: expected a tensor on the engine's device cuda:{dev}")
+            if tuple(positions.shape) not in ((t,), (b, t)) or (t > 1 and positions.stride(-1) != 1):
+                raise StemsError(1, "positions: expected [tokens] or [batch][tokens], the last stride 1")
+            pos, pos_stride = positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0
+        tensors, results = (RotaryTensor * 2)(), []
+        for i, (x, y) in enumerate(pairs):
+            if y is None:
+                y = _empty(x.shape, x.dtype, dev, stream)
+            else:
+                _layer_tensor(y, "out", dev, x.dtype, x.shape)
+                _inner(y, "out")
+            xs, ys = x.stride(), y.stride()
+            tensors[i] = RotaryTensor(x.data_ptr(), y.data_ptr(), x.shape[2], xs[0], xs[1], xs[2], ys[0], ys[1], ys[2])
+            results.append(y)
+        cfg = RotaryConfig(C.sizeof(RotaryConfig), code, _choice(_LAYOUTS, layout, "layout"), int(bool(inverse)), b, t, d,
+                           rotary_dim, _choice(_SCALINGS, scaling, "scaling"), offset, base, factor, original_length,
+                           beta_fast, beta_slow, magnitude)
+        rc = lib().stg_rotary(self._h, C.byref(cfg), tensors, len(pairs), pos, pos_stride, _stream_of(stream, q))
+        if rc != 0:
+            self._check(rc, "rotary")
+        return results[0] if k is None else tuple(results)
+
+    @staticmethod
+    def _rows(t, what):
+        """(batch, positions, batch stride, position stride) of [batch][...][channels], the
+        middle dimensions being one run of positions."""
+        if t.dim() < 2:
+            raise StemsError(1, f"{what}: expected [batch][...][channels]")
+        _inner(t, what)
+        if t.dim() == 3:
+            return t.shape[0], t.shape[1], t.stride(0), t.stride(1)
+        if t.dim() == 2:
+            return t.shape[0], 1, t.stride(0), t.shape[1]
+        n, step = _run(t.shape[1:-1], t.stride()[1:-1], t.shape[-1])
+        if step is None:
+            raise StemsError(1, f"{what}: the positions' dimensions must be one run (call contiguous())")
+        return t.shape[0], n, t.stride(0), step
+
+    def _norm_config(self, x, groups, gamma, beta, activation, eps, y, dx=None):
+        dev = self.device
+        code = _layer_tensor(x, "x", dev)
+        b, n, xb, xp = self._rows(x, "x")
+        ch = x.shape[-1]
+        pcode = None
+        for t, what in ((gamma, "gamma"), (beta, "beta")):
+            if t is not None:
+                pc = _layer_tensor(t, what, dev, shape=(ch,))
+                if pcode is not None and pc != pcode:
+                    raise StemsError(1, "gamma and beta must have one dtype")
+                pcode = pc
+                _inner(t, what)
+        _, _, yb, yp = self._rows(y, "y")
+        db, dp = self._rows(dx, "dx")[2:] if dx is not None else (yb, yp)
+        return GroupNormConfig(C.sizeof(GroupNormConfig), code, 0 if pcode is None else pcode,
+                               _choice(ACTIVATIONS, activation, "activation"), b, n, ch, groups, xb, xp, yb, yp, db, dp, eps)
+
+    def _workspace(self, fn, cfg, backward, what, stream):
+        n = C.c_size_t()
+        rc = fn(C.byref(cfg), backward, C.byref(n))
+        if rc != 0:
+            raise StemsError(rc, what)
+        if not n.value:
+            return None, 0, None
+        import torch
+        ws = _empty((n.value,), torch.uint8, self.device, stream)
+        return ws.data_ptr(), n.value, ws
+
+    def group_norm(self, x, groups, gamma=None, beta=None, activation="none", eps=1e-5, out=None, return_stats=False,
+                   stream=None):
+        """Group norm with an activation (stg_group_norm) of channels-last x [batch][...][channels]:
+        y, or (y, mean, rstd), the statistics float32 [batch][groups], when a backward pass
+        will need them. gamma / beta [channels] in x's dtype or float32. out may be x."""
+        dev = self.device
+        _layer_tensor(x, "x", dev)
+        y = _empty(x.shape, x.dtype, dev, stream) if out is None else out
+        if out is not None:
+            _layer_tensor(out, "out", dev, x.dtype, x.shape)
+        cfg = self._norm_config(x, groups, gamma, beta, activation, eps, y)
+        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 0, "group_norm", stream)
+        mean = rstd = None
+        if return_stats:
+            import torch
+            mean, rstd = (_empty((x.shape[0], groups), torch.float32, dev, stream) for _ in range(2))
+        rc = lib().stg_group_norm(self._h, C.byref(cfg), x.data_ptr(), gamma.data_ptr() if gamma is not None else None,
+                                  beta.data_ptr() if beta is not None else None, y.data_ptr(),
+                                  mean.data_ptr() if return_stats else None, rstd.data_ptr() if return_stats else None,
+                                  ws, n, _stream_of(stream, x))
+        if rc != 0:
+            self._check(rc, "group_norm")
+        return (y, mean, rstd) if return_stats else y
+
+    def group_norm_backward(self, dy, x, groups, gamma, beta, mean, rstd, activation="none", eps=1e-5, need_dx=True,
+                            stream=None):
+        """(dx, dgamma, dbeta) of group_norm from dy and the forward pass's x, mean and rstd; the
+        last two None without gamma / beta, dx None without need_dx."""
+        import torch
+        dev = self.device
+        _layer_tensor(x, "x", dev)
+        _layer_tensor(dy, "dy", dev, x.dtype, x.shape)
+        for t, what in ((mean, "mean"), (rstd, "rstd")):
+            _layer_tensor(t, what, dev, torch.float32, (x.shape[0], groups))
+            if not t.is_contiguous():
+                raise StemsError(1, f"{what}: expected a contiguous tensor")
+        dx = _empty(x.shape, x.dtype, dev, stream) if need_dx else None
+        cfg = self._norm_config(x, groups, gamma, beta, activation, eps, dy, dx)
+        dgamma, dbeta = (None if t is None else _empty(t.shape, t.dtype, dev, stream) for t in (gamma, beta))
+        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 1, "group_norm_backward", stream)
+        ptrs = [None if t is None else t.data_ptr() for t in (dy, x, gamma, beta, mean, rstd, dx, dgamma, dbeta)]
+        rc = lib().stg_group_norm_backward(self._h, C.byref(cfg), *ptrs, ws, n, _stream_of(stream, x))
+        if rc != 0:
+            self._check(rc, "group_norm_backward")
+        return dx, dgamma, dbeta
+
+    def _gated_config(self, x, wg, wu, bg, bu, activation, y):
+        dev = self.device
+        code = _layer_tensor(x, "x", dev)
+        if x.dim() < 2:
+            raise StemsError(1, "x: expected [...][features]")
+        k = x.shape[-1]
+        if not hasattr(wg, "shape") or len(wg.shape) != 2:
+            raise StemsError(1, "w_gate: expected [width][features]")
+        n = wg.shape[0]
+        for t, what in ((wg, "w_gate"), (wu, "w_up")):
+            _layer_tensor(t, what, dev, x.dtype, (n, k))
+            _inner(t, what)
+        for t, what in ((bg, "b_gate"), (bu, "b_up")):
+            if t is not None:
+                _layer_tensor(t, what, dev, x.dtype, (n,))
+                _inner(t, what)
+        _layer_tensor(y, "y", dev, x.dtype, (*x.shape[:-1], n))
+        return GatedConfig(C.sizeof(GatedConfig), code, _choice(ACTIVATIONS, activation, "activation"), k, n,
+                           x.numel() // k if k else 0, self._row_stride(x, "x"), wg.stride(0), wu.stride(0),
+                           self._row_stride(y, "y"), k, k, k)
+
+    @staticmethod
+    def _row_stride(t, what):
+        """The one stride of the rows of [...][features]."""
+        _inner(t, what)
+        step = _run(t.shape[:-1], t.stride()[:-1], t.shape[-1])[1]
+        if step is None:
+            raise StemsError(1, f"{what}: the rows must have one stride (call contiguous())")
+        return step
+
+    def gated(self, x, w_gate, w_up, b_gate=None, b_up=None, activation="silu", out=None, stream=None):
+        """act(x w_gate^T + b_gate) (x w_up^T + b_up) (stg_gated): x [...][features], weights
+        [width][features], biases [width]; y [...][width]."""
+        dev = self.device
+        _layer_tensor(x, "x", dev)
+        if out is None:
+            if not hasattr(w_gate, "shape") or x.dim() < 2:
+                raise StemsError(1, "expected x [...][features] and w_gate [width][features]")
+            out = _empty((*x.shape[:-1], w_gate.shape[0]), x.dtype, dev, stream)
+        cfg = self._gated_config(x, w_gate, w_up, b_gate, b_up, activation, out)
+        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 0, "gated", stream)
+        rc = lib().stg_gated(self._h, C.byref(cfg), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+                             b_gate.data_ptr() if b_gate is not None else None,
+                             b_up.data_ptr() if b_up is not None else None, out.data_ptr(), ws, n, _stream_of(stream, x))
+        if rc != 0:
+            self._check(rc, "gated")
+        return out
+
+    def gated_backward(self, dy, x, w_gate, w_up, b_gate=None, b_up=None, activation="silu", need_dx=True, need_dw=True,
+                       stream=None):
+        """(dx, dw_gate, dw_up), then the biases' gradients for the biases given, of gated from dy
+        and the forward pass's inputs. need_dx / need_dw False leave None in their places."""
+        dev = self.device
+        _layer_tensor(dy, "dy", dev)
+        cfg = self._gated_config(x, w_gate, w_up, b_gate, b_up, activation, dy)
+        dx = _empty(x.shape, x.dtype, dev, stream) if need_dx else None
+        dws = [_empty(w.shape, w.dtype, dev, stream) if need_dw else None for w in (w_gate, w_up)]
+        dbs = [None if t is None else _empty(t.shape, t.dtype, dev, stream) for t in (b_gate, b_up)]
+        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 1, "gated_backward", stream)
+        ptrs = [None if t is None else t.data_ptr() for t in (dy, x, w_gate, w_up, b_gate, b_up, dx, *dws, *dbs)]
+        rc = lib().stg_gated_backward(self._h, C.byref(cfg), *ptrs, ws, n, _stream_of(stream, x))
+        if rc != 0:
+            self._check(rc, "gated_backward")
+        return (dx, *dws, *(t for t in dbs if t is not None))
+
     # -- plans ---------------------------------------------------------------------------
     def plan_htdemucs(self, n_samples, n_channels=2, n_sources=4, segment=343980, overlap=-1.0,
                       mono_norm=True, cac_norm=True, shifts=0, seed=0, sample_rate=44100, n_models=1,
@@ -525,6 +847,49 @@ class Plan:
 
     def finish(self, mix, out, stream=None):
         self.engine._check(lib().stg_finish(self._h, _ptr(mix), _ptr(out), _stream_of(stream, out)), "finish")
+
+    def mask_head_sizes(self):
+        """(stems, bands, frames, sum of the bands' mask entries per frame) of a RoFormer plan."""
+        s, b, t, c = C.c_int32(), C.c_int32(), C.c_int32(), C.c_int64()
+        self.engine._check(lib().stg_mask_head_sizes(self._h, C.byref(s), C.byref(b), C.byref(t), C.byref(c)),
+                           "mask_head_sizes")
+        return s.value, b.value, t.value, c.value
+
+    def mask_head(self, hidden, weight, bias=None, out=None, stream=None):
+        """RoFormer's last layer (stg_mask_head): hidden [chunks][stems][bands][frames][hidden],
+        weight [stems][2 sum din][hidden] and bias [stems][2 sum din] band after band, a band's
+        value rows before its gate rows -> float32 masks [chunks][mask floats per chunk], the
+        layout back() and separate() read. out: such a tensor, or a device pointer (the network
+        output a separate_network callback is given)."""
+        import torch
+        dev = self.engine.device
+        s, b, t, cols = self._head_sizes = getattr(self, "_head_sizes", None) or self.mask_head_sizes()
+        code = _layer_tensor(hidden, "hidden", dev)
+        if hidden.dim() != 5 or tuple(hidden.shape[1:4]) != (s, b, t):
+            raise StemsError(1, f"hidden: expected [chunks][{s}][{b}][{t}][hidden]")
+        n, k = hidden.shape[0], hidden.shape[4]
+        _layer_tensor(weight, "weight", dev, hidden.dtype, (s, 2 * cols, k))
+        if bias is not None:
+            _layer_tensor(bias, "bias", dev, hidden.dtype, (s, 2 * cols))
+        for x, what in ((hidden, "hidden"), (weight, "weight"), (bias, "bias")):
+            if x is not None and not x.is_contiguous():
+                raise StemsError(1, f"{what}: expected a contiguous tensor")
+        if out is None:
+            out = _empty((n, self.mask_floats_per_chunk), torch.float32, dev, stream)
+        elif not isinstance(out, int):
+            _layer_tensor(out, "out", dev, torch.float32)
+            if out.numel() != n * self.mask_floats_per_chunk or not out.is_contiguous():
+                raise StemsError(1, "out: expected a contiguous [chunks][mask floats per chunk]")
+        cfg = MaskHeadConfig(C.sizeof(MaskHeadConfig), code, k, n)
+        need = C.c_size_t()
+        self.engine._check(lib().stg_mask_head_workspace(self._h, C.byref(cfg), C.byref(need)), "mask_head")
+        ws = _empty((need.value,), torch.uint8, dev, stream) if need.value else None
+        rc = lib().stg_mask_head(self._h, C.byref(cfg), hidden.data_ptr(), weight.data_ptr(),
+                                 bias.data_ptr() if bias is not None else None, out if isinstance(out, int) else out.data_ptr(),
+                                 ws.data_ptr() if ws is not None else None, need.value, _stream_of(stream, hidden))
+        if rc != 0:
+            self.engine._check(rc, "mask_head")
+        return out
 
     def separate_network(self, mix, out, network, chunks_per_batch=0, stream=None):
         """network(first_chunk, n_chunks, net_in_ptr, net_out_ptr, stream_handle) runs the model."""

@@ -46,6 +46,11 @@ struct FftTables {
     DevBuf win, tw;
 };
 
+// One tile of the mask head's output columns (gated.cu): its band, first column, the band's
+// first entry and its width.
+constexpr int kHeadTileN = 64;
+struct HeadTile { int band, n0, off, din; };
+
 } // namespace stg
 
 // the handles of the C ABI live in the global namespace, as the header declares them
@@ -105,6 +110,8 @@ struct stg_plan {
     DevBuf d_mixn, d_mono, d_cac_part, d_cac_stats;   // scratch of the HTDemucs normalisations
     DevBuf d_mask_t;                                  // t-major masks (HTDemucs, TFC-TDF)
     DevBuf d_zspec;                                   // HTDemucs spectra
+    DevBuf d_head;                                    // RoFormer: the mask head's column tiles (HeadTile)
+    int head_tiles = 0;
     const float* mono_src = nullptr;                  // the track d_mixn was normalised from
     DevBuf s_mix, s_mask, s_out;   // device staging for stg_separate_host
     // stg_separate_host: a copy stream that brings the masks in batch by batch, and the events
@@ -145,6 +152,14 @@ struct stg_plan {
         upload(d_ebeg, H.ebeg, "band table");
         upload(d_ent, H.ent, "band table");
         upload(d_binv, H.binv, "band table");
+        if (!H.band_din.empty()) {
+            std::vector<HeadTile> tiles;
+            int off = 0;
+            for (int b = 0; b < (int)H.band_din.size(); off += H.band_din[b++])
+                for (int n0 = 0; n0 < H.band_din[b]; n0 += kHeadTileN) tiles.push_back(HeadTile{b, n0, off, H.band_din[b]});
+            head_tiles = (int)tiles.size();
+            upload(d_head, tiles, "mask head tiles");
+        }
         if (!H.bag.empty()) {
             upload(d_bag, H.bag, "bag weights");
             upload(d_bag_tot, H.bag_tot, "bag weights");

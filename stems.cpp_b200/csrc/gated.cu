@@ -1,0 +1,512 @@
+// gated.cu -- the gated projection, its backward pass and RoFormer's mask head
+// (include/stems_gpu_v1.h: stg_gated, stg_gated_backward, stg_mask_head): entry points and the
+// kernels on the CUDA cores.
+//
+// With g = x Wg^T + bg and u = x Wu^T + bu: y = act(g) u. Backward:
+//   dg = dy u act'(g), du = dy act(g);  dx = dg Wg + du Wu;  dWg = dg^T x, dWu = du^T x;
+//   dbg, dbu = column sums of dg, du.
+#include "gated.h"
+
+namespace stg {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTileK = 16;
+constexpr int kPitch = 132;        // floats between two k rows of a tile
+
+__device__ __forceinline__ float sigmoid_exact(float z) { return 1.0f / (1.0f + expf(-z)); }
+
+__device__ __forceinline__ float gate_act(int a, float z) {
+    switch (a) {
+        case STG_ACT_RELU: return z < 0.0f ? 0.0f : z;
+        case STG_ACT_SILU: return z * sigmoid_exact(z);
+        case STG_ACT_GELU: return 0.5f * z * erfcf(-z * 0.70710678118654752f);
+        case STG_ACT_SIGMOID: return sigmoid_exact(z);
+        default: return z;
+    }
+}
+__device__ __forceinline__ float gate_grad(int a, float z) {
+    switch (a) {
+        case STG_ACT_RELU: return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
+        case STG_ACT_SILU: { const float s = sigmoid_exact(z); return s * fmaf(z, 1.0f - s, 1.0f); }
+        case STG_ACT_GELU: return fmaf(0.3989422804014327f * z, expf(-0.5f * z * z), 0.5f * erfcf(-z * 0.70710678118654752f));
+        case STG_ACT_SIGMOID: { const float s = sigmoid_exact(z); return s * (1.0f - s); }
+        default: return 1.0f;
+    }
+}
+
+// A 128 x 16 tile of an operand on its way to shared memory, [k][128]. KMAJOR: element (i, k)
+// is at p[i * ld + k], otherwise at p[k * ld + i]. A thread takes eight neighbours in memory.
+template <class T, bool KMAJOR> struct TileLoad {
+    float v[8];
+    __device__ __forceinline__ void fetch(const T* p, int64_t ld, int64_t i0, int64_t ni, int64_t k0, int64_t nk) {
+        const int t = threadIdx.x;
+        const int64_t r = KMAJOR ? i0 + (t >> 1) : k0 + (t >> 4);
+        const int64_t c = KMAJOR ? k0 + (t & 1) * 8 : i0 + (t & 15) * 8;
+        const bool row_ok = r < (KMAJOR ? ni : nk);
+        const int64_t nc = KMAJOR ? nk : ni;
+        const T* q = p + r * ld + c;
+        if (row_ok && c + 8 <= nc && (reinterpret_cast<uintptr_t>(q) & 15) == 0) {
+            constexpr int W = 16 / sizeof(T);
+#pragma unroll
+            for (int j = 0; j < 8; j += W) {
+                const Pack<T, W> w = *reinterpret_cast<const Pack<T, W>*>(q + j);
+#pragma unroll
+                for (int e = 0; e < W; e++) v[j + e] = to_float(w.v[e]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = row_ok && c + j < nc ? to_float(q[j]) : 0.0f;
+        }
+    }
+    __device__ __forceinline__ void store(float* s, int row_base = 0) const {
+        const int t = threadIdx.x;
+        if (KMAJOR) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) s[((t & 1) * 8 + j) * kPitch + row_base + (t >> 1)] = v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j += 4)
+                *reinterpret_cast<float4*>(s + (t >> 4) * kPitch + (t & 15) * 8 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        }
+    }
+};
+
+__device__ __forceinline__ void fma2(uint64_t& d, uint64_t a, uint64_t b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ uint64_t twice(float a) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(a));
+    return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+
+// 128 x 128 outputs per block, 8 x 8 per thread: rows 4 ty + {0..3} and 64 + that, columns
+// 4 tx + {0..3} and 64 + that. In the dual modes the second 64 columns are the up projection of
+// the same outputs as the first, so a thread holds both factors of its outputs. Products and
+// sums are float with one rounding each (packed in pairs); K runs in order.
+template <class T, int MODE>
+__global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ GatedParams p) {
+    constexpr bool DUAL = MODE == GATED_FWD || MODE == GATED_HEAD || MODE == GATED_PRE;
+    constexpr bool AK = MODE != GATED_DW, BK = DUAL;   // contraction contiguous in memory
+    __shared__ __align__(16) float As[2][kTileK * kPitch], Bs[2][kTileK * kPitch];
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+
+    // the tile
+    int64_t m0, ni, nk, nj;           // first row, rows, contraction, columns of an operand
+    int n0;
+    const T *a = nullptr, *b0 = nullptr, *b1 = nullptr, *a2 = nullptr;
+    int64_t lda, ldb0, ldb1;
+    HeadTile ht{};
+    int64_t head_row = 0, bias0 = 0;  // mask head: first frame of the tile's band in x; row of the band's first weight
+    int64_t kbeg = 0;
+    if (MODE == GATED_HEAD) {
+        ht = p.tiles[blockIdx.x % p.n_tiles];
+        const int64_t rest = blockIdx.x / p.n_tiles, mt = (p.frames + kGatedTileM - 1) / kGatedTileM;
+        const int64_t cs = rest / mt;                    // chunk * stems + stem
+        m0 = (rest - cs * mt) * kGatedTileM;
+        n0 = ht.n0;
+        ni = p.frames; nk = p.k; nj = ht.din;
+        head_row = (cs * p.bands + ht.band) * p.frames;
+        a = static_cast<const T*>(p.x) + head_row * p.k;
+        lda = p.k;
+        bias0 = (cs % p.stems) * 2 * p.band_cols + 2 * (int64_t)ht.off;
+        b0 = static_cast<const T*>(p.wg) + bias0 * p.k;
+        b1 = b0 + (int64_t)ht.din * p.k;
+        ldb0 = ldb1 = p.k;
+        head_row = cs;                                   // for the output
+    } else if (DUAL) {
+        const int nt = (p.n + kGatedTileN - 1) / kGatedTileN;
+        m0 = (int64_t)(blockIdx.x / nt) * kGatedTileM;
+        n0 = (int)(blockIdx.x % nt) * kGatedTileN;
+        ni = p.m; nk = p.k; nj = p.n;
+        a = static_cast<const T*>(p.x);
+        b0 = static_cast<const T*>(p.wg);
+        b1 = static_cast<const T*>(p.wu);
+        lda = p.x_row; ldb0 = p.wg_row; ldb1 = p.wu_row;
+    } else if (MODE == GATED_DX) {
+        const int nt = (p.k + 127) / 128;
+        m0 = (int64_t)(blockIdx.x / nt) * kGatedTileM;
+        n0 = (int)(blockIdx.x % nt) * 128;
+        ni = p.m; nk = p.n; nj = p.k;
+        a = static_cast<const T*>(p.dg);
+        a2 = static_cast<const T*>(p.du);
+        b0 = static_cast<const T*>(p.wg);
+        b1 = static_cast<const T*>(p.wu);
+        lda = p.pre_row; ldb0 = p.wg_row; ldb1 = p.wu_row;
+    } else {
+        const int nt = (p.k + 127) / 128;
+        m0 = (int64_t)(blockIdx.x / nt) * kGatedTileM;
+        n0 = (int)(blockIdx.x % nt) * 128;
+        const bool up = blockIdx.y & 1;
+        kbeg = (int64_t)(blockIdx.y >> 1) * p.split_rows;
+        ni = p.n; nk = min(p.m, kbeg + p.split_rows); nj = p.k;
+        a = static_cast<const T*>(up ? p.du : p.dg);
+        b0 = static_cast<const T*>(p.x);
+        lda = p.pre_row; ldb0 = ldb1 = p.x_row;
+    }
+
+    uint64_t acc[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[i][j] = 0;
+
+    const int64_t steps1 = (nk - kbeg + kTileK - 1) / kTileK, steps = steps1 * (MODE == GATED_DX ? 2 : 1);
+    TileLoad<T, AK> la;
+    TileLoad<T, BK> lb;
+    // the dual modes' B tile: rows 0..63 from Wg, 64..127 from Wu
+    auto fetch = [&](int64_t s) {
+        const bool second = MODE == GATED_DX && s >= steps1;
+        const int64_t k0 = kbeg + (second ? s - steps1 : s) * kTileK;
+        la.fetch(second ? a2 : a, lda, m0, ni, k0, nk);
+        if (DUAL) {
+            const bool up = threadIdx.x >= 128;   // threads 128.. carry rows 64..
+            lb.fetch(up ? b1 : b0, up ? ldb1 : ldb0, n0 - (up ? 64 : 0), nj, k0, nk);
+        } else {
+            lb.fetch(second ? b1 : b0, second ? ldb1 : ldb0, n0, nj, k0, nk);
+        }
+    };
+    if (steps > 0) {
+        fetch(0);
+        la.store(As[0]);
+        lb.store(Bs[0]);
+    }
+    __syncthreads();
+    for (int64_t s = 0; s < steps; s++) {
+        const int cur = (int)(s & 1);
+        if (s + 1 < steps) fetch(s + 1);
+        const float *pa = As[cur] + 4 * ty, *pb = Bs[cur] + 4 * tx;
+#pragma unroll
+        for (int k = 0; k < kTileK; k++) {
+            const float4 a0 = *reinterpret_cast<const float4*>(pa + k * kPitch), a1 = *reinterpret_cast<const float4*>(pa + k * kPitch + 64);
+            const ulonglong2 c0 = *reinterpret_cast<const ulonglong2*>(pb + k * kPitch), c1 = *reinterpret_cast<const ulonglong2*>(pb + k * kPitch + 64);
+            const float av[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+            const uint64_t bv[4] = {c0.x, c0.y, c1.x, c1.y};
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint64_t d = twice(av[i]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) fma2(acc[i][j], d, bv[j]);
+            }
+        }
+        if (s + 1 < steps) {
+            la.store(As[cur ^ 1]);
+            lb.store(Bs[cur ^ 1]);
+        }
+        __syncthreads();
+    }
+
+    float v[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 h = halves(acc[i][j]);
+            v[i][2 * j] = h.x;
+            v[i][2 * j + 1] = h.y;
+        }
+    auto row_of = [&](int i) { return m0 + 4 * ty + (i & 3) + (i >> 2) * 64; };
+
+    if (DUAL) {
+        float bg[4], bu[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int c = n0 + 4 * tx + j;
+            bg[j] = bu[j] = 0.0f;
+            if (p.bg && c < nj) {
+                bg[j] = to_float(static_cast<const T*>(p.bg)[bias0 + c]);
+                if (MODE == GATED_HEAD) bu[j] = to_float(static_cast<const T*>(p.bg)[bias0 + ht.din + c]);
+            }
+            if (MODE != GATED_HEAD && p.bu && c < nj) bu[j] = to_float(static_cast<const T*>(p.bu)[c]);
+        }
+        float sg[4] = {}, su[4] = {};
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int64_t r = row_of(i);
+            if (r >= ni) continue;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int c = n0 + 4 * tx + j;
+                if (c >= nj) continue;
+                const float g = v[i][j] + bg[j], u = v[i][4 + j] + bu[j];
+                if (MODE == GATED_FWD) {
+                    static_cast<T*>(p.y)[r * p.y_row + c] = from_float<T>(gate_act(p.act, g) * u);
+                } else if (MODE == GATED_HEAD) {   // value rows come first: g is the value, u its gate
+                    p.masks[(head_row * p.band_cols + ht.off) * p.frames + r * ht.din + c] = g * sigmoid_exact(u);
+                } else {
+                    const float dy = to_float(static_cast<const T*>(p.dy)[r * p.y_row + c]);
+                    const float dg = dy * u * gate_grad(p.act, g), du = dy * gate_act(p.act, g);
+                    static_cast<T*>(p.dg)[r * p.pre_row + c] = from_float<T>(dg);
+                    static_cast<T*>(p.du)[r * p.pre_row + c] = from_float<T>(du);
+                    sg[j] += dg;
+                    su[j] += du;
+                }
+            }
+        }
+        if (MODE == GATED_PRE && p.col_sums) {
+            // the 16 threads of a column group, through shared memory in a fixed order
+            float* red = As[0];   // [ty][2][64]
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                red[ty * 128 + 4 * tx + j] = sg[j];
+                red[ty * 128 + 64 + 4 * tx + j] = su[j];
+            }
+            __syncthreads();
+            if (threadIdx.x < 128) {
+                float t = 0.0f;
+                for (int r = 0; r < 16; r++) t += red[r * 128 + threadIdx.x];
+                const int c = n0 + (threadIdx.x & 63);
+                if (c < p.n) p.col_sums[((m0 / kGatedTileM) * 2 + (threadIdx.x >> 6)) * p.n + c] = t;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int64_t r = row_of(i);
+            if (r >= ni) continue;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int c = n0 + 4 * tx + (j & 3) + (j >> 2) * 64;
+                if (c >= nj) continue;
+                if (MODE == GATED_DX) static_cast<T*>(p.dx)[r * p.dx_row + c] = from_float<T>(v[i][j]);
+                else p.dw_part[((int64_t)blockIdx.y * p.n + r) * p.k + c] = v[i][j];
+            }
+        }
+    }
+}
+
+// dW from its partial sums [splits][2][n][k], added in order.
+template <class T>
+__global__ void __launch_bounds__(kThreads) dw_join(const float* part, int splits, int64_t n, int64_t k, T* dwg, int64_t dwg_row,
+                                                    T* dwu, int64_t dwu_row) {
+    const int64_t total = 2 * n * k;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+        float s = 0.0f;
+        for (int q = 0; q < splits; q++) s += part[q * total + i];
+        const bool up = i >= n * k;
+        const int64_t j = up ? i - n * k : i, r = j / k, c = j - r * k;
+        T* d = up ? dwu : dwg;
+        if (d) d[r * (up ? dwu_row : dwg_row) + c] = from_float<T>(s);
+    }
+}
+
+// dbg and dbu from the tiles' column sums [tiles][2][n]: a warp per column.
+template <class T>
+__global__ void __launch_bounds__(128) db_join(const float* sums, int64_t tiles, int n, T* dbg, T* dbu) {
+    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (i >= 2 * (int64_t)n) return;
+    float s = 0.0f;
+    for (int64_t t = lane; t < tiles; t += 32) s += sums[t * 2 * n + i];
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    if (lane == 0) {
+        T* d = i < n ? dbg : dbu;
+        if (d) d[i < n ? i : i - n] = from_float<T>(s);
+    }
+}
+
+// ---- host -------------------------------------------------------------------------------------
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+void check_config(const stg_gated_config* c, bool backward) {
+    check_sized(c, "gated");
+    check(valid_dtype(c->dtype), "gated: unknown dtype");
+    check(valid_activation(c->activation), "gated: unknown activation");
+    check(c->features >= 1 && c->width >= 1 && c->rows >= 0, "gated: features and width must be at least 1, rows at least 0");
+    if (c->rows > INT32_MAX) fail(STG_UNSUPPORTED, "gated: too many rows");
+    check(c->x_row >= 0 && c->wg_row >= 0 && c->wu_row >= 0 && c->y_row >= 0, "gated: negative stride");
+    check((c->y_row >= c->width || c->rows <= 1) || backward, "gated: the output's rows overlap");
+}
+
+struct GatedLayout { size_t dg = 0, du = 0, sums = 0, dw = 0, bytes = 0; int64_t pre_row = 0; int splits = 1; int64_t split_rows = 0; };
+
+GatedLayout backward_layout(const stg_gated_config& c) {
+    GatedLayout l;
+    const size_t es = elem_size(c.dtype);
+    l.pre_row = ceil_div(c.width, 8) * 8;
+    l.du = up256((size_t)c.rows * l.pre_row * es);
+    l.sums = l.du + up256((size_t)c.rows * l.pre_row * es);
+    l.dw = l.sums + up256(sizeof(float) * (size_t)ceil_div(c.rows, kGatedTileM) * 2 * c.width);
+    // dW has 2 width x features outputs and a sum over all rows: rows are split until the tiles
+    // fill the GPU twice, while a part keeps at least 256 rows
+    const int64_t tiles = 2 * ceil_div(c.width, 128) * ceil_div(c.features, 128);
+    l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(2 * 148, tiles), c.rows / 256, 64}));
+    l.split_rows = std::max<int64_t>(16, ceil_div(ceil_div(c.rows, l.splits), 16) * 16);
+    l.splits = (int)std::max<int64_t>(1, ceil_div(c.rows, l.split_rows));
+    l.bytes = l.dw + up256(sizeof(float) * (size_t)l.splits * 2 * c.width * c.features);
+    return l;
+}
+
+GatedParams params_of(const stg_gated_config& c) {
+    GatedParams p{};
+    p.m = c.rows; p.n = c.width; p.k = c.features;
+    p.act = c.activation;
+    p.x_row = c.x_row; p.wg_row = c.wg_row; p.wu_row = c.wu_row; p.y_row = c.y_row; p.dx_row = c.dx_row;
+    return p;
+}
+
+dim3 tile_grid(int64_t tiles, int64_t y = 1) {
+    if (tiles > INT32_MAX || y > 65535) fail(STG_UNSUPPORTED, "gated: too many tiles");
+    return dim3((unsigned)tiles, (unsigned)y);
+}
+
+} // namespace
+
+} // namespace stg
+
+extern "C" {
+
+STG_API stg_status stg_gated_workspace(const stg_gated_config* c, int32_t backward, size_t* bytes) {
+    return guard(nullptr, [&] {
+        check_config(c, backward != 0);
+        check(bytes && (backward == 0 || backward == 1), "gated: null buffer");
+        *bytes = backward && c->rows ? backward_layout(*c).bytes : 0;
+    });
+}
+
+STG_API stg_status stg_gated(stg_engine* e, const stg_gated_config* c, const void* d_x, const void* d_wg, const void* d_wu,
+                             const void* d_bg, const void* d_bu, void* d_y, void* d_ws, size_t ws_bytes, void* stream) {
+    if (!e) return STG_INVALID_ARGUMENT;
+    return guard(e, [&] {
+        check_config(c, false);
+        const size_t es = elem_size(c->dtype);
+        for (const void* q : {d_x, d_wg, d_wu, d_bg, d_bu, (const void*)d_y}) check(aligned(q, es), "gated: a buffer is not aligned to its elements");
+        if (!c->rows) return;
+        check(d_x && d_wg && d_wu && d_y, "gated: null buffer");
+        GatedParams p = params_of(*c);
+        p.x = d_x; p.wg = d_wg; p.wu = d_wu; p.bg = d_bg; p.bu = d_bu; p.y = d_y;
+        DeviceScope scope(e);
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        const dim3 grid = tile_grid(ceil_div(p.m, kGatedTileM) * ceil_div(p.n, kGatedTileN));
+        with_dtype(c->dtype, [&](auto* tag) {
+            using T = std::remove_pointer_t<decltype(tag)>;
+            gated_simt<T, GATED_FWD><<<grid, kThreads, 0, st>>>(p);
+        });
+        cuda_check(cudaGetLastError(), "gated kernel");
+    });
+}
+
+STG_API stg_status stg_gated_backward(stg_engine* e, const stg_gated_config* c, const void* d_dy, const void* d_x, const void* d_wg,
+                                      const void* d_wu, const void* d_bg, const void* d_bu, void* d_dx, void* d_dwg, void* d_dwu,
+                                      void* d_dbg, void* d_dbu, void* d_ws, size_t ws_bytes, void* stream) {
+    if (!e) return STG_INVALID_ARGUMENT;
+    return guard(e, [&] {
+        check_config(c, true);
+        const size_t es = elem_size(c->dtype);
+        for (const void* q : {d_dy, d_x, d_wg, d_wu, d_bg, d_bu, (const void*)d_dx, (const void*)d_dwg, (const void*)d_dwu, (const void*)d_dbg, (const void*)d_dbu})
+            check(aligned(q, es), "gated: a buffer is not aligned to its elements");
+        check(!d_dx || c->dx_row >= c->features || c->rows <= 1, "gated: the rows of dx overlap");
+        check((!d_dwg || c->dwg_row >= c->features || c->width == 1) && (!d_dwu || c->dwu_row >= c->features || c->width == 1),
+              "gated: the rows of a weight's gradient overlap");
+        DeviceScope scope(e);
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (!c->rows) {   // sums over no rows
+            auto zero = [&](void* d, int64_t row, int64_t w, int64_t h) {
+                if (d) cuda_check(cudaMemset2DAsync(d, (size_t)std::max(row, w) * es, 0, (size_t)w * es, (size_t)h, st), "gated memset");
+            };
+            zero(d_dwg, c->dwg_row, c->features, c->width);
+            zero(d_dwu, c->dwu_row, c->features, c->width);
+            zero(d_dbg, c->width, c->width, 1);
+            zero(d_dbu, c->width, c->width, 1);
+            return;
+        }
+        check(d_dy && d_x && d_wg && d_wu, "gated: null buffer");
+        if (!d_dx && !d_dwg && !d_dwu && !d_dbg && !d_dbu) return;
+        const GatedLayout lay = backward_layout(*c);
+        check(d_ws && aligned(d_ws, 256) && ws_bytes >= lay.bytes, "gated: workspace is missing, unaligned or too small");
+        char* ws = static_cast<char*>(d_ws);
+        GatedParams p = params_of(*c);
+        p.dy = d_dy; p.x = d_x; p.wg = d_wg; p.wu = d_wu; p.bg = d_bg; p.bu = d_bu; p.dx = d_dx;
+        p.dg = ws;
+        p.du = ws + lay.du;
+        p.pre_row = lay.pre_row;
+        p.col_sums = d_dbg || d_dbu ? reinterpret_cast<float*>(ws + lay.sums) : nullptr;
+        p.dw_part = reinterpret_cast<float*>(ws + lay.dw);
+        p.splits = lay.splits;
+        p.split_rows = lay.split_rows;
+        const int64_t mt = ceil_div(p.m, kGatedTileM);
+        with_dtype(c->dtype, [&](auto* tag) {
+            using T = std::remove_pointer_t<decltype(tag)>;
+            gated_simt<T, GATED_PRE><<<tile_grid(mt * ceil_div(p.n, kGatedTileN)), kThreads, 0, st>>>(p);
+            if (p.col_sums)
+                db_join<T><<<(unsigned)ceil_div(2 * (int64_t)p.n, 4), 128, 0, st>>>(p.col_sums, mt, p.n, static_cast<T*>(d_dbg), static_cast<T*>(d_dbu));
+            if (d_dx) gated_simt<T, GATED_DX><<<tile_grid(mt * ceil_div(p.k, 128)), kThreads, 0, st>>>(p);
+            if (d_dwg || d_dwu) {
+                gated_simt<T, GATED_DW><<<tile_grid(ceil_div(p.n, 128) * ceil_div(p.k, 128), 2 * p.splits), kThreads, 0, st>>>(p);
+                const int64_t blocks = std::min<int64_t>(ceil_div(2 * (int64_t)p.n * p.k, kThreads), 148 * 8);
+                dw_join<T><<<(unsigned)blocks, kThreads, 0, st>>>(p.dw_part, p.splits, p.n, p.k, static_cast<T*>(d_dwg), c->dwg_row,
+                                                                  static_cast<T*>(d_dwu), c->dwu_row);
+            }
+        });
+        cuda_check(cudaGetLastError(), "gated kernel");
+    });
+}
+
+static void check_head(const stg_plan* p, const stg_mask_head_config* c) {
+    check_sized(c, "mask head");
+    check(p->H.arch == ARCH_ROFORMER && !p->H.band_din.empty(), "mask head: not a RoFormer plan");
+    check(valid_dtype(c->dtype), "mask head: unknown dtype");
+    check(c->hidden >= 1 && c->n_chunks >= 0, "mask head: hidden must be at least 1, n_chunks at least 0");
+}
+
+STG_API stg_status stg_mask_head_sizes(const stg_plan* p, int32_t* stems, int32_t* bands, int32_t* frames, int64_t* columns) {
+    if (!p) return STG_INVALID_ARGUMENT;
+    return guard(p->engine, [&] {
+        check(p->H.arch == ARCH_ROFORMER && !p->H.band_din.empty(), "mask head: not a RoFormer plan");
+        check(stems && bands && frames && columns, "mask head: null buffer");
+        *stems = p->H.S;
+        *bands = (int32_t)p->H.band_din.size();
+        *frames = p->H.g.T;
+        *columns = p->H.stem_stride / p->H.g.T;
+    });
+}
+
+STG_API stg_status stg_mask_head_workspace(const stg_plan* p, const stg_mask_head_config* c, size_t* bytes) {
+    if (!p) return STG_INVALID_ARGUMENT;
+    return guard(p->engine, [&] {
+        check_head(p, c);
+        check(bytes, "mask head: null buffer");
+        *bytes = 0;
+    });
+}
+
+STG_API stg_status stg_mask_head(stg_plan* plan, const stg_mask_head_config* c, const void* d_hidden, const void* d_weight,
+                                 const void* d_bias, float* d_masks, void* d_ws, size_t ws_bytes, void* stream) {
+    if (!plan) return STG_INVALID_ARGUMENT;
+    return guard(plan->engine, [&] {
+        check_head(plan, c);
+        const size_t es = elem_size(c->dtype);
+        for (const void* q : {d_hidden, d_weight, d_bias}) check(aligned(q, es), "mask head: a buffer is not aligned to its elements");
+        if (!c->n_chunks) return;
+        check(d_hidden && d_weight && d_masks, "mask head: null buffer");
+        plan->H.check_mask(d_masks);
+        GatedParams p{};
+        p.x = d_hidden; p.wg = d_weight; p.bg = d_bias; p.masks = d_masks;
+        p.k = c->hidden;
+        p.frames = plan->H.g.T;
+        p.bands = (int)plan->H.band_din.size();
+        p.stems = plan->H.S;
+        p.band_cols = plan->H.stem_stride / plan->H.g.T;
+        p.tiles = plan->d_head.as<HeadTile>();
+        p.n_tiles = plan->head_tiles;
+        DeviceScope scope(plan->engine);
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        const dim3 grid = tile_grid((int64_t)c->n_chunks * p.stems * ceil_div(p.frames, kGatedTileM) * p.n_tiles);
+        with_dtype(c->dtype, [&](auto* tag) {
+            using T = std::remove_pointer_t<decltype(tag)>;
+            gated_simt<T, GATED_HEAD><<<grid, kThreads, 0, st>>>(p);
+        });
+        cuda_check(cudaGetLastError(), "mask head kernel");
+    });
+}
+
+} // extern "C"

@@ -1,0 +1,43 @@
+// gated.h -- what the gated projection's entry points (gated.cu) and its kernels share.
+#pragma once
+#include "layers.h"
+
+namespace stg {
+
+constexpr int kGatedTileN = kHeadTileN;   // output columns of a tile: as many gate and up columns side by side
+constexpr int kGatedTileM = 128;
+
+// The four products of the gated projection. Rows of x are m, outputs n, features k.
+enum GatedMode : int {
+    GATED_FWD,    // y = act(x Wg^T + bg) (x Wu^T + bu)
+    GATED_HEAD,   // the same per band, the sigmoid on the second factor, float output
+    GATED_PRE,    // dg = dy u act'(g) and du = dy act(g), and their column sums
+    GATED_DX,     // dx = dg Wg + du Wu
+    GATED_DW,     // dWg = dg^T x, dWu = du^T x
+};
+
+struct GatedParams {
+    int64_t m;
+    int n, k;
+    int act;
+    const void *x, *wg, *wu, *bg, *bu, *dy;
+    int64_t x_row, wg_row, wu_row, y_row, dx_row;
+    void *y, *dx;
+    // backward scratch: dg and du [m][pre_row] in the element type, column sums [tiles][2][n]
+    void *dg, *du;
+    int64_t pre_row;
+    float* col_sums;
+    // dWg and dWu: partial sums over `splits` ranges of rows, [splits][2][n][k] float
+    float* dw_part;
+    int splits;
+    int64_t split_rows;
+    // mask head: tiles over the bands' columns
+    const HeadTile* tiles;
+    int n_tiles;                       // tiles of one stem
+    int64_t frames;                    // rows of a band
+    int bands, stems;
+    int64_t band_cols;                 // sum of din
+    float* masks;
+};
+
+} // namespace stg

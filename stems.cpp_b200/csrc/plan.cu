@@ -313,6 +313,7 @@ void build_roformer(HostPlan& P, const stg_roformer_config& c, int64_t len) {
         }
         foff += sz;
         off += din;
+        P.band_din.push_back(din);
     }
     if (off * T > INT32_MAX) fail(STG_UNSUPPORTED, "roformer: band table too large");
     P.stem_stride = off * T;

@@ -68,6 +68,7 @@ struct HostPlan {
     std::vector<int> ebeg;         // RoFormer CSR over bins
     std::vector<int2> ent;
     std::vector<float> binv;
+    std::vector<int> band_din;     // RoFormer: mask entries of each band per frame
     // the network between the halves: layouts and floats per chunk of its input and output
     int front_layout = FRONT_COMPLEX, back_layout = BACK_COMPLEX;
     int front_bins = 0, back_bins = 0;

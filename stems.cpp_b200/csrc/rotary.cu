@@ -1,0 +1,296 @@
+// rotary.cu -- rotary positions for queries and keys (include/stems_gpu_v1.h: stg_rotary).
+//
+// Pair i of a token at position p turns by a = p f_i: (x0, x1) -> m (x0 cos a - x1 sin a,
+// x1 cos a + x0 sin a). The work is one read and one write of the tensors; what could spoil it
+// is the sines and cosines, which every head of a token shares. A block therefore takes a few
+// tokens with all their heads, of queries and keys together, computes the tokens' table of
+// (cos, sin) once into shared memory and streams the heads past it in 16-byte vectors.
+#include "layers.h"
+
+#include <cmath>
+
+namespace stg {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxHalf = 256;      // rotary_dim at most 512
+constexpr int kTableEntries = 2048;   // (cos, sin) pairs a block keeps: 16 KB
+
+struct RotaryTensor {
+    const void* x;
+    void* y;
+    int64_t xb, xt, xh, yb, yt, yh;
+};
+
+struct RotaryParams {
+    RotaryTensor t[2];
+    int heads0, heads;              // of the first tensor, of both
+    int half, rotary, dim;
+    int64_t tokens, n;              // a batch item's tokens, all tokens
+    int tokens_per_block, heads_per_block;
+    int copy_tail;
+    FastDiv per_head;               // items of a head: rotated ones, then copied ones
+    int rot_items, tail_items;
+    FastDiv heads_div;
+    const int32_t* pos;
+    int64_t pos_batch;
+    int offset;
+    float magnitude;
+    double turns[kMaxHalf];         // f_i / 2 pi, negative for the inverse
+};
+
+// cos and sin of 2 pi t, t in turns. The fraction r in [-1/2, 1/2] is exact in double; it goes to
+// float as a leading part and a rest, and the rest's effect is added to first order, so the
+// result is good to about one unit of the last place at any position.
+__device__ __forceinline__ float2 cos_sin_turns(double t) {
+    const double r = 2.0 * (t - rint(t));   // half turns
+    const float hi = (float)r;
+    const float lo = (float)(r - (double)hi) * 3.14159265358979f;
+    float s, c;
+    sincospif(hi, &s, &c);
+    return make_float2(fmaf(-s, lo, c), fmaf(c, lo, s));
+}
+
+// V elements per access. LAYOUT 0: an item is a run of max(V, 2) neighbouring elements, whole
+// pairs; LAYOUT 1: V elements of the first half and their partners in the second. Tail items
+// are V elements past the rotated part.
+template <class T, int V, int LAYOUT>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+    extern __shared__ float2 table[];
+    const int64_t tok0 = (int64_t)blockIdx.x * p.tokens_per_block;
+    const int n_tok = (int)min((int64_t)p.tokens_per_block, p.n - tok0);
+    const int head0 = blockIdx.y * p.heads_per_block;
+    const int n_heads = min(p.heads_per_block, p.heads - head0);
+
+    for (int e = threadIdx.x; e < n_tok * p.half; e += kThreads) {
+        const int tk = e / p.half, i = e - tk * p.half;
+        const int64_t tok = tok0 + tk, b = tok / p.tokens, t = tok - b * p.tokens;
+        const int32_t pos = p.pos ? p.pos[b * p.pos_batch + t] : p.offset + (int32_t)t;
+        float2 cs = cos_sin_turns((double)pos * p.turns[i]);
+        cs.x *= p.magnitude;
+        cs.y *= p.magnitude;
+        table[e] = cs;
+    }
+    __syncthreads();
+
+    using P = Pack<T, V>;
+    const int per_tok = n_heads * (int)p.per_head.d;
+    const FastDiv& heads_div = p.heads_div;
+    for (int it = threadIdx.x; it < n_tok * per_tok; it += kThreads) {
+        const int hd = (int)p.per_head.div((uint32_t)it);          // token-major (token, head)
+        const int item = it - hd * (int)p.per_head.d;
+        // a block's last head range may be short: its heads count is then not the constant
+        const int tk = n_heads == (int)heads_div.d ? (int)heads_div.div((uint32_t)hd) : hd / n_heads;
+        const int h = head0 + hd - tk * n_heads;
+        const int64_t tok = tok0 + tk;
+        const int64_t b = tok / p.tokens, t = tok - b * p.tokens;
+        const RotaryTensor& R = p.t[h >= p.heads0];
+        const int hh = h >= p.heads0 ? h - p.heads0 : h;
+        const T* x = static_cast<const T*>(R.x) + b * R.xb + t * R.xt + hh * R.xh;
+        T* y = static_cast<T*>(R.y) + b * R.yb + t * R.yt + hh * R.yh;
+        const float2* cs = table + tk * p.half;
+        if (item >= p.rot_items) {
+            const int at = p.rotary + (item - p.rot_items) * V;
+            *reinterpret_cast<P*>(y + at) = *reinterpret_cast<const P*>(x + at);
+        } else if (LAYOUT == 0) {
+            constexpr int E = V < 2 ? 2 : V;   // with one element per access, a pair is two
+            const int at = item * E;
+            T in[E], out[E];
+#pragma unroll
+            for (int k = 0; k < E; k += V) {
+                const P v = *reinterpret_cast<const P*>(x + at + k);
+#pragma unroll
+                for (int j = 0; j < V; j++) in[k + j] = v.v[j];
+            }
+#pragma unroll
+            for (int k = 0; k < E; k += 2) {
+                const float2 w = cs[(at + k) >> 1];
+                const float a = to_float(in[k]), c = to_float(in[k + 1]);
+                out[k] = from_float<T>(fmaf(a, w.x, -c * w.y));
+                out[k + 1] = from_float<T>(fmaf(c, w.x, a * w.y));
+            }
+#pragma unroll
+            for (int k = 0; k < E; k += V) {
+                P v;
+#pragma unroll
+                for (int j = 0; j < V; j++) v.v[j] = out[k + j];
+                *reinterpret_cast<P*>(y + at + k) = v;
+            }
+        } else {
+            const int at = item * V;
+            const P a = *reinterpret_cast<const P*>(x + at), c = *reinterpret_cast<const P*>(x + at + p.half);
+            P u, v;
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const float2 w = cs[at + j];
+                const float fa = to_float(a.v[j]), fc = to_float(c.v[j]);
+                u.v[j] = from_float<T>(fmaf(fa, w.x, -fc * w.y));
+                v.v[j] = from_float<T>(fmaf(fc, w.x, fa * w.y));
+            }
+            *reinterpret_cast<P*>(y + at) = u;
+            *reinterpret_cast<P*>(y + at + p.half) = v;
+        }
+    }
+}
+
+template <class T, int V>
+void launch(RotaryParams& p, int layout, cudaStream_t st) {
+    const int e = layout == 0 && V < 2 ? 2 : V;
+    p.rot_items = (layout == 0 ? p.rotary : p.half) / e;
+    p.tail_items = p.copy_tail ? (p.dim - p.rotary) / V : 0;
+    const int per_head = p.rot_items + p.tail_items;
+    // tokens so that a thread has about four items and the table fits; heads split over blocks
+    // only when so few tokens would leave most of the GPU idle (then each part repeats the table)
+    p.heads_per_block = p.heads;
+    p.tokens_per_block = 1;
+    while (p.tokens_per_block < 64 && (int64_t)p.tokens_per_block * per_head * p.heads < 4 * kThreads &&
+           2 * p.tokens_per_block * p.half <= kTableEntries)
+        p.tokens_per_block *= 2;
+    const int64_t blocks = (p.n + p.tokens_per_block - 1) / p.tokens_per_block;
+    if (blocks < 148) {
+        const int want = (int)std::min<int64_t>((296 + blocks - 1) / blocks, ((int64_t)per_head * p.heads + kThreads - 1) / kThreads);
+        p.heads_per_block = std::max(1, (p.heads + want - 1) / std::max(1, want));
+    }
+    // a block's items stay far below 2^31
+    while ((int64_t)p.tokens_per_block * per_head * p.heads_per_block >= (1 << 30)) p.heads_per_block = (p.heads_per_block + 1) / 2;
+    const int parts = (p.heads + p.heads_per_block - 1) / p.heads_per_block;
+    p.per_head = FastDiv((uint32_t)per_head);
+    p.heads_div = FastDiv((uint32_t)p.heads_per_block);
+    if (blocks > INT32_MAX || parts > 65535) fail(STG_UNSUPPORTED, "rotary: too many tokens or heads");
+    const dim3 grid((unsigned)blocks, (unsigned)parts);
+    const size_t smem = sizeof(float2) * (size_t)p.tokens_per_block * p.half;
+    if (layout == 0) rotary_kernel<T, V, 0><<<grid, kThreads, smem, st>>>(p);
+    else rotary_kernel<T, V, 1><<<grid, kThreads, smem, st>>>(p);
+    cuda_check(cudaGetLastError(), "rotary kernel");
+}
+
+template <class T, int V>
+void launch_widest(RotaryParams& p, int layout, int width, cudaStream_t st) {
+    if constexpr (V > 1) {
+        if (width < V) return launch_widest<T, V / 2>(p, layout, width, st);
+    }
+    launch<T, V>(p, layout, st);
+}
+
+void check_config(const stg_rotary_config* c) {
+    check_sized(c, "rotary");
+    check(valid_dtype(c->dtype), "rotary: unknown dtype");
+    check(c->layout == 0 || c->layout == 1, "rotary: layout must be 0 or 1");
+    check(c->inverse == 0 || c->inverse == 1, "rotary: inverse must be 0 or 1");
+    check(c->batch >= 0 && c->tokens >= 0, "rotary: negative size");
+    check(c->head_dim >= 1 && c->head_dim <= 65536, "rotary: head_dim must be 1..65536");
+    const int r = c->rotary_dim ? c->rotary_dim : c->head_dim;
+    check(r >= 2 && r % 2 == 0 && r <= c->head_dim, "rotary: rotary_dim must be even and at most head_dim");
+    if (r > 2 * kMaxHalf) fail(STG_UNSUPPORTED, "rotary: rotary_dim above 512");
+    check(c->scaling >= 0 && c->scaling <= 3, "rotary: unknown scaling");
+    check(c->base == 0.0 || (c->base > 0.0 && c->base != 1.0 && std::isfinite(c->base)), "rotary: base must be positive and not 1");
+    check(std::isfinite(c->magnitude), "rotary: magnitude must be finite");
+    if (c->scaling != 0) check(c->factor >= 1.0 && std::isfinite(c->factor), "rotary: factor must be at least 1");
+    if (c->scaling == 2) check(r > 2, "rotary: NTK scaling needs rotary_dim above 2");
+    if (c->scaling == 3) {
+        check(c->original_length > 0.0 && std::isfinite(c->original_length), "rotary: original_length must be positive");
+        const bool none = c->beta_fast == 0.0 && c->beta_slow == 0.0;
+        check(none || (c->beta_slow > 0.0 && c->beta_fast > c->beta_slow && std::isfinite(c->beta_fast)),
+              "rotary: beta_fast must be above beta_slow, both positive");
+    }
+    if (c->batch > 0 && c->tokens > INT64_MAX / 2 / c->batch) fail(STG_UNSUPPORTED, "rotary: too many tokens");
+}
+
+// f_i and m of a checked configuration.
+double frequencies(const stg_rotary_config& c, double* f) {
+    const int r = c.rotary_dim ? c.rotary_dim : c.head_dim, half = r / 2;
+    double base = c.base == 0.0 ? 10000.0 : c.base, m = 1.0;
+    const double s = c.factor;
+    if (c.scaling == 2) base *= std::pow(s, (double)r / (r - 2));
+    for (int i = 0; i < half; i++) f[i] = std::pow(base, -2.0 * i / r);
+    if (c.scaling == 1)
+        for (int i = 0; i < half; i++) f[i] /= s;
+    if (c.scaling == 3) {
+        const bool none = c.beta_fast == 0.0 && c.beta_slow == 0.0;
+        const double fast = none ? 32.0 : c.beta_fast, slow = none ? 1.0 : c.beta_slow;
+        auto dim_of = [&](double turns) { return r * std::log(c.original_length / (turns * 2.0 * M_PI)) / (2.0 * std::log(base)); };
+        const double lo = std::max(std::floor(dim_of(fast)), 0.0);
+        const double hi = std::min(std::ceil(dim_of(slow)), (double)(half - 1));
+        for (int i = 0; i < half; i++) {
+            const double g = std::min(std::max((i - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
+            f[i] = (1.0 - g) * f[i] + g * f[i] / s;
+        }
+        m = 0.1 * std::log(s) + 1.0;
+    }
+    return c.magnitude != 0.0 ? c.magnitude : m;
+}
+
+} // namespace
+
+} // namespace stg
+
+extern "C" {
+
+STG_API stg_status stg_rotary_frequencies(const stg_rotary_config* c, double* f, double* magnitude) {
+    return guard(nullptr, [&] {
+        check_config(c);
+        check(f && magnitude, "rotary: null buffer");
+        *magnitude = frequencies(*c, f);
+    });
+}
+
+STG_API stg_status stg_rotary(stg_engine* e, const stg_rotary_config* c, const stg_rotary_tensor* tensors,
+                              int32_t n_tensors, const int32_t* d_positions, int64_t position_batch_stride, void* stream) {
+    if (!e) return STG_INVALID_ARGUMENT;
+    return guard(e, [&] {
+        check_config(c);
+        check(tensors && (n_tensors == 1 || n_tensors == 2), "rotary: one or two tensors");
+        check(position_batch_stride >= 0, "rotary: negative stride");
+        check(aligned(d_positions, 4), "rotary: positions are not aligned");
+        if (!d_positions && c->tokens > 0)
+            check(c->offset + (c->tokens - 1) <= INT32_MAX, "rotary: a position does not fit 32 bits");
+        RotaryParams p{};
+        const size_t es = elem_size(c->dtype);
+        p.dim = c->head_dim;
+        p.rotary = c->rotary_dim ? c->rotary_dim : c->head_dim;
+        p.half = p.rotary / 2;
+        p.tokens = c->tokens;
+        p.n = c->batch * c->tokens;
+        int64_t heads = 0;
+        // the widest vector that the sizes, strides and addresses allow
+        int width = (int)(16 / es);
+        auto fit = [&](int64_t n) { while (n % width) width /= 2; };
+        fit(c->layout == 0 ? p.rotary : p.half);
+        bool in_place = true;
+        for (int k = 0; k < n_tensors; k++) {
+            const stg_rotary_tensor& t = tensors[k];
+            check(t.heads >= 0 && t.heads <= (1 << 20), "rotary: heads must be 0..2^20");
+            check(t.x_batch >= 0 && t.x_token >= 0 && t.x_head >= 0 && t.y_batch >= 0 && t.y_token >= 0 && t.y_head >= 0,
+                  "rotary: negative stride");
+            p.t[k] = RotaryTensor{t.d_x, t.d_y, t.x_batch, t.x_token, t.x_head, t.y_batch, t.y_token, t.y_head};
+            if (k == 0) p.heads0 = (int)t.heads;
+            heads += t.heads;
+            if (!t.heads || !p.n) continue;
+            check(t.d_x && t.d_y, "rotary: null buffer");
+            check(aligned(t.d_x, es) && aligned(t.d_y, es), "rotary: a buffer is not aligned to its elements");
+            check((t.y_batch || c->batch == 1) && (t.y_token || c->tokens == 1) && (t.y_head || t.heads == 1),
+                  "rotary: an output stride of 0");
+            if (t.d_x != t.d_y || t.x_batch != t.y_batch || t.x_token != t.y_token || t.x_head != t.y_head) in_place = false;
+            for (int64_t s : {t.x_batch, t.x_token, t.x_head, t.y_batch, t.y_token, t.y_head}) fit(s);
+            while (!aligned(t.d_x, width * es) || !aligned(t.d_y, width * es)) width /= 2;
+        }
+        p.heads = (int)heads;
+        if (!p.n || !heads) return;
+        p.copy_tail = p.rotary < p.dim && !in_place;
+        if (p.copy_tail) { fit(p.dim - p.rotary); fit(p.rotary); }
+        p.pos = d_positions;
+        p.pos_batch = position_batch_stride;
+        p.offset = c->offset;
+        p.magnitude = (float)frequencies(*c, p.turns);
+        for (int i = 0; i < p.half; i++) p.turns[i] *= (c->inverse ? -1.0 : 1.0) / (2.0 * M_PI);
+        DeviceScope scope(e);
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        with_dtype(c->dtype, [&](auto* tag) {
+            using T = std::remove_pointer_t<decltype(tag)>;
+            launch_widest<T, (int)(16 / sizeof(T))>(p, c->layout, width, st);
+        });
+    });
+}
+
+} // extern "C"
