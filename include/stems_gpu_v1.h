@@ -586,6 +586,11 @@ STG_API stg_status stg_gated_backward(stg_engine* engine, const stg_gated_config
                                       const void* d_bu, void* d_dx, void* d_dwg, void* d_dwu, void* d_dbg,
                                       void* d_dbu, void* d_workspace, size_t workspace_bytes, void* stream);
 
+/* Waits for the engine's device; STG_INTERNAL_ERROR when a kernel of the gated projection or the
+ * mask head gave up waiting for its own copies or products since the library was loaded (after
+ * ten seconds, where it would otherwise hang: a failure of the device, not of a call). */
+STG_API stg_status stg_engine_status(stg_engine* engine);
+
 /* The last layer of RoFormer's mask estimators (src/roformer.cpp:190-214) over a batch of
  * chunks, every stem and band in one launch: per chunk, stem s and band b of the plan,
  * v = h Wv^T + bv and g = h Wg^T + bg, mask = v sigmoid(g) (torch's GLU), written as float in the

@@ -203,6 +203,7 @@ _SIGNATURES = {
     "stg_gated": (C.c_int32, [C.c_void_p, C.POINTER(GatedConfig)] + [C.c_void_p] * 7 + [C.c_size_t, C.c_void_p]),
     "stg_gated_backward": (C.c_int32, [C.c_void_p, C.POINTER(GatedConfig)] + [C.c_void_p] * 12 +
                            [C.c_size_t, C.c_void_p]),
+    "stg_engine_status": (C.c_int32, [C.c_void_p]),
     "stg_mask_head_sizes": (C.c_int32, [C.c_void_p, _I32P, _I32P, _I32P, C.POINTER(C.c_int64)]),
     "stg_mask_head_workspace": (C.c_int32, [C.c_void_p, C.POINTER(MaskHeadConfig), C.POINTER(C.c_size_t)]),
     "stg_mask_head": (C.c_int32, [C.c_void_p, C.POINTER(MaskHeadConfig)] + [C.c_void_p] * 5 + [C.c_size_t, C.c_void_p]),
@@ -391,6 +392,10 @@ class Engine:
     def set_profiling(self, enabled: bool = True):
         """Record CUDA events around every run's kernels (see Plan.last_timing)."""
         self._check(lib().stg_engine_set_profiling(self._h, int(enabled)), "set_profiling")
+
+    def status(self):
+        """Waits for the device and raises if a kernel of gated or mask_head gave up a wait."""
+        self._check(lib().stg_engine_status(self._h), "status")
 
     def _check(self, rc, what):
         if rc != 0:

@@ -8,7 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libstems_gpu.so")
 SOURCES = ["kernels.cu", "pair.cu", "split.cu", "plan.cu", "engine.cu", "noalloc.cu", "norm.cu", "convert.cu", "vr.cu", "gguf.cu",
-           "rotary.cu", "groupnorm.cu", "gated.cu"]
+           "rotary.cu", "groupnorm.cu", "gated.cu", "gated_mma.cu"]
 HEADERS = ["fft.cuh", "frame.cuh", "kernels.h", "plan.h", "engine.h", "layers.h", "gated.h"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-shared", "--threads=0"]

@@ -26,13 +26,18 @@ STG_API stg_status stg_engine_create(int device, stg_engine** out) {
     int n = 0;
     if (cudaGetDeviceCount(&n) != cudaSuccess) { cudaGetLastError(); return STG_INTERNAL_ERROR; }
     if (device < 0 || device >= n) return STG_INVALID_ARGUMENT;
-    cudaDeviceProp prop{};
-    if (cudaGetDeviceProperties(&prop, device) != cudaSuccess) { cudaGetLastError(); return STG_INTERNAL_ERROR; }
-    if (prop.major < 10) return STG_UNSUPPORTED;   // built for sm_100a only
+    int major = 0, sms = 0;   // two attributes: the whole property table takes milliseconds
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+        cudaGetLastError();
+        return STG_INTERNAL_ERROR;
+    }
+    if (major < 10) return STG_UNSUPPORTED;   // built for sm_100a only
     if (cudaSetDevice(device) != cudaSuccess) { cudaGetLastError(); return STG_INTERNAL_ERROR; }
     stg_engine* e = new (std::nothrow) stg_engine;
     if (!e) return STG_OUT_OF_MEMORY;
     e->device = device;
+    e->sms = sms;
     *out = e;
     return STG_OK;
 }

@@ -59,6 +59,7 @@ using namespace stg;
 // ---- engine -------------------------------------------------------------------------------
 struct stg_engine {
     int device = 0;
+    int sms = 0;                   // multiprocessors
     bool profiling = false;
     std::string last_error;
     std::map<int, std::unique_ptr<FftTables>> tables;

@@ -312,6 +312,16 @@ __global__ void __launch_bounds__(128) db_join(const float* sums, int64_t tiles,
     }
 }
 
+// A matrix with its rows `pitch` elements apart, for operands whose rows are no whole 16 bytes.
+template <class T>
+__global__ void __launch_bounds__(kThreads) repack(const T* src, int64_t src_row, T* dst, int64_t pitch, int64_t rows, int cols) {
+    const int64_t total = rows * cols;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t r = i / cols, c = i - r * cols;
+        dst[r * pitch + c] = src[r * src_row + c];
+    }
+}
+
 // ---- host -------------------------------------------------------------------------------------
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -327,7 +337,31 @@ void check_config(const stg_gated_config* c, bool backward) {
     check((c->y_row >= c->width || c->rows <= 1) || backward, "gated: the output's rows overlap");
 }
 
-struct GatedLayout { size_t dg = 0, du = 0, sums = 0, dw = 0, bytes = 0; int64_t pre_row = 0; int splits = 1; int64_t split_rows = 0; };
+// Which operands the tensor-core path needs a repacked copy of (bytes, 0: none): it reads by
+// TMA, whose rows are a multiple of 16 bytes apart.
+struct Copies { size_t x = 0, wg = 0, wu = 0; size_t bytes() const { return x + wg + wu; } };
+size_t copy_bytes(int64_t rows, int64_t row, int cols) {
+    return rows <= 1 || row % 8 == 0 ? 0 : up256((size_t)rows * (size_t)(ceil_div(cols, 8) * 8) * 2);
+}
+Copies copies_of(const stg_gated_config& c) {
+    Copies r;
+    if (c.dtype == STG_F32 || !c.rows) return r;
+    r.x = copy_bytes(c.rows, c.x_row, c.features);
+    r.wg = copy_bytes(c.width, c.wg_row, c.features);
+    r.wu = copy_bytes(c.width, c.wu_row, c.features);
+    return r;
+}
+template <class T> void copy_operand(const void*& p, int64_t& row, size_t bytes, int64_t rows, int cols, char*& ws, cudaStream_t st) {
+    if (!bytes) return;
+    const int64_t pitch = ceil_div(cols, 8) * 8;
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(rows * cols, kThreads), 148 * 8);
+    repack<T><<<blocks, kThreads, 0, st>>>(static_cast<const T*>(p), row, reinterpret_cast<T*>(ws), pitch, rows, cols);
+    p = ws;
+    row = pitch;
+    ws += bytes;
+}
+
+struct GatedLayout { size_t dg = 0, du = 0, sums = 0, dw = 0, copies = 0, bytes = 0; int64_t pre_row = 0; int splits = 1; int64_t split_rows = 0; };
 
 GatedLayout backward_layout(const stg_gated_config& c) {
     GatedLayout l;
@@ -335,14 +369,16 @@ GatedLayout backward_layout(const stg_gated_config& c) {
     l.pre_row = ceil_div(c.width, 8) * 8;
     l.du = up256((size_t)c.rows * l.pre_row * es);
     l.sums = l.du + up256((size_t)c.rows * l.pre_row * es);
-    l.dw = l.sums + up256(sizeof(float) * (size_t)ceil_div(c.rows, kGatedTileM) * 2 * c.width);
+    l.dw = l.sums + up256(sizeof(float) * (size_t)ceil_div(c.rows, kGatedTileM) * 4 * 2 * c.width);
     // dW has 2 width x features outputs and a sum over all rows: rows are split until the tiles
-    // fill the GPU twice, while a part keeps at least 256 rows
-    const int64_t tiles = 2 * ceil_div(c.width, 128) * ceil_div(c.features, 128);
-    l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(2 * 148, tiles), c.rows / 256, 64}));
-    l.split_rows = std::max<int64_t>(16, ceil_div(ceil_div(c.rows, l.splits), 16) * 16);
+    // fill the GPU, while a part keeps at least 256 rows
+    const int64_t tiles = 2 * ceil_div(c.width, 128) * ceil_div(c.features, c.dtype == STG_F32 ? 128 : 256);
+    const int64_t want = c.dtype == STG_F32 ? ceil_div(2 * 148, tiles) : std::max<int64_t>(1, 148 / tiles);
+    l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, c.rows / 256, 64}));
+    l.split_rows = std::max<int64_t>(64, ceil_div(ceil_div(c.rows, l.splits), 64) * 64);
     l.splits = (int)std::max<int64_t>(1, ceil_div(c.rows, l.split_rows));
-    l.bytes = l.dw + up256(sizeof(float) * (size_t)l.splits * 2 * c.width * c.features);
+    l.copies = l.dw + up256(sizeof(float) * (size_t)l.splits * 2 * c.width * c.features);
+    l.bytes = l.copies + copies_of(c).bytes();
     return l;
 }
 
@@ -352,6 +388,11 @@ GatedParams params_of(const stg_gated_config& c) {
     p.act = c.activation;
     p.x_row = c.x_row; p.wg_row = c.wg_row; p.wu_row = c.wu_row; p.y_row = c.y_row; p.dx_row = c.dx_row;
     return p;
+}
+
+// f16 and bf16 go to the tensor cores where the operands that are not copied start on 16 bytes.
+bool on_tensor_cores(const stg_gated_config& c, const Copies& copies, const GatedParams& p) {
+    return c.dtype != STG_F32 && (copies.x || aligned(p.x, 16)) && (copies.wg || aligned(p.wg, 16)) && (copies.wu || aligned(p.wu, 16));
 }
 
 dim3 tile_grid(int64_t tiles, int64_t y = 1) {
@@ -369,7 +410,7 @@ STG_API stg_status stg_gated_workspace(const stg_gated_config* c, int32_t backwa
     return guard(nullptr, [&] {
         check_config(c, backward != 0);
         check(bytes && (backward == 0 || backward == 1), "gated: null buffer");
-        *bytes = backward && c->rows ? backward_layout(*c).bytes : 0;
+        *bytes = !c->rows ? 0 : backward ? backward_layout(*c).bytes : copies_of(*c).bytes();
     });
 }
 
@@ -386,10 +427,18 @@ STG_API stg_status stg_gated(stg_engine* e, const stg_gated_config* c, const voi
         p.x = d_x; p.wg = d_wg; p.wu = d_wu; p.bg = d_bg; p.bu = d_bu; p.y = d_y;
         DeviceScope scope(e);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
-        const dim3 grid = tile_grid(ceil_div(p.m, kGatedTileM) * ceil_div(p.n, kGatedTileN));
+        const Copies copies = copies_of(*c);
+        check(!copies.bytes() || (d_ws && aligned(d_ws, 256) && ws_bytes >= copies.bytes()), "gated: workspace is missing, unaligned or too small");
         with_dtype(c->dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
-            gated_simt<T, GATED_FWD><<<grid, kThreads, 0, st>>>(p);
+            if (on_tensor_cores(*c, copies, p)) {
+                char* ws = static_cast<char*>(d_ws);
+                copy_operand<T>(p.x, p.x_row, copies.x, p.m, p.k, ws, st);
+                copy_operand<T>(p.wg, p.wg_row, copies.wg, p.n, p.k, ws, st);
+                copy_operand<T>(p.wu, p.wu_row, copies.wu, p.n, p.k, ws, st);
+                return launch_gated_mma(GATED_FWD, c->dtype == STG_BF16, p, 0, e->sms, st);
+            }
+            gated_simt<T, GATED_FWD><<<tile_grid(ceil_div(p.m, kGatedTileM) * ceil_div(p.n, kGatedTileN)), kThreads, 0, st>>>(p);
         });
         cuda_check(cudaGetLastError(), "gated kernel");
     });
@@ -434,20 +483,49 @@ STG_API stg_status stg_gated_backward(stg_engine* e, const stg_gated_config* c, 
         p.splits = lay.splits;
         p.split_rows = lay.split_rows;
         const int64_t mt = ceil_div(p.m, kGatedTileM);
+        auto join_dw = [&](auto* tag) {
+            using T = std::remove_pointer_t<decltype(tag)>;
+            const int64_t blocks = std::min<int64_t>(ceil_div(2 * (int64_t)p.n * p.k, kThreads), 148 * 8);
+            dw_join<T><<<(unsigned)blocks, kThreads, 0, st>>>(p.dw_part, p.splits, p.n, p.k, static_cast<T*>(d_dwg), c->dwg_row,
+                                                              static_cast<T*>(d_dwu), c->dwu_row);
+        };
         with_dtype(c->dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
+            const Copies copies = copies_of(*c);
+            if (on_tensor_cores(*c, copies, p)) {
+                char* cw = ws + lay.copies;
+                copy_operand<T>(p.x, p.x_row, copies.x, p.m, p.k, cw, st);
+                copy_operand<T>(p.wg, p.wg_row, copies.wg, p.n, p.k, cw, st);
+                copy_operand<T>(p.wu, p.wu_row, copies.wu, p.n, p.k, cw, st);
+                auto product = [&](GatedMode mode) { launch_gated_mma(mode, c->dtype == STG_BF16, p, 0, e->sms, st); };
+                product(GATED_PRE);
+                if (p.col_sums)
+                    db_join<T><<<(unsigned)ceil_div(2 * (int64_t)p.n, 4), 128, 0, st>>>(p.col_sums, 4 * mt, p.n, static_cast<T*>(d_dbg), static_cast<T*>(d_dbu));
+                if (d_dx) product(GATED_DX);
+                if (d_dwg || d_dwu) {
+                    product(GATED_DW);
+                    join_dw((T*)nullptr);
+                }
+                return;
+            }
             gated_simt<T, GATED_PRE><<<tile_grid(mt * ceil_div(p.n, kGatedTileN)), kThreads, 0, st>>>(p);
             if (p.col_sums)
                 db_join<T><<<(unsigned)ceil_div(2 * (int64_t)p.n, 4), 128, 0, st>>>(p.col_sums, mt, p.n, static_cast<T*>(d_dbg), static_cast<T*>(d_dbu));
             if (d_dx) gated_simt<T, GATED_DX><<<tile_grid(mt * ceil_div(p.k, 128)), kThreads, 0, st>>>(p);
             if (d_dwg || d_dwu) {
                 gated_simt<T, GATED_DW><<<tile_grid(ceil_div(p.n, 128) * ceil_div(p.k, 128), 2 * p.splits), kThreads, 0, st>>>(p);
-                const int64_t blocks = std::min<int64_t>(ceil_div(2 * (int64_t)p.n * p.k, kThreads), 148 * 8);
-                dw_join<T><<<(unsigned)blocks, kThreads, 0, st>>>(p.dw_part, p.splits, p.n, p.k, static_cast<T*>(d_dwg), c->dwg_row,
-                                                                  static_cast<T*>(d_dwu), c->dwu_row);
+                join_dw((T*)nullptr);
             }
         });
         cuda_check(cudaGetLastError(), "gated kernel");
+    });
+}
+
+STG_API stg_status stg_engine_status(stg_engine* e) {
+    if (!e) return STG_INVALID_ARGUMENT;
+    return guard(e, [&] {
+        DeviceScope scope(e);
+        if (gated_gave_up()) fail(STG_INTERNAL_ERROR, "a kernel of the gated projection gave up a wait: its result is incomplete");
     });
 }
 
@@ -456,6 +534,17 @@ static void check_head(const stg_plan* p, const stg_mask_head_config* c) {
     check(p->H.arch == ARCH_ROFORMER && !p->H.band_din.empty(), "mask head: not a RoFormer plan");
     check(valid_dtype(c->dtype), "mask head: unknown dtype");
     check(c->hidden >= 1 && c->n_chunks >= 0, "mask head: hidden must be at least 1, n_chunks at least 0");
+}
+
+static int64_t head_rows(const stg_plan* p, const stg_mask_head_config* c) {
+    return (int64_t)c->n_chunks * p->H.S * (int64_t)p->H.band_din.size() * p->H.g.T;
+}
+static Copies head_copies(const stg_plan* p, const stg_mask_head_config* c) {
+    Copies r;
+    if (c->dtype == STG_F32 || !c->n_chunks) return r;
+    r.x = copy_bytes(head_rows(p, c), c->hidden, c->hidden);
+    r.wg = copy_bytes(p->H.S * 2 * (p->H.stem_stride / p->H.g.T), c->hidden, c->hidden);
+    return r;
 }
 
 STG_API stg_status stg_mask_head_sizes(const stg_plan* p, int32_t* stems, int32_t* bands, int32_t* frames, int64_t* columns) {
@@ -475,7 +564,7 @@ STG_API stg_status stg_mask_head_workspace(const stg_plan* p, const stg_mask_hea
     return guard(p->engine, [&] {
         check_head(p, c);
         check(bytes, "mask head: null buffer");
-        *bytes = 0;
+        *bytes = head_copies(p, c).bytes();
     });
 }
 
@@ -501,8 +590,18 @@ STG_API stg_status stg_mask_head(stg_plan* plan, const stg_mask_head_config* c, 
         DeviceScope scope(plan->engine);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
         const dim3 grid = tile_grid((int64_t)c->n_chunks * p.stems * ceil_div(p.frames, kGatedTileM) * p.n_tiles);
+        const Copies copies = head_copies(plan, c);
+        check(!copies.bytes() || (d_ws && aligned(d_ws, 256) && ws_bytes >= copies.bytes()), "mask head: workspace is missing, unaligned or too small");
+        const int64_t rows = head_rows(plan, c);
         with_dtype(c->dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
+            if (c->dtype != STG_F32 && rows <= INT32_MAX && (copies.x || aligned(d_hidden, 16)) && (copies.wg || aligned(d_weight, 16))) {
+                char* ws = static_cast<char*>(d_ws);
+                p.x_row = p.wg_row = p.k;
+                copy_operand<T>(p.x, p.x_row, copies.x, rows, p.k, ws, st);
+                copy_operand<T>(p.wg, p.wg_row, copies.wg, p.stems * 2 * p.band_cols, p.k, ws, st);
+                return launch_gated_mma(GATED_HEAD, c->dtype == STG_BF16, p, rows, plan->engine->sms, st);
+            }
             gated_simt<T, GATED_HEAD><<<grid, kThreads, 0, st>>>(p);
         });
         cuda_check(cudaGetLastError(), "mask head kernel");

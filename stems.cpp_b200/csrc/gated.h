@@ -40,4 +40,12 @@ struct GatedParams {
     float* masks;
 };
 
+// One of the products on the tensor cores (gated_mma.cu), f16 or bf16. Matrices of g that are
+// read or written by TMA (x, Wg, Wu, dg, du) start on 16 bytes with rows a multiple of 16 bytes apart.
+// head_rows: rows of x in the mask head, below 2^31.
+void launch_gated_mma(GatedMode mode, bool bf16, const GatedParams& g, int64_t head_rows, int sms, cudaStream_t st);
+// Whether a kernel of launch_gated_mma gave up a wait since the library was loaded (it then
+// returned with its result incomplete). Waits for the device.
+int gated_gave_up();
+
 } // namespace stg

@@ -488,3 +488,7 @@ def test_layers_in_graphs_and_on_streams(pkg, engine, name):
     for out in both:
         assert all(torch.equal(a, b) for a, b in zip(out, want))
     assert all(torch.equal(a, b) for a, b in zip(inputs, before))
+
+
+def test_no_kernel_gave_up(engine):
+    engine.status()

@@ -69,6 +69,7 @@ def test_null_engines_and_plans_are_rejected(pkg):
     assert L.stg_mask_head(None, C.byref(head), *[None] * 5, 0, None) == 1
     assert L.stg_mask_head_workspace(None, C.byref(head), C.byref(n)) == 1
     assert L.stg_mask_head_sizes(None, None, None, None, None) == 1
+    assert L.stg_engine_status(None) == 1
 
 
 @pytest.mark.parametrize("bad, code", [
