@@ -48,7 +48,7 @@ struct FftTables {
 
 // One tile of the mask head's output columns (gated.cu): its band, first column, the band's
 // first entry and its width.
-constexpr int kHeadTileN = 64;
+constexpr int kHeadTileN = 64, kHeadWideN = 128;   // on the CUDA cores, on the tensor cores
 struct HeadTile { int band, n0, off, din; };
 
 } // namespace stg
@@ -112,7 +112,7 @@ struct stg_plan {
     DevBuf d_mask_t;                                  // t-major masks (HTDemucs, TFC-TDF)
     DevBuf d_zspec;                                   // HTDemucs spectra
     DevBuf d_head;                                    // RoFormer: the mask head's column tiles (HeadTile)
-    int head_tiles = 0;
+    int head_tiles = 0, head_wide = 0;                // kHeadTileN-wide ones, then kHeadWideN-wide ones
     const float* mono_src = nullptr;                  // the track d_mixn was normalised from
     DevBuf s_mix, s_mask, s_out;   // device staging for stg_separate_host
     // stg_separate_host: a copy stream that brings the masks in batch by batch, and the events
@@ -154,11 +154,19 @@ struct stg_plan {
         upload(d_ent, H.ent, "band table");
         upload(d_binv, H.binv, "band table");
         if (!H.band_din.empty()) {
-            std::vector<HeadTile> tiles;
+            std::vector<HeadTile> tiles, wide;
             int off = 0;
-            for (int b = 0; b < (int)H.band_din.size(); off += H.band_din[b++])
+            for (int b = 0; b < (int)H.band_din.size(); off += H.band_din[b++]) {
                 for (int n0 = 0; n0 < H.band_din[b]; n0 += kHeadTileN) tiles.push_back(HeadTile{b, n0, off, H.band_din[b]});
+                for (int n0 = 0; n0 < H.band_din[b]; n0 += kHeadWideN) wide.push_back(HeadTile{b, n0, off, H.band_din[b]});
+            }
+            // the widest first: the last ones to start are then the short ones
+            std::stable_sort(wide.begin(), wide.end(), [](const HeadTile& x, const HeadTile& y) {
+                return std::min(kHeadWideN, x.din - x.n0) > std::min(kHeadWideN, y.din - y.n0);
+            });
             head_tiles = (int)tiles.size();
+            head_wide = (int)wide.size();
+            tiles.insert(tiles.end(), wide.begin(), wide.end());
             upload(d_head, tiles, "mask head tiles");
         }
         if (!H.bag.empty()) {

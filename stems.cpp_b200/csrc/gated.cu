@@ -369,14 +369,16 @@ GatedLayout backward_layout(const stg_gated_config& c) {
     l.pre_row = ceil_div(c.width, 8) * 8;
     l.du = up256((size_t)c.rows * l.pre_row * es);
     l.sums = l.du + up256((size_t)c.rows * l.pre_row * es);
-    l.dw = l.sums + up256(sizeof(float) * (size_t)ceil_div(c.rows, kGatedTileM) * 4 * 2 * c.width);
     // dW has 2 width x features outputs and a sum over all rows: rows are split until the tiles
     // fill the GPU, while a part keeps at least 256 rows
-    const int64_t tiles = 2 * ceil_div(c.width, 128) * ceil_div(c.features, c.dtype == STG_F32 ? 128 : 256);
-    const int64_t want = c.dtype == STG_F32 ? ceil_div(2 * 148, tiles) : std::max<int64_t>(1, 148 / tiles);
+    // (f32: 128 x 128 tiles, two blocks per SM; else pairs of SMs and their 256 x 224 tiles)
+    const bool f32 = c.dtype == STG_F32;
+    const int64_t tiles = 2 * ceil_div(c.width, f32 ? 128 : 256) * ceil_div(c.features, f32 ? 128 : 224);
+    const int64_t want = f32 ? ceil_div(2 * 148, tiles) : std::max<int64_t>(1, 74 / tiles);
     l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, c.rows / 256, 64}));
     l.split_rows = std::max<int64_t>(64, ceil_div(ceil_div(c.rows, l.splits), 64) * 64);
     l.splits = (int)std::max<int64_t>(1, ceil_div(c.rows, l.split_rows));
+    l.dw = l.sums + up256(sizeof(float) * (size_t)std::max<int64_t>(ceil_div(c.rows, kGatedTileM), l.splits * ceil_div(c.features, 64)) * 2 * c.width);
     l.copies = l.dw + up256(sizeof(float) * (size_t)l.splits * 2 * c.width * c.features);
     l.bytes = l.copies + copies_of(c).bytes();
     return l;
@@ -499,12 +501,12 @@ STG_API stg_status stg_gated_backward(stg_engine* e, const stg_gated_config* c, 
                 copy_operand<T>(p.wu, p.wu_row, copies.wu, p.n, p.k, cw, st);
                 auto product = [&](GatedMode mode) { launch_gated_mma(mode, c->dtype == STG_BF16, p, 0, e->sms, st); };
                 product(GATED_PRE);
-                if (p.col_sums)
-                    db_join<T><<<(unsigned)ceil_div(2 * (int64_t)p.n, 4), 128, 0, st>>>(p.col_sums, 4 * mt, p.n, static_cast<T*>(d_dbg), static_cast<T*>(d_dbu));
                 if (d_dx) product(GATED_DX);
-                if (d_dwg || d_dwu) {
+                if (d_dwg || d_dwu || p.col_sums) {
                     product(GATED_DW);
-                    join_dw((T*)nullptr);
+                    if (p.col_sums)
+                        db_join<T><<<(unsigned)ceil_div(2 * (int64_t)p.n, 4), 128, 0, st>>>(p.col_sums, gated_col_sums(p, e->sms), p.n, static_cast<T*>(d_dbg), static_cast<T*>(d_dbu));
+                    if (d_dwg || d_dwu) join_dw((T*)nullptr);
                 }
                 return;
             }
@@ -600,6 +602,8 @@ STG_API stg_status stg_mask_head(stg_plan* plan, const stg_mask_head_config* c, 
                 p.x_row = p.wg_row = p.k;
                 copy_operand<T>(p.x, p.x_row, copies.x, rows, p.k, ws, st);
                 copy_operand<T>(p.wg, p.wg_row, copies.wg, p.stems * 2 * p.band_cols, p.k, ws, st);
+                p.tiles += plan->head_tiles;
+                p.n_tiles = plan->head_wide;
                 return launch_gated_mma(GATED_HEAD, c->dtype == STG_BF16, p, rows, plan->engine->sms, st);
             }
             gated_simt<T, GATED_HEAD><<<grid, kThreads, 0, st>>>(p);

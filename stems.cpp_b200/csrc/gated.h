@@ -23,7 +23,7 @@ struct GatedParams {
     const void *x, *wg, *wu, *bg, *bu, *dy;
     int64_t x_row, wg_row, wu_row, y_row, dx_row;
     void *y, *dx;
-    // backward scratch: dg and du [m][pre_row] in the element type, column sums [tiles][2][n]
+    // backward scratch: dg and du [m][pre_row] in the element type, column sums [128-row tiles, or gated_col_sums][2][n]
     void *dg, *du;
     int64_t pre_row;
     float* col_sums;
@@ -44,6 +44,8 @@ struct GatedParams {
 // read or written by TMA (x, Wg, Wu, dg, du) start on 16 bytes with rows a multiple of 16 bytes apart.
 // head_rows: rows of x in the mask head, below 2^31.
 void launch_gated_mma(GatedMode mode, bool bf16, const GatedParams& g, int64_t head_rows, int sms, cudaStream_t st);
+// How many partial column sums GATED_DW leaves: one per split and column tile, at most splits * ceil(k / 64).
+int64_t gated_col_sums(const GatedParams& g, int sms);
 // Whether a kernel of launch_gated_mma gave up a wait since the library was loaded (it then
 // returned with its result incomplete). Waits for the device.
 int gated_gave_up();

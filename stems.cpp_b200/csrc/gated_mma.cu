@@ -1,14 +1,16 @@
 // gated_mma.cu -- the gated projection's products on the tensor cores, f16 and bf16
 // (gated.h: GatedMode; the mathematics is in gated.cu).
 //
-// One persistent block per SM walks 128-row output tiles. A producer thread brings 64-deep
-// slices of the operands into a ring of shared-memory stages by TMA (128-byte swizzle); one
-// thread issues tcgen05.mma with float accumulators in TMEM; eight warps read finished
-// accumulators back, apply the epilogue and store. Two accumulator sets let the epilogue of a
-// tile run under the products of the next. In the forward modes a stage holds Wg's and Wu's
-// rows of the same output columns one behind the other, so one instruction computes both
-// projections and a thread of the epilogue finds g and u of an output in its own TMEM lane: the
-// projections never leave the SM.
+// Two neighbouring SMs work as a pair (a cluster of two blocks, tcgen05 cta_group::2) and walk
+// 256-row output tiles: each block holds its own 128 rows of A and half the columns of B, so
+// a slice of the contraction costs an SM 32 KB of loads for the work of a 128 x 256 tile where a
+// block alone would load 48 KB (alone, the products waited for the loads and reached half the
+// tensor cores' rate). A producer thread brings 64-deep slices into a ring of shared-memory
+// stages by TMA (128-byte swizzle); one thread of the pair issues the products, float
+// accumulators in TMEM; sixteen warps per block read finished accumulators back, apply the
+// epilogue and store. In the forward modes one block of the pair loads Wg's rows and the other
+// Wu's rows of the same outputs, so one instruction computes both projections and an epilogue
+// thread finds g and u of an output in its own TMEM lane: the projections never leave the SM.
 //
 // Where an operand's contraction is not its contiguous axis (W in dx = dg Wg + du Wu; all of
 // dW = dg^T x), the tile goes to shared memory as it lies and the instruction reads it
@@ -21,10 +23,14 @@ namespace stg {
 
 namespace {
 
-constexpr int kThreads = 384;      // warp 0 TMA, warp 1 MMA, warp 2 TMEM, warps 4..11 epilogue
-constexpr int kEpilogueWarps = 8;
+constexpr int kEpilogueWarps = 16;
+constexpr int kThreads = 128 + 32 * kEpilogueWarps;   // warp 0 TMA, warp 1 products, warp 2 TMEM, warps 4.. epilogue
 constexpr int kDepth = 64;         // contraction per stage: 128 bytes, one swizzle row
-constexpr int kABytes = kGatedTileM * kDepth * 2;
+constexpr int kPairM = 256;        // rows of a pair's tile
+constexpr int kABytes = 128 * kDepth * 2, kBBytes = 128 * kDepth * 2;   // of one block
+constexpr int kStageBytes = kABytes + kBBytes;
+constexpr int kAccCols = 256;      // TMEM columns of an accumulator set
+constexpr int kSumCol = 240;       // dW: the column of the set that sums dg over the rows
 
 // Kernels that gave up a wait (never, unless a copy or a product failed): see wait().
 __device__ unsigned int g_gave_up;
@@ -32,9 +38,11 @@ __device__ unsigned int g_gave_up;
 struct MmaParams {
     GatedParams g;
     CUtensorMap a[2], b[2], c[2];
-    int64_t tiles;
-    int tiles_n;                   // column tiles of a row of tiles
+    int tiles;
+    FastDiv tiles_n;               // column tiles of a row of tiles (mask head: row tiles of a band)
+    FastDiv rest_n;                // row tiles of a part in dW, column tiles of a stem in the mask head
     int cols;                      // columns of a tile (the instruction's N; outputs x 2 in the forward modes)
+    int sums;                      // dW: also sum dg and du over the rows
     int store_by_tma;
 };
 
@@ -46,8 +54,14 @@ __device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
 __device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void bar_arrive(uint64_t* b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+// The address of a barrier (or anything at the same place) in the pair's first block.
+__device__ __forceinline__ uint32_t in_leader(const void* p) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_addr(p)));
+    return r;
+}
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
     uint32_t ok;
@@ -75,15 +89,16 @@ __device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, volatile in
     }
     return false;
 }
+// Called by whole warps; all lanes get the same answer.
 __device__ __forceinline__ bool wait(uint64_t* b, uint32_t parity, volatile int* dead) {
-#pragma unroll 1
-    for (int i = 0; i < 16; i++)
-        if (bar_try(b, parity)) return true;
-    return wait_slow(b, parity, dead);
+    bool ok = bar_try(b, parity);
+    if (!ok) ok = wait_slow(b, parity, dead);
+    return __all_sync(~0u, ok);
 }
-__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* m, int x, int y, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-                     smem_addr(dst)), "l"(m), "r"(x), "r"(y), "r"(smem_addr(bar)) : "memory");
+// Into this block's shared memory; the bytes count at a barrier of the pair's first block.
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* m, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                     smem_addr(dst)), "l"(m), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void tma_store(const CUtensorMap* m, int x, int y, const void* src) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(m), "r"(x), "r"(y), "r"(
@@ -92,26 +107,39 @@ __device__ __forceinline__ void tma_store(const CUtensorMap* m, int x, int y, co
 __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
                  "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
 }
-// The barrier's phase completes when the products issued so far have.
+// The barrier at this place in both blocks: its phase completes when the products issued so far have.
 __device__ __forceinline__ void mma_commit(uint64_t* b) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(b)) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(b)),
+                 "h"((uint16_t)3) : "memory");
 }
-__device__ __forceinline__ void tmem_load32(uint32_t (&v)[32], uint32_t addr) {
+__device__ __forceinline__ void tmem_load16(uint32_t (&v)[16], uint32_t addr) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
-        "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
-          "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
-          "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(addr));
+}
+__device__ __forceinline__ uint32_t tmem_load1(uint32_t addr) {
+    uint32_t v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(addr));
+    return v;
 }
 __device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+// One lane of a converged warp, the same one each time.
+__device__ __forceinline__ bool elect() {
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+    return r != 0;
+}
 
 // Shared-memory matrix descriptor, 128-byte swizzle: address and offsets in 16-byte units, bit
 // 46 the descriptor's version, layout 2 in bits 61..63. K-major: rows of 128 bytes, groups of
@@ -131,21 +159,26 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// ---- activations: results are rounded to 16 bits, so the fast exponential and division do -----------
-template <int ACT> __device__ __forceinline__ float act(float z) {
-    if (ACT == STG_ACT_RELU) return z < 0.0f ? 0.0f : z;
-    if (ACT == STG_ACT_SILU) return z * sigmoidf(z);
-    if (ACT == STG_ACT_GELU) return 0.5f * z * erfcf(-z * 0.70710678118654752f);
-    if (ACT == STG_ACT_SIGMOID) return sigmoidf(z);
-    return z;
+// ---- activations: results are rounded to 16 bits, so the approximate exponential and reciprocal
+// (2^-22 relative each) do. ----------------------------------------------------------------------------
+__device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float rcp(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+// 1 / (1 + 2^(-z log2 e)); 0 where the power is infinite.
+__device__ __forceinline__ float fast_sigmoid(float z) { return rcp(1.0f + ex2(-1.4426950408889634f * z)); }
+
+// a += x, b += y in one packed instruction.
+__device__ __forceinline__ void add2(uint32_t& a, uint32_t& b, float x, float y) {
+    asm("{\n.reg .b64 u, v;\nmov.b64 u, {%0, %1};\nmov.b64 v, {%2, %3};\nadd.rn.f32x2 u, u, v;\nmov.b64 {%0, %1}, u;\n}"
+        : "+r"(a), "+r"(b) : "f"(x), "f"(y));
 }
+
 // act(z) and its derivative.
 template <int ACT> __device__ __forceinline__ void act_both(float z, float& a, float& d) {
     if (ACT == STG_ACT_RELU) {
         a = z < 0.0f ? 0.0f : z;
         d = z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
     } else if (ACT == STG_ACT_SILU) {
-        const float s = sigmoidf(z);
+        const float s = fast_sigmoid(z);
         a = z * s;
         d = fmaf(a, 1.0f - s, s);
     } else if (ACT == STG_ACT_GELU) {
@@ -153,59 +186,68 @@ template <int ACT> __device__ __forceinline__ void act_both(float z, float& a, f
         a = z * h;
         d = fmaf(0.3989422804014327f * z, __expf(-0.5f * z * z), h);
     } else if (ACT == STG_ACT_SIGMOID) {
-        a = sigmoidf(z);
+        a = fast_sigmoid(z);
         d = a * (1.0f - a);
     } else {
         a = z;
         d = 1.0f;
     }
 }
+template <int ACT> __device__ __forceinline__ float act(float z) {
+    float a, d;
+    act_both<ACT>(z, a, d);
+    return a;
+}
 
-// Where a tile lies.
+// Where a pair's tile lies.
 struct Tile {
     int64_t m0;      // first output row
     int n0;          // first output column
-    int a_y, b_y;    // coordinates of the operands' rows
-    int up_y;
-    int kb;          // stages
-    int part;        // DW: gate or up, and split
+    int cols;        // the instruction's N
+    int a_y;         // A: first row (of the contraction, in dW)
+    int b_y, up_y;   // forward modes: first rows of the two weights
+    int kb;          // slices of the contraction
+    int part;        // dW: 2 split + (0 gate, 1 up)
+    int tile_n;      // dW: number of the column tile
     HeadTile h;
     int64_t cs;      // mask head: chunk * stems + stem
 };
 
-template <int MODE> __device__ __forceinline__ Tile tile_at(const MmaParams& p, int64_t t) {
+template <int MODE> __device__ __forceinline__ Tile tile_at(const MmaParams& p, uint32_t t) {
     Tile r{};
     const GatedParams& g = p.g;
+    r.cols = p.cols;
     if (MODE == GATED_HEAD) {
         // frames first: a band's rows and its weights are then read by neighbours in time
-        const int64_t mt = (g.frames + kGatedTileM - 1) / kGatedTileM, rest = t / mt;
-        r.m0 = (t - rest * mt) * kGatedTileM;
-        r.cs = rest / g.n_tiles;
-        r.h = g.tiles[rest - r.cs * g.n_tiles];
+        const uint32_t rest = p.tiles_n.div(t), cs = p.rest_n.div(rest);
+        r.m0 = (int64_t)(t - rest * p.tiles_n.d) * kPairM;
+        r.cs = cs;
+        r.h = g.tiles[rest - cs * p.rest_n.d];
         r.n0 = r.h.n0;
+        r.cols = 2 * ((min(kHeadWideN, r.h.din - r.n0) + 31) / 32 * 32);
         r.a_y = (int)((r.cs * g.bands + r.h.band) * g.frames + r.m0);
-        r.b_y = (int)((r.cs % g.stems) * 2 * g.band_cols + 2 * (int64_t)r.h.off + r.n0);
+        r.b_y = (int)(((uint32_t)r.cs % (uint32_t)g.stems) * 2 * g.band_cols + 2 * (int64_t)r.h.off + r.n0);
         r.up_y = r.b_y + r.h.din;
         r.kb = (g.k + kDepth - 1) / kDepth;
     } else if (MODE == GATED_FWD || MODE == GATED_PRE) {
-        const int64_t mt = t / p.tiles_n;
-        r.m0 = mt * kGatedTileM;
-        r.n0 = (int)(t - mt * p.tiles_n) * (p.cols / 2);
+        const uint32_t mt = p.tiles_n.div(t);
+        r.m0 = (int64_t)mt * kPairM;
+        r.n0 = (int)(t - mt * p.tiles_n.d) * (p.cols / 2);
         r.a_y = (int)r.m0;
         r.b_y = r.up_y = r.n0;
         r.kb = (g.k + kDepth - 1) / kDepth;
     } else if (MODE == GATED_DX) {
-        const int64_t mt = t / p.tiles_n;
-        r.m0 = mt * kGatedTileM;
-        r.n0 = (int)(t - mt * p.tiles_n) * p.cols;
+        const uint32_t mt = p.tiles_n.div(t);
+        r.m0 = (int64_t)mt * kPairM;
+        r.n0 = (int)(t - mt * p.tiles_n.d) * p.cols;
         r.a_y = (int)r.m0;
         r.kb = 2 * ((g.n + kDepth - 1) / kDepth);
     } else {
-        const int tm = (g.n + kGatedTileM - 1) / kGatedTileM;
-        const int64_t q = t / p.tiles_n;
-        r.n0 = (int)(t - q * p.tiles_n) * p.cols;
-        r.part = (int)(q / tm);                          // 2 split + (gate, up)
-        r.m0 = (q - (int64_t)r.part * tm) * kGatedTileM;
+        const uint32_t q = p.tiles_n.div(t), part = p.rest_n.div(q);
+        r.tile_n = (int)(t - q * p.tiles_n.d);
+        r.n0 = r.tile_n * p.cols;
+        r.part = (int)part;
+        r.m0 = (int64_t)(q - part * p.rest_n.d) * kPairM;
         const int64_t beg = (r.part >> 1) * g.split_rows;
         r.a_y = (int)beg;
         r.kb = (int)((min(g.m, beg + g.split_rows) - beg + kDepth - 1) / kDepth);
@@ -213,306 +255,343 @@ template <int MODE> __device__ __forceinline__ Tile tile_at(const MmaParams& p, 
     return r;
 }
 
-template <int MODE> __host__ __device__ constexpr int b_bytes() { return MODE == GATED_HEAD ? 128 * kDepth * 2 : 256 * kDepth * 2; }
 // Per epilogue warp: 32 rows x 32 columns of output, for dg and du each (float in the mask head,
 // rows 33 apart), and 64 floats of each bias.
 template <int MODE> __host__ __device__ constexpr int out_bytes() {
     return MODE == GATED_PRE ? 4096 : MODE == GATED_HEAD ? 32 * 33 * 4 : MODE == GATED_DW ? 0 : 2048;
 }
-template <int MODE> __host__ __device__ constexpr int stages() { return MODE == GATED_HEAD ? 5 : MODE == GATED_PRE ? 3 : 4; }
+template <int MODE> __host__ __device__ constexpr int stages() { return MODE == GATED_HEAD || MODE == GATED_PRE ? 4 : 5; }
+// dW: a tile of ones, 16 columns
+template <int MODE> __host__ __device__ constexpr int ones_bytes() { return MODE == GATED_DW ? 64 * kDepth * 2 : 0; }
 template <int MODE> constexpr size_t smem_bytes() {
-    return (size_t)stages<MODE>() * (kABytes + b_bytes<MODE>()) + (size_t)kEpilogueWarps * (out_bytes<MODE>() + 512) + 256;
+    return (size_t)stages<MODE>() * kStageBytes + ones_bytes<MODE>() + (size_t)kEpilogueWarps * (out_bytes<MODE>() + 512) + 256;
 }
 
 template <class T, int MODE, int ACT>
-__global__ void __launch_bounds__(kThreads, 1) gated_mma(const __grid_constant__ MmaParams p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_mma(const __grid_constant__ MmaParams p) {
     constexpr bool DUAL = MODE == GATED_FWD || MODE == GATED_HEAD || MODE == GATED_PRE;
     constexpr int kStages = stages<MODE>();
-    constexpr int kStageBytes = kABytes + b_bytes<MODE>();
-    constexpr int kAccCols = MODE == GATED_HEAD ? 128 : 256;   // TMEM columns of an accumulator set
+    // Two accumulator sets let the epilogue of a tile run under the products of the next. The mask
+    // head's float results see the accumulators' roundings (the tensor cores cut, so they add
+    // up along a sum): its two sets are instead two partial sums of one tile, of alternate slices.
+    constexpr int kSets = MODE == GATED_HEAD ? 1 : 2;
     extern __shared__ __align__(1024) uint8_t base[];   // the swizzle counts from 1024-byte boundaries
-    uint8_t* out_stage = base + kStages * kStageBytes;
+    uint8_t* ones = base + kStages * kStageBytes;
+    uint8_t* out_stage = ones + ones_bytes<MODE>();
     float* bias_stage = reinterpret_cast<float*>(out_stage + kEpilogueWarps * out_bytes<MODE>());
     uint64_t* bars = reinterpret_cast<uint64_t*>(bias_stage + kEpilogueWarps * 128);
+    // full and acc_empty are used in the pair's first block, empty and acc_full in both
     uint64_t *full = bars, *empty = bars + kStages, *acc_full = bars + 2 * kStages, *acc_empty = acc_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // the warp's number, known to be uniform
+    const int rank = blockIdx.x & 1;
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const GatedParams& g = p.g;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; s++) { bar_init(full + s, 1); bar_init(empty + s, 1); }
-        for (int s = 0; s < 2; s++) { bar_init(acc_full + s, 1); bar_init(acc_empty + s, kEpilogueWarps); }
+        for (int s = 0; s < 2; s++) { bar_init(acc_full + s, 1); bar_init(acc_empty + s, MODE == GATED_FWD || MODE == GATED_PRE ? kEpilogueWarps : 2 * kEpilogueWarps); }
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (MODE == GATED_DW)   // the same value everywhere: no layout to mind
+        for (int i = threadIdx.x; i < ones_bytes<MODE>() / 4; i += kThreads) reinterpret_cast<uint32_t*>(ones)[i] = pack2<T>(1.0f, 1.0f);
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(2 * kAccCols) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(2 * kAccCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     fence_before();
     __syncthreads();
+    cluster_sync();
     fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0 && lane == 0) {
-        // ---- producer ----------------------------------------------------------------------------
+    // The producer and the product warp run converged with one lane issuing: their addresses and
+    // descriptors then stay in uniform registers. (With one diverged lane the per-slice arithmetic
+    // took about 550 cycles and the tensor cores waited for it.)
+    if (warp == 0) {
+        // ---- producer: this block's rows of A, and its half of B ------------------------------------
+        const bool one = elect();
         int s = 0;
         uint32_t phase = 0;
-        int64_t issued = 0;
-        const int nb = (p.cols + 63) / 64;
-        for (int64_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
+        int issued = 0;      // saturates at kStages
+        for (int t = pair; t < p.tiles; t += pairs) {
             const Tile q = tile_at<MODE>(p, t);
+            const int nb = DUAL ? 1 : (q.cols / 2 + 63) / 64;
+            const uint32_t bytes = kABytes + (DUAL ? (uint32_t)q.cols / 2 * kDepth * 2 : (uint32_t)nb * 8192);
             for (int k = 0; k < q.kb; k++) {
                 if (issued >= kStages && !wait(empty + s, phase ^ 1, dead)) break;
                 uint8_t* a = base + s * kStageBytes;
                 uint8_t* b = a + kABytes;
-                if (DUAL) {
-                    bar_expect(full + s, kABytes + (uint32_t)p.cols * kDepth * 2);
-                    tma_load(a, &p.a[0], k * kDepth, q.a_y, full + s);
-                    tma_load(b, &p.b[0], k * kDepth, q.b_y, full + s);
-                    tma_load(b + (p.cols / 2) * kDepth * 2, &p.b[1], k * kDepth, q.up_y, full + s);
+                const uint32_t bar = in_leader(full + s);
+                if (one && rank == 0) bar_expect(full + s, 2 * bytes);
+                if (!one) {
+                } else if (DUAL) {
+                    tma_load(a, &p.a[0], k * kDepth, q.a_y + rank * 128, bar);
+                    const int y = rank ? q.up_y : q.b_y;
+                    if (MODE == GATED_HEAD)
+                        for (int c = 0; c < q.cols / 2; c += 32) tma_load(b + c * kDepth * 2, &p.b[0], k * kDepth, y + c, bar);
+                    else tma_load(b, &p.b[rank], k * kDepth, y, bar);
                 } else if (MODE == GATED_DX) {
                     const int half = q.kb / 2, up = k >= half, j = (up ? k - half : k) * kDepth;
-                    bar_expect(full + s, kABytes + (uint32_t)nb * 8192);
-                    tma_load(a, &p.a[up], j, q.a_y, full + s);
-                    for (int c = 0; c < nb; c++) tma_load(b + c * 8192, &p.b[up], q.n0 + c * 64, j, full + s);
+                    tma_load(a, &p.a[up], j, q.a_y + rank * 128, bar);
+                    for (int c = 0; c < nb; c++) tma_load(b + c * 8192, &p.b[up], q.n0 + rank * (q.cols / 2) + c * 64, j, bar);
                 } else {
                     const int r = q.a_y + k * kDepth;
-                    bar_expect(full + s, kABytes + (uint32_t)nb * 8192);
-                    tma_load(a, &p.a[q.part & 1], (int)q.m0, r, full + s);
-                    tma_load(a + 8192, &p.a[q.part & 1], (int)q.m0 + 64, r, full + s);
-                    for (int c = 0; c < nb; c++) tma_load(b + c * 8192, &p.b[0], q.n0 + c * 64, r, full + s);
+                    tma_load(a, &p.a[q.part & 1], (int)q.m0 + rank * 128, r, bar);
+                    tma_load(a + 8192, &p.a[q.part & 1], (int)q.m0 + rank * 128 + 64, r, bar);
+                    for (int c = 0; c < nb; c++) tma_load(b + c * 8192, &p.b[0], q.n0 + rank * (q.cols / 2) + c * 64, r, bar);
                 }
-                issued++;
+                issued = min(issued + 1, kStages);
                 if (++s == kStages) { s = 0; phase ^= 1; }
             }
         }
-        // after a failed wait: let the copies in flight land before the block goes
-        if (*dead)
-            for (int i = 0; i < kStages && i < issued; i++) {
-                const int64_t n = issued - 1 - i;
-                for (int tries = 0; tries < 1000000 && !bar_try(full + n % kStages, (uint32_t)(n / kStages) & 1); tries++) {}
-            }
-    } else if (warp == 1 && lane == 0) {
-        // ---- products ----------------------------------------------------------------------------
+        // after a failed wait: time for the copies in flight to land before the block goes
+        if (*dead) {
+            const uint64_t t0 = now_ns();
+            while (now_ns() - t0 < 10000000) {}
+        }
+    } else if (warp == 1 && rank == 0) {
+        // ---- products, for both blocks ---------------------------------------------------------------
         constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
         constexpr uint32_t kAMn = MODE == GATED_DW, kBMn = !DUAL;
-        // D float; A and B types; majors; N / 8; M / 16
-        const uint32_t idesc = 1u << 4 | kType << 7 | kType << 10 | kAMn << 15 | kBMn << 16 | (uint32_t)(p.cols >> 3) << 17 | (uint32_t)(kGatedTileM >> 4) << 24;
-        int s = 0, acc = 0;
+        // D float; A and B types; majors; M / 16. N / 8 is added per tile
+        constexpr uint32_t idesc0 = 1u << 4 | kType << 7 | kType << 10 | kAMn << 15 | kBMn << 16 | (uint32_t)(kPairM >> 4) << 24;
+        // descriptors of the first stage; a stage or a step of 16 further on adds to the address field
+        const uint64_t a0 = smem_desc(smem_addr(base), kAMn ? 8192 : 16), b0 = smem_desc(smem_addr(base) + kABytes, kBMn ? 8192 : 16);
+        const uint64_t ones0 = MODE == GATED_DW ? smem_desc(smem_addr(ones), 8192) : 0;
+        constexpr uint32_t a_step = (kAMn ? 2048 : 32) >> 4, b_step = (kBMn ? 2048 : 32) >> 4;
+        const bool one = elect();
+        int s = 0;
         uint32_t phase = 0;
-        int64_t n = 0;
-        for (int64_t t = blockIdx.x; t < p.tiles; t += gridDim.x, n++) {
+        int n = 0;
+        for (int t = pair; t < p.tiles; t += pairs, n++) {
             const Tile q = tile_at<MODE>(p, t);
-            if (n >= 2 && !wait(acc_empty + acc, (uint32_t)((n >> 1) - 1) & 1, dead)) break;
+            const int set = n % kSets;
+            if (n >= kSets && !wait(acc_empty + set, (uint32_t)(n / kSets - 1) & 1, dead)) break;
             fence_after();
-            const uint32_t d = tmem + acc * kAccCols;
+            const uint32_t d0 = tmem + set * kAccCols, idesc = idesc0 | (uint32_t)(q.cols >> 3) << 17;
             bool ok = true;
             for (int k = 0; k < q.kb; k++) {
                 if (!(ok = wait(full + s, phase, dead))) break;
                 fence_after();
-                const uint32_t a = smem_addr(base + s * kStageBytes), b = a + kABytes;
+                const uint64_t a = a0 + (uint32_t)(s * (kStageBytes >> 4)), b = b0 + (uint32_t)(s * (kStageBytes >> 4));
+                const uint32_t d = MODE == GATED_HEAD ? d0 + (k & 1) * kAccCols : d0;
+                const bool add = k > (MODE == GATED_HEAD ? 1 : 0);
+                // the sums dg^T 1 of a slice, shared between the column tiles, which read the same dg
+                const bool sum = MODE == GATED_DW && p.sums && (uint32_t)k % p.tiles_n.d == (uint32_t)q.tile_n;
+                if (one) {
 #pragma unroll
-                for (int i = 0; i < kDepth / 16; i++)
-                    mma(d, smem_desc(a + i * (kAMn ? 2048 : 32), kAMn ? 8192 : 16), smem_desc(b + i * (kBMn ? 2048 : 32), kBMn ? 8192 : 16), idesc,
-                        k > 0 || i > 0);
-                mma_commit(empty + s);
+                    for (int i = 0; i < kDepth / 16; i++) {
+                        mma(d, a + i * a_step, b + i * b_step, idesc, add || i > 0);
+                        if (MODE == GATED_DW && sum)
+                            mma(d + kSumCol, a + i * a_step, ones0 + i * b_step, idesc0 | 2u << 17, k >= (int)p.tiles_n.d || i > 0);
+                    }
+                    mma_commit(empty + s);
+                }
                 if (++s == kStages) { s = 0; phase ^= 1; }
             }
             if (!ok) break;
-            mma_commit(acc_full + acc);
-            acc ^= 1;
+            if (one) mma_commit(acc_full + set);
         }
     } else if (warp >= 4) {
-        // ---- epilogue ----------------------------------------------------------------------------
-        const int e = warp - 4, quad = warp & 3, half = e >> 2;   // TMEM lanes 32 quad.., half of the columns
+        // ---- epilogue --------------------------------------------------------------------------------
+        // A warp reads TMEM lanes 32 quad.. and every kStep-th 32-column piece. In gated and its
+        // first backward product, whose tiles are short, eight warps take the even tiles and
+        // eight the odd ones, so that the waits of one half run under the work of the other.
+        constexpr int kHalves = MODE == GATED_FWD || MODE == GATED_PRE ? 2 : 1, kStep = 4 / kHalves;
+        const int e = warp - 4, quad = warp & 3, group = (e >> 2) % kStep;
         uint8_t* stage = out_stage + e * out_bytes<MODE>();
         float* bias = bias_stage + e * 128;
-        int64_t n = 0;
-        for (int64_t t = blockIdx.x; t < p.tiles; t += gridDim.x, n++) {
+        int n = 0;
+        for (int t = pair; t < p.tiles; t += pairs, n++) {
+            if (kHalves == 2 && (n & 1) != (e >> 3)) continue;
             const Tile q = tile_at<MODE>(p, t);
-            const int acc = (int)(n & 1);
-            const int width = DUAL ? p.cols / 2 : p.cols;         // outputs of the tile's row
-            // two warps share a quadrant: 32-column pieces, the first half of them to one
-            const int pieces = (width + 31) / 32, mine0 = half ? (pieces + 1) / 2 : 0, mine1 = half ? pieces : (pieces + 1) / 2;
-            const int64_t row = q.m0 + quad * 32 + lane;
-            if (DUAL) {
+            const int set = n % kSets;
+            const int width = DUAL ? q.cols / 2 : q.cols;         // outputs of the tile's row
+            const int pieces = (width + 31) / 32;
+            const int64_t row0 = q.m0 + rank * 128 + quad * 32, row = row0 + lane;
+            if (DUAL) {   // at most four pieces to a tile, so kHalves to a warp
                 const int nj = MODE == GATED_HEAD ? q.h.din : g.n;
-                __syncwarp();
-                for (int i = lane; i < 64; i += 32) {
-                    const int c = q.n0 + mine0 * 32 + i;
-                    float bg = 0.0f, bu = 0.0f;
-                    if (c < nj) {
-                        if (MODE == GATED_HEAD) {
-                            const int64_t at = (q.cs % g.stems) * 2 * g.band_cols + 2 * (int64_t)q.h.off + c;
-                            if (g.bg) { bg = to_float(static_cast<const T*>(g.bg)[at]); bu = to_float(static_cast<const T*>(g.bg)[at + nj]); }
-                        } else {
-                            if (g.bg) bg = to_float(static_cast<const T*>(g.bg)[c]);
-                            if (g.bu) bu = to_float(static_cast<const T*>(g.bu)[c]);
-                        }
+                float bg[kHalves], bu[kHalves];
+#pragma unroll
+                for (int i = 0; i < kHalves; i++) {
+                    const int c = q.n0 + (group + i * kStep) * 32 + lane;
+                    bg[i] = bu[i] = 0.0f;
+                    if (c >= nj) continue;
+                    if (MODE == GATED_HEAD) {
+                        const int64_t at = ((uint32_t)q.cs % (uint32_t)g.stems) * 2 * g.band_cols + 2 * (int64_t)q.h.off + c;
+                        if (g.bg) { bg[i] = to_float(static_cast<const T*>(g.bg)[at]); bu[i] = to_float(static_cast<const T*>(g.bg)[at + nj]); }
+                    } else {
+                        if (g.bg) bg[i] = to_float(static_cast<const T*>(g.bg)[c]);
+                        if (g.bu) bu[i] = to_float(static_cast<const T*>(g.bu)[c]);
                     }
-                    bias[i] = bg;
-                    bias[64 + i] = bu;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kHalves; i++) {
+                    bias[64 * i + lane] = bg[i];
+                    bias[64 * i + 32 + lane] = bu[i];
                 }
                 __syncwarp();
             }
-            if (!wait(acc_full + acc, (uint32_t)(n >> 1) & 1, dead)) break;
+            if (!wait(acc_full + set, (uint32_t)(n / kSets) & 1, dead)) break;
             fence_after();
-            const uint32_t lanes = tmem + acc * kAccCols + ((uint32_t)(quad * 32) << 16);
-            for (int c = mine0; c < mine1; c++) {
-                uint32_t v[32], w[32];
-                tmem_load32(v, lanes + c * 32);
-                if (DUAL) tmem_load32(w, lanes + width + c * 32);
+            const uint32_t lanes = tmem + set * kAccCols + ((uint32_t)(quad * 32) << 16);
+            if (MODE == GATED_DW && p.sums && group == 3) {
+                const uint32_t sum = tmem_load1(lanes + kSumCol);
                 tmem_wait();
-                if (c + 1 == mine1) {   // the accumulators are in registers: the next products may have them
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(acc_empty + acc);
-                }
-                const int j0 = q.n0 + c * 32, lc = (c - mine0) * 32;
-                if (MODE == GATED_DW) {
-                    // 32 floats of the row: whole 128-byte lines where the rows are aligned
-                    if (row < g.n) {
-                        float* o = g.dw_part + ((int64_t)q.part * g.n + row) * g.k + j0;
-                        if ((g.k & 3) == 0 && j0 + 32 <= g.k) {
+                // a column tile past the slices has summed none
+                if (row < g.n) g.col_sums[((int64_t)((q.part >> 1) * (int)p.tiles_n.d + q.tile_n) * 2 + (q.part & 1)) * g.n + row] = q.tile_n < q.kb ? __uint_as_float(sum) : 0.0f;
+            }
+            for (int c = group; c < pieces; c += kStep) {
+                const float* pb = bias + (c - group) / kStep * 64;
+                const int j0 = q.n0 + c * 32;
+                const bool store = MODE != GATED_DW && MODE != GATED_HEAD && p.store_by_tma;
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(o + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                        } else {
+                for (int hh = 0; hh < 2; hh++) {   // 16 columns at a time, to stay within the registers
+                    const int j = j0 + hh * 16, lc = hh * 16;
+                    uint32_t v[16], w[16];
+                    tmem_load16(v, lanes + c * 32 + lc);
+                    if (DUAL) tmem_load16(w, lanes + width + c * 32 + lc);
+                    tmem_wait();
+                    if (MODE == GATED_HEAD && q.kb > 1) {   // the other partial sum
+                        uint32_t x[16];
+                        tmem_load16(x, lanes + kAccCols + c * 32 + lc);
+                        tmem_wait();
 #pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if (j0 + i < g.k) o[i] = __uint_as_float(v[i]);
-                        }
+                        for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(x[i]));
+                        tmem_load16(x, lanes + kAccCols + width + c * 32 + lc);
+                        tmem_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__uint_as_float(w[i]) + __uint_as_float(x[i]));
                     }
-                    continue;
-                }
-                if (MODE == GATED_HEAD) {
-                    float* sm = reinterpret_cast<float*>(stage);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 bv = *reinterpret_cast<const float4*>(bias + lc + i), bw = *reinterpret_cast<const float4*>(bias + 64 + lc + i);
-                        const float bva[4] = {bv.x, bv.y, bv.z, bv.w}, bwa[4] = {bw.x, bw.y, bw.z, bw.w};
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            sm[lane * 33 + i + k] = (__uint_as_float(v[i + k]) + bva[k]) * sigmoidf(__uint_as_float(w[i + k]) + bwa[k]);
+                    if (hh == 1 && c + kStep >= pieces) {   // all in registers: the next products may have the set
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive_cluster(in_leader(acc_empty + set));
                     }
-                    __syncwarp();
-                    const int64_t r0 = q.m0 + quad * 32;
-                    const int rows = (int)min((int64_t)32, g.frames - r0);
-                    float* o = g.masks + (q.cs * g.band_cols + q.h.off) * g.frames + r0 * q.h.din + j0 + lane;
-                    if (j0 + lane < q.h.din)
-                        for (int r = 0; r < rows; r++) o[(int64_t)r * q.h.din] = sm[r * 33 + lane];
-                    __syncwarp();
-                    continue;
-                }
-                uint32_t o[16], o2[16];
-                if (MODE == GATED_FWD) {
+                    if (MODE == GATED_DW) {
+                        if (row < g.n) {
+                            float* o = g.dw_part + ((int64_t)q.part * g.n + row) * g.k + j;
+                            if ((g.k & 3) == 0 && j + 16 <= g.k) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 bv = *reinterpret_cast<const float4*>(bias + lc + i), bw = *reinterpret_cast<const float4*>(bias + 64 + lc + i);
-                        const float y0 = act<ACT>(__uint_as_float(v[i]) + bv.x) * (__uint_as_float(w[i]) + bw.x);
-                        const float y1 = act<ACT>(__uint_as_float(v[i + 1]) + bv.y) * (__uint_as_float(w[i + 1]) + bw.y);
-                        const float y2 = act<ACT>(__uint_as_float(v[i + 2]) + bv.z) * (__uint_as_float(w[i + 2]) + bw.z);
-                        const float y3 = act<ACT>(__uint_as_float(v[i + 3]) + bv.w) * (__uint_as_float(w[i + 3]) + bw.w);
-                        o[i / 2] = pack2<T>(y0, y1);
-                        o[i / 2 + 1] = pack2<T>(y2, y3);
-                    }
-                } else if (MODE == GATED_PRE) {
-                    // dg and du in place of g and u, then their sums over the warp's rows
-                    const T* dy = static_cast<const T*>(g.dy) + row * g.y_row + j0;
-                    const bool row_ok = row < g.m;
-                    const bool vec = row_ok && j0 + 32 <= g.n && (reinterpret_cast<uintptr_t>(dy) & 15) == 0;
+                                for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(o + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                            } else {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        float d[8];
-                        if (vec) {
-                            const Pack<T, 8> x = *reinterpret_cast<const Pack<T, 8>*>(dy + i);
-#pragma unroll
-                            for (int k = 0; k < 8; k++) d[k] = to_float(x.v[k]);
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 8; k++) d[k] = row_ok && j0 + i + k < g.n ? to_float(dy[i + k]) : 0.0f;
-                        }
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            const float gg = __uint_as_float(v[i + k]) + bias[lc + i + k], uu = __uint_as_float(w[i + k]) + bias[64 + lc + i + k];
-                            float a, s;
-                            act_both<ACT>(gg, a, s);
-                            // a row or column past the end has d = 0, but its g and u are not defined
-                            const bool in = row_ok && j0 + i + k < g.n;
-                            v[i + k] = __float_as_uint(in ? d[k] * uu * s : 0.0f);
-                            w[i + k] = __float_as_uint(in ? d[k] * a : 0.0f);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        o[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-                        o2[i] = pack2<T>(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
-                    }
-                    if (g.col_sums) {
-                        // Sums of 32 columns over 32 lanes in 31 steps each: a lane and its partner split
-                        // the columns between them and add, until a lane holds one column: its own number's.
-#pragma unroll
-                        for (int h = 16; h > 0; h >>= 1) {
-                            const bool hi = lane & h;
-#pragma unroll
-                            for (int i = 0; i < 16; i++) {
-                                if (i >= h) break;
-                                const float kv = __uint_as_float(hi ? v[i + h] : v[i]), sv = __uint_as_float(hi ? v[i] : v[i + h]);
-                                const float kw = __uint_as_float(hi ? w[i + h] : w[i]), sw = __uint_as_float(hi ? w[i] : w[i + h]);
-                                v[i] = __float_as_uint(kv + __shfl_xor_sync(~0u, sv, h));
-                                w[i] = __float_as_uint(kw + __shfl_xor_sync(~0u, sw, h));
+                                for (int i = 0; i < 16; i++)
+                                    if (j + i < g.k) o[i] = __uint_as_float(v[i]);
                             }
                         }
-                        if (j0 + lane < g.n) {
-                            float* sums = g.col_sums + ((q.m0 / 32 + quad) * 2) * g.n + j0 + lane;
-                            sums[0] = __uint_as_float(v[0]);
-                            sums[g.n] = __uint_as_float(w[0]);
+                        continue;
+                    }
+                    if (DUAL) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const float4 x = *reinterpret_cast<const float4*>(pb + lc + i), y = *reinterpret_cast<const float4*>(pb + 32 + lc + i);
+                            add2(v[i], v[i + 1], x.x, x.y);
+                            add2(v[i + 2], v[i + 3], x.z, x.w);
+                            add2(w[i], w[i + 1], y.x, y.y);
+                            add2(w[i + 2], w[i + 3], y.z, y.w);
                         }
                     }
-                } else {
+                    if (MODE == GATED_HEAD) {
+                        float* sm = reinterpret_cast<float*>(stage) + lane * 33 + lc;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-                }
-                T* out = static_cast<T*>(MODE == GATED_FWD ? g.y : MODE == GATED_PRE ? g.dg : g.dx);
-                const int64_t pitch = MODE == GATED_FWD ? g.y_row : MODE == GATED_PRE ? g.pre_row : g.dx_row;
-                const int nj = MODE == GATED_DX ? g.k : g.n;
-                if (p.store_by_tma) {
-                    // 32 rows of 64 bytes as the 64-byte swizzle has them: 16-byte piece c of row r at c ^ (r / 2 & 3)
-                    if (lane == 0) stores_read();
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int to = lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
-                        *reinterpret_cast<uint4*>(stage + to) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                        if (MODE == GATED_PRE)
-                            *reinterpret_cast<uint4*>(stage + 2048 + to) = make_uint4(o2[4 * i], o2[4 * i + 1], o2[4 * i + 2], o2[4 * i + 3]);
+                        for (int i = 0; i < 16; i++) sm[i] = __uint_as_float(v[i]) * fast_sigmoid(__uint_as_float(w[i]));
+                        continue;
                     }
+                    uint32_t o[8], o2[8];
+                    if (MODE == GATED_FWD) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2)
+                            o[i / 2] = pack2<T>(act<ACT>(__uint_as_float(v[i])) * __uint_as_float(w[i]),
+                                                act<ACT>(__uint_as_float(v[i + 1])) * __uint_as_float(w[i + 1]));
+                    } else if (MODE == GATED_PRE) {
+                        const T* dy = static_cast<const T*>(g.dy) + row * g.y_row + j;
+                        Pack<T, 8> d[2];
+                        if (row < g.m && j + 16 <= g.n && (reinterpret_cast<uintptr_t>(dy) & 15) == 0) {
+                            d[0] = *reinterpret_cast<const Pack<T, 8>*>(dy);
+                            d[1] = *reinterpret_cast<const Pack<T, 8>*>(dy + 8);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; i++) d[i / 8].v[i % 8] = row < g.m && j + i < g.n ? dy[i] : from_float<T>(0.0f);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            float dg[2], du[2];
+#pragma unroll
+                            for (int k = 0; k < 2; k++) {
+                                const float x = to_float(d[(i + k) / 8].v[(i + k) % 8]);
+                                float a, s;
+                                act_both<ACT>(__uint_as_float(v[i + k]), a, s);
+                                dg[k] = x * __uint_as_float(w[i + k]) * s;
+                                du[k] = x * a;
+                            }
+                            o[i / 2] = pack2<T>(dg[0], dg[1]);
+                            o2[i / 2] = pack2<T>(du[0], du[1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) o[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                    }
+                    if (store) {
+                        if (hh == 0) {   // the stage's last store has read it
+                            if (lane == 0) stores_read();
+                            __syncwarp();
+                        }
+                        // rows of 64 bytes as the 64-byte swizzle has them: 16-byte piece c of row r at c ^ (r / 2 & 3)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const int to = lane * 64 + (((2 * hh + i) ^ ((lane >> 1) & 3)) << 4);
+                            *reinterpret_cast<uint4*>(stage + to) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                            if (MODE == GATED_PRE)
+                                *reinterpret_cast<uint4*>(stage + 2048 + to) = make_uint4(o2[4 * i], o2[4 * i + 1], o2[4 * i + 2], o2[4 * i + 3]);
+                        }
+                    } else if (MODE != GATED_PRE && row < g.m) {
+                        T* out = static_cast<T*>(MODE == GATED_FWD ? g.y : g.dx);
+                        const int64_t pitch = MODE == GATED_FWD ? g.y_row : g.dx_row;
+                        const int nj = MODE == GATED_DX ? g.k : g.n;
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (j + i < nj) out[row * pitch + j + i] = reinterpret_cast<const T*>(&o[i / 2])[i & 1];
+                    }
+                }
+                if (MODE == GATED_HEAD) {
+                    __syncwarp();
+                    const int rows = (int)max((int64_t)0, min((int64_t)32, g.frames - row0));
+                    const float* sm = reinterpret_cast<const float*>(stage) + lane;
+                    float* o = g.masks + (q.cs * g.band_cols + q.h.off) * g.frames + row0 * q.h.din + j0 + lane;
+                    if (j0 + lane < q.h.din) {
+#pragma unroll 8
+                        for (int r = 0; r < rows; r++) o[(int64_t)r * q.h.din] = sm[r * 33];
+                    }
+                    __syncwarp();
+                }
+                if (store) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    const int64_t y = q.m0 + quad * 32;
-                    if (lane == 0 && j0 < nj && y < g.m) {
-                        tma_store(&p.c[0], j0, (int)y, stage);
-                        if (MODE == GATED_PRE) tma_store(&p.c[1], j0, (int)y, stage + 2048);
+                    if (lane == 0 && j0 < (MODE == GATED_DX ? g.k : g.n) && row0 < g.m) {
+                        tma_store(&p.c[0], j0, (int)row0, stage);
+                        if (MODE == GATED_PRE) tma_store(&p.c[1], j0, (int)row0, stage + 2048);
                         store_commit();
-                    }
-                } else if (row < g.m) {
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        if (j0 + i >= nj) break;
-                        const T* s = reinterpret_cast<const T*>(&o[i / 2]);
-                        out[row * pitch + j0 + i] = s[i & 1];
-                        if (MODE == GATED_PRE) static_cast<T*>(g.du)[row * pitch + j0 + i] = reinterpret_cast<const T*>(&o2[i / 2])[i & 1];
                     }
                 }
             }
-            if (mine0 == mine1 && lane == 0) bar_arrive(acc_empty + acc);   // no piece of this tile
+            if (group >= pieces) {   // no piece of this tile (or only the sums)
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive_cluster(in_leader(acc_empty + set));
+            }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     fence_before();
     __syncthreads();
-    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kAccCols));
+    cluster_sync();   // neither block goes while the other may still signal or read it
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kAccCols));
 }
 
 // ---- host -------------------------------------------------------------------------------------
@@ -548,7 +627,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 template <class T, int MODE, int ACT> void launch(const MmaParams& p, int sms, cudaStream_t st) {
     const auto kernel = gated_mma<T, MODE, ACT>;
     cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<MODE>()), "gated kernel");
-    kernel<<<(unsigned)std::min<int64_t>(p.tiles, sms), kThreads, smem_bytes<MODE>(), st>>>(p);
+    kernel<<<2 * (unsigned)std::min<int64_t>(p.tiles, sms / 2), kThreads, smem_bytes<MODE>(), st>>>(p);
     cuda_check(cudaGetLastError(), "gated kernel");
 }
 
@@ -562,25 +641,44 @@ template <class T, int MODE> void launch_act(const MmaParams& p, int sms, cudaSt
     }
 }
 
+// The width of dx's and dW's column tiles: whole 32-column pieces as the epilogue stores them (so that
+// no piece reaches into the next tile), of the tile count that takes the fewest column steps per
+// pair, counting 32 more per tile for the rows of A that each tile loads again. dW's
+// sums over the rows have the accumulators' last columns.
+int column_tile(int k, int64_t rest, int64_t pairs, bool sums) {
+    const int most = sums ? kSumCol / 32 * 32 : 256;
+    int64_t best = INT64_MAX, width = 0;
+    for (int64_t t = ceil_div(k, most); t <= ceil_div(k, 64); t++) {
+        const int64_t cols = ceil_div(ceil_div(k, t), 32) * 32, cost = ceil_div(rest * ceil_div(k, cols), pairs) * (cols + 32);
+        if (cost < best) { best = cost; width = cols; }
+    }
+    return (int)width;
+}
+
 } // namespace
+
+int64_t gated_col_sums(const GatedParams& g, int sms) {
+    return g.splits * ceil_div(g.k, column_tile(g.k, 2 * g.splits * ceil_div(g.n, kPairM), sms / 2, true));
+}
 
 void launch_gated_mma(GatedMode mode, bool bf16, const GatedParams& g, int64_t head_rows, int sms, cudaStream_t st) {
     MmaParams p{};
     p.g = g;
-    const int64_t mt = ceil_div(mode == GATED_HEAD ? g.frames : g.m, kGatedTileM);
+    const int64_t mt = ceil_div(mode == GATED_HEAD ? g.frames : g.m, kPairM), pairs = sms / 2;
+    int64_t tiles = 0, tiles_n = 1, rest_n = 1;
     if (mode == GATED_HEAD) {
-        p.cols = 2 * kGatedTileN;
-        p.tiles = head_rows / g.frames / g.bands * mt * g.n_tiles;
-        encode(&p.a[0], bf16, g.x, head_rows, g.k, g.x_row, kDepth, kGatedTileM);
-        encode(&p.b[0], bf16, g.wg, g.stems * 2 * g.band_cols, g.k, g.wg_row, kDepth, kGatedTileN);
-        p.b[1] = p.b[0];
+        tiles_n = mt;
+        rest_n = g.n_tiles;
+        tiles = head_rows / g.frames / g.bands * mt * g.n_tiles;
+        encode(&p.a[0], bf16, g.x, head_rows, g.k, g.x_row, kDepth, 128);
+        encode(&p.b[0], bf16, g.wg, g.stems * 2 * g.band_cols, g.k, g.wg_row, kDepth, 32);
     } else if (mode == GATED_FWD || mode == GATED_PRE) {
         // 128 outputs to a tile; 64 when that would leave SMs without a tile
-        const int n = mt * ceil_div(g.n, 128) < sms ? 64 : 128;
+        const int n = mt * ceil_div(g.n, 128) < pairs ? 64 : 128;
         p.cols = 2 * n;
-        p.tiles_n = (int)ceil_div(g.n, n);
-        p.tiles = mt * p.tiles_n;
-        encode(&p.a[0], bf16, g.x, g.m, g.k, g.x_row, kDepth, kGatedTileM);
+        tiles_n = ceil_div(g.n, n);
+        tiles = mt * tiles_n;
+        encode(&p.a[0], bf16, g.x, g.m, g.k, g.x_row, kDepth, 128);
         encode(&p.b[0], bf16, g.wg, g.n, g.k, g.wg_row, kDepth, n);
         encode(&p.b[1], bf16, g.wu, g.n, g.k, g.wu_row, kDepth, n);
         if (mode == GATED_FWD) {
@@ -592,26 +690,29 @@ void launch_gated_mma(GatedMode mode, bool bf16, const GatedParams& g, int64_t h
             encode(&p.c[1], bf16, g.du, g.m, g.n, g.pre_row, 32, 32, true);
         }
     } else {
-        // the fewest column tiles of at most 256, of one width: whole 32-column pieces, as the epilogue
-        // stores them, so that no piece reaches into the next tile
-        p.tiles_n = (int)ceil_div(g.k, 256);
-        p.cols = (int)ceil_div(ceil_div(g.k, p.tiles_n), 32) * 32;
-        p.tiles_n = (int)ceil_div(g.k, p.cols);
+        p.sums = mode == GATED_DW && g.col_sums;
+        const int64_t rest = mode == GATED_DX ? mt : 2 * g.splits * ceil_div(g.n, kPairM);
+        p.cols = column_tile(g.k, rest, pairs, p.sums);
+        tiles_n = ceil_div(g.k, p.cols);
+        rest_n = ceil_div(g.n, kPairM);
+        tiles = rest * tiles_n;
         if (mode == GATED_DX) {
-            p.tiles = mt * p.tiles_n;
-            encode(&p.a[0], bf16, g.dg, g.m, g.n, g.pre_row, kDepth, kGatedTileM);
-            encode(&p.a[1], bf16, g.du, g.m, g.n, g.pre_row, kDepth, kGatedTileM);
+            encode(&p.a[0], bf16, g.dg, g.m, g.n, g.pre_row, kDepth, 128);
+            encode(&p.a[1], bf16, g.du, g.m, g.n, g.pre_row, kDepth, 128);
             encode(&p.b[0], bf16, g.wg, g.n, g.k, g.wg_row, 64, kDepth);
             encode(&p.b[1], bf16, g.wu, g.n, g.k, g.wu_row, 64, kDepth);
             p.store_by_tma = aligned(g.dx, 16) && (g.dx_row % 8 == 0 || g.m == 1);
             if (p.store_by_tma) encode(&p.c[0], bf16, g.dx, g.m, g.k, g.dx_row, 32, 32, true);
         } else {
-            p.tiles = 2 * g.splits * ceil_div(g.n, kGatedTileM) * p.tiles_n;
             encode(&p.a[0], bf16, g.dg, g.m, g.n, g.pre_row, 64, kDepth);
             encode(&p.a[1], bf16, g.du, g.m, g.n, g.pre_row, 64, kDepth);
             encode(&p.b[0], bf16, g.x, g.m, g.k, g.x_row, 64, kDepth);
         }
     }
+    if (tiles > INT32_MAX) fail(STG_UNSUPPORTED, "gated: too many tiles");
+    p.tiles = (int)tiles;
+    p.tiles_n = FastDiv((uint32_t)tiles_n);
+    p.rest_n = FastDiv((uint32_t)rest_n);
     auto go = [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
         if (mode == GATED_HEAD) launch<T, GATED_HEAD, STG_ACT_SIGMOID>(p, sms, st);

@@ -187,9 +187,10 @@ def gated_backward(dy, x, wg, wu, bg, bu, kind):
     for v, ev in ((dg, rdg), (du, rdu)):
         out.append(v.t() @ d[0])
         err.append(ev.t() @ d[0].abs() + 2 * (m + 2) * F32 * ((v.abs() + ev).t() @ d[0].abs()))
-    for v, ev in ((dg, edg), (du, edu)):
+    # the tensor cores sum the rounded gradients, the CUDA cores (float32) the ones before rounding
+    for v, ev in ((dg, edg if t == torch.float32 else rdg), (du, edu if t == torch.float32 else rdu)):
         out.append(v.sum(0))
-        err.append(ev.sum(0) + (m + 2) * F32 * v.abs().sum(0))
+        err.append(ev.sum(0) + 2 * (m + 2) * F32 * (v.abs() + ev).sum(0))
     return out, [e + half_ulp(t) * o.abs() + tiny(t) for o, e in zip(out, err)]
 
 
