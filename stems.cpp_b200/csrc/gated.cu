@@ -282,43 +282,86 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
     }
 }
 
-// dW from its partial sums [splits][2][n][k], added in order.
+// The biases' gradients from the column sums [sums][2][n] (the first sum_blocks blocks, 32 columns
+// each) and dW from its partial sums [splits][2][n][k], both added in a fixed order.
 template <class T>
-__global__ void __launch_bounds__(kThreads) dw_join(const float* part, int splits, int64_t n, int64_t k, T* dwg, int64_t dwg_row,
-                                                    T* dwu, int64_t dwu_row) {
-    const int64_t total = 2 * n * k;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+__global__ void __launch_bounds__(kThreads) join_parts(const __grid_constant__ GatedParams p, int64_t sums, unsigned sum_blocks, T* dwg,
+                                                       int64_t dwg_row, T* dwu, int64_t dwu_row, T* dbg, T* dbu) {
+    if (blockIdx.x < sum_blocks) {
+        __shared__ float red[8][33];
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const int64_t i = (int64_t)blockIdx.x * 32 + lane, n2 = 2 * (int64_t)p.n;
         float s = 0.0f;
-        for (int q = 0; q < splits; q++) s += part[q * total + i];
-        const bool up = i >= n * k;
-        const int64_t j = up ? i - n * k : i, r = j / k, c = j - r * k;
-        T* d = up ? dwu : dwg;
-        if (d) d[r * (up ? dwu_row : dwg_row) + c] = from_float<T>(s);
+        if (i < n2)
+#pragma unroll 4
+            for (int64_t t = warp; t < sums; t += 8) s += p.col_sums[t * n2 + i];
+        red[warp][lane] = s;
+        __syncthreads();
+        if (warp || i >= n2) return;
+        for (int w = 1; w < 8; w++) s += red[w][lane];
+        T* d = i < p.n ? dbg : dbu;
+        if (d) d[i < p.n ? i : i - p.n] = from_float<T>(s);
+        return;
+    }
+    const int64_t total = 2 * (int64_t)p.n * p.k, blocks = gridDim.x - sum_blocks;
+    const bool wide = p.k % 4 == 0;
+    for (int64_t i = ((blockIdx.x - sum_blocks) * (int64_t)kThreads + threadIdx.x) * 4; i < total; i += blocks * kThreads * 4) {
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int q = 0; q < p.splits; q++) {
+            const float* from = p.dw_part + q * total + i;
+            if (wide) {
+                const float4 v = *reinterpret_cast<const float4*>(from);
+                s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (i + e < total) s[e] += from[e];
+            }
+        }
+        const int64_t row4 = i / p.k;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (i + e >= total) break;
+            const int64_t row = wide ? row4 : (i + e) / p.k, c = i + e - row * p.k;   // row of [dWg; dWu]
+            const bool up = row >= p.n;
+            T* d = up ? dwu : dwg;
+            if (d) d[(up ? row - p.n : row) * (up ? dwu_row : dwg_row) + c] = from_float<T>(s[e]);
+        }
     }
 }
 
-// dbg and dbu from the tiles' column sums [tiles][2][n]: a warp per column.
+// Copies of up to three matrices of one width, their rows `pitch` elements apart, for operands
+// whose rows are no whole 16 bytes. A thread makes 16 bytes of a copy; elements past the width are 0.
+struct RepackParams {
+    const void* src[3];
+    void* dst[3];
+    int64_t row[3], rows[3];
+    int cols;
+    FastDiv pieces;      // of 16 bytes in a row
+};
 template <class T>
-__global__ void __launch_bounds__(128) db_join(const float* sums, int64_t tiles, int n, T* dbg, T* dbu) {
-    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (i >= 2 * (int64_t)n) return;
-    float s = 0.0f;
-    for (int64_t t = lane; t < tiles; t += 32) s += sums[t * 2 * n + i];
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-    if (lane == 0) {
-        T* d = i < n ? dbg : dbu;
-        if (d) d[i < n ? i : i - n] = from_float<T>(s);
-    }
-}
-
-// A matrix with its rows `pitch` elements apart, for operands whose rows are no whole 16 bytes.
-template <class T>
-__global__ void __launch_bounds__(kThreads) repack(const T* src, int64_t src_row, T* dst, int64_t pitch, int64_t rows, int cols) {
-    const int64_t total = rows * cols;
+__global__ void __launch_bounds__(kThreads) repack(const __grid_constant__ RepackParams p) {
+    const int z = blockIdx.y;
+    const int64_t total = p.rows[z] * p.pieces.d;
+    const T* src = static_cast<const T*>(p.src[z]);
+    const bool pairs = p.row[z] % 2 == 0 && reinterpret_cast<uintptr_t>(src) % 4 == 0;
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-        const int64_t r = i / cols, c = i - r * cols;
-        dst[r * pitch + c] = src[r * src_row + c];
+        const int64_t r = total < (1ll << 31) ? p.pieces.div((uint32_t)i) : i / p.pieces.d;
+        const int c = (int)(i - r * p.pieces.d) * 8;
+        const T* from = src + r * p.row[z] + c;
+        Pack<T, 8> v;
+        if (pairs && c + 8 <= p.cols) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const Pack<T, 2> w = *reinterpret_cast<const Pack<T, 2>*>(from + e);
+                v.v[e] = w.v[0];
+                v.v[e + 1] = w.v[1];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v.v[e] = c + e < p.cols ? from[e] : from_float<T>(0.0f);
+        }
+        *reinterpret_cast<Pack<T, 8>*>(static_cast<T*>(p.dst[z]) + i * 8) = v;
     }
 }
 
@@ -351,14 +394,31 @@ Copies copies_of(const stg_gated_config& c) {
     r.wu = copy_bytes(c.width, c.wu_row, c.features);
     return r;
 }
-template <class T> void copy_operand(const void*& p, int64_t& row, size_t bytes, int64_t rows, int cols, char*& ws, cudaStream_t st) {
-    if (!bytes) return;
-    const int64_t pitch = ceil_div(cols, 8) * 8;
-    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(rows * cols, kThreads), 148 * 8);
-    repack<T><<<blocks, kThreads, 0, st>>>(static_cast<const T*>(p), row, reinterpret_cast<T*>(ws), pitch, rows, cols);
-    p = ws;
-    row = pitch;
-    ws += bytes;
+// Makes the copies in ws and points p at them.
+template <class T> void copy_operands(GatedParams& p, const Copies& copies, int64_t x_rows, int64_t w_rows, char* ws, cudaStream_t st) {
+    if (!copies.bytes()) return;
+    RepackParams r{};
+    r.cols = p.k;
+    r.pieces = FastDiv((uint32_t)ceil_div(p.k, 8));
+    int n = 0;
+    int64_t most = 0;
+    auto add = [&](const void*& src, int64_t& row, size_t bytes, int64_t rows) {
+        if (!bytes) return;
+        r.src[n] = src;
+        r.dst[n] = ws;
+        r.row[n] = row;
+        r.rows[n] = rows;
+        n++;
+        most = std::max(most, rows);
+        src = ws;
+        row = ceil_div(p.k, 8) * 8;
+        ws += bytes;
+    };
+    add(p.x, p.x_row, copies.x, x_rows);
+    add(p.wg, p.wg_row, copies.wg, w_rows);
+    add(p.wu, p.wu_row, copies.wu, w_rows);
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(most * r.pieces.d, kThreads), 148 * 16);
+    repack<T><<<dim3(blocks, n), kThreads, 0, st>>>(r);
 }
 
 struct GatedLayout { size_t dg = 0, du = 0, sums = 0, dw = 0, copies = 0, bytes = 0; int64_t pre_row = 0; int splits = 1; int64_t split_rows = 0; };
@@ -434,10 +494,7 @@ STG_API stg_status stg_gated(stg_engine* e, const stg_gated_config* c, const voi
         with_dtype(c->dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
             if (on_tensor_cores(*c, copies, p)) {
-                char* ws = static_cast<char*>(d_ws);
-                copy_operand<T>(p.x, p.x_row, copies.x, p.m, p.k, ws, st);
-                copy_operand<T>(p.wg, p.wg_row, copies.wg, p.n, p.k, ws, st);
-                copy_operand<T>(p.wu, p.wu_row, copies.wu, p.n, p.k, ws, st);
+                copy_operands<T>(p, copies, p.m, p.n, static_cast<char*>(d_ws), st);
                 return launch_gated_mma(GATED_FWD, c->dtype == STG_BF16, p, 0, e->sms, st);
             }
             gated_simt<T, GATED_FWD><<<tile_grid(ceil_div(p.m, kGatedTileM) * ceil_div(p.n, kGatedTileN)), kThreads, 0, st>>>(p);
@@ -485,39 +542,31 @@ STG_API stg_status stg_gated_backward(stg_engine* e, const stg_gated_config* c, 
         p.splits = lay.splits;
         p.split_rows = lay.split_rows;
         const int64_t mt = ceil_div(p.m, kGatedTileM);
-        auto join_dw = [&](auto* tag) {
+        auto join = [&](auto* tag, int64_t sums) {   // the partial sums of dW and of the biases' gradients
             using T = std::remove_pointer_t<decltype(tag)>;
-            const int64_t blocks = std::min<int64_t>(ceil_div(2 * (int64_t)p.n * p.k, kThreads), 148 * 8);
-            dw_join<T><<<(unsigned)blocks, kThreads, 0, st>>>(p.dw_part, p.splits, p.n, p.k, static_cast<T*>(d_dwg), c->dwg_row,
-                                                              static_cast<T*>(d_dwu), c->dwu_row);
+            const bool dw = d_dwg || d_dwu;
+            if (!dw && !p.col_sums) return;
+            const unsigned sum_blocks = p.col_sums ? (unsigned)ceil_div(2 * (int64_t)p.n, 32) : 0;
+            const unsigned dw_blocks = dw ? (unsigned)std::min<int64_t>(ceil_div(2 * (int64_t)p.n * p.k, 4 * kThreads), 148 * 8) : 0;
+            join_parts<T><<<sum_blocks + dw_blocks, kThreads, 0, st>>>(p, sums, sum_blocks, static_cast<T*>(d_dwg), c->dwg_row, static_cast<T*>(d_dwu),
+                                                                       c->dwu_row, static_cast<T*>(d_dbg), static_cast<T*>(d_dbu));
         };
         with_dtype(c->dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
             const Copies copies = copies_of(*c);
             if (on_tensor_cores(*c, copies, p)) {
-                char* cw = ws + lay.copies;
-                copy_operand<T>(p.x, p.x_row, copies.x, p.m, p.k, cw, st);
-                copy_operand<T>(p.wg, p.wg_row, copies.wg, p.n, p.k, cw, st);
-                copy_operand<T>(p.wu, p.wu_row, copies.wu, p.n, p.k, cw, st);
+                copy_operands<T>(p, copies, p.m, p.n, ws + lay.copies, st);
                 auto product = [&](GatedMode mode) { launch_gated_mma(mode, c->dtype == STG_BF16, p, 0, e->sms, st); };
                 product(GATED_PRE);
                 if (d_dx) product(GATED_DX);
-                if (d_dwg || d_dwu || p.col_sums) {
-                    product(GATED_DW);
-                    if (p.col_sums)
-                        db_join<T><<<(unsigned)ceil_div(2 * (int64_t)p.n, 4), 128, 0, st>>>(p.col_sums, gated_col_sums(p, e->sms), p.n, static_cast<T*>(d_dbg), static_cast<T*>(d_dbu));
-                    if (d_dwg || d_dwu) join_dw((T*)nullptr);
-                }
+                if (d_dwg || d_dwu || p.col_sums) product(GATED_DW);
+                join((T*)nullptr, gated_col_sums(p, e->sms));
                 return;
             }
             gated_simt<T, GATED_PRE><<<tile_grid(mt * ceil_div(p.n, kGatedTileN)), kThreads, 0, st>>>(p);
-            if (p.col_sums)
-                db_join<T><<<(unsigned)ceil_div(2 * (int64_t)p.n, 4), 128, 0, st>>>(p.col_sums, mt, p.n, static_cast<T*>(d_dbg), static_cast<T*>(d_dbu));
             if (d_dx) gated_simt<T, GATED_DX><<<tile_grid(mt * ceil_div(p.k, 128)), kThreads, 0, st>>>(p);
-            if (d_dwg || d_dwu) {
-                gated_simt<T, GATED_DW><<<tile_grid(ceil_div(p.n, 128) * ceil_div(p.k, 128), 2 * p.splits), kThreads, 0, st>>>(p);
-                join_dw((T*)nullptr);
-            }
+            if (d_dwg || d_dwu) gated_simt<T, GATED_DW><<<tile_grid(ceil_div(p.n, 128) * ceil_div(p.k, 128), 2 * p.splits), kThreads, 0, st>>>(p);
+            join((T*)nullptr, mt);
         });
         cuda_check(cudaGetLastError(), "gated kernel");
     });
@@ -598,10 +647,8 @@ STG_API stg_status stg_mask_head(stg_plan* plan, const stg_mask_head_config* c, 
         with_dtype(c->dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
             if (c->dtype != STG_F32 && rows <= INT32_MAX && (copies.x || aligned(d_hidden, 16)) && (copies.wg || aligned(d_weight, 16))) {
-                char* ws = static_cast<char*>(d_ws);
                 p.x_row = p.wg_row = p.k;
-                copy_operand<T>(p.x, p.x_row, copies.x, rows, p.k, ws, st);
-                copy_operand<T>(p.wg, p.wg_row, copies.wg, p.stems * 2 * p.band_cols, p.k, ws, st);
+                copy_operands<T>(p, copies, rows, p.stems * 2 * p.band_cols, static_cast<char*>(d_ws), st);
                 p.tiles += plan->head_tiles;
                 p.n_tiles = plan->head_wide;
                 return launch_gated_mma(GATED_HEAD, c->dtype == STG_BF16, p, rows, plan->engine->sms, st);

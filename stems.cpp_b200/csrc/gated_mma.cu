@@ -122,11 +122,6 @@ __device__ __forceinline__ void tmem_load16(uint32_t (&v)[16], uint32_t addr) {
           "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(addr));
 }
-__device__ __forceinline__ uint32_t tmem_load1(uint32_t addr) {
-    uint32_t v;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(addr));
-    return v;
-}
 __device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
@@ -255,12 +250,12 @@ template <int MODE> __device__ __forceinline__ Tile tile_at(const MmaParams& p, 
     return r;
 }
 
-// Per epilogue warp: 32 rows x 32 columns of output, for dg and du each (float in the mask head,
-// rows 33 apart), and 64 floats of each bias.
+// Per epilogue warp: 32 rows x 32 columns of output, for dg and du each (in the mask head 16 columns of
+// float, rows 17 apart), and 64 floats of each bias.
 template <int MODE> __host__ __device__ constexpr int out_bytes() {
-    return MODE == GATED_PRE ? 4096 : MODE == GATED_HEAD ? 32 * 33 * 4 : MODE == GATED_DW ? 0 : 2048;
+    return MODE == GATED_PRE ? 4096 : MODE == GATED_HEAD ? 32 * 17 * 4 : MODE == GATED_DW ? 0 : 2048;
 }
-template <int MODE> __host__ __device__ constexpr int stages() { return MODE == GATED_HEAD || MODE == GATED_PRE ? 4 : 5; }
+template <int MODE> __host__ __device__ constexpr int stages() { return MODE == GATED_PRE ? 4 : 5; }
 // dW: a tile of ones, 16 columns
 template <int MODE> __host__ __device__ constexpr int ones_bytes() { return MODE == GATED_DW ? 64 * kDepth * 2 : 0; }
 template <int MODE> constexpr size_t smem_bytes() {
@@ -380,7 +375,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_m
                 const uint64_t a = a0 + (uint32_t)(s * (kStageBytes >> 4)), b = b0 + (uint32_t)(s * (kStageBytes >> 4));
                 const uint32_t d = MODE == GATED_HEAD ? d0 + (k & 1) * kAccCols : d0;
                 const bool add = k > (MODE == GATED_HEAD ? 1 : 0);
-                // the sums dg^T 1 of a slice, shared between the column tiles, which read the same dg
+                // The sums dg^T 1 of a slice, shared between the column tiles, which read the same dg. (Adding
+                // across lanes in GATED_PRE's epilogue, or there by mma.sync, took 12 and 16 us more at 24030 x
+                // 1408; here it is 8.)
                 const bool sum = MODE == GATED_DW && p.sums && (uint32_t)k % p.tiles_n.d == (uint32_t)q.tile_n;
                 if (one) {
 #pragma unroll
@@ -403,6 +400,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_m
         // eight the odd ones, so that the waits of one half run under the work of the other.
         constexpr int kHalves = MODE == GATED_FWD || MODE == GATED_PRE ? 2 : 1, kStep = 4 / kHalves;
         const int e = warp - 4, quad = warp & 3, group = (e >> 2) % kStep;
+        const bool store = MODE != GATED_DW && MODE != GATED_HEAD && p.store_by_tma;
+        // dy of the next 16 columns of this warp, on its way while the present ones are used; 0 past the sides
+        Pack<T, 8> dy[2], ahead[2];
+        auto ahead_of = [&](int64_t r, int j, Pack<T, 8> (&to)[2]) {
+            const T* from = static_cast<const T*>(g.dy) + r * g.y_row + j;
+            if (r < g.m && j + 16 <= g.n && (reinterpret_cast<uintptr_t>(from) & 15) == 0) {
+                to[0] = *reinterpret_cast<const Pack<T, 8>*>(from);
+                to[1] = *reinterpret_cast<const Pack<T, 8>*>(from + 8);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) to[i / 8].v[i % 8] = r < g.m && j + i < g.n ? from[i] : from_float<T>(0.0f);
+            }
+        };
+        if (MODE == GATED_PRE) {
+            const int first = pair + (e >> 3) * pairs;   // this warp's first tile
+            if (first < p.tiles) {
+                const Tile q = tile_at<MODE>(p, first);
+                ahead_of(q.m0 + rank * 128 + quad * 32 + lane, q.n0 + group * 32, ahead);
+            }
+        }
         uint8_t* stage = out_stage + e * out_bytes<MODE>();
         float* bias = bias_stage + e * 128;
         int n = 0;
@@ -441,135 +458,165 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_m
             fence_after();
             const uint32_t lanes = tmem + set * kAccCols + ((uint32_t)(quad * 32) << 16);
             if (MODE == GATED_DW && p.sums && group == 3) {
-                const uint32_t sum = tmem_load1(lanes + kSumCol);
+                uint32_t sum;
+                asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(sum) : "r"(lanes + kSumCol));
                 tmem_wait();
                 // a column tile past the slices has summed none
-                if (row < g.n) g.col_sums[((int64_t)((q.part >> 1) * (int)p.tiles_n.d + q.tile_n) * 2 + (q.part & 1)) * g.n + row] = q.tile_n < q.kb ? __uint_as_float(sum) : 0.0f;
+                if (row < g.n)
+                    g.col_sums[((int64_t)((q.part >> 1) * (int)p.tiles_n.d + q.tile_n) * 2 + (q.part & 1)) * g.n + row] = q.tile_n < q.kb ? __uint_as_float(sum) : 0.0f;
             }
-            for (int c = group; c < pieces; c += kStep) {
-                const float* pb = bias + (c - group) / kStep * 64;
-                const int j0 = q.n0 + c * 32;
-                const bool store = MODE != GATED_DW && MODE != GATED_HEAD && p.store_by_tma;
+            // 16 columns of a piece, bias added, through the epilogue to the stage or to memory
+            auto half = [&](uint32_t (&v)[16], uint32_t (&w)[16], int c, int hh) {
+                const int lc = hh * 16, j = q.n0 + c * 32 + lc;
+                if (MODE == GATED_DW) {
+                    if (row < g.n) {
+                        float* o = g.dw_part + ((int64_t)q.part * g.n + row) * g.k + j;
+                        if ((g.k & 3) == 0 && j + 16 <= g.k) {
 #pragma unroll
-                for (int hh = 0; hh < 2; hh++) {   // 16 columns at a time, to stay within the registers
-                    const int j = j0 + hh * 16, lc = hh * 16;
-                    uint32_t v[16], w[16];
-                    tmem_load16(v, lanes + c * 32 + lc);
-                    if (DUAL) tmem_load16(w, lanes + width + c * 32 + lc);
-                    tmem_wait();
-                    if (MODE == GATED_HEAD && q.kb > 1) {   // the other partial sum
-                        uint32_t x[16];
-                        tmem_load16(x, lanes + kAccCols + c * 32 + lc);
-                        tmem_wait();
-#pragma unroll
-                        for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(x[i]));
-                        tmem_load16(x, lanes + kAccCols + width + c * 32 + lc);
-                        tmem_wait();
-#pragma unroll
-                        for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__uint_as_float(w[i]) + __uint_as_float(x[i]));
-                    }
-                    if (hh == 1 && c + kStep >= pieces) {   // all in registers: the next products may have the set
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) bar_arrive_cluster(in_leader(acc_empty + set));
-                    }
-                    if (MODE == GATED_DW) {
-                        if (row < g.n) {
-                            float* o = g.dw_part + ((int64_t)q.part * g.n + row) * g.k + j;
-                            if ((g.k & 3) == 0 && j + 16 <= g.k) {
-#pragma unroll
-                                for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(o + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 16; i++)
-                                    if (j + i < g.k) o[i] = __uint_as_float(v[i]);
-                            }
-                        }
-                        continue;
-                    }
-                    if (DUAL) {
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            const float4 x = *reinterpret_cast<const float4*>(pb + lc + i), y = *reinterpret_cast<const float4*>(pb + 32 + lc + i);
-                            add2(v[i], v[i + 1], x.x, x.y);
-                            add2(v[i + 2], v[i + 3], x.z, x.w);
-                            add2(w[i], w[i + 1], y.x, y.y);
-                            add2(w[i + 2], w[i + 3], y.z, y.w);
-                        }
-                    }
-                    if (MODE == GATED_HEAD) {
-                        float* sm = reinterpret_cast<float*>(stage) + lane * 33 + lc;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) sm[i] = __uint_as_float(v[i]) * fast_sigmoid(__uint_as_float(w[i]));
-                        continue;
-                    }
-                    uint32_t o[8], o2[8];
-                    if (MODE == GATED_FWD) {
-#pragma unroll
-                        for (int i = 0; i < 16; i += 2)
-                            o[i / 2] = pack2<T>(act<ACT>(__uint_as_float(v[i])) * __uint_as_float(w[i]),
-                                                act<ACT>(__uint_as_float(v[i + 1])) * __uint_as_float(w[i + 1]));
-                    } else if (MODE == GATED_PRE) {
-                        const T* dy = static_cast<const T*>(g.dy) + row * g.y_row + j;
-                        Pack<T, 8> d[2];
-                        if (row < g.m && j + 16 <= g.n && (reinterpret_cast<uintptr_t>(dy) & 15) == 0) {
-                            d[0] = *reinterpret_cast<const Pack<T, 8>*>(dy);
-                            d[1] = *reinterpret_cast<const Pack<T, 8>*>(dy + 8);
+                            for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(o + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) d[i / 8].v[i % 8] = row < g.m && j + i < g.n ? dy[i] : from_float<T>(0.0f);
+                            for (int i = 0; i < 16; i++)
+                                if (j + i < g.k) o[i] = __uint_as_float(v[i]);
                         }
-#pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            float dg[2], du[2];
-#pragma unroll
-                            for (int k = 0; k < 2; k++) {
-                                const float x = to_float(d[(i + k) / 8].v[(i + k) % 8]);
-                                float a, s;
-                                act_both<ACT>(__uint_as_float(v[i + k]), a, s);
-                                dg[k] = x * __uint_as_float(w[i + k]) * s;
-                                du[k] = x * a;
-                            }
-                            o[i / 2] = pack2<T>(dg[0], dg[1]);
-                            o2[i / 2] = pack2<T>(du[0], du[1]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) o[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
                     }
-                    if (store) {
-                        if (hh == 0) {   // the stage's last store has read it
-                            if (lane == 0) stores_read();
-                            __syncwarp();
-                        }
-                        // rows of 64 bytes as the 64-byte swizzle has them: 16-byte piece c of row r at c ^ (r / 2 & 3)
+                    return;
+                }
+                if (DUAL) {
+                    const float* pb = bias + (c - group) / kStep * 64 + lc;
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const int to = lane * 64 + (((2 * hh + i) ^ ((lane >> 1) & 3)) << 4);
-                            *reinterpret_cast<uint4*>(stage + to) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                            if (MODE == GATED_PRE)
-                                *reinterpret_cast<uint4*>(stage + 2048 + to) = make_uint4(o2[4 * i], o2[4 * i + 1], o2[4 * i + 2], o2[4 * i + 3]);
-                        }
-                    } else if (MODE != GATED_PRE && row < g.m) {
-                        T* out = static_cast<T*>(MODE == GATED_FWD ? g.y : g.dx);
-                        const int64_t pitch = MODE == GATED_FWD ? g.y_row : g.dx_row;
-                        const int nj = MODE == GATED_DX ? g.k : g.n;
-#pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            if (j + i < nj) out[row * pitch + j + i] = reinterpret_cast<const T*>(&o[i / 2])[i & 1];
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(pb + i), y = *reinterpret_cast<const float4*>(pb + 32 + i);
+                        add2(v[i], v[i + 1], x.x, x.y);
+                        add2(v[i + 2], v[i + 3], x.z, x.w);
+                        add2(w[i], w[i + 1], y.x, y.y);
+                        add2(w[i + 2], w[i + 3], y.z, y.w);
                     }
                 }
                 if (MODE == GATED_HEAD) {
+                    // through shared memory, so that a row's 16 floats are stored side by side
+                    float* sm = reinterpret_cast<float*>(stage);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) sm[lane * 17 + i] = __uint_as_float(v[i]) * fast_sigmoid(__uint_as_float(w[i]));
                     __syncwarp();
-                    const int rows = (int)max((int64_t)0, min((int64_t)32, g.frames - row0));
-                    const float* sm = reinterpret_cast<const float*>(stage) + lane;
-                    float* o = g.masks + (q.cs * g.band_cols + q.h.off) * g.frames + row0 * q.h.din + j0 + lane;
-                    if (j0 + lane < q.h.din) {
+                    const int rows = (int)max((int64_t)0, min((int64_t)32, g.frames - row0)), col = j + (lane & 15);
+                    float* o = g.masks + (q.cs * g.band_cols + q.h.off) * g.frames + row0 * q.h.din + col;
+                    if (col < q.h.din) {
 #pragma unroll 8
-                        for (int r = 0; r < rows; r++) o[(int64_t)r * q.h.din] = sm[r * 33];
+                        for (int r = lane >> 4; r < rows; r += 2) o[(int64_t)r * q.h.din] = sm[r * 17 + (lane & 15)];
                     }
                     __syncwarp();
+                    return;
                 }
+                uint32_t o[8], o2[8];
+                if (MODE == GATED_FWD) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2)
+                        o[i / 2] = pack2<T>(act<ACT>(__uint_as_float(v[i])) * __uint_as_float(w[i]),
+                                            act<ACT>(__uint_as_float(v[i + 1])) * __uint_as_float(w[i + 1]));
+                } else if (MODE == GATED_PRE) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        float dg[2], du[2];
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const float x = to_float(dy[(i + k) / 8].v[(i + k) % 8]);
+                            float a, s;
+                            act_both<ACT>(__uint_as_float(v[i + k]), a, s);
+                            dg[k] = x * __uint_as_float(w[i + k]) * s;
+                            du[k] = x * a;
+                        }
+                        o[i / 2] = pack2<T>(dg[0], dg[1]);
+                        o2[i / 2] = pack2<T>(du[0], du[1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) o[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                }
+                if (store) {
+                    if (hh == 0) {   // the stage's last store has read it
+                        if (lane == 0) stores_read();
+                        __syncwarp();
+                    }
+                    // rows of 64 bytes as the 64-byte swizzle has them: 16-byte piece c of row r at c ^ (r / 2 & 3)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const int to = lane * 64 + (((2 * hh + i) ^ ((lane >> 1) & 3)) << 4);
+                        *reinterpret_cast<uint4*>(stage + to) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        if (MODE == GATED_PRE)
+                            *reinterpret_cast<uint4*>(stage + 2048 + to) = make_uint4(o2[4 * i], o2[4 * i + 1], o2[4 * i + 2], o2[4 * i + 3]);
+                    }
+                } else if (MODE != GATED_PRE && row < g.m) {
+                    T* out = static_cast<T*>(MODE == GATED_FWD ? g.y : g.dx);
+                    const int64_t pitch = MODE == GATED_FWD ? g.y_row : g.dx_row;
+                    const int nj = MODE == GATED_DX ? g.k : g.n;
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (j + i < nj) out[row * pitch + j + i] = reinterpret_cast<const T*>(&o[i / 2])[i & 1];
+                }
+            };
+            auto load = [&](uint32_t (&v)[16], uint32_t (&w)[16], int c, int hh) {
+                tmem_load16(v, lanes + c * 32 + hh * 16);
+                if (DUAL) tmem_load16(w, lanes + width + c * 32 + hh * 16);
+            };
+            auto loaded = [&](uint32_t (&v)[16], uint32_t (&w)[16], int c, int hh) {
+                tmem_wait();
+                if (MODE == GATED_HEAD && q.kb > 1) {   // the other partial sum
+                    uint32_t x[16];
+#pragma unroll
+                    for (int which = 0; which < 2; which++) {
+                        tmem_load16(x, lanes + kAccCols + which * width + c * 32 + hh * 16);
+                        tmem_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            uint32_t& y = which ? w[i] : v[i];
+                            y = __float_as_uint(__uint_as_float(y) + __uint_as_float(x[i]));
+                        }
+                    }
+                }
+            };
+            // The next 16 columns are on their way from TMEM while these go through the epilogue. (Not in
+            // GATED_PRE, which has dy ahead instead: both together spill.)
+            constexpr bool kAhead = MODE != GATED_PRE;
+            uint32_t v0[16], w0[16], v1[16], w1[16];
+            if (kAhead && group < pieces) {
+                load(v0, w0, group, 0);
+                loaded(v0, w0, group, 0);
+            }
+            for (int c = group; c < pieces; c += kStep) {
+                const int j0 = q.n0 + c * 32;
+                const bool last = c + kStep >= pieces;
+                if (kAhead) load(v1, w1, c, 1);
+                else {
+                    load(v0, w0, c, 0);
+                    loaded(v0, w0, c, 0);
+                }
+                if (MODE == GATED_PRE) {
+                    dy[0] = ahead[0];
+                    dy[1] = ahead[1];
+                    ahead_of(row, j0 + 16, ahead);
+                }
+                half(v0, w0, c, 0);
+                if (!kAhead) load(v1, w1, c, 1);
+                loaded(v1, w1, c, 1);
+                if (!last) {
+                    if (kAhead) load(v0, w0, c + kStep, 0);
+                } else {   // all in registers: the next products may have the set
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive_cluster(in_leader(acc_empty + set));
+                }
+                if (MODE == GATED_PRE) {
+                    dy[0] = ahead[0];
+                    dy[1] = ahead[1];
+                    if (!last) ahead_of(row, j0 + kStep * 32, ahead);
+                    else if (t + 2 * pairs < p.tiles) {   // of this warp's next tile
+                        const Tile nq = tile_at<MODE>(p, t + 2 * pairs);
+                        ahead_of(nq.m0 + rank * 128 + quad * 32 + lane, nq.n0 + group * 32, ahead);
+                    }
+                }
+                half(v1, w1, c, 1);
+                if (kAhead && !last) loaded(v0, w0, c + kStep, 0);
                 if (store) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
@@ -580,7 +627,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_m
                     }
                 }
             }
-            if (group >= pieces) {   // no piece of this tile (or only the sums)
+            if (group >= pieces) {   // no piece of this tile
                 fence_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive_cluster(in_leader(acc_empty + set));
@@ -690,8 +737,8 @@ void launch_gated_mma(GatedMode mode, bool bf16, const GatedParams& g, int64_t h
             encode(&p.c[1], bf16, g.du, g.m, g.n, g.pre_row, 32, 32, true);
         }
     } else {
-        p.sums = mode == GATED_DW && g.col_sums;
         const int64_t rest = mode == GATED_DX ? mt : 2 * g.splits * ceil_div(g.n, kPairM);
+        p.sums = mode == GATED_DW && g.col_sums;
         p.cols = column_tile(g.k, rest, pairs, p.sums);
         tiles_n = ceil_div(g.k, p.cols);
         rest_n = ceil_div(g.n, kPairM);
