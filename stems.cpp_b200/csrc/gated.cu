@@ -15,24 +15,13 @@ constexpr int kThreads = 256;
 constexpr int kTileK = 16;
 constexpr int kPitch = 132;        // floats between two k rows of a tile
 
-__device__ __forceinline__ float sigmoid_exact(float z) { return 1.0f / (1.0f + expf(-z)); }
-
-__device__ __forceinline__ float gate_act(int a, float z) {
-    switch (a) {
-        case STG_ACT_RELU: return z < 0.0f ? 0.0f : z;
-        case STG_ACT_SILU: return z * sigmoid_exact(z);
-        case STG_ACT_GELU: return 0.5f * z * erfcf(-z * 0.70710678118654752f);
-        case STG_ACT_SIGMOID: return sigmoid_exact(z);
-        default: return z;
-    }
-}
-__device__ __forceinline__ float gate_grad(int a, float z) {
-    switch (a) {
-        case STG_ACT_RELU: return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
-        case STG_ACT_SILU: { const float s = sigmoid_exact(z); return s * fmaf(z, 1.0f - s, 1.0f); }
-        case STG_ACT_GELU: return fmaf(0.3989422804014327f * z, expf(-0.5f * z * z), 0.5f * erfcf(-z * 0.70710678118654752f));
-        case STG_ACT_SIGMOID: { const float s = sigmoid_exact(z); return s * (1.0f - s); }
-        default: return 1.0f;
+__device__ __forceinline__ void gate_both(int kind, float z, float& a, float& d) {
+    switch (kind) {
+        case STG_ACT_RELU: return act_both<STG_ACT_RELU, false>(z, a, d);
+        case STG_ACT_SILU: return act_both<STG_ACT_SILU, false>(z, a, d);
+        case STG_ACT_GELU: return act_both<STG_ACT_GELU, false>(z, a, d);
+        case STG_ACT_SIGMOID: return act_both<STG_ACT_SIGMOID, false>(z, a, d);
+        default: return act_both<STG_ACT_NONE, false>(z, a, d);
     }
 }
 
@@ -236,13 +225,15 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
                 const int c = n0 + 4 * tx + j;
                 if (c >= nj) continue;
                 const float g = v[i][j] + bg[j], u = v[i][4 + j] + bu[j];
+                float a, d;
+                if (MODE != GATED_HEAD) gate_both(p.act, g, a, d);
                 if (MODE == GATED_FWD) {
-                    static_cast<T*>(p.y)[r * p.y_row + c] = from_float<T>(gate_act(p.act, g) * u);
+                    static_cast<T*>(p.y)[r * p.y_row + c] = from_float<T>(a * u);
                 } else if (MODE == GATED_HEAD) {   // value rows come first: g is the value, u its gate
-                    p.masks[(head_row * p.band_cols + ht.off) * p.frames + r * ht.din + c] = g * sigmoid_exact(u);
+                    p.masks[(head_row * p.band_cols + ht.off) * p.frames + r * ht.din + c] = g * sigmoid<false>(u);
                 } else {
                     const float dy = to_float(static_cast<const T*>(p.dy)[r * p.y_row + c]);
-                    const float dg = dy * u * gate_grad(p.act, g), du = dy * gate_act(p.act, g);
+                    const float dg = dy * u * d, du = dy * a;
                     static_cast<T*>(p.dg)[r * p.pre_row + c] = from_float<T>(dg);
                     static_cast<T*>(p.du)[r * p.pre_row + c] = from_float<T>(du);
                     sg[j] += dg;

@@ -154,44 +154,10 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// ---- activations: results are rounded to 16 bits, so the approximate exponential and reciprocal
-// (2^-22 relative each) do. ----------------------------------------------------------------------------
-__device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-__device__ __forceinline__ float rcp(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-// 1 / (1 + 2^(-z log2 e)); 0 where the power is infinite.
-__device__ __forceinline__ float fast_sigmoid(float z) { return rcp(1.0f + ex2(-1.4426950408889634f * z)); }
-
 // a += x, b += y in one packed instruction.
 __device__ __forceinline__ void add2(uint32_t& a, uint32_t& b, float x, float y) {
     asm("{\n.reg .b64 u, v;\nmov.b64 u, {%0, %1};\nmov.b64 v, {%2, %3};\nadd.rn.f32x2 u, u, v;\nmov.b64 {%0, %1}, u;\n}"
         : "+r"(a), "+r"(b) : "f"(x), "f"(y));
-}
-
-// act(z) and its derivative.
-template <int ACT> __device__ __forceinline__ void act_both(float z, float& a, float& d) {
-    if (ACT == STG_ACT_RELU) {
-        a = z < 0.0f ? 0.0f : z;
-        d = z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
-    } else if (ACT == STG_ACT_SILU) {
-        const float s = fast_sigmoid(z);
-        a = z * s;
-        d = fmaf(a, 1.0f - s, s);
-    } else if (ACT == STG_ACT_GELU) {
-        const float h = 0.5f * erfcf(-z * 0.70710678118654752f);
-        a = z * h;
-        d = fmaf(0.3989422804014327f * z, __expf(-0.5f * z * z), h);
-    } else if (ACT == STG_ACT_SIGMOID) {
-        a = fast_sigmoid(z);
-        d = a * (1.0f - a);
-    } else {
-        a = z;
-        d = 1.0f;
-    }
-}
-template <int ACT> __device__ __forceinline__ float act(float z) {
-    float a, d;
-    act_both<ACT>(z, a, d);
-    return a;
 }
 
 // Where a pair's tile lies.
@@ -497,7 +463,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_m
                     // through shared memory, so that a row's 16 floats are stored side by side
                     float* sm = reinterpret_cast<float*>(stage);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) sm[lane * 17 + i] = __uint_as_float(v[i]) * fast_sigmoid(__uint_as_float(w[i]));
+                    for (int i = 0; i < 16; i++) sm[lane * 17 + i] = __uint_as_float(v[i]) * sigmoid<true>(__uint_as_float(w[i]));
                     __syncwarp();
                     const int rows = (int)max((int64_t)0, min((int64_t)32, g.frames - row0)), col = j + (lane & 15);
                     float* o = g.masks + (q.cs * g.band_cols + q.h.off) * g.frames + row0 * q.h.din + col;
@@ -512,8 +478,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_m
                 if (MODE == GATED_FWD) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 2)
-                        o[i / 2] = pack2<T>(act<ACT>(__uint_as_float(v[i])) * __uint_as_float(w[i]),
-                                            act<ACT>(__uint_as_float(v[i + 1])) * __uint_as_float(w[i + 1]));
+                        o[i / 2] = pack2<T>(act<ACT, true>(__uint_as_float(v[i])) * __uint_as_float(w[i]),
+                                            act<ACT, true>(__uint_as_float(v[i + 1])) * __uint_as_float(w[i + 1]));
                 } else if (MODE == GATED_PRE) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
@@ -522,7 +488,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_m
                         for (int k = 0; k < 2; k++) {
                             const float x = to_float(dy[(i + k) / 8].v[(i + k) % 8]);
                             float a, s;
-                            act_both<ACT>(__uint_as_float(v[i + k]), a, s);
+                            act_both<ACT, true>(__uint_as_float(v[i + k]), a, s);
                             dg[k] = x * __uint_as_float(w[i + k]) * s;
                             du[k] = x * a;
                         }

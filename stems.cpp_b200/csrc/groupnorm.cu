@@ -8,11 +8,23 @@
 //   dbeta = sum dz,  dgamma = sum dz xh  (over items and positions),
 //   dx = rstd (d - sum(d) / m - xh sum(d xh) / m),  d = gamma dz.
 //
-// Three kernels each way. A block of the first takes a range of positions with all channels:
-// its threads stand side by side along the channels (16-byte vectors, whole rows, so every
-// sector is used whatever the group size) and step down the positions, each with sums of its
-// own channels. The second joins the blocks' parts in a fixed order. The third reads x again.
+// The floor is one read of x (and dy) and one write, so what a block has read for the statistics
+// it keeps in shared memory for the second look, and one launch does both: the positions of
+// an item are dealt to a set of blocks, each takes the moments of its share, the set meets, joins
+// the moments in a fixed order and applies them.
+//   - An item that fits the shared memory of up to eight blocks is a cluster's, which
+//     meets in hardware and reads each other's moments there; items do not wait for each other.
+//   - Larger items take all SMs (as many items at a time as fit the GPU's shared memory, at
+//     least one) in a cooperative launch; what does not fit is read again, from L2 where it can be.
+//   - Very many groups or channels, whose moments would themselves be much to exchange, take
+//     three launches: moments, their joining, a second reading.
+// A block's threads stand side by side along the channels (16-byte vectors, whole rows, so every
+// sector is used whatever the group size) and step down the positions.
 #include "layers.h"
+
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
 
 namespace stg {
 
@@ -30,34 +42,15 @@ struct NormParams {
     int64_t positions, xb, xp, yb, yp, db, dp;
     int channels, groups, cpg;       // cpg: channels of a group
     int batch, chunks, rows;         // chunks per item, positions of a chunk (the last may have fewer)
+    int used;                        // chunks of an item that have a position: fewer only in a cluster
     int columns;                     // vectors of a row
     FastDiv columns_div;             // by min(columns, kThreads)
     float eps;
     int param_float;
+    // one-launch kernels: items at a time, steps a thread keeps, blocks of an item (= chunks)
+    int at_once, kept;
+    int mono;                        // a vector's channels are of one group
 };
-
-// ---- activations: float for f32 with CUDA's accurate functions, the fast ones (about 2^-21
-// relative) where the result is rounded to 16 bits anyway -----------------------------------------
-template <bool kFast> __device__ __forceinline__ float sigmoid(float z) {
-    return kFast ? sigmoidf(z) : 1.0f / (1.0f + expf(-z));
-}
-template <int ACT, bool kFast> __device__ __forceinline__ float act(float z) {
-    if (ACT == STG_ACT_RELU) return z < 0.0f ? 0.0f : z;   // keeps NaN
-    if (ACT == STG_ACT_SILU) return z * sigmoid<kFast>(z);
-    if (ACT == STG_ACT_GELU) return 0.5f * z * erfcf(-z * 0.70710678118654752f);
-    if (ACT == STG_ACT_SIGMOID) return sigmoid<kFast>(z);
-    return z;
-}
-template <int ACT, bool kFast> __device__ __forceinline__ float act_grad(float z) {
-    if (ACT == STG_ACT_RELU) return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
-    if (ACT == STG_ACT_SILU) { const float s = sigmoid<kFast>(z); return s * fmaf(z, 1.0f - s, 1.0f); }
-    if (ACT == STG_ACT_GELU) {
-        const float e = kFast ? __expf(-0.5f * z * z) : expf(-0.5f * z * z);
-        return fmaf(0.3989422804014327f * z, e, 0.5f * erfcf(-z * 0.70710678118654752f));
-    }
-    if (ACT == STG_ACT_SIGMOID) { const float s = sigmoid<kFast>(z); return s * (1.0f - s); }
-    return 1.0f;
-}
 
 // Mean and sum of squared deviations of n values, joined pairwise (Chan, Golub, LeVeque 1979).
 struct Moments { float n, mean, m2; };
@@ -282,7 +275,7 @@ __global__ void __launch_bounds__(128) grad_join(const __grid_constant__ NormPar
     float db = 0.0f, dg = 0.0f;
     for (int b = 0; b < p.batch; b++) {
         float s1 = 0.0f, s2 = 0.0f;
-        for (int k = lane; k < p.chunks; k += 32) {
+        for (int k = lane; k < p.used; k += 32) {
             const float2 v = p.part[((int64_t)b * p.chunks + k) * p.channels + c];
             s1 += v.x;
             s2 += v.y;
@@ -291,7 +284,7 @@ __global__ void __launch_bounds__(128) grad_join(const __grid_constant__ NormPar
             s1 += __shfl_xor_sync(~0u, s1, o);
             s2 += __shfl_xor_sync(~0u, s2, o);
         }
-        if (lane == 0) p.sums[(int64_t)b * p.channels + c] = make_float2(s1, s2);
+        if (lane == 0 && p.sums) p.sums[(int64_t)b * p.channels + c] = make_float2(s1, s2);
         db += s1;
         dg += s2;
     }
@@ -360,6 +353,402 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(const __grid_const
     }
 }
 
+// ---- one launch -------------------------------------------------------------------------------
+
+constexpr int kFused = 512;          // threads
+constexpr int kFusedGroups = 2048;   // most groups
+constexpr int kClusterMost = 8;
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// The 8 bytes at the same place in another block of the cluster.
+__device__ __forceinline__ float2 peer_read(const float2* p, int rank) {
+    uint32_t a;
+    float2 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+    return v;
+}
+
+struct Share { int item, chunk, n; int64_t l0; };
+template <bool GRID> __device__ __forceinline__ Share share_of(const NormParams& p, int round) {
+    Share s;
+    const int slot = blockIdx.x / p.chunks;
+    s.chunk = blockIdx.x - slot * p.chunks;
+    s.item = GRID ? (slot < p.at_once ? round * p.at_once + slot : p.batch) : slot;
+    s.l0 = (int64_t)s.chunk * p.rows;
+    s.n = s.item < p.batch ? (int)min((int64_t)p.rows, p.positions - s.l0) : 0;
+    return s;
+}
+
+// Moments of the block's groups from its threads' parts: [step][width] of them, of `per` channels
+// each, mean and M2 of the rows that place r has. Several warps to a group when groups are few.
+__device__ __forceinline__ void block_moments(const NormParams& p, const Place& q, int n, const float2* part, int vec, float2* group, Moments* red) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kFused / 32;
+    const int per = p.mono ? vec : 1, row = p.channels / per, w = p.cpg / per;   // parts of a row, of a group in a row
+    const int rows = min(q.step, n), team = max(1, warps / p.groups);
+    for (int g0 = 0; g0 < p.groups; g0 += warps / team) {
+        const int g = g0 + warp / team, member = warp % team;
+        Moments m{0.0f, 0.0f, 0.0f};
+        if (g < p.groups && warp < warps / team * team) {
+            for (int i = member * 32 + lane; i < rows * w; i += team * 32) {
+                const int r = i / w, c = g * w + i - r * w;
+                const float2 v = part[r * row + c];
+                join(m, Moments{(float)((n - r + q.step - 1) / q.step) * (float)per, v.x, v.y});
+            }
+            warp_join(m);
+            if (team == 1) {
+                if (lane == 0) group[g] = make_float2(m.mean, m.m2);
+            } else if (lane == 0) red[warp] = m;
+        }
+        if (team > 1) {   // then every group has its team at once: one round
+            __syncthreads();
+            if (threadIdx.x < p.groups) {
+                Moments t = red[threadIdx.x * team];
+                for (int k = 1; k < team; k++) join(t, red[threadIdx.x * team + k]);
+                group[threadIdx.x] = make_float2(t.mean, t.m2);
+            }
+        }
+    }
+    __syncthreads();
+}
+
+template <class T, int V, int ACT, bool GRID>
+__global__ void __launch_bounds__(kFused, 1) norm_fused(const __grid_constant__ NormParams p) {
+    constexpr bool fast = sizeof(T) == 2;
+    constexpr int U = 8;                        // positions in flight per thread
+    using P = Pack<T, V>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    P* keep = reinterpret_cast<P*>(smem);       // [kept][threads]
+    float2* part = reinterpret_cast<float2*>(smem + (size_t)p.kept * kFused * sizeof(P));
+    float2* group = part + kFused * (p.mono ? 1 : V);   // [groups]: the block's moments
+    float2* stat = group + p.groups;                    // [groups]: the item's mean and rstd
+    __shared__ Moments red[kFused / 32];
+    Place q;
+    q.width = p.columns;
+    q.step = kFused / q.width;
+    q.r = (int)p.columns_div.div(threadIdx.x);
+    q.col = threadIdx.x - q.r * q.width;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ch = q.col * V;
+    const bool on = q.r < q.step;
+    const int rounds = GRID ? (p.batch + p.at_once - 1) / p.at_once : 1;
+    for (int round = 0; round < rounds; round++) {
+        const Share s = share_of<GRID>(p, round);
+        const T* x = static_cast<const T*>(p.x) + s.item * p.xb + s.l0 * p.xp + ch;
+        const int steps = s.n > 0 ? (s.n + q.step - 1) / q.step : 0;
+        if (s.n > 0) {
+            if (on && q.r < s.n) {
+                // differences from the first value met, so that a mean far from zero costs no digits
+                float pivot[V], a[V], b[V];
+                const P first = *reinterpret_cast<const P*>(x + (int64_t)q.r * p.xp);
+#pragma unroll
+                for (int j = 0; j < V; j++) { pivot[j] = to_float(first.v[p.mono ? 0 : j]); a[j] = b[j] = 0.0f; }
+                for (int it = 0; it < steps; it += U) {
+                    P v[U];
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const int l = q.r + (it + u) * q.step;
+                        if (l < s.n) v[u] = *reinterpret_cast<const P*>(x + (int64_t)l * p.xp);
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const int l = q.r + (it + u) * q.step;
+                        if (l >= s.n) break;
+                        if (it + u < p.kept) keep[(it + u) * kFused + threadIdx.x] = v[u];
+#pragma unroll
+                        for (int j = 0; j < V; j++) {
+                            const float d = to_float(v[u].v[j]) - pivot[j];
+                            a[j] += d;
+                            b[j] = fmaf(d, d, b[j]);
+                        }
+                    }
+                }
+                const float cnt = (float)((s.n - q.r + q.step - 1) / q.step);
+                auto moments = [&](float sum, float sq, float n, float at) {   // + 0 sum: a NaN stays one
+                    const float m = sum / n;
+                    return make_float2(at + m, fmaxf(fmaf(-sum, m, sq), 0.0f) + 0.0f * sum);
+                };
+                if (p.mono) {
+                    float sa = a[0], sb = b[0];
+#pragma unroll
+                    for (int j = 1; j < V; j++) { sa += a[j]; sb += b[j]; }
+                    part[q.r * q.width + q.col] = moments(sa, sb, cnt * V, pivot[0]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; j++) part[(q.r * q.width + q.col) * V + j] = moments(a[j], b[j], cnt, pivot[j]);
+                }
+            }
+            __syncthreads();
+            block_moments(p, q, s.n, part, V, group, red);
+            if (GRID)
+                for (int g = threadIdx.x; g < p.groups; g += kFused) p.part[((int64_t)s.item * p.groups + g) * p.chunks + s.chunk] = group[g];
+        }
+        __syncwarp();
+        if (GRID) cg::this_grid().sync();
+        else {
+            cluster_arrive();
+            cluster_wait();
+        }
+        if (s.n > 0) {
+            for (int g = warp; g < p.groups; g += kFused / 32) {
+                Moments m{0.0f, 0.0f, 0.0f};
+                for (int c = lane; c < p.used; c += 32) {
+                    const float n = (float)min((int64_t)p.rows, p.positions - (int64_t)c * p.rows) * (float)p.cpg;
+                    const float2 v = GRID ? __ldcg(p.part + ((int64_t)s.item * p.groups + g) * p.chunks + c) : peer_read(group + g, c);
+                    join(m, Moments{n, v.x, v.y});
+                }
+                warp_join(m);
+                if (lane == 0) {
+                    const float r = 1.0f / sqrtf(m.m2 / ((float)p.positions * (float)p.cpg) + p.eps);
+                    stat[g] = make_float2(m.mean, r);
+                    if (s.chunk == 0 && p.mean) {
+                        p.mean[(int64_t)s.item * p.groups + g] = m.mean;
+                        p.rstd[(int64_t)s.item * p.groups + g] = r;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (!GRID) cluster_arrive();   // waited for below: no block goes while others still read its moments
+        __syncthreads();
+        if (s.n > 0 && on) {
+            float mu[V], a[V], sh[V];
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const float2 st = stat[(ch + j) / p.cpg];
+                mu[j] = st.x;
+                a[j] = st.y * param(p.gamma, ch + j, p.param_float, 1.0f, (const T*)nullptr);
+                sh[j] = param(p.beta, ch + j, p.param_float, 0.0f, (const T*)nullptr);
+            }
+            T* y = static_cast<T*>(p.y) + s.item * p.yb + s.l0 * p.yp + ch;
+            auto one = [&](P v, int l) {
+#pragma unroll
+                for (int j = 0; j < V; j++) v.v[j] = from_float<T>(act<ACT, fast>(fmaf(to_float(v.v[j]) - mu[j], a[j], sh[j])));
+                *reinterpret_cast<P*>(y + (int64_t)l * p.yp) = v;
+            };
+            // what was read last and not kept is in L2 yet: from the end
+            int it = steps - 1;
+            constexpr int W = 4;
+            for (; it >= p.kept; it -= W) {
+                P v[W];
+#pragma unroll
+                for (int u = 0; u < W; u++) {
+                    const int l = q.r + (it - u) * q.step;
+                    if (it - u >= p.kept && l < s.n) v[u] = *reinterpret_cast<const P*>(x + (int64_t)l * p.xp);
+                }
+#pragma unroll
+                for (int u = 0; u < W; u++) {
+                    const int l = q.r + (it - u) * q.step;
+                    if (it - u >= p.kept && l < s.n) one(v[u], l);
+                }
+            }
+#pragma unroll 2
+            for (it = min(steps, p.kept) - 1; it >= 0; it--) {
+                const int l = q.r + it * q.step;
+                if (l < s.n) one(keep[it * kFused + threadIdx.x], l);
+            }
+        }
+        if (GRID) __syncthreads();   // stat and the kept values are the next round's
+        else {
+            __syncwarp();
+            cluster_wait();
+        }
+    }
+}
+
+// Backward: the block's sums of dz and dz xh per channel, of gamma times them per group; the set's
+// blocks meet over the group sums. Channel sums go out per block for dgamma and dbeta.
+template <class T, int V, int ACT, bool GRID>
+__global__ void __launch_bounds__(kFused, 1) norm_grad_fused(const __grid_constant__ NormParams p) {
+    constexpr bool fast = sizeof(T) == 2;
+    constexpr int U = 4;
+    using P = Pack<T, V>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    P* keep = reinterpret_cast<P*>(smem);       // [kept][x, dy][threads]
+    float2* part = reinterpret_cast<float2*>(smem + (size_t)p.kept * 2 * kFused * sizeof(P));   // [step][channels]
+    float2* chan = part + kFused * V;           // [channels]
+    float2* group = chan + p.channels;          // [groups]: the block's sums
+    float2* stat = group + p.groups;            // [groups]: the item's means of d and d xh
+    Place q;
+    q.width = p.columns;
+    q.step = kFused / q.width;
+    q.r = (int)p.columns_div.div(threadIdx.x);
+    q.col = threadIdx.x - q.r * q.width;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ch = q.col * V;
+    const bool on = q.r < q.step;
+    const int rounds = GRID ? (p.batch + p.at_once - 1) / p.at_once : 1;
+    float ga[V], be[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        ga[j] = on ? param(p.gamma, ch + j, p.param_float, 1.0f, (const T*)nullptr) : 0.0f;
+        be[j] = on ? param(p.beta, ch + j, p.param_float, 0.0f, (const T*)nullptr) : 0.0f;
+    }
+    for (int round = 0; round < rounds; round++) {
+        const Share s = share_of<GRID>(p, round);
+        const T* x = static_cast<const T*>(p.x) + s.item * p.xb + s.l0 * p.xp + ch;
+        const T* dy = static_cast<const T*>(p.dy) + s.item * p.yb + s.l0 * p.yp + ch;
+        const int steps = s.n > 0 ? (s.n + q.step - 1) / q.step : 0;
+        float mu[V], rs[V];
+        if (s.n > 0) {
+            if (on) {
+                float a[V], b[V];
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const int64_t g = (int64_t)s.item * p.groups + (ch + j) / p.cpg;
+                    mu[j] = p.mean[g];
+                    rs[j] = p.rstd[g];
+                    a[j] = b[j] = 0.0f;
+                }
+                for (int it = 0; it < steps; it += U) {
+                    P v[U], w[U];
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const int l = q.r + (it + u) * q.step;
+                        if (l < s.n) {
+                            v[u] = *reinterpret_cast<const P*>(x + (int64_t)l * p.xp);
+                            w[u] = *reinterpret_cast<const P*>(dy + (int64_t)l * p.yp);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const int l = q.r + (it + u) * q.step;
+                        if (l >= s.n) break;
+                        if (it + u < p.kept) {
+                            keep[(it + u) * 2 * kFused + threadIdx.x] = v[u];
+                            keep[(it + u) * 2 * kFused + kFused + threadIdx.x] = w[u];
+                        }
+#pragma unroll
+                        for (int j = 0; j < V; j++) {
+                            const float xh = (to_float(v[u].v[j]) - mu[j]) * rs[j];
+                            const float dz = to_float(w[u].v[j]) * act_grad<ACT, fast>(fmaf(xh, ga[j], be[j]));
+                            a[j] += dz;
+                            b[j] = fmaf(dz, xh, b[j]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < V; j++) part[(q.r * q.width + q.col) * V + j] = make_float2(a[j], b[j]);
+            }
+            __syncthreads();
+            for (int c = threadIdx.x; c < p.channels; c += kFused) {
+                float2 t = make_float2(0.0f, 0.0f);
+                for (int r = 0; r < q.step; r++) {
+                    const float2 v = part[r * p.channels + c];
+                    t.x += v.x;
+                    t.y += v.y;
+                }
+                chan[c] = t;
+                p.part[((int64_t)s.item * p.chunks + s.chunk) * p.channels + c] = t;
+            }
+            __syncthreads();
+            for (int g = warp; g < p.groups; g += kFused / 32) {
+                float a = 0.0f, b = 0.0f;
+                for (int k = lane; k < p.cpg; k += 32) {
+                    const int c = g * p.cpg + k;
+                    const float gc = param(p.gamma, c, p.param_float, 1.0f, (const T*)nullptr);
+                    a = fmaf(gc, chan[c].x, a);
+                    b = fmaf(gc, chan[c].y, b);
+                }
+                for (int o = 16; o > 0; o >>= 1) {
+                    a += __shfl_xor_sync(~0u, a, o);
+                    b += __shfl_xor_sync(~0u, b, o);
+                }
+                if (lane == 0) {
+                    group[g] = make_float2(a, b);
+                    if (GRID) p.sums[((int64_t)s.item * p.groups + g) * p.chunks + s.chunk] = make_float2(a, b);
+                }
+            }
+        }
+        __syncwarp();
+        if (GRID) cg::this_grid().sync();
+        else {
+            cluster_arrive();
+            cluster_wait();
+        }
+        if (s.n > 0 && p.dx) {
+            const float m = (float)p.positions * (float)p.cpg;
+            for (int g = warp; g < p.groups; g += kFused / 32) {
+                float a = 0.0f, b = 0.0f;
+                for (int c = lane; c < p.used; c += 32) {
+                    const float2 v = GRID ? __ldcg(p.sums + ((int64_t)s.item * p.groups + g) * p.chunks + c) : peer_read(group + g, c);
+                    a += v.x;
+                    b += v.y;
+                }
+                for (int o = 16; o > 0; o >>= 1) {
+                    a += __shfl_xor_sync(~0u, a, o);
+                    b += __shfl_xor_sync(~0u, b, o);
+                }
+                if (lane == 0) stat[g] = make_float2(a / m, b / m);
+            }
+        }
+        __syncwarp();
+        if (!GRID) cluster_arrive();
+        __syncthreads();
+        if (s.n > 0 && p.dx && on) {
+            float2 mo[V];
+#pragma unroll
+            for (int j = 0; j < V; j++) mo[j] = stat[(ch + j) / p.cpg];
+            T* dx = static_cast<T*>(p.dx) + s.item * p.db + s.l0 * p.dp + ch;
+            auto one = [&](const P& v, const P& w, int l) {
+                P o;
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const float xh = (to_float(v.v[j]) - mu[j]) * rs[j];
+                    const float d = to_float(w.v[j]) * act_grad<ACT, fast>(fmaf(xh, ga[j], be[j])) * ga[j];
+                    o.v[j] = from_float<T>(rs[j] * (d - mo[j].x - xh * mo[j].y));
+                }
+                *reinterpret_cast<P*>(dx + (int64_t)l * p.dp) = o;
+            };
+            int it = steps - 1;
+            constexpr int W = 2;
+            for (; it >= p.kept; it -= W) {
+                P v[W], w[W];
+#pragma unroll
+                for (int u = 0; u < W; u++) {
+                    const int l = q.r + (it - u) * q.step;
+                    if (it - u >= p.kept && l < s.n) {
+                        v[u] = *reinterpret_cast<const P*>(x + (int64_t)l * p.xp);
+                        w[u] = *reinterpret_cast<const P*>(dy + (int64_t)l * p.yp);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < W; u++) {
+                    const int l = q.r + (it - u) * q.step;
+                    if (it - u >= p.kept && l < s.n) one(v[u], w[u], l);
+                }
+            }
+            for (it = min(steps, p.kept) - 1; it >= 0; it--) {
+                const int l = q.r + it * q.step;
+                if (l < s.n) one(keep[it * 2 * kFused + threadIdx.x], keep[it * 2 * kFused + kFused + threadIdx.x], l);
+            }
+        }
+        if (GRID) __syncthreads();
+        else {
+            __syncwarp();
+            cluster_wait();
+        }
+    }
+    if (GRID && (p.dgamma || p.dbeta)) {   // every item's parts were complete at the last meeting
+        const int all = (int)gridDim.x * (kFused / 32);
+        for (int c = blockIdx.x * (kFused / 32) + warp; c < p.channels; c += all) {
+            float a = 0.0f, b = 0.0f;
+            for (int k = lane; k < p.batch * p.chunks; k += 32) {
+                const float2 v = __ldcg(p.part + (int64_t)k * p.channels + c);
+                a += v.x;
+                b += v.y;
+            }
+            for (int o = 16; o > 0; o >>= 1) {
+                a += __shfl_xor_sync(~0u, a, o);
+                b += __shfl_xor_sync(~0u, b, o);
+            }
+            if (lane == 0) {
+                if (p.dbeta) set_param(p.dbeta, c, p.param_float, a, (const T*)nullptr);
+                if (p.dgamma) set_param(p.dgamma, c, p.param_float, b, (const T*)nullptr);
+            }
+        }
+    }
+}
+
 // ---- host -------------------------------------------------------------------------------------
 
 void check_config(const stg_group_norm_config* c) {
@@ -386,20 +775,80 @@ int chunks_of(const stg_group_norm_config& c) {
     return (int)((c.positions + rows - 1) / std::max<int64_t>(rows, 1));
 }
 
-struct NormLayout { size_t part = 0, sums = 0, stats = 0, bytes = 0; };
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
-NormLayout layout_of(const stg_group_norm_config& c, bool backward) {
-    NormLayout l;
-    if (!c.batch || !c.positions) return l;
-    const size_t chunks = (size_t)chunks_of(c);
-    if (backward) {
-        l.sums = up(sizeof(float2) * (size_t)c.batch * chunks * c.channels);
-        l.bytes = l.sums + up(sizeof(float2) * (size_t)c.batch * c.channels);
-    } else {
-        l.stats = up(sizeof(float2) * (size_t)c.batch * chunks * c.groups);
-        l.bytes = l.stats + 2 * up(sizeof(float) * (size_t)c.batch * c.groups);
+
+enum Path { THREE_LAUNCHES, CLUSTER, GRID };
+// How a call runs with vectors of `vec` channels on `sms` SMs, and the scratch it takes.
+struct NormPlan {
+    Path path = THREE_LAUNCHES;
+    int chunks = 0, at_once = 1, kept = 0;
+    int64_t rows = 0;
+    size_t smem = 0;
+    size_t second = 0, third = 0, bytes = 0;   // offsets of the scratch's parts
+};
+NormPlan plan_of(const stg_group_norm_config& c, bool backward, int vec, int sms) {
+    NormPlan r;
+    if (!c.batch || !c.positions) return r;
+    const int columns = c.channels / vec, cpg = c.channels / c.groups;
+    const size_t vb = (size_t)vec * elem_size(c.dtype) * (backward ? 2 : 1), block_step = vb * kFused;
+    const bool mono = cpg % vec == 0;
+    // shared memory besides the kept values: the threads' parts, channel and group sums
+    const size_t other = backward ? sizeof(float2) * ((size_t)kFused * vec + c.channels + 2 * (size_t)c.groups)
+                                  : sizeof(float2) * ((size_t)kFused * (mono ? 1 : vec) + 2 * (size_t)c.groups);
+    const size_t most = 225 * 1024;
+    if (columns <= kFused && c.groups <= kFusedGroups && other + 8 * block_step <= most) {
+        const int64_t step = kFused / columns, room = (int64_t)((most - other) / block_step);   // steps a block can keep
+        const int64_t item_steps = (c.positions + step - 1) / step;
+        int64_t blocks = (item_steps + room - 1) / room;
+        if (blocks <= kClusterMost) {
+            // as many blocks as fill the GPU once, each with at least four steps
+            int64_t size = 1;
+            while (size < kClusterMost && (size < blocks || (size * 2 * c.batch <= sms && size * 8 <= item_steps))) size *= 2;
+            r.path = CLUSTER;
+            r.chunks = (int)size;
+            r.rows = (c.positions + size - 1) / size;
+            r.kept = (int)((r.rows + step - 1) / step);
+        } else {
+            r.at_once = (int)std::max<int64_t>(1, std::min<int64_t>(c.batch, sms * room / item_steps));
+            const int64_t per = sms / r.at_once;
+            if (per * c.groups <= 32768) {   // what every block reads of the others' sums: at most 256 KB
+                r.path = GRID;
+                r.rows = (c.positions + per - 1) / per;
+                r.chunks = (int)((c.positions + r.rows - 1) / r.rows);
+                r.kept = (int)std::min<int64_t>(room, (r.rows + step - 1) / step);
+            }
+        }
+        if (r.path != THREE_LAUNCHES && r.rows <= (1 << 30)) {
+            r.smem = other + (size_t)r.kept * block_step;
+            const size_t sets = (size_t)c.batch * r.chunks;
+            if (backward) {
+                r.second = up(sizeof(float2) * sets * c.channels);
+                r.bytes = r.second + (r.path == GRID ? up(sizeof(float2) * sets * c.groups) : 0);
+            } else r.bytes = r.path == GRID ? up(sizeof(float2) * sets * c.groups) : 0;
+            return r;
+        }
     }
-    return l;
+    r = NormPlan{};
+    r.chunks = chunks_of(c);
+    r.rows = (c.positions + r.chunks - 1) / r.chunks;
+    if (r.rows > (1 << 30)) fail(STG_UNSUPPORTED, "group norm: too many positions");
+    if (backward) {
+        r.second = up(sizeof(float2) * (size_t)c.batch * r.chunks * c.channels);
+        r.bytes = r.second + up(sizeof(float2) * (size_t)c.batch * c.channels);
+    } else {
+        r.second = up(sizeof(float2) * (size_t)c.batch * r.chunks * c.groups);
+        r.third = r.second + up(sizeof(float) * (size_t)c.batch * c.groups);
+        r.bytes = r.third + up(sizeof(float) * (size_t)c.batch * c.groups);
+    }
+    return r;
+}
+constexpr int kSms = 148;
+// Enough for either vector width: which one a call can use its buffers' addresses decide.
+size_t workspace_of(const stg_group_norm_config& c, bool backward) {
+    size_t n = plan_of(c, backward, 1, kSms).bytes;
+    const int w = 16 / (int)elem_size(c.dtype);
+    if (c.channels % w == 0) n = std::max(n, plan_of(c, backward, w, kSms).bytes);
+    return n;
 }
 
 NormParams params_of(const stg_group_norm_config& c) {
@@ -414,32 +863,44 @@ NormParams params_of(const stg_group_norm_config& c) {
     p.batch = (int)c.batch;
     p.eps = (float)c.eps;
     p.param_float = c.param_dtype == STG_F32;
-    if (c.batch && c.positions) {
-        p.chunks = chunks_of(c);
-        const int64_t rows = (c.positions + p.chunks - 1) / p.chunks;
-        if (rows > (1 << 30)) fail(STG_UNSUPPORTED, "group norm: too many positions");
-        p.rows = (int)rows;
-        p.chunks = (int)((c.positions + rows - 1) / rows);
-    }
     return p;
 }
 
-template <class Fn> void with_activation(int a, Fn&& fn) {
-    switch (a) {
-        case STG_ACT_RELU: return fn(std::integral_constant<int, STG_ACT_RELU>{});
-        case STG_ACT_SILU: return fn(std::integral_constant<int, STG_ACT_SILU>{});
-        case STG_ACT_GELU: return fn(std::integral_constant<int, STG_ACT_GELU>{});
-        case STG_ACT_SIGMOID: return fn(std::integral_constant<int, STG_ACT_SIGMOID>{});
-        default: return fn(std::integral_constant<int, STG_ACT_NONE>{});
-    }
-}
 // Widest (16 bytes) or scalar vectors, as sizes, strides and addresses allow.
-template <class T, class Fn> void with_width(bool wide, NormParams& p, Fn&& fn) {
-    constexpr int W = 16 / sizeof(T);
-    p.columns = wide ? p.channels / W : p.channels;
-    p.columns_div = FastDiv((uint32_t)std::min(p.columns, kThreads));
-    if (wide) fn(std::integral_constant<int, W>{});
+template <class T, class Fn> void with_width(bool wide, Fn&& fn) {
+    if (wide) fn(std::integral_constant<int, 16 / (int)sizeof(T)>{});
     else fn(std::integral_constant<int, 1>{});
+}
+void set_plan(NormParams& p, const NormPlan& plan, int vec) {
+    p.columns = p.channels / vec;
+    p.columns_div = FastDiv((uint32_t)std::min(p.columns, plan.path == THREE_LAUNCHES ? kThreads : kFused));
+    p.chunks = plan.chunks;
+    p.rows = (int)plan.rows;
+    p.used = (int)((p.positions + plan.rows - 1) / plan.rows);
+    p.at_once = plan.at_once;
+    p.kept = plan.kept;
+    p.mono = p.cpg % vec == 0;
+}
+template <class K> void launch_fused(K kernel, const NormParams& p, const NormPlan& plan, int sms, cudaStream_t st) {
+    cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan.smem), "group norm kernel");
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    const int64_t blocks = plan.path == GRID ? (int64_t)plan.at_once * plan.chunks : (int64_t)p.batch * plan.chunks;
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kFused);
+    cfg.dynamicSmemBytes = plan.smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (plan.path == GRID) {
+        attr[0].id = cudaLaunchAttributeCooperative;
+        attr[0].val.cooperative = 1;
+    } else {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = plan.chunks;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    }
+    cuda_check(cudaLaunchKernelEx(&cfg, kernel, p), "group norm kernel");
 }
 bool wide_fits(const stg_group_norm_config& c, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
     const int w = 16 / (int)elem_size(c.dtype);
@@ -462,7 +923,7 @@ STG_API stg_status stg_group_norm_workspace(const stg_group_norm_config* c, int3
     return guard(nullptr, [&] {
         check_config(c);
         check(bytes && (backward == 0 || backward == 1), "group norm: null buffer");
-        *bytes = layout_of(*c, backward != 0).bytes;
+        *bytes = workspace_of(*c, backward != 0);
     });
 }
 
@@ -479,28 +940,38 @@ STG_API stg_status stg_group_norm(stg_engine* e, const stg_group_norm_config* c,
         check_output_strides(c->y_batch, c->y_position, *c);
         if (!c->batch || !c->positions) return;
         check(d_x && d_y, "group norm: null buffer");
-        const NormLayout lay = layout_of(*c, false);
-        check(d_ws && aligned(d_ws, 256) && ws_bytes >= lay.bytes, "group norm: workspace is missing, unaligned or too small");
+        const bool wide = wide_fits(*c, {d_x, d_y}, {c->x_batch, c->x_position, c->y_batch, c->y_position});
+        const NormPlan plan = plan_of(*c, false, wide ? 16 / (int)es : 1, std::min(e->sms, kSms));
+        check(!plan.bytes || (d_ws && aligned(d_ws, 256) && ws_bytes >= plan.bytes), "group norm: workspace is missing, unaligned or too small");
         NormParams p = params_of(*c);
         char* ws = static_cast<char*>(d_ws);
         p.x = d_x; p.y = d_y; p.gamma = d_gamma; p.beta = d_beta;
         p.part = reinterpret_cast<float2*>(ws);
-        p.mean = d_mean ? d_mean : reinterpret_cast<float*>(ws + lay.stats);
-        p.rstd = d_rstd ? d_rstd : p.mean + up(sizeof(float) * (size_t)c->batch * c->groups) / sizeof(float);
-        const bool wide = wide_fits(*c, {d_x, d_y}, {c->x_batch, c->x_position, c->y_batch, c->y_position});
+        p.mean = d_mean;
+        p.rstd = d_rstd;
         DeviceScope scope(e);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
-        const dim3 grid((unsigned)p.chunks, (unsigned)p.batch);
         with_dtype(c->dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
-            with_width<T>(wide, p, [&](auto v) {
+            with_width<T>(wide, [&](auto v) {
                 constexpr int V = decltype(v)::value;
-                const size_t smem = sizeof(Moments) * (size_t)p.groups;
-                if (smem + sizeof(float2) * kThreads * V > 48 * 1024)
-                    cuda_check(cudaFuncSetAttribute(moments_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "group norm kernel");
-                moments_kernel<T, V><<<grid, kThreads, smem, st>>>(p);
-                moments_join<<<(unsigned)(((int64_t)p.batch * p.groups + 3) / 4), 128, 0, st>>>(p);
-                with_activation(c->activation, [&](auto a) { apply_kernel<T, V, decltype(a)::value><<<grid, kThreads, 0, st>>>(p); });
+                set_plan(p, plan, V);
+                with_activation(c->activation, [&](auto a) {
+                    constexpr int A = decltype(a)::value;
+                    if (plan.path == CLUSTER) return launch_fused(norm_fused<T, V, A, false>, p, plan, e->sms, st);
+                    if (plan.path == GRID) return launch_fused(norm_fused<T, V, A, true>, p, plan, e->sms, st);
+                    if (!p.mean) {
+                        p.mean = reinterpret_cast<float*>(ws + plan.second);
+                        p.rstd = reinterpret_cast<float*>(ws + plan.third);
+                    }
+                    const dim3 grid((unsigned)p.chunks, (unsigned)p.batch);
+                    const size_t smem = sizeof(Moments) * (size_t)p.groups;
+                    if (smem + sizeof(float2) * kThreads * V > 48 * 1024)
+                        cuda_check(cudaFuncSetAttribute(moments_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "group norm kernel");
+                    moments_kernel<T, V><<<grid, kThreads, smem, st>>>(p);
+                    moments_join<<<(unsigned)(((int64_t)p.batch * p.groups + 3) / 4), 128, 0, st>>>(p);
+                    apply_kernel<T, V, A><<<grid, kThreads, 0, st>>>(p);
+                });
             });
         });
         cuda_check(cudaGetLastError(), "group norm kernel");
@@ -527,8 +998,9 @@ STG_API stg_status stg_group_norm_backward(stg_engine* e, const stg_group_norm_c
         }
         check(d_x && d_dy && d_mean && d_rstd, "group norm: null buffer");
         if (!d_dx && !d_dgamma && !d_dbeta) return;
-        const NormLayout lay = layout_of(*c, true);
-        check(d_ws && aligned(d_ws, 256) && ws_bytes >= lay.bytes, "group norm: workspace is missing, unaligned or too small");
+        const bool wide = wide_fits(*c, {d_x, d_dy, d_dx}, {c->x_batch, c->x_position, c->y_batch, c->y_position, c->dx_batch, c->dx_position});
+        const NormPlan plan = plan_of(*c, true, wide ? 16 / (int)es : 1, std::min(e->sms, kSms));
+        check(d_ws && aligned(d_ws, 256) && ws_bytes >= plan.bytes, "group norm: workspace is missing, unaligned or too small");
         NormParams p = params_of(*c);
         char* ws = static_cast<char*>(d_ws);
         p.x = d_x; p.dy = d_dy; p.dx = d_dx; p.gamma = d_gamma; p.beta = d_beta;
@@ -536,17 +1008,24 @@ STG_API stg_status stg_group_norm_backward(stg_engine* e, const stg_group_norm_c
         p.mean = const_cast<float*>(d_mean);
         p.rstd = const_cast<float*>(d_rstd);
         p.part = reinterpret_cast<float2*>(ws);
-        p.sums = reinterpret_cast<float2*>(ws + lay.sums);
-        const bool wide = wide_fits(*c, {d_x, d_dy, d_dx}, {c->x_batch, c->x_position, c->y_batch, c->y_position, c->dx_batch, c->dx_position});
-        const dim3 grid((unsigned)p.chunks, (unsigned)p.batch);
+        p.sums = plan.path == CLUSTER ? nullptr : reinterpret_cast<float2*>(ws + plan.second);
         with_dtype(c->dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
-            with_width<T>(wide, p, [&](auto v) {
+            with_width<T>(wide, [&](auto v) {
                 constexpr int V = decltype(v)::value;
+                set_plan(p, plan, V);
                 with_activation(c->activation, [&](auto a) {
                     constexpr int A = decltype(a)::value;
+                    const unsigned join_blocks = (unsigned)((p.channels + 3) / 4);
+                    if (plan.path == CLUSTER) {
+                        launch_fused(norm_grad_fused<T, V, A, false>, p, plan, e->sms, st);
+                        if (p.dgamma || p.dbeta) grad_join<T><<<join_blocks, 128, 0, st>>>(p);
+                        return;
+                    }
+                    if (plan.path == GRID) return launch_fused(norm_grad_fused<T, V, A, true>, p, plan, e->sms, st);
+                    const dim3 grid((unsigned)p.chunks, (unsigned)p.batch);
                     grad_sums_kernel<T, V, A><<<grid, kThreads, 0, st>>>(p);
-                    grad_join<T><<<(unsigned)((p.channels + 3) / 4), 128, 0, st>>>(p);
+                    grad_join<T><<<join_blocks, 128, 0, st>>>(p);
                     if (p.dx) {
                         const size_t smem = sizeof(float2) * (size_t)p.groups;
                         if (smem > 48 * 1024)

@@ -121,7 +121,8 @@ NORM = [
     # batch, positions, channels, groups
     (1, 1, 1, 1), (1, 1, 8, 1), (2, 1, 6, 3), (1, 2, 8, 8), (3, 17, 48, 4), (2, 336, 48, 1), (1, 1000, 75, 5), (2, 129, 96, 96),
     (1, 5000, 64, 2), (4, 3, 2056, 8), (1, 40, 2051, 7), (2, 3, 8192, 1), (1, 50, 8192, 8192), (5, 700, 24, 3), (1, 30011, 16, 4), (2, 9000, 192, 4),
-    (65, 9, 32, 8), (1, 33, 36, 1),
+    (65, 9, 32, 8), (1, 33, 36, 1), (7, 9, 16, 2),
+    (5, 30000, 24, 2), (1, 400000, 40, 5), (3, 70001, 33, 3), (2, 20000, 520, 520),
 ]
 
 
@@ -225,16 +226,20 @@ def test_group_norm_refusals(pkg, engine):
             call()
         assert err.value.code in (1, 2)
     import ctypes as C
-    cfg = pkg.GroupNormConfig(C.sizeof(pkg.GroupNormConfig), 0, 0, 0, 2, 6, 8, 2, 48, 8, 48, 8, 48, 8, 1e-5)
-    y = torch.zeros_like(x)
-    args = (engine._h, C.byref(cfg), x.data_ptr(), None, None, y.data_ptr(), None, None)
     n = C.c_size_t()
-    assert pkg.lib().stg_group_norm_workspace(C.byref(cfg), 0, C.byref(n)) == 0
-    ws = torch.empty(n.value + 256, dtype=torch.uint8, device="cuda")
-    assert pkg.lib().stg_group_norm(*args, ws.data_ptr(), n.value, None) == 0
-    assert pkg.lib().stg_group_norm(*args, None, 0, None) == 1
-    assert pkg.lib().stg_group_norm(*args, ws.data_ptr(), n.value - 1, None) == 1
-    assert pkg.lib().stg_group_norm(*args, ws.data_ptr() + 8, n.value, None) == 1
+    for positions, channels, groups in ((5, 4096, 4096), (60000, 16, 4)):     # three launches; all SMs at once
+        cfg = pkg.GroupNormConfig(C.sizeof(pkg.GroupNormConfig), 0, 0, 0, 1, positions, channels, groups, 0, channels, 0, channels, 0,
+                                  channels, 1e-5)
+        cfg.x_batch = cfg.y_batch = cfg.dx_batch = positions * channels
+        x = torch.zeros(1, positions, channels, device="cuda")
+        y = torch.zeros_like(x)
+        args = (engine._h, C.byref(cfg), x.data_ptr(), None, None, y.data_ptr(), None, None)
+        assert pkg.lib().stg_group_norm_workspace(C.byref(cfg), 0, C.byref(n)) == 0 and n.value > 0
+        ws = torch.empty(n.value + 256, dtype=torch.uint8, device="cuda")
+        assert pkg.lib().stg_group_norm(*args, ws.data_ptr(), n.value, None) == 0
+        assert pkg.lib().stg_group_norm(*args, None, 0, None) == 1
+        assert pkg.lib().stg_group_norm(*args, ws.data_ptr(), 0, None) == 1
+        assert pkg.lib().stg_group_norm(*args, ws.data_ptr() + 8, n.value, None) == 1
     assert "workspace" in engine.last_error()
 
 
