@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(const __grid_const
 
 // ---- one launch -------------------------------------------------------------------------------
 
-constexpr int kFused = 512;          // threads
+constexpr int kFused = 1024, kFusedGrad = 512;   // threads forward and backward: what the registers allow
 constexpr int kFusedGroups = 2048;   // most groups
 constexpr int kClusterMost = 8;
 
@@ -368,6 +368,16 @@ __device__ __forceinline__ float2 peer_read(const float2* p, int rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
     return v;
+}
+
+// Pair i of a vector as floats, and back. A vector of one is a pair with nothing beside it.
+template <class T, int V> __device__ __forceinline__ f2 get(const Pack<T, V>& v, int i) {
+    if constexpr (V == 1) return make_f2(to_float(v.v[0]), 0.0f);
+    else return load2(&v.v[2 * i]);
+}
+template <class T, int V> __device__ __forceinline__ void put(Pack<T, V>& v, int i, f2 a) {
+    if constexpr (V == 1) v.v[0] = from_float<T>(split(a).x);
+    else store2(&v.v[2 * i], a);
 }
 
 struct Share { int item, chunk, n; int64_t l0; };
@@ -416,7 +426,8 @@ __device__ __forceinline__ void block_moments(const NormParams& p, const Place& 
 template <class T, int V, int ACT, bool GRID>
 __global__ void __launch_bounds__(kFused, 1) norm_fused(const __grid_constant__ NormParams p) {
     constexpr bool fast = sizeof(T) == 2;
-    constexpr int U = 8;                        // positions in flight per thread
+    constexpr int U = 4;                        // positions in flight per thread
+    constexpr int N = (V + 1) / 2;
     using P = Pack<T, V>;
     extern __shared__ __align__(16) uint8_t smem[];
     P* keep = reinterpret_cast<P*>(smem);       // [kept][threads]
@@ -439,43 +450,55 @@ __global__ void __launch_bounds__(kFused, 1) norm_fused(const __grid_constant__ 
         if (s.n > 0) {
             if (on && q.r < s.n) {
                 // differences from the first value met, so that a mean far from zero costs no digits
-                float pivot[V], a[V], b[V];
-                const P first = *reinterpret_cast<const P*>(x + (int64_t)q.r * p.xp);
+                f2 pivot[N], a[N], b[N];
+                {
+                    const P first = *reinterpret_cast<const P*>(x + (int64_t)q.r * p.xp);
 #pragma unroll
-                for (int j = 0; j < V; j++) { pivot[j] = to_float(first.v[p.mono ? 0 : j]); a[j] = b[j] = 0.0f; }
-                for (int it = 0; it < steps; it += U) {
+                    for (int i = 0; i < N; i++) {
+                        const float2 f = split(get(first, i));
+                        pivot[i] = p.mono ? make_f2(-to_float(first.v[0])) : make_f2(-f.x, -f.y);
+                        a[i] = b[i] = make_f2(0.0f);
+                    }
+                }
+                const T* at = x + (int64_t)q.r * p.xp;
+                const int64_t step = (int64_t)q.step * p.xp;
+                const int mine = (s.n - q.r + q.step - 1) / q.step;
+                for (int it = 0; it < mine; it += U) {
                     P v[U];
 #pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        const int l = q.r + (it + u) * q.step;
-                        if (l < s.n) v[u] = *reinterpret_cast<const P*>(x + (int64_t)l * p.xp);
-                    }
+                    for (int u = 0; u < U; u++, at += step)
+                        if (it + u < mine) v[u] = *reinterpret_cast<const P*>(at);
 #pragma unroll
                     for (int u = 0; u < U; u++) {
-                        const int l = q.r + (it + u) * q.step;
-                        if (l >= s.n) break;
+                        if (it + u >= mine) break;
                         if (it + u < p.kept) keep[(it + u) * kFused + threadIdx.x] = v[u];
 #pragma unroll
-                        for (int j = 0; j < V; j++) {
-                            const float d = to_float(v[u].v[j]) - pivot[j];
-                            a[j] += d;
-                            b[j] = fmaf(d, d, b[j]);
+                        for (int i = 0; i < N; i++) {
+                            const f2 d = get(v[u], i) + pivot[i];
+                            a[i] = a[i] + d;
+                            b[i] = fma2(d, d, b[i]);
                         }
                     }
                 }
-                const float cnt = (float)((s.n - q.r + q.step - 1) / q.step);
-                auto moments = [&](float sum, float sq, float n, float at) {   // + 0 sum: a NaN stays one
+                auto moments = [&](float sum, float sq, float n, float neg) {   // + 0 sum: a NaN stays one
                     const float m = sum / n;
-                    return make_float2(at + m, fmaxf(fmaf(-sum, m, sq), 0.0f) + 0.0f * sum);
+                    return make_float2(m - neg, fmaxf(fmaf(-sum, m, sq), 0.0f) + 0.0f * sum);
                 };
-                if (p.mono) {
-                    float sa = a[0], sb = b[0];
+                if (V == 1) {
+                    part[q.r * q.width + q.col] = moments(split(a[0]).x, split(b[0]).x, (float)mine, split(pivot[0]).x);
+                } else if (p.mono) {
 #pragma unroll
-                    for (int j = 1; j < V; j++) { sa += a[j]; sb += b[j]; }
-                    part[q.r * q.width + q.col] = moments(sa, sb, cnt * V, pivot[0]);
+                    for (int i = 1; i < N; i++) { a[0] = a[0] + a[i]; b[0] = b[0] + b[i]; }
+                    const float2 sa = split(a[0]), sb = split(b[0]);
+                    part[q.r * q.width + q.col] = moments(sa.x + sa.y, sb.x + sb.y, (float)mine * V, split(pivot[0]).x);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < V; j++) part[(q.r * q.width + q.col) * V + j] = moments(a[j], b[j], cnt, pivot[j]);
+                    for (int i = 0; i < N; i++) {
+                        const float2 sa = split(a[i]), sb = split(b[i]), sp = split(pivot[i]);
+                        float2* to = part + (q.r * q.width + q.col) * V + 2 * i;
+                        to[0] = moments(sa.x, sb.x, (float)mine, sp.x);
+                        to[1] = moments(sa.y, sb.y, (float)mine, sp.y);
+                    }
                 }
             }
             __syncthreads();
@@ -512,23 +535,38 @@ __global__ void __launch_bounds__(kFused, 1) norm_fused(const __grid_constant__ 
         if (!GRID) cluster_arrive();   // waited for below: no block goes while others still read its moments
         __syncthreads();
         if (s.n > 0 && on) {
-            float mu[V], a[V], sh[V];
+            // z = (x - mu) a + sh. For 16-bit x as x a + (sh - mu a): what that rounds, 2^-24 of mu a, is far
+            // below the 2^-9 (2^-12) of mu a that x itself was rounded by.
+            f2 mu[N], a[N], sh[N];
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float2 st = stat[(ch + j) / p.cpg];
-                mu[j] = st.x;
-                a[j] = st.y * param(p.gamma, ch + j, p.param_float, 1.0f, (const T*)nullptr);
-                sh[j] = param(p.beta, ch + j, p.param_float, 0.0f, (const T*)nullptr);
+            for (int i = 0; i < N; i++) {
+                float m[2], s1[2], s0[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int c = V == 1 ? ch : ch + 2 * i + k;
+                    const float2 st = stat[c / p.cpg];
+                    m[k] = st.x;
+                    s1[k] = st.y * param(p.gamma, c, p.param_float, 1.0f, (const T*)nullptr);
+                    s0[k] = param(p.beta, c, p.param_float, 0.0f, (const T*)nullptr);
+                    if (fast) s0[k] = fmaf(-m[k], s1[k], s0[k]);
+                }
+                mu[i] = make_f2(-m[0], -m[1]);
+                a[i] = make_f2(s1[0], s1[1]);
+                sh[i] = make_f2(s0[0], s0[1]);
             }
             T* y = static_cast<T*>(p.y) + s.item * p.yb + s.l0 * p.yp + ch;
             auto one = [&](P v, int l) {
 #pragma unroll
-                for (int j = 0; j < V; j++) v.v[j] = from_float<T>(act<ACT, fast>(fmaf(to_float(v.v[j]) - mu[j], a[j], sh[j])));
+                for (int i = 0; i < N; i++) {
+                    f2 z = get(v, i);
+                    if (!fast) z = z + mu[i];
+                    put(v, i, act2<ACT, fast>(fma2(z, a[i], sh[i])));
+                }
                 *reinterpret_cast<P*>(y + (int64_t)l * p.yp) = v;
             };
             // what was read last and not kept is in L2 yet: from the end
             int it = steps - 1;
-            constexpr int W = 4;
+            constexpr int W = 2;
             for (; it >= p.kept; it -= W) {
                 P v[W];
 #pragma unroll
@@ -559,78 +597,87 @@ __global__ void __launch_bounds__(kFused, 1) norm_fused(const __grid_constant__ 
 // Backward: the block's sums of dz and dz xh per channel, of gamma times them per group; the set's
 // blocks meet over the group sums. Channel sums go out per block for dgamma and dbeta.
 template <class T, int V, int ACT, bool GRID>
-__global__ void __launch_bounds__(kFused, 1) norm_grad_fused(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(kFusedGrad, 1) norm_grad_fused(const __grid_constant__ NormParams p) {
     constexpr bool fast = sizeof(T) == 2;
-    constexpr int U = 4;
+    constexpr int U = 4, N = (V + 1) / 2;
     using P = Pack<T, V>;
     extern __shared__ __align__(16) uint8_t smem[];
     P* keep = reinterpret_cast<P*>(smem);       // [kept][x, dy][threads]
-    float2* part = reinterpret_cast<float2*>(smem + (size_t)p.kept * 2 * kFused * sizeof(P));   // [step][channels]
-    float2* chan = part + kFused * V;           // [channels]
+    float2* part = reinterpret_cast<float2*>(smem + (size_t)p.kept * 2 * kFusedGrad * sizeof(P));   // [step][channels]
+    float2* chan = part + kFusedGrad * V;           // [channels]
     float2* group = chan + p.channels;          // [groups]: the block's sums
     float2* stat = group + p.groups;            // [groups]: the item's means of d and d xh
     Place q;
     q.width = p.columns;
-    q.step = kFused / q.width;
+    q.step = kFusedGrad / q.width;
     q.r = (int)p.columns_div.div(threadIdx.x);
     q.col = threadIdx.x - q.r * q.width;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ch = q.col * V;
     const bool on = q.r < q.step;
     const int rounds = GRID ? (p.batch + p.at_once - 1) / p.at_once : 1;
-    float ga[V], be[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-        ga[j] = on ? param(p.gamma, ch + j, p.param_float, 1.0f, (const T*)nullptr) : 0.0f;
-        be[j] = on ? param(p.beta, ch + j, p.param_float, 0.0f, (const T*)nullptr) : 0.0f;
-    }
     for (int round = 0; round < rounds; round++) {
         const Share s = share_of<GRID>(p, round);
         const T* x = static_cast<const T*>(p.x) + s.item * p.xb + s.l0 * p.xp + ch;
         const T* dy = static_cast<const T*>(p.dy) + s.item * p.yb + s.l0 * p.yp + ch;
         const int steps = s.n > 0 ? (s.n + q.step - 1) / q.step : 0;
-        float mu[V], rs[V];
+        // z = (x - mu) za + zb; the sums are of dz and dz (x - mu), the latter scaled by rstd at the end
+        f2 mu[N], za[N], zb[N];
         if (s.n > 0) {
             if (on) {
-                float a[V], b[V];
+                f2 a[N], b[N];
+                float rs[2 * N];
 #pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const int64_t g = (int64_t)s.item * p.groups + (ch + j) / p.cpg;
-                    mu[j] = p.mean[g];
-                    rs[j] = p.rstd[g];
-                    a[j] = b[j] = 0.0f;
+                for (int i = 0; i < N; i++) {
+                    float m[2], s1[2], s0[2];
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const int c = V == 1 ? ch : ch + 2 * i + k;
+                        const int64_t g = (int64_t)s.item * p.groups + c / p.cpg;
+                        m[k] = -p.mean[g];
+                        rs[2 * i + k] = p.rstd[g];
+                        s1[k] = rs[2 * i + k] * param(p.gamma, c, p.param_float, 1.0f, (const T*)nullptr);
+                        s0[k] = param(p.beta, c, p.param_float, 0.0f, (const T*)nullptr);
+                    }
+                    mu[i] = make_f2(m[0], m[1]);
+                    za[i] = make_f2(s1[0], s1[1]);
+                    zb[i] = make_f2(s0[0], s0[1]);
+                    a[i] = b[i] = make_f2(0.0f);
                 }
-                for (int it = 0; it < steps; it += U) {
+                const T *ax = x + (int64_t)q.r * p.xp, *ad = dy + (int64_t)q.r * p.yp;
+                const int64_t sx = (int64_t)q.step * p.xp, sd = (int64_t)q.step * p.yp;
+                const int mine = q.r < s.n ? (s.n - q.r + q.step - 1) / q.step : 0;
+                for (int it = 0; it < mine; it += U) {
                     P v[U], w[U];
 #pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        const int l = q.r + (it + u) * q.step;
-                        if (l < s.n) {
-                            v[u] = *reinterpret_cast<const P*>(x + (int64_t)l * p.xp);
-                            w[u] = *reinterpret_cast<const P*>(dy + (int64_t)l * p.yp);
+                    for (int u = 0; u < U; u++, ax += sx, ad += sd)
+                        if (it + u < mine) {
+                            v[u] = *reinterpret_cast<const P*>(ax);
+                            w[u] = *reinterpret_cast<const P*>(ad);
                         }
-                    }
 #pragma unroll
                     for (int u = 0; u < U; u++) {
-                        const int l = q.r + (it + u) * q.step;
-                        if (l >= s.n) break;
+                        if (it + u >= mine) break;
                         if (it + u < p.kept) {
-                            keep[(it + u) * 2 * kFused + threadIdx.x] = v[u];
-                            keep[(it + u) * 2 * kFused + kFused + threadIdx.x] = w[u];
+                            keep[(it + u) * 2 * kFusedGrad + threadIdx.x] = v[u];
+                            keep[(it + u) * 2 * kFusedGrad + kFusedGrad + threadIdx.x] = w[u];
                         }
 #pragma unroll
-                        for (int j = 0; j < V; j++) {
-                            const float xh = (to_float(v[u].v[j]) - mu[j]) * rs[j];
-                            const float dz = to_float(w[u].v[j]) * act_grad<ACT, fast>(fmaf(xh, ga[j], be[j]));
-                            a[j] += dz;
-                            b[j] = fmaf(dz, xh, b[j]);
+                        for (int i = 0; i < N; i++) {
+                            const f2 xm = get(v[u], i) + mu[i];
+                            const f2 dz = get(w[u], i) * act_grad2<ACT, fast>(fma2(xm, za[i], zb[i]));
+                            a[i] = a[i] + dz;
+                            b[i] = fma2(dz, xm, b[i]);
                         }
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < V; j++) part[(q.r * q.width + q.col) * V + j] = make_float2(a[j], b[j]);
+                for (int j = 0; j < V; j++) {
+                    const float2 sa = split(a[j / 2]), sb = split(b[j / 2]);
+                    part[(q.r * q.width + q.col) * V + j] = make_float2(j & 1 ? sa.y : sa.x, (j & 1 ? sb.y : sb.x) * rs[j]);
+                }
             }
             __syncthreads();
-            for (int c = threadIdx.x; c < p.channels; c += kFused) {
+            for (int c = threadIdx.x; c < p.channels; c += kFusedGrad) {
                 float2 t = make_float2(0.0f, 0.0f);
                 for (int r = 0; r < q.step; r++) {
                     const float2 v = part[r * p.channels + c];
@@ -641,7 +688,7 @@ __global__ void __launch_bounds__(kFused, 1) norm_grad_fused(const __grid_consta
                 p.part[((int64_t)s.item * p.chunks + s.chunk) * p.channels + c] = t;
             }
             __syncthreads();
-            for (int g = warp; g < p.groups; g += kFused / 32) {
+            for (int g = warp; g < p.groups; g += kFusedGrad / 32) {
                 float a = 0.0f, b = 0.0f;
                 for (int k = lane; k < p.cpg; k += 32) {
                     const int c = g * p.cpg + k;
@@ -667,7 +714,7 @@ __global__ void __launch_bounds__(kFused, 1) norm_grad_fused(const __grid_consta
         }
         if (s.n > 0 && p.dx) {
             const float m = (float)p.positions * (float)p.cpg;
-            for (int g = warp; g < p.groups; g += kFused / 32) {
+            for (int g = warp; g < p.groups; g += kFusedGrad / 32) {
                 float a = 0.0f, b = 0.0f;
                 for (int c = lane; c < p.used; c += 32) {
                     const float2 v = GRID ? __ldcg(p.sums + ((int64_t)s.item * p.groups + g) * p.chunks + c) : peer_read(group + g, c);
@@ -685,17 +732,29 @@ __global__ void __launch_bounds__(kFused, 1) norm_grad_fused(const __grid_consta
         if (!GRID) cluster_arrive();
         __syncthreads();
         if (s.n > 0 && p.dx && on) {
-            float2 mo[V];
+            // dx = rstd gamma dz - (x - mu) rstd^2 mean(d xh) - rstd mean(d)
+            f2 c1[N], c2[N];
 #pragma unroll
-            for (int j = 0; j < V; j++) mo[j] = stat[(ch + j) / p.cpg];
+            for (int i = 0; i < N; i++) {
+                float u1[2], u2[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int g = (V == 1 ? ch : ch + 2 * i + k) / p.cpg;
+                    const float r = p.rstd[(int64_t)s.item * p.groups + g];
+                    u1[k] = -r * stat[g].x;
+                    u2[k] = -r * r * stat[g].y;
+                }
+                c1[i] = make_f2(u1[0], u1[1]);
+                c2[i] = make_f2(u2[0], u2[1]);
+            }
             T* dx = static_cast<T*>(p.dx) + s.item * p.db + s.l0 * p.dp + ch;
             auto one = [&](const P& v, const P& w, int l) {
                 P o;
 #pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float xh = (to_float(v.v[j]) - mu[j]) * rs[j];
-                    const float d = to_float(w.v[j]) * act_grad<ACT, fast>(fmaf(xh, ga[j], be[j])) * ga[j];
-                    o.v[j] = from_float<T>(rs[j] * (d - mo[j].x - xh * mo[j].y));
+                for (int i = 0; i < N; i++) {
+                    const f2 xm = get(v, i) + mu[i];
+                    const f2 dz = get(w, i) * act_grad2<ACT, fast>(fma2(xm, za[i], zb[i]));
+                    put(o, i, fma2(dz, za[i], fma2(xm, c2[i], c1[i])));
                 }
                 *reinterpret_cast<P*>(dx + (int64_t)l * p.dp) = o;
             };
@@ -719,7 +778,7 @@ __global__ void __launch_bounds__(kFused, 1) norm_grad_fused(const __grid_consta
             }
             for (it = min(steps, p.kept) - 1; it >= 0; it--) {
                 const int l = q.r + it * q.step;
-                if (l < s.n) one(keep[it * 2 * kFused + threadIdx.x], keep[it * 2 * kFused + kFused + threadIdx.x], l);
+                if (l < s.n) one(keep[it * 2 * kFusedGrad + threadIdx.x], keep[it * 2 * kFusedGrad + kFusedGrad + threadIdx.x], l);
             }
         }
         if (GRID) __syncthreads();
@@ -729,8 +788,8 @@ __global__ void __launch_bounds__(kFused, 1) norm_grad_fused(const __grid_consta
         }
     }
     if (GRID && (p.dgamma || p.dbeta)) {   // every item's parts were complete at the last meeting
-        const int all = (int)gridDim.x * (kFused / 32);
-        for (int c = blockIdx.x * (kFused / 32) + warp; c < p.channels; c += all) {
+        const int all = (int)gridDim.x * (kFusedGrad / 32);
+        for (int c = blockIdx.x * (kFusedGrad / 32) + warp; c < p.channels; c += all) {
             float a = 0.0f, b = 0.0f;
             for (int k = lane; k < p.batch * p.chunks; k += 32) {
                 const float2 v = __ldcg(p.part + (int64_t)k * p.channels + c);
@@ -790,14 +849,15 @@ NormPlan plan_of(const stg_group_norm_config& c, bool backward, int vec, int sms
     NormPlan r;
     if (!c.batch || !c.positions) return r;
     const int columns = c.channels / vec, cpg = c.channels / c.groups;
-    const size_t vb = (size_t)vec * elem_size(c.dtype) * (backward ? 2 : 1), block_step = vb * kFused;
+    const int threads = backward ? kFusedGrad : kFused;
+    const size_t vb = (size_t)vec * elem_size(c.dtype) * (backward ? 2 : 1), block_step = vb * threads;
     const bool mono = cpg % vec == 0;
     // shared memory besides the kept values: the threads' parts, channel and group sums
-    const size_t other = backward ? sizeof(float2) * ((size_t)kFused * vec + c.channels + 2 * (size_t)c.groups)
-                                  : sizeof(float2) * ((size_t)kFused * (mono ? 1 : vec) + 2 * (size_t)c.groups);
+    const size_t other = backward ? sizeof(float2) * ((size_t)threads * vec + c.channels + 2 * (size_t)c.groups)
+                                  : sizeof(float2) * ((size_t)threads * (mono ? 1 : vec) + 2 * (size_t)c.groups);
     const size_t most = 225 * 1024;
-    if (columns <= kFused && c.groups <= kFusedGroups && other + 8 * block_step <= most) {
-        const int64_t step = kFused / columns, room = (int64_t)((most - other) / block_step);   // steps a block can keep
+    if (columns <= threads && c.groups <= kFusedGroups && other + 8 * block_step <= most) {
+        const int64_t step = threads / columns, room = (int64_t)((most - other) / block_step);   // steps a block can keep
         const int64_t item_steps = (c.positions + step - 1) / step;
         int64_t blocks = (item_steps + room - 1) / room;
         if (blocks <= kClusterMost) {
@@ -871,9 +931,9 @@ template <class T, class Fn> void with_width(bool wide, Fn&& fn) {
     if (wide) fn(std::integral_constant<int, 16 / (int)sizeof(T)>{});
     else fn(std::integral_constant<int, 1>{});
 }
-void set_plan(NormParams& p, const NormPlan& plan, int vec) {
+void set_plan(NormParams& p, const NormPlan& plan, int vec, int fused) {
     p.columns = p.channels / vec;
-    p.columns_div = FastDiv((uint32_t)std::min(p.columns, plan.path == THREE_LAUNCHES ? kThreads : kFused));
+    p.columns_div = FastDiv((uint32_t)std::min(p.columns, plan.path == THREE_LAUNCHES ? kThreads : fused));
     p.chunks = plan.chunks;
     p.rows = (int)plan.rows;
     p.used = (int)((p.positions + plan.rows - 1) / plan.rows);
@@ -881,13 +941,13 @@ void set_plan(NormParams& p, const NormPlan& plan, int vec) {
     p.kept = plan.kept;
     p.mono = p.cpg % vec == 0;
 }
-template <class K> void launch_fused(K kernel, const NormParams& p, const NormPlan& plan, int sms, cudaStream_t st) {
+template <class K> void launch_fused(K kernel, const NormParams& p, const NormPlan& plan, int threads, cudaStream_t st) {
     cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan.smem), "group norm kernel");
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
     const int64_t blocks = plan.path == GRID ? (int64_t)plan.at_once * plan.chunks : (int64_t)p.batch * plan.chunks;
     cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(kFused);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = plan.smem;
     cfg.stream = st;
     cfg.attrs = attr;
@@ -955,11 +1015,11 @@ STG_API stg_status stg_group_norm(stg_engine* e, const stg_group_norm_config* c,
             using T = std::remove_pointer_t<decltype(tag)>;
             with_width<T>(wide, [&](auto v) {
                 constexpr int V = decltype(v)::value;
-                set_plan(p, plan, V);
+                set_plan(p, plan, V, kFused);
                 with_activation(c->activation, [&](auto a) {
                     constexpr int A = decltype(a)::value;
-                    if (plan.path == CLUSTER) return launch_fused(norm_fused<T, V, A, false>, p, plan, e->sms, st);
-                    if (plan.path == GRID) return launch_fused(norm_fused<T, V, A, true>, p, plan, e->sms, st);
+                    if (plan.path == CLUSTER) return launch_fused(norm_fused<T, V, A, false>, p, plan, kFused, st);
+                    if (plan.path == GRID) return launch_fused(norm_fused<T, V, A, true>, p, plan, kFused, st);
                     if (!p.mean) {
                         p.mean = reinterpret_cast<float*>(ws + plan.second);
                         p.rstd = reinterpret_cast<float*>(ws + plan.third);
@@ -1013,16 +1073,16 @@ STG_API stg_status stg_group_norm_backward(stg_engine* e, const stg_group_norm_c
             using T = std::remove_pointer_t<decltype(tag)>;
             with_width<T>(wide, [&](auto v) {
                 constexpr int V = decltype(v)::value;
-                set_plan(p, plan, V);
+                set_plan(p, plan, V, kFusedGrad);
                 with_activation(c->activation, [&](auto a) {
                     constexpr int A = decltype(a)::value;
                     const unsigned join_blocks = (unsigned)((p.channels + 3) / 4);
                     if (plan.path == CLUSTER) {
-                        launch_fused(norm_grad_fused<T, V, A, false>, p, plan, e->sms, st);
+                        launch_fused(norm_grad_fused<T, V, A, false>, p, plan, kFusedGrad, st);
                         if (p.dgamma || p.dbeta) grad_join<T><<<join_blocks, 128, 0, st>>>(p);
                         return;
                     }
-                    if (plan.path == GRID) return launch_fused(norm_grad_fused<T, V, A, true>, p, plan, e->sms, st);
+                    if (plan.path == GRID) return launch_fused(norm_grad_fused<T, V, A, true>, p, plan, kFusedGrad, st);
                     const dim3 grid((unsigned)p.chunks, (unsigned)p.batch);
                     grad_sums_kernel<T, V, A><<<grid, kThreads, 0, st>>>(p);
                     grad_join<T><<<join_blocks, 128, 0, st>>>(p);

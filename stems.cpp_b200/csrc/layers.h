@@ -123,6 +123,96 @@ template <int ACT, bool kFast> __device__ __forceinline__ float act_grad(float z
     return d;
 }
 
+// ---- pairs: two floats to an instruction --------------------------------------------------------
+struct f2 { uint64_t v; };
+__device__ __forceinline__ f2 make_f2(float x, float y) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ f2 make_f2(float x) { return make_f2(x, x); }
+__device__ __forceinline__ float2 split(f2 a) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v)); return r; }
+__device__ __forceinline__ f2 operator+(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ f2 operator*(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+template <class Fn> __device__ __forceinline__ f2 each(f2 a, Fn&& fn) { const float2 v = split(a); return make_f2(fn(v.x), fn(v.y)); }
+
+__device__ __forceinline__ f2 load2(const float* p) { return make_f2(p[0], p[1]); }
+__device__ __forceinline__ f2 load2(const __half* p) { const float2 v = __half22float2(*reinterpret_cast<const __half2*>(p)); return make_f2(v.x, v.y); }
+__device__ __forceinline__ f2 load2(const __nv_bfloat16* p) {   // a bf16 is the upper half of a float
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+    return make_f2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ void store2(float* p, f2 a) { const float2 v = split(a); p[0] = v.x; p[1] = v.y; }
+__device__ __forceinline__ void store2(__half* p, f2 a) { const float2 v = split(a); *reinterpret_cast<__half2*>(p) = __floats2half2_rn(v.x, v.y); }
+__device__ __forceinline__ void store2(__nv_bfloat16* p, f2 a) {
+    const float2 v = split(a);
+    *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y);
+}
+
+// exp(-z) for float results: 2^t, t = -z log2 e rounded, times 1 + ln 2 (what t lost), so that what
+// is left is the approximate power's own 2^-22. Infinite powers are kept finite for that product.
+__device__ __forceinline__ f2 exp_neg(f2 z) {
+    const f2 c = make_f2(-1.4426950216293335f), t = z * c;
+    const f2 lost = each(fma2(z, make_f2(-1.9259629911266175e-8f), fma2(z, c, t * make_f2(-1.0f))),
+                         [](float x) { return fabsf(x) < 1.0f ? x : 0.0f; });   // (infinite z lose nothing)
+    const f2 e = each(t, [](float x) { return fminf(ex2(x), 3.0e38f); });
+    return fma2(e, lost * make_f2(0.6931471805599453f), e);
+}
+template <bool kFast> __device__ __forceinline__ f2 sigmoid2(f2 z) {
+    const f2 e = kFast ? each(z * make_f2(-1.4426950408889634f), [](float x) { return ex2(x); }) : exp_neg(z);
+    return each(e + make_f2(1.0f), [](float x) { return rcp(x); });
+}
+constexpr float kGaussStep = 0.27f;
+__device__ constexpr float kGauss[9] = {0.107720181f, 0.107550503f, 0.10175919f, 0.0722401889f, 0.107399681f, -0.068621354f, 0.169291745f, -0.126255433f, 0.0289153096f};
+// |z| and Phi(-|z|), exp(-z^2 / 2): see gauss(). For float results P has degree 8 on t = 1 / (1 + 0.27 x)
+// (3e-8) and the power makes up for the rounding of z^2.
+template <bool kFast> __device__ __forceinline__ f2 gauss2(f2 z, f2& size, f2& e) {
+    size = each(z, [](float x) { return fminf(fabsf(x), 100.0f); });
+    const f2 t = each(fma2(make_f2(kFast ? 0.36f : kGaussStep), size, make_f2(1.0f)), [](float x) { return rcp(x); });
+    f2 p;
+    if (kFast) {
+        e = each(z * z * make_f2(-0.72134752044448170f), [](float x) { return ex2(x); });
+        p = fma2(t, make_f2(0.047056273f), make_f2(-0.17976463f));
+        p = fma2(t, p, make_f2(0.18095392f));
+        p = fma2(t, p, make_f2(0.026549397f));
+        p = fma2(t, p, make_f2(0.13971923f));
+        p = fma2(t, p, make_f2(0.14177246f));
+        p = fma2(t, p, make_f2(0.14371304f));
+    } else {
+        const f2 zz = each(z * z, [](float x) { return fminf(x, 400.0f); });   // past 14 both factors vanish
+        const f2 lost = fma2(z, z, z * z * make_f2(-1.0f));
+        e = exp_neg(zz * make_f2(0.5f));
+        e = fma2(e, each(lost, [](float x) { return fabsf(x) < 1.0f ? -0.5f * x : 0.0f; }), e);
+        p = make_f2(kGauss[8]);
+#pragma unroll
+        for (int i = 7; i >= 0; i--) p = fma2(t, p, make_f2(kGauss[i]));
+    }
+    return p * t * e;
+}
+// act(z), and act(z) and its derivative, of pairs.
+template <int ACT, bool kFast> __device__ __forceinline__ f2 act2(f2 z) {
+    if (ACT == STG_ACT_RELU) return each(z, [](float x) { return x < 0.0f ? 0.0f : x; });
+    if (ACT == STG_ACT_SILU) return z * sigmoid2<kFast>(z);
+    if (ACT == STG_ACT_GELU) {   // max(z, 0) - |z| Phi(-|z|)
+        f2 size, e;
+        const f2 tail = gauss2<kFast>(z, size, e);
+        return fma2(size * make_f2(-1.0f), tail, each(z, [](float x) { return x < 0.0f ? 0.0f : x; }));
+    }
+    if (ACT == STG_ACT_SIGMOID) return sigmoid2<kFast>(z);
+    return z;
+}
+template <int ACT, bool kFast> __device__ __forceinline__ f2 act_grad2(f2 z) {
+    if (ACT == STG_ACT_RELU) return each(z, [](float x) { return x > 0.0f ? 1.0f : (x <= 0.0f ? 0.0f : x); });
+    if (ACT == STG_ACT_SILU || ACT == STG_ACT_SIGMOID) {
+        const f2 s = sigmoid2<kFast>(z), rest = fma2(s, make_f2(-1.0f), make_f2(1.0f));
+        return ACT == STG_ACT_SIGMOID ? s * rest : fma2(z * s, rest, s);
+    }
+    if (ACT == STG_ACT_GELU) {
+        f2 size, e;
+        const float2 tail = split(gauss2<kFast>(z, size, e)), x = split(z);
+        const f2 phi = make_f2(x.x < 0.0f ? tail.x : 1.0f - tail.x, x.y < 0.0f ? tail.y : 1.0f - tail.y);
+        return fma2(z * make_f2(0.3989422804014327f), e, phi);
+    }
+    return make_f2(1.0f);
+}
+
 // Calls fn with the activation as an integral_constant.
 template <class Fn> void with_activation(int a, Fn&& fn) {
     switch (a) {
