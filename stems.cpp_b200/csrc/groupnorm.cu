@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(const __grid_const
 
 // ---- one launch -------------------------------------------------------------------------------
 
-constexpr int kFused = 1024, kFusedGrad = 512;   // threads forward and backward: what the registers allow
+constexpr int kFused = 512;          // threads: with 1024 the registers do not hold a vector's sums
 constexpr int kFusedGroups = 2048;   // most groups
 constexpr int kClusterMost = 8;
 
@@ -370,16 +370,6 @@ __device__ __forceinline__ float2 peer_read(const float2* p, int rank) {
     return v;
 }
 
-// Pair i of a vector as floats, and back. A vector of one is a pair with nothing beside it.
-template <class T, int V> __device__ __forceinline__ f2 get(const Pack<T, V>& v, int i) {
-    if constexpr (V == 1) return make_f2(to_float(v.v[0]), 0.0f);
-    else return load2(&v.v[2 * i]);
-}
-template <class T, int V> __device__ __forceinline__ void put(Pack<T, V>& v, int i, f2 a) {
-    if constexpr (V == 1) v.v[0] = from_float<T>(split(a).x);
-    else store2(&v.v[2 * i], a);
-}
-
 struct Share { int item, chunk, n; int64_t l0; };
 template <bool GRID> __device__ __forceinline__ Share share_of(const NormParams& p, int round) {
     Share s;
@@ -391,33 +381,44 @@ template <bool GRID> __device__ __forceinline__ Share share_of(const NormParams&
     return s;
 }
 
-// Moments of the block's groups from its threads' parts: [step][width] of them, of `per` channels
-// each, mean and M2 of the rows that place r has. Several warps to a group when groups are few.
-__device__ __forceinline__ void block_moments(const NormParams& p, const Place& q, int n, const float2* part, int vec, float2* group, Moments* red) {
+// Moments of the block's groups from its threads' parts: [step][row] of them, of `per` channels each,
+// mean and M2 of the rows that place r has. The mean of the means first, then the deviations from
+// it, both from the group's first part on; several warps to a group when groups are few.
+__device__ __forceinline__ void block_moments(const NormParams& p, const Place& q, int n, const float2* part, int vec, float2* group, float2* red) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kFused / 32;
     const int per = p.mono ? vec : 1, row = p.channels / per, w = p.cpg / per;   // parts of a row, of a group in a row
     const int rows = min(q.step, n), team = max(1, warps / p.groups);
+    const int base = n / q.step, more = n - base * q.step;       // place r has base rows, and one more below `more`
+    const int member = warp % team, lead = member * 32 + lane;
+    const int r0 = lead / w, c0 = lead - r0 * w, dr = team * 32 / w, dc = team * 32 - dr * w;
+    const float inv = 1.0f / ((float)n * (float)p.cpg);
     for (int g0 = 0; g0 < p.groups; g0 += warps / team) {
-        const int g = g0 + warp / team, member = warp % team;
-        Moments m{0.0f, 0.0f, 0.0f};
-        if (g < p.groups && warp < warps / team * team) {
-            for (int i = member * 32 + lane; i < rows * w; i += team * 32) {
-                const int r = i / w, c = g * w + i - r * w;
-                const float2 v = part[r * row + c];
-                join(m, Moments{(float)((n - r + q.step - 1) / q.step) * (float)per, v.x, v.y});
+        const int g = g0 + warp / team;
+        const bool live = g < p.groups && warp < warps / team * team;
+        const float2* at = part + g * w;
+        const float from = live ? at[0].x : 0.0f;
+        float mean = 0.0f;
+        for (int pass = 0; pass < 2; pass++) {
+            float sum = 0.0f;
+            if (live)
+                for (int r = r0, c = c0; r < rows;) {
+                    const float2 v = at[r * row + c];
+                    const float cnt = (float)((base + (r < more)) * per), d = v.x - from - mean;
+                    sum += pass ? fmaf(cnt * d, d, v.y) : cnt * d;
+                    r += dr;
+                    if ((c += dc) >= w) { c -= w; r++; }
+                }
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            if (team > 1) {   // then every group has its team at once: one round
+                if (lane == 0) reinterpret_cast<float*>(red)[warp] = sum;
+                __syncthreads();
+                sum = 0.0f;
+                if (live)
+                    for (int k = 0; k < team; k++) sum += reinterpret_cast<float*>(red)[warp - member + k];
+                __syncthreads();
             }
-            warp_join(m);
-            if (team == 1) {
-                if (lane == 0) group[g] = make_float2(m.mean, m.m2);
-            } else if (lane == 0) red[warp] = m;
-        }
-        if (team > 1) {   // then every group has its team at once: one round
-            __syncthreads();
-            if (threadIdx.x < p.groups) {
-                Moments t = red[threadIdx.x * team];
-                for (int k = 1; k < team; k++) join(t, red[threadIdx.x * team + k]);
-                group[threadIdx.x] = make_float2(t.mean, t.m2);
-            }
+            if (pass == 0) mean = sum * inv;
+            else if (live && member == 0 && lane == 0) group[g] = make_float2(from + mean, sum);
         }
     }
     __syncthreads();
@@ -426,15 +427,14 @@ __device__ __forceinline__ void block_moments(const NormParams& p, const Place& 
 template <class T, int V, int ACT, bool GRID>
 __global__ void __launch_bounds__(kFused, 1) norm_fused(const __grid_constant__ NormParams p) {
     constexpr bool fast = sizeof(T) == 2;
-    constexpr int U = 4;                        // positions in flight per thread
-    constexpr int N = (V + 1) / 2;
+    constexpr int U = 8, N = (V + 1) / 2;       // positions in flight per thread, pairs of a vector
     using P = Pack<T, V>;
     extern __shared__ __align__(16) uint8_t smem[];
     P* keep = reinterpret_cast<P*>(smem);       // [kept][threads]
     float2* part = reinterpret_cast<float2*>(smem + (size_t)p.kept * kFused * sizeof(P));
     float2* group = part + kFused * (p.mono ? 1 : V);   // [groups]: the block's moments
     float2* stat = group + p.groups;                    // [groups]: the item's mean and rstd
-    __shared__ Moments red[kFused / 32];
+    __shared__ float2 red[kFused / 64];
     Place q;
     q.width = p.columns;
     q.step = kFused / q.width;
@@ -446,24 +446,43 @@ __global__ void __launch_bounds__(kFused, 1) norm_fused(const __grid_constant__ 
     for (int round = 0; round < rounds; round++) {
         const Share s = share_of<GRID>(p, round);
         const T* x = static_cast<const T*>(p.x) + s.item * p.xb + s.l0 * p.xp + ch;
-        const int steps = s.n > 0 ? (s.n + q.step - 1) / q.step : 0;
         if (s.n > 0) {
             if (on && q.r < s.n) {
                 // differences from the first value met, so that a mean far from zero costs no digits
                 f2 pivot[N], a[N], b[N];
+                const T* at = x + (int64_t)q.r * p.xp;
                 {
-                    const P first = *reinterpret_cast<const P*>(x + (int64_t)q.r * p.xp);
+                    const P first = *reinterpret_cast<const P*>(at);
 #pragma unroll
                     for (int i = 0; i < N; i++) {
-                        const float2 f = split(get(first, i));
-                        pivot[i] = p.mono ? make_f2(-to_float(first.v[0])) : make_f2(-f.x, -f.y);
-                        a[i] = b[i] = make_f2(0.0f);
+                        const float2 f = split(get(first, i)), f0 = split(get(first, 0));
+                        pivot[i] = p.mono ? make_f2(-f0.x, -f0.x) : make_f2(-f.x, -f.y);
+                        a[i] = b[i] = make_f2(0.0f, 0.0f);
                     }
                 }
-                const T* at = x + (int64_t)q.r * p.xp;
                 const int64_t step = (int64_t)q.step * p.xp;
                 const int mine = (s.n - q.r + q.step - 1) / q.step;
-                for (int it = 0; it < mine; it += U) {
+                auto take = [&](const P& v) {
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const f2 d = get(v, i) + pivot[i];
+                        a[i] = a[i] + d;
+                        b[i] = fma2(d, d, b[i]);
+                    }
+                };
+                int it = 0;
+                P* k = keep + threadIdx.x;
+                for (; it + U <= min(mine, p.kept); it += U, k += U * kFused) {
+                    P v[U];
+#pragma unroll
+                    for (int u = 0; u < U; u++, at += step) v[u] = *reinterpret_cast<const P*>(at);
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        k[u * kFused] = v[u];
+                        take(v[u]);
+                    }
+                }
+                for (; it < mine; it += U) {
                     P v[U];
 #pragma unroll
                     for (int u = 0; u < U; u++, at += step)
@@ -472,12 +491,7 @@ __global__ void __launch_bounds__(kFused, 1) norm_fused(const __grid_constant__ 
                     for (int u = 0; u < U; u++) {
                         if (it + u >= mine) break;
                         if (it + u < p.kept) keep[(it + u) * kFused + threadIdx.x] = v[u];
-#pragma unroll
-                        for (int i = 0; i < N; i++) {
-                            const f2 d = get(v[u], i) + pivot[i];
-                            a[i] = a[i] + d;
-                            b[i] = fma2(d, d, b[i]);
-                        }
+                        take(v[u]);
                     }
                 }
                 auto moments = [&](float sum, float sq, float n, float neg) {   // + 0 sum: a NaN stays one
@@ -545,46 +559,46 @@ __global__ void __launch_bounds__(kFused, 1) norm_fused(const __grid_constant__ 
                 for (int k = 0; k < 2; k++) {
                     const int c = V == 1 ? ch : ch + 2 * i + k;
                     const float2 st = stat[c / p.cpg];
-                    m[k] = st.x;
+                    m[k] = -st.x;
                     s1[k] = st.y * param(p.gamma, c, p.param_float, 1.0f, (const T*)nullptr);
                     s0[k] = param(p.beta, c, p.param_float, 0.0f, (const T*)nullptr);
-                    if (fast) s0[k] = fmaf(-m[k], s1[k], s0[k]);
+                    if (fast) s0[k] = fmaf(m[k], s1[k], s0[k]);
                 }
-                mu[i] = make_f2(-m[0], -m[1]);
+                mu[i] = make_f2(m[0], m[1]);
                 a[i] = make_f2(s1[0], s1[1]);
                 sh[i] = make_f2(s0[0], s0[1]);
             }
-            T* y = static_cast<T*>(p.y) + s.item * p.yb + s.l0 * p.yp + ch;
-            auto one = [&](P v, int l) {
+            const PairAct<ACT, fast> fn;
+            const int64_t sx = (int64_t)q.step * p.xp, sy = (int64_t)q.step * p.yp;
+            auto one = [&](P v, T* y) {
 #pragma unroll
                 for (int i = 0; i < N; i++) {
-                    f2 z = get(v, i);
-                    if (!fast) z = z + mu[i];
-                    put(v, i, act2<ACT, fast>(fma2(z, a[i], sh[i])));
+                    const f2 f = get(v, i);
+                    put(v, i, fn.value(fma2(fast ? f : f + mu[i], a[i], sh[i])));
                 }
-                *reinterpret_cast<P*>(y + (int64_t)l * p.yp) = v;
+                *reinterpret_cast<P*>(y) = v;
             };
+            const int mine = q.r < s.n ? (s.n - q.r + q.step - 1) / q.step : 0;
             // what was read last and not kept is in L2 yet: from the end
-            int it = steps - 1;
-            constexpr int W = 2;
+            int it = mine - 1;
+            const T* at = x + (q.r + (int64_t)it * q.step) * p.xp;
+            T* y = static_cast<T*>(p.y) + s.item * p.yb + s.l0 * p.yp + ch + (q.r + (int64_t)it * q.step) * p.yp;
+            constexpr int W = 4;
             for (; it >= p.kept; it -= W) {
                 P v[W];
 #pragma unroll
-                for (int u = 0; u < W; u++) {
-                    const int l = q.r + (it - u) * q.step;
-                    if (it - u >= p.kept && l < s.n) v[u] = *reinterpret_cast<const P*>(x + (int64_t)l * p.xp);
-                }
+                for (int u = 0; u < W; u++, at -= sx)
+                    if (it - u >= p.kept) v[u] = *reinterpret_cast<const P*>(at);
 #pragma unroll
-                for (int u = 0; u < W; u++) {
-                    const int l = q.r + (it - u) * q.step;
-                    if (it - u >= p.kept && l < s.n) one(v[u], l);
-                }
+                for (int u = 0; u < W; u++)
+                    if (it - u >= p.kept) {
+                        one(v[u], y);
+                        y -= sy;
+                    }
             }
+            const P* k = keep + min(mine, p.kept) * kFused + threadIdx.x;
 #pragma unroll 2
-            for (it = min(steps, p.kept) - 1; it >= 0; it--) {
-                const int l = q.r + it * q.step;
-                if (l < s.n) one(keep[it * kFused + threadIdx.x], l);
-            }
+            for (it = min(mine, p.kept); it > 0; it--, y -= sy) one(*(k -= kFused), y);
         }
         if (GRID) __syncthreads();   // stat and the kept values are the next round's
         else {
@@ -597,19 +611,20 @@ __global__ void __launch_bounds__(kFused, 1) norm_fused(const __grid_constant__ 
 // Backward: the block's sums of dz and dz xh per channel, of gamma times them per group; the set's
 // blocks meet over the group sums. Channel sums go out per block for dgamma and dbeta.
 template <class T, int V, int ACT, bool GRID>
-__global__ void __launch_bounds__(kFusedGrad, 1) norm_grad_fused(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(kFused, 1) norm_grad_fused(const __grid_constant__ NormParams p) {
     constexpr bool fast = sizeof(T) == 2;
     constexpr int U = 4, N = (V + 1) / 2;
+    const PairAct<ACT, fast> fn;
     using P = Pack<T, V>;
     extern __shared__ __align__(16) uint8_t smem[];
     P* keep = reinterpret_cast<P*>(smem);       // [kept][x, dy][threads]
-    float2* part = reinterpret_cast<float2*>(smem + (size_t)p.kept * 2 * kFusedGrad * sizeof(P));   // [step][channels]
-    float2* chan = part + kFusedGrad * V;           // [channels]
+    float2* part = reinterpret_cast<float2*>(smem + (size_t)p.kept * 2 * kFused * sizeof(P));   // [step][channels]
+    float2* chan = part + kFused * V;           // [channels]
     float2* group = chan + p.channels;          // [groups]: the block's sums
     float2* stat = group + p.groups;            // [groups]: the item's means of d and d xh
     Place q;
     q.width = p.columns;
-    q.step = kFusedGrad / q.width;
+    q.step = kFused / q.width;
     q.r = (int)p.columns_div.div(threadIdx.x);
     q.col = threadIdx.x - q.r * q.width;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ch = q.col * V;
@@ -619,9 +634,10 @@ __global__ void __launch_bounds__(kFusedGrad, 1) norm_grad_fused(const __grid_co
         const Share s = share_of<GRID>(p, round);
         const T* x = static_cast<const T*>(p.x) + s.item * p.xb + s.l0 * p.xp + ch;
         const T* dy = static_cast<const T*>(p.dy) + s.item * p.yb + s.l0 * p.yp + ch;
-        const int steps = s.n > 0 ? (s.n + q.step - 1) / q.step : 0;
         // z = (x - mu) za + zb; the sums are of dz and dz (x - mu), the latter scaled by rstd at the end
         f2 mu[N], za[N], zb[N];
+        const int mine = q.r < s.n ? (s.n - q.r + q.step - 1) / q.step : 0;
+        const int64_t sx = (int64_t)q.step * p.xp, sd = (int64_t)q.step * p.yp;
         if (s.n > 0) {
             if (on) {
                 f2 a[N], b[N];
@@ -641,34 +657,41 @@ __global__ void __launch_bounds__(kFusedGrad, 1) norm_grad_fused(const __grid_co
                     mu[i] = make_f2(m[0], m[1]);
                     za[i] = make_f2(s1[0], s1[1]);
                     zb[i] = make_f2(s0[0], s0[1]);
-                    a[i] = b[i] = make_f2(0.0f);
+                    a[i] = b[i] = make_f2(0.0f, 0.0f);
                 }
+                auto take = [&](const P& v, const P& w) {
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const f2 xm = get(v, i) + mu[i];
+                        const f2 dz = get(w, i) * fn.slope(fma2(xm, za[i], zb[i]));
+                        a[i] = a[i] + dz;
+                        b[i] = fma2(dz, xm, b[i]);
+                    }
+                };
                 const T *ax = x + (int64_t)q.r * p.xp, *ad = dy + (int64_t)q.r * p.yp;
-                const int64_t sx = (int64_t)q.step * p.xp, sd = (int64_t)q.step * p.yp;
-                const int mine = q.r < s.n ? (s.n - q.r + q.step - 1) / q.step : 0;
-                for (int it = 0; it < mine; it += U) {
+                int it = 0;
+                P* k = keep + threadIdx.x;
+                for (; it + U <= min(mine, p.kept); it += U, k += U * 2 * kFused) {
                     P v[U], w[U];
 #pragma unroll
-                    for (int u = 0; u < U; u++, ax += sx, ad += sd)
-                        if (it + u < mine) {
-                            v[u] = *reinterpret_cast<const P*>(ax);
-                            w[u] = *reinterpret_cast<const P*>(ad);
-                        }
+                    for (int u = 0; u < U; u++, ax += sx, ad += sd) {
+                        v[u] = *reinterpret_cast<const P*>(ax);
+                        w[u] = *reinterpret_cast<const P*>(ad);
+                    }
 #pragma unroll
                     for (int u = 0; u < U; u++) {
-                        if (it + u >= mine) break;
-                        if (it + u < p.kept) {
-                            keep[(it + u) * 2 * kFusedGrad + threadIdx.x] = v[u];
-                            keep[(it + u) * 2 * kFusedGrad + kFusedGrad + threadIdx.x] = w[u];
-                        }
-#pragma unroll
-                        for (int i = 0; i < N; i++) {
-                            const f2 xm = get(v[u], i) + mu[i];
-                            const f2 dz = get(w[u], i) * act_grad2<ACT, fast>(fma2(xm, za[i], zb[i]));
-                            a[i] = a[i] + dz;
-                            b[i] = fma2(dz, xm, b[i]);
-                        }
+                        k[u * 2 * kFused] = v[u];
+                        k[u * 2 * kFused + kFused] = w[u];
+                        take(v[u], w[u]);
                     }
+                }
+                for (; it < mine; it++, ax += sx, ad += sd) {
+                    const P v = *reinterpret_cast<const P*>(ax), w = *reinterpret_cast<const P*>(ad);
+                    if (it < p.kept) {
+                        keep[it * 2 * kFused + threadIdx.x] = v;
+                        keep[it * 2 * kFused + kFused + threadIdx.x] = w;
+                    }
+                    take(v, w);
                 }
 #pragma unroll
                 for (int j = 0; j < V; j++) {
@@ -677,7 +700,7 @@ __global__ void __launch_bounds__(kFusedGrad, 1) norm_grad_fused(const __grid_co
                 }
             }
             __syncthreads();
-            for (int c = threadIdx.x; c < p.channels; c += kFusedGrad) {
+            for (int c = threadIdx.x; c < p.channels; c += kFused) {
                 float2 t = make_float2(0.0f, 0.0f);
                 for (int r = 0; r < q.step; r++) {
                     const float2 v = part[r * p.channels + c];
@@ -688,7 +711,7 @@ __global__ void __launch_bounds__(kFusedGrad, 1) norm_grad_fused(const __grid_co
                 p.part[((int64_t)s.item * p.chunks + s.chunk) * p.channels + c] = t;
             }
             __syncthreads();
-            for (int g = warp; g < p.groups; g += kFusedGrad / 32) {
+            for (int g = warp; g < p.groups; g += kFused / 32) {
                 float a = 0.0f, b = 0.0f;
                 for (int k = lane; k < p.cpg; k += 32) {
                     const int c = g * p.cpg + k;
@@ -714,7 +737,7 @@ __global__ void __launch_bounds__(kFusedGrad, 1) norm_grad_fused(const __grid_co
         }
         if (s.n > 0 && p.dx) {
             const float m = (float)p.positions * (float)p.cpg;
-            for (int g = warp; g < p.groups; g += kFusedGrad / 32) {
+            for (int g = warp; g < p.groups; g += kFused / 32) {
                 float a = 0.0f, b = 0.0f;
                 for (int c = lane; c < p.used; c += 32) {
                     const float2 v = GRID ? __ldcg(p.sums + ((int64_t)s.item * p.groups + g) * p.chunks + c) : peer_read(group + g, c);
@@ -747,38 +770,40 @@ __global__ void __launch_bounds__(kFusedGrad, 1) norm_grad_fused(const __grid_co
                 c1[i] = make_f2(u1[0], u1[1]);
                 c2[i] = make_f2(u2[0], u2[1]);
             }
-            T* dx = static_cast<T*>(p.dx) + s.item * p.db + s.l0 * p.dp + ch;
-            auto one = [&](const P& v, const P& w, int l) {
+            auto one = [&](const P& v, const P& w, T* dx) {
                 P o;
 #pragma unroll
                 for (int i = 0; i < N; i++) {
                     const f2 xm = get(v, i) + mu[i];
-                    const f2 dz = get(w, i) * act_grad2<ACT, fast>(fma2(xm, za[i], zb[i]));
+                    const f2 dz = get(w, i) * fn.slope(fma2(xm, za[i], zb[i]));
                     put(o, i, fma2(dz, za[i], fma2(xm, c2[i], c1[i])));
                 }
-                *reinterpret_cast<P*>(dx + (int64_t)l * p.dp) = o;
+                *reinterpret_cast<P*>(dx) = o;
             };
-            int it = steps - 1;
+            int it = mine - 1;
+            const int64_t last = q.r + (int64_t)it * q.step, so = (int64_t)q.step * p.dp;
+            const T *ax = x + last * p.xp, *ad = dy + last * p.yp;
+            T* dx = static_cast<T*>(p.dx) + s.item * p.db + (s.l0 + last) * p.dp + ch;
             constexpr int W = 2;
             for (; it >= p.kept; it -= W) {
                 P v[W], w[W];
 #pragma unroll
-                for (int u = 0; u < W; u++) {
-                    const int l = q.r + (it - u) * q.step;
-                    if (it - u >= p.kept && l < s.n) {
-                        v[u] = *reinterpret_cast<const P*>(x + (int64_t)l * p.xp);
-                        w[u] = *reinterpret_cast<const P*>(dy + (int64_t)l * p.yp);
+                for (int u = 0; u < W; u++, ax -= sx, ad -= sd)
+                    if (it - u >= p.kept) {
+                        v[u] = *reinterpret_cast<const P*>(ax);
+                        w[u] = *reinterpret_cast<const P*>(ad);
                     }
-                }
 #pragma unroll
-                for (int u = 0; u < W; u++) {
-                    const int l = q.r + (it - u) * q.step;
-                    if (it - u >= p.kept && l < s.n) one(v[u], w[u], l);
-                }
+                for (int u = 0; u < W; u++)
+                    if (it - u >= p.kept) {
+                        one(v[u], w[u], dx);
+                        dx -= so;
+                    }
             }
-            for (it = min(steps, p.kept) - 1; it >= 0; it--) {
-                const int l = q.r + it * q.step;
-                if (l < s.n) one(keep[it * 2 * kFusedGrad + threadIdx.x], keep[it * 2 * kFusedGrad + kFusedGrad + threadIdx.x], l);
+            const P* k = keep + min(mine, p.kept) * 2 * kFused + threadIdx.x;
+            for (it = min(mine, p.kept); it > 0; it--, dx -= so) {
+                k -= 2 * kFused;
+                one(k[0], k[kFused], dx);
             }
         }
         if (GRID) __syncthreads();
@@ -788,8 +813,8 @@ __global__ void __launch_bounds__(kFusedGrad, 1) norm_grad_fused(const __grid_co
         }
     }
     if (GRID && (p.dgamma || p.dbeta)) {   // every item's parts were complete at the last meeting
-        const int all = (int)gridDim.x * (kFusedGrad / 32);
-        for (int c = blockIdx.x * (kFusedGrad / 32) + warp; c < p.channels; c += all) {
+        const int all = (int)gridDim.x * (kFused / 32);
+        for (int c = blockIdx.x * (kFused / 32) + warp; c < p.channels; c += all) {
             float a = 0.0f, b = 0.0f;
             for (int k = lane; k < p.batch * p.chunks; k += 32) {
                 const float2 v = __ldcg(p.part + (int64_t)k * p.channels + c);
@@ -849,15 +874,14 @@ NormPlan plan_of(const stg_group_norm_config& c, bool backward, int vec, int sms
     NormPlan r;
     if (!c.batch || !c.positions) return r;
     const int columns = c.channels / vec, cpg = c.channels / c.groups;
-    const int threads = backward ? kFusedGrad : kFused;
-    const size_t vb = (size_t)vec * elem_size(c.dtype) * (backward ? 2 : 1), block_step = vb * threads;
+    const size_t vb = (size_t)vec * elem_size(c.dtype) * (backward ? 2 : 1), block_step = vb * kFused;
     const bool mono = cpg % vec == 0;
     // shared memory besides the kept values: the threads' parts, channel and group sums
-    const size_t other = backward ? sizeof(float2) * ((size_t)threads * vec + c.channels + 2 * (size_t)c.groups)
-                                  : sizeof(float2) * ((size_t)threads * (mono ? 1 : vec) + 2 * (size_t)c.groups);
+    const size_t other = backward ? sizeof(float2) * ((size_t)kFused * vec + c.channels + 2 * (size_t)c.groups)
+                                  : sizeof(float2) * ((size_t)kFused * (mono ? 1 : vec) + 2 * (size_t)c.groups);
     const size_t most = 225 * 1024;
-    if (columns <= threads && c.groups <= kFusedGroups && other + 8 * block_step <= most) {
-        const int64_t step = threads / columns, room = (int64_t)((most - other) / block_step);   // steps a block can keep
+    if (columns <= kFused && c.groups <= kFusedGroups && other + 8 * block_step <= most) {
+        const int64_t step = kFused / columns, room = (int64_t)((most - other) / block_step);   // steps a block can keep
         const int64_t item_steps = (c.positions + step - 1) / step;
         int64_t blocks = (item_steps + room - 1) / room;
         if (blocks <= kClusterMost) {
@@ -1073,16 +1097,16 @@ STG_API stg_status stg_group_norm_backward(stg_engine* e, const stg_group_norm_c
             using T = std::remove_pointer_t<decltype(tag)>;
             with_width<T>(wide, [&](auto v) {
                 constexpr int V = decltype(v)::value;
-                set_plan(p, plan, V, kFusedGrad);
+                set_plan(p, plan, V, kFused);
                 with_activation(c->activation, [&](auto a) {
                     constexpr int A = decltype(a)::value;
                     const unsigned join_blocks = (unsigned)((p.channels + 3) / 4);
                     if (plan.path == CLUSTER) {
-                        launch_fused(norm_grad_fused<T, V, A, false>, p, plan, kFusedGrad, st);
+                        launch_fused(norm_grad_fused<T, V, A, false>, p, plan, kFused, st);
                         if (p.dgamma || p.dbeta) grad_join<T><<<join_blocks, 128, 0, st>>>(p);
                         return;
                     }
-                    if (plan.path == GRID) return launch_fused(norm_grad_fused<T, V, A, true>, p, plan, kFusedGrad, st);
+                    if (plan.path == GRID) return launch_fused(norm_grad_fused<T, V, A, true>, p, plan, kFused, st);
                     const dim3 grid((unsigned)p.chunks, (unsigned)p.batch);
                     grad_sums_kernel<T, V, A><<<grid, kThreads, 0, st>>>(p);
                     grad_join<T><<<join_blocks, 128, 0, st>>>(p);

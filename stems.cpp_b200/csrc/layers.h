@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace stg {
 
 // The engine's device for one call; the caller's current device again afterwards.
@@ -60,50 +62,90 @@ template <class Fn> void with_dtype(int dtype, Fn&& fn) {
 }
 
 // ---- activations --------------------------------------------------------------------------------
-// Float results (kFast false) use CUDA's expf, erfcf and division. Results that are rounded to 16
-// bits use the approximate exponential and reciprocal (2^-22 relative each): a function then
-// costs two special-function instructions and a few multiplications, where the
-// accurate ones made group norm with GELU compute-bound (213 us where the memory takes 40).
+// Built on the approximate power of two and reciprocal (2^-22 relative each). For results that are
+// rounded to 16 bits (kFast) those do as they are; float results make up for the roundings of
+// the exponent, which is what is left of an exponential's error otherwise. CUDA's accurate erfcf,
+// expf and division made group norm with GELU compute-bound (213 us where the memory takes 40).
 __device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 __device__ __forceinline__ float rcp(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-// 1 / (1 + 2^(-z log2 e)); 0 where the power is infinite.
-template <bool kFast> __device__ __forceinline__ float sigmoid(float z) {
-    return kFast ? rcp(1.0f + ex2(-1.4426950408889634f * z)) : 1.0f / (1.0f + expf(-z));
+__device__ __forceinline__ float relu(float x) { float r; asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x)); return r; }   // keeps NaN
+// exp(-z) for float results: 2^t, t = -z log2 e rounded, times 1 + ln 2 (what t lost), so that what
+// is left is the approximate power's own 2^-22. Infinite powers are kept finite for that product.
+__device__ __forceinline__ float exp_neg(float z) {
+    const float t = z * -1.4426950216293335f;
+    const float lost = fmaf(z, -1.9259629911266175e-8f, fmaf(z, -1.4426950216293335f, -t));
+    const float e = fminf(ex2(t), 3.0e38f);
+    return fmaf(e, fabsf(lost) < 1.0f ? lost * 0.6931471805599453f : 0.0f, e);   // infinite z lose nothing
 }
-// Phi(z), the normal distribution function, and e = exp(-z^2 / 2). Phi(-|z|) = e R(|z|) with R(x) =
-// erfcx(x / sqrt 2) / 2, which falls smoothly from 1/2 to 1 / (x sqrt(2 pi)) and is fitted here by
-// t P(t), t = 1 / (1 + 0.36 x), P of degree 6: minimax on [0, 14] (iteratively reweighted least
-// squares in double), 1.2e-6 relative in float. Past 13 e is zero in float.
-__device__ __forceinline__ float gauss(float z, float& e) {
-    const float t = rcp(fmaf(0.36f, fabsf(z), 1.0f));
-    e = ex2(-0.72134752044448170f * z * z);
-    float p = fmaf(t, 0.047056273f, -0.17976463f);
-    p = fmaf(t, p, 0.18095392f);
-    p = fmaf(t, p, 0.026549397f);
-    p = fmaf(t, p, 0.13971923f);
-    p = fmaf(t, p, 0.14177246f);
-    p = fmaf(t, p, 0.14371304f);
-    const float tail = p * t * e;
-    return z < 0.0f ? tail : 1.0f - tail;   // a NaN in z is one in tail
+// 1 / (1 + e^-z); 0 where the power is infinite.
+template <bool kFast> __device__ __forceinline__ float sigmoid(float z) {
+    return rcp(1.0f + (kFast ? ex2(-1.4426950408889634f * z) : exp_neg(z)));
+}
+// Phi(-x), the normal distribution's tail, for x >= 0, as 2^S(x): S = log2 Phi(-x) is smooth and
+// nearly a parabola, here a polynomial of degree 10 (minimax in the error of the power, by
+// iteratively reweighted least squares in double): in float 4e-6 relative for x <= 4, 2e-5 at 9, where
+// Phi is 1e-19 and the polynomial ends. One special function and no division: the rational form it
+// replaces (1 / (1 + c x) and exp(-x^2 / 2)) took two and four instructions more.
+__device__ __forceinline__ float normal_tail(float x) {
+    float s = -1.87925829e-09f;
+    s = fmaf(s, x, 8.08722736e-08f);
+    s = fmaf(s, x, -1.3956618e-06f);
+    s = fmaf(s, x, 1.1034977e-05f);
+    s = fmaf(s, x, -8.45205791e-06f);
+    s = fmaf(s, x, -0.000698472729f);
+    s = fmaf(s, x, 0.00804607337f);
+    s = fmaf(s, x, -0.0534383855f);
+    s = fmaf(s, x, -0.458760105f);
+    s = fmaf(s, x, -1.15118688f);
+    s = fmaf(s, x, -0.999997556f);
+    return ex2(s);
+}
+// Phi(-x) and e = exp(-x^2 / 2) for float results: Phi(-x) = e R(x), R(x) = erfcx(x / sqrt 2) / 2 fitted by
+// t P(t), t = 1 / (1 + 0.27 x), P of degree 8 (2.4e-8 on [0, 14], by the same means); e makes up for
+// the rounding of x^2.
+__device__ __forceinline__ float normal_tail(float x, float& e) {
+    const float t = rcp(fmaf(0.27f, x, 1.0f));
+    const float xx = fminf(x * x, 400.0f), lost = fmaf(x, x, -x * x);   // past 14 both factors vanish
+    e = exp_neg(0.5f * xx);
+    e = fmaf(e, fabsf(lost) < 1.0f ? -0.5f * lost : 0.0f, e);
+    float p = 0.0289153096f;
+    p = fmaf(t, p, -0.126255433f);
+    p = fmaf(t, p, 0.169291745f);
+    p = fmaf(t, p, -0.068621354f);
+    p = fmaf(t, p, 0.107399681f);
+    p = fmaf(t, p, 0.0722401889f);
+    p = fmaf(t, p, 0.10175919f);
+    p = fmaf(t, p, 0.107550503f);
+    p = fmaf(t, p, 0.107720181f);
+    return p * t * e;
+}
+// act(z).
+template <int ACT, bool kFast> __device__ __forceinline__ float act(float z) {
+    if (ACT == STG_ACT_RELU) return relu(z);
+    if (ACT == STG_ACT_SILU) return z * sigmoid<kFast>(z);
+    if (ACT == STG_ACT_GELU) {   // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+        float e;
+        const float u = fminf(fabsf(z), kFast ? 9.0f : 100.0f);
+        return fmaf(-u, kFast ? normal_tail(u) : normal_tail(u, e), relu(z));
+    }
+    if (ACT == STG_ACT_SIGMOID) return sigmoid<kFast>(z);
+    return z;
 }
 // act(z) and its derivative.
 template <int ACT, bool kFast> __device__ __forceinline__ void act_both(float z, float& a, float& d) {
     if (ACT == STG_ACT_RELU) {
-        a = z < 0.0f ? 0.0f : z;                             // keeps NaN
+        a = relu(z);
         d = z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
     } else if (ACT == STG_ACT_SILU) {
         const float s = sigmoid<kFast>(z);
         a = z * s;
         d = fmaf(a, 1.0f - s, s);
     } else if (ACT == STG_ACT_GELU) {
-        float e, phi;
-        if (kFast) phi = gauss(z, e);
-        else {
-            phi = 0.5f * erfcf(-z * 0.70710678118654752f);
-            e = expf(-0.5f * z * z);
-        }
-        a = z * phi;
-        d = fmaf(0.3989422804014327f * z, e, phi);
+        float e;
+        const float u = fminf(fabsf(z), kFast ? 9.0f : 100.0f), tail = kFast ? normal_tail(u) : normal_tail(u, e);
+        if (kFast) e = ex2(-0.72134752044448170f * z * z);
+        a = fmaf(-u, tail, relu(z));
+        d = fmaf(0.3989422804014327f * z, e, z < 0.0f ? tail : 1.0f - tail);
     } else if (ACT == STG_ACT_SIGMOID) {
         a = sigmoid<kFast>(z);
         d = a * (1.0f - a);
@@ -111,11 +153,6 @@ template <int ACT, bool kFast> __device__ __forceinline__ void act_both(float z,
         a = z;
         d = 1.0f;
     }
-}
-template <int ACT, bool kFast> __device__ __forceinline__ float act(float z) {
-    float a, d;
-    act_both<ACT, kFast>(z, a, d);
-    return a;
 }
 template <int ACT, bool kFast> __device__ __forceinline__ float act_grad(float z) {
     float a, d;
@@ -126,92 +163,97 @@ template <int ACT, bool kFast> __device__ __forceinline__ float act_grad(float z
 // ---- pairs: two floats to an instruction --------------------------------------------------------
 struct f2 { uint64_t v; };
 __device__ __forceinline__ f2 make_f2(float x, float y) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y)); return r; }
-__device__ __forceinline__ f2 make_f2(float x) { return make_f2(x, x); }
+// A constant for both, kept in registers: left to the compiler it is made again at each use, which
+// costs as much as the packed instruction saves.
+__device__ __forceinline__ f2 held_f2(float x) { f2 r; asm volatile("mov.b64 %0, {%1, %1};" : "=l"(r.v) : "f"(x)); return r; }
 __device__ __forceinline__ float2 split(f2 a) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v)); return r; }
 __device__ __forceinline__ f2 operator+(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
 __device__ __forceinline__ f2 operator*(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
 __device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
 template <class Fn> __device__ __forceinline__ f2 each(f2 a, Fn&& fn) { const float2 v = split(a); return make_f2(fn(v.x), fn(v.y)); }
 
-__device__ __forceinline__ f2 load2(const float* p) { return make_f2(p[0], p[1]); }
-__device__ __forceinline__ f2 load2(const __half* p) { const float2 v = __half22float2(*reinterpret_cast<const __half2*>(p)); return make_f2(v.x, v.y); }
-__device__ __forceinline__ f2 load2(const __nv_bfloat16* p) {   // a bf16 is the upper half of a float
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
-    return make_f2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+// Pair i of a vector as floats, and back. A vector of one is a pair with nothing beside it.
+template <class T, int V> __device__ __forceinline__ f2 get(const Pack<T, V>& v, int i) {
+    if constexpr (V == 1) return make_f2(to_float(v.v[0]), 0.0f);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) {   // a bf16 is the upper half of a float
+        const uint32_t u = reinterpret_cast<const uint32_t*>(&v)[i];
+        return make_f2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    } else if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(reinterpret_cast<const __half2*>(&v)[i]);
+        return make_f2(f.x, f.y);
+    } else return make_f2(v.v[2 * i], v.v[2 * i + 1]);
 }
-__device__ __forceinline__ void store2(float* p, f2 a) { const float2 v = split(a); p[0] = v.x; p[1] = v.y; }
-__device__ __forceinline__ void store2(__half* p, f2 a) { const float2 v = split(a); *reinterpret_cast<__half2*>(p) = __floats2half2_rn(v.x, v.y); }
-__device__ __forceinline__ void store2(__nv_bfloat16* p, f2 a) {
-    const float2 v = split(a);
-    *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y);
+template <class T, int V> __device__ __forceinline__ void put(Pack<T, V>& v, int i, f2 a) {
+    const float2 f = split(a);
+    if constexpr (V == 1) v.v[0] = from_float<T>(f.x);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) reinterpret_cast<__nv_bfloat162*>(&v)[i] = __floats2bfloat162_rn(f.x, f.y);
+    else if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2*>(&v)[i] = __floats2half2_rn(f.x, f.y);
+    else { v.v[2 * i] = f.x; v.v[2 * i + 1] = f.y; }
 }
 
-// exp(-z) for float results: 2^t, t = -z log2 e rounded, times 1 + ln 2 (what t lost), so that what
-// is left is the approximate power's own 2^-22. Infinite powers are kept finite for that product.
-__device__ __forceinline__ f2 exp_neg(f2 z) {
-    const f2 c = make_f2(-1.4426950216293335f), t = z * c;
-    const f2 lost = each(fma2(z, make_f2(-1.9259629911266175e-8f), fma2(z, c, t * make_f2(-1.0f))),
-                         [](float x) { return fabsf(x) < 1.0f ? x : 0.0f; });   // (infinite z lose nothing)
-    const f2 e = each(t, [](float x) { return fminf(ex2(x), 3.0e38f); });
-    return fma2(e, lost * make_f2(0.6931471805599453f), e);
-}
-template <bool kFast> __device__ __forceinline__ f2 sigmoid2(f2 z) {
-    const f2 e = kFast ? each(z * make_f2(-1.4426950408889634f), [](float x) { return ex2(x); }) : exp_neg(z);
-    return each(e + make_f2(1.0f), [](float x) { return rcp(x); });
-}
-constexpr float kGaussStep = 0.27f;
-__device__ constexpr float kGauss[9] = {0.107720181f, 0.107550503f, 0.10175919f, 0.0722401889f, 0.107399681f, -0.068621354f, 0.169291745f, -0.126255433f, 0.0289153096f};
-// |z| and Phi(-|z|), exp(-z^2 / 2): see gauss(). For float results P has degree 8 on t = 1 / (1 + 0.27 x)
-// (3e-8) and the power makes up for the rounding of z^2.
-template <bool kFast> __device__ __forceinline__ f2 gauss2(f2 z, f2& size, f2& e) {
-    size = each(z, [](float x) { return fminf(fabsf(x), 100.0f); });
-    const f2 t = each(fma2(make_f2(kFast ? 0.36f : kGaussStep), size, make_f2(1.0f)), [](float x) { return rcp(x); });
-    f2 p;
-    if (kFast) {
-        e = each(z * z * make_f2(-0.72134752044448170f), [](float x) { return ex2(x); });
-        p = fma2(t, make_f2(0.047056273f), make_f2(-0.17976463f));
-        p = fma2(t, p, make_f2(0.18095392f));
-        p = fma2(t, p, make_f2(0.026549397f));
-        p = fma2(t, p, make_f2(0.13971923f));
-        p = fma2(t, p, make_f2(0.14177246f));
-        p = fma2(t, p, make_f2(0.14371304f));
-    } else {
-        const f2 zz = each(z * z, [](float x) { return fminf(x, 400.0f); });   // past 14 both factors vanish
-        const f2 lost = fma2(z, z, z * z * make_f2(-1.0f));
-        e = exp_neg(zz * make_f2(0.5f));
-        e = fma2(e, each(lost, [](float x) { return fabsf(x) < 1.0f ? -0.5f * x : 0.0f; }), e);
-        p = make_f2(kGauss[8]);
+// act() and act_grad() of pairs. Float results go through the plain functions; 16-bit ones keep their
+// constants in registers.
+template <int ACT, bool kFast> struct PairAct {
+    __device__ __forceinline__ f2 value(f2 z) const { return each(z, [](float x) { return act<ACT, kFast>(x); }); }
+    __device__ __forceinline__ f2 slope(f2 z) const { return each(z, [](float x) { return act_grad<ACT, kFast>(x); }); }
+};
+template <> struct PairAct<STG_ACT_NONE, true> {
+    __device__ __forceinline__ f2 value(f2 z) const { return z; }
+    __device__ __forceinline__ f2 slope(f2) const { return make_f2(1.0f, 1.0f); }
+};
+template <> struct PairAct<STG_ACT_NONE, false> : PairAct<STG_ACT_NONE, true> {};
+struct PairSigmoid {
+    f2 log2e = held_f2(-1.4426950408889634f), one = held_f2(1.0f);
+    __device__ __forceinline__ f2 sigmoid(f2 z) const { return each(each(z * log2e, ex2) + one, rcp); }
+    __device__ __forceinline__ f2 rest(f2 s) const { return each(s, [](float x) { return 1.0f - x; }); }
+};
+template <> struct PairAct<STG_ACT_SILU, true> : PairSigmoid {
+    __device__ __forceinline__ f2 value(f2 z) const { return z * sigmoid(z); }
+    __device__ __forceinline__ f2 slope(f2 z) const {
+        const f2 s = sigmoid(z);
+        return fma2(z * s, rest(s), s);
+    }
+};
+template <> struct PairAct<STG_ACT_SIGMOID, true> : PairSigmoid {
+    __device__ __forceinline__ f2 value(f2 z) const { return sigmoid(z); }
+    __device__ __forceinline__ f2 slope(f2 z) const {
+        const f2 s = sigmoid(z);
+        return s * rest(s);
+    }
+};
+template <> struct PairAct<STG_ACT_GELU, true> {   // normal_tail's polynomial in -|z|
+    f2 c[11] = {held_f2(-0.999997556f),
+               held_f2(1.15118688f),
+               held_f2(-0.458760105f),
+               held_f2(0.0534383855f),
+               held_f2(0.00804607337f),
+               held_f2(0.000698472729f),
+               held_f2(-8.45205791e-06f),
+               held_f2(-1.1034977e-05f),
+               held_f2(-1.3956618e-06f),
+               held_f2(-8.08722736e-08f),
+               held_f2(-1.87925829e-09f)};
+    // w = max(-|z|, -9); Phi(w)
+    __device__ __forceinline__ f2 tail(f2 z, f2& w) const {
+        w = each(z, [](float x) { return fmaxf(-fabsf(x), -9.0f); });
+        f2 s = c[10];
 #pragma unroll
-        for (int i = 7; i >= 0; i--) p = fma2(t, p, make_f2(kGauss[i]));
+        for (int i = 9; i >= 0; i--) s = fma2(s, w, c[i]);
+        return each(s, ex2);
     }
-    return p * t * e;
-}
-// act(z), and act(z) and its derivative, of pairs.
-template <int ACT, bool kFast> __device__ __forceinline__ f2 act2(f2 z) {
-    if (ACT == STG_ACT_RELU) return each(z, [](float x) { return x < 0.0f ? 0.0f : x; });
-    if (ACT == STG_ACT_SILU) return z * sigmoid2<kFast>(z);
-    if (ACT == STG_ACT_GELU) {   // max(z, 0) - |z| Phi(-|z|)
-        f2 size, e;
-        const f2 tail = gauss2<kFast>(z, size, e);
-        return fma2(size * make_f2(-1.0f), tail, each(z, [](float x) { return x < 0.0f ? 0.0f : x; }));
+    __device__ __forceinline__ f2 value(f2 z) const {
+        f2 w;
+        const f2 t = tail(z, w);
+        return fma2(w, t, each(z, relu));
     }
-    if (ACT == STG_ACT_SIGMOID) return sigmoid2<kFast>(z);
-    return z;
-}
-template <int ACT, bool kFast> __device__ __forceinline__ f2 act_grad2(f2 z) {
-    if (ACT == STG_ACT_RELU) return each(z, [](float x) { return x > 0.0f ? 1.0f : (x <= 0.0f ? 0.0f : x); });
-    if (ACT == STG_ACT_SILU || ACT == STG_ACT_SIGMOID) {
-        const f2 s = sigmoid2<kFast>(z), rest = fma2(s, make_f2(-1.0f), make_f2(1.0f));
-        return ACT == STG_ACT_SIGMOID ? s * rest : fma2(z * s, rest, s);
+    __device__ __forceinline__ f2 slope(f2 z) const {
+        f2 w;
+        const float2 t = split(tail(z, w)), x = split(z);
+        const f2 phi = make_f2(x.x < 0.0f ? t.x : 1.0f - t.x, x.y < 0.0f ? t.y : 1.0f - t.y);
+        const f2 e = each(z * z, [](float v) { return 0.3989422804014327f * ex2(-0.72134752044448170f * v); });
+        return fma2(z, e, phi);
     }
-    if (ACT == STG_ACT_GELU) {
-        f2 size, e;
-        const float2 tail = split(gauss2<kFast>(z, size, e)), x = split(z);
-        const f2 phi = make_f2(x.x < 0.0f ? tail.x : 1.0f - tail.x, x.y < 0.0f ? tail.y : 1.0f - tail.y);
-        return fma2(z * make_f2(0.3989422804014327f), e, phi);
-    }
-    return make_f2(1.0f);
-}
+};
 
 // Calls fn with the activation as an integral_constant.
 template <class Fn> void with_activation(int a, Fn&& fn) {
