@@ -8,23 +8,18 @@
 //   dbeta = sum dz,  dgamma = sum dz xh  (over items and positions),
 //   dx = rstd (d - sum(d) / m - xh sum(d xh) / m),  d = gamma dz.
 //
-// The floor is one read of x (and dy) and one write, so what a block has read for the statistics
-// it keeps in shared memory for the second look, and one launch does both: the positions of
-// an item are dealt to a set of blocks, each takes the moments of its share, the set meets, joins
-// the moments in a fixed order and applies them.
-//   - An item that fits the shared memory of up to eight blocks is a cluster's, which
-//     meets in hardware and reads each other's moments there; items do not wait for each other.
-//   - Larger items take all SMs (as many items at a time as fit the GPU's shared memory, at
-//     least one) in a cooperative launch; what does not fit is read again, from L2 where it can be.
-//   - Very many groups or channels, whose moments would themselves be much to exchange, take
-//     three launches: moments, their joining, a second reading.
+// The floor is one read of x (and dy) and one write.
+//   - An item that fits the shared memory of up to eight blocks is a cluster's: each block keeps
+//     its positions in shared memory, the blocks meet in hardware and read each other's moments
+//     there. One launch, one read, and items do not wait for each other.
+//   - Larger items take three launches: moments by block, their joining, and a second reading in the
+//     opposite order, so that what the first left in L2 is met there. A cooperative launch that
+//     kept 26 MB in the SMs' shared memory instead stood still at each item's meeting: 121 us for
+//     4 x 172032 x 96 bf16.
 // A block's threads stand side by side along the channels (16-byte vectors, whole rows, so every
-// sector is used whatever the group size) and step down the positions.
+// sector is used whatever the group size) and step down the positions. Each takes the differences
+// from the first value it meets, so that a mean far from zero costs no digits.
 #include "layers.h"
-
-#include <cooperative_groups.h>
-
-namespace cg = cooperative_groups;
 
 namespace stg {
 
@@ -47,8 +42,7 @@ struct NormParams {
     FastDiv columns_div;             // by min(columns, kThreads)
     float eps;
     int param_float;
-    // one-launch kernels: items at a time, steps a thread keeps, blocks of an item (= chunks)
-    int at_once, kept;
+    int kept;                        // cluster: steps a thread keeps
     int mono;                        // a vector's channels are of one group
 };
 
@@ -85,88 +79,322 @@ template <class T> __device__ __forceinline__ void set_param(void* p, int i, boo
     else static_cast<T*>(p)[i] = from_float<T>(v);
 }
 
+// A vector's last read, and a result that is not read here: both leave L2 first.
+template <class P, class T> __device__ __forceinline__ P load_stream(const T* p) {
+    P v;
+    if constexpr (sizeof(P) == 16) {
+        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+        v = *reinterpret_cast<const P*>(&u);
+    } else v = *reinterpret_cast<const P*>(p);
+    return v;
+}
+template <class T, class P> __device__ __forceinline__ void store_stream(T* p, const P& v) {
+    if constexpr (sizeof(P) == 16) __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
+    else *reinterpret_cast<P*>(p) = v;
+}
+
 // The thread's place in a block: column vector `col` of the current column tile and one of
 // `step` positions taken side by side.
 struct Place { int width, step, r, col; };
-__device__ __forceinline__ Place place(const NormParams& p) {
+template <int THREADS> __device__ __forceinline__ Place place(const NormParams& p) {
     Place q;
     q.width = (int)p.columns_div.d;
-    q.step = kThreads / q.width;
+    q.step = THREADS / q.width;
     q.r = (int)p.columns_div.div(threadIdx.x);
     q.col = threadIdx.x - q.r * q.width;
     return q;
 }
+// Positions of n that place q has.
+__device__ __forceinline__ int mine_of(const Place& q, int n) { return q.r < n ? (n - q.r + q.step - 1) / q.step : 0; }
 
-// Moments of a chunk's groups. Each thread sums its channels' differences from the first value
-// it meets, so that a mean far from zero costs no digits.
+// load() then use() n times, in that order each, with the loads U to 2U ahead.
+template <class P, int U, class Load, class Use> __device__ __forceinline__ void stream(int n, Load&& load, Use&& use) {
+    P now[U], next[U];
+    if (n >= U) {
+#pragma unroll
+        for (int u = 0; u < U; u++) load(now[u]);
+#pragma unroll 2
+        for (; n >= 2 * U; n -= U) {
+#pragma unroll
+            for (int u = 0; u < U; u++) load(next[u]);
+#pragma unroll
+            for (int u = 0; u < U; u++) use(now[u]);
+#pragma unroll
+            for (int u = 0; u < U; u++) now[u] = next[u];
+        }
+        n -= U;
+        // the rest is on its way while the last whole batch is used
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (u < n) load(next[u]);
+#pragma unroll
+        for (int u = 0; u < U; u++) use(now[u]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (u < n) load(next[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (u < n) use(next[u]);
+}
+template <class P> struct Two { P x, dy; };
+
+// A thread's sums of its channels.
+template <class T, int V> struct Sums {
+    static constexpr int N = (V + 1) / 2;
+    f2 pivot[N], a[N], b[N];
+    __device__ __forceinline__ void start(const Pack<T, V>& first, bool mono) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float2 f = split(get(first, i)), f0 = split(get(first, 0));
+            pivot[i] = mono ? make_f2(-f0.x, -f0.x) : make_f2(-f.x, -f.y);
+            a[i] = b[i] = make_f2(0.0f, 0.0f);
+        }
+    }
+    __device__ __forceinline__ void take(const Pack<T, V>& v) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const f2 d = get(v, i) + pivot[i];
+            a[i] = a[i] + d;
+            b[i] = fma2(d, d, b[i]);
+        }
+    }
+    // Mean and M2 of the `mine` positions: one part for the vector when its channels are of one
+    // group, else one for each channel.
+    __device__ __forceinline__ void finish(int mine, bool mono, float2* part, int at) {
+        auto moments = [](float sum, float sq, float n, float neg) {   // + 0 sum: a NaN stays one
+            const float m = sum / n;
+            return make_float2(m - neg, fmaxf(fmaf(-sum, m, sq), 0.0f) + 0.0f * sum);
+        };
+        if (V == 1) {
+            part[at] = moments(split(a[0]).x, split(b[0]).x, (float)mine, split(pivot[0]).x);
+        } else if (mono) {
+#pragma unroll
+            for (int i = 1; i < N; i++) { a[0] = a[0] + a[i]; b[0] = b[0] + b[i]; }
+            const float2 sa = split(a[0]), sb = split(b[0]);
+            part[at] = moments(sa.x + sa.y, sb.x + sb.y, (float)mine * V, split(pivot[0]).x);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float2 sa = split(a[i]), sb = split(b[i]), sp = split(pivot[i]);
+                part[at * V + 2 * i] = moments(sa.x, sb.x, (float)mine, sp.x);
+                part[at * V + 2 * i + 1] = moments(sa.y, sb.y, (float)mine, sp.y);
+            }
+        }
+    }
+};
+
+// Moments of the groups with channels in [ch0, ch1) from a block's parts of them: [step][row],
+// mean and M2 of the positions that place r has. The mean of the means first, then the deviations
+// from it, both from the group's first part on; several warps to a group when groups are few. A
+// group that began before ch0 is joined to what group[] has of it.
+template <int THREADS>
+__device__ __forceinline__ void block_moments(const NormParams& p, const Place& q, int n, int vec, int ch0, int ch1, const float2* part, float2* group,
+                                              float* red) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = THREADS / 32;
+    const int per = p.mono ? vec : 1, row = q.width * vec / per, rows = min(q.step, n);
+    const int base = n / q.step, more = n - base * q.step;       // place r has base positions, and one more below `more`
+    const int first = ch0 / p.cpg, count = (ch1 - 1) / p.cpg + 1 - first, team = max(1, warps / count), member = warp % team;
+    for (int g0 = 0; g0 < count; g0 += warps / team) {
+        const int g = first + g0 + warp / team;
+        const bool live = g - first < count && warp < warps / team * team;
+        const int from_ch = max(g * p.cpg, ch0), w = live ? (min((g + 1) * p.cpg, ch1) - from_ch) / per : 1;
+        const float2* at = part + (from_ch - ch0) / per;
+        const int lead = member * 32 + lane, r0 = lead / w, c0 = lead - r0 * w, dr = team * 32 / w, dc = team * 32 - dr * w;
+        const float from = live ? at[0].x : 0.0f;
+        float mean = 0.0f;
+        for (int pass = 0; pass < 2; pass++) {
+            float sum = 0.0f;
+            if (live)
+                for (int r = r0, c = c0; r < rows;) {
+                    const float2 v = at[r * row + c];
+                    const float cnt = (float)((base + (r < more)) * per), d = v.x - from - mean;
+                    sum += pass ? fmaf(cnt * d, d, v.y) : cnt * d;
+                    r += dr;
+                    if ((c += dc) >= w) { c -= w; r++; }
+                }
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            if (team > 1) {   // then every group has its team at once: one round
+                if (lane == 0) red[warp] = sum;
+                __syncthreads();
+                sum = 0.0f;
+                if (live)
+                    for (int k = 0; k < team; k++) sum += red[warp - member + k];
+                __syncthreads();
+            }
+            if (pass == 0) mean = sum / ((float)n * (float)(w * per));
+            else if (live && member == 0 && lane == 0) {
+                Moments m{(float)n * (float)(w * per), from + mean, sum};
+                if (g * p.cpg < ch0) {
+                    Moments t{(float)n * (float)(ch0 - g * p.cpg), group[g].x, group[g].y};
+                    join(t, m);
+                    m = t;
+                }
+                group[g] = make_float2(m.mean, m.m2);
+            }
+        }
+    }
+    __syncthreads();
+}
+
+// z = (x + mu) a + sh for a thread's channels. For 16-bit x as x a + (sh + mu a): what that rounds, 2^-24
+// of mu a, is far below the 2^-9 (2^-12) of mu a that x itself was rounded by.
+template <class T, int V, int ACT> struct Affine {
+    static constexpr int N = (V + 1) / 2;
+    static constexpr bool fast = sizeof(T) == 2;
+    f2 mu[N], a[N], sh[N];
+    PairAct<ACT, fast> fn;
+    // stat(g): mean and rstd of a group
+    template <class Fn> __device__ __forceinline__ void start(const NormParams& p, int ch, Fn&& stat) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            float m[2], s1[2], s0[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int c = V == 1 ? ch : ch + 2 * i + k;
+                const float2 st = stat(c / p.cpg);
+                m[k] = -st.x;
+                s1[k] = st.y * param(p.gamma, c, p.param_float, 1.0f, (const T*)nullptr);
+                s0[k] = param(p.beta, c, p.param_float, 0.0f, (const T*)nullptr);
+                if (fast) s0[k] = fmaf(m[k], s1[k], s0[k]);
+            }
+            mu[i] = make_f2(m[0], m[1]);
+            a[i] = make_f2(s1[0], s1[1]);
+            sh[i] = make_f2(s0[0], s0[1]);
+        }
+    }
+    __device__ __forceinline__ void put_at(T* y, Pack<T, V> v) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const f2 f = get(v, i);
+            put(v, i, fn.value(fma2(fast ? f : f + mu[i], a[i], sh[i])));
+        }
+        store_stream(y, v);
+    }
+};
+
+// Backward: z = (x + mu) za + zb; the sums are of dz and dz (x + mu), the latter scaled by rstd at the end;
+// dx = dz za + (x + mu) c2 + c1, c2 = -rstd^2 mean(d xh), c1 = -rstd mean(d).
+template <class T, int V, int ACT> struct Slope {
+    static constexpr int N = (V + 1) / 2;
+    f2 mu[N], za[N], zb[N];
+    float rs[2 * N];
+    PairAct<ACT, sizeof(T) == 2> fn;
+    __device__ __forceinline__ void start(const NormParams& p, int item, int ch) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            float m[2], s1[2], s0[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int c = V == 1 ? ch : ch + 2 * i + k;
+                const int64_t g = (int64_t)item * p.groups + c / p.cpg;
+                m[k] = -p.mean[g];
+                rs[2 * i + k] = p.rstd[g];
+                s1[k] = rs[2 * i + k] * param(p.gamma, c, p.param_float, 1.0f, (const T*)nullptr);
+                s0[k] = param(p.beta, c, p.param_float, 0.0f, (const T*)nullptr);
+            }
+            mu[i] = make_f2(m[0], m[1]);
+            za[i] = make_f2(s1[0], s1[1]);
+            zb[i] = make_f2(s0[0], s0[1]);
+        }
+    }
+    __device__ __forceinline__ void take(const Pack<T, V>& v, const Pack<T, V>& w, f2 (&a)[N], f2 (&b)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const f2 xm = get(v, i) + mu[i];
+            const f2 dz = get(w, i) * fn.slope(fma2(xm, za[i], zb[i]));
+            a[i] = a[i] + dz;
+            b[i] = fma2(dz, xm, b[i]);
+        }
+    }
+    __device__ __forceinline__ void parts(const f2 (&a)[N], const f2 (&b)[N], float2* part) const {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const float2 sa = split(a[j / 2]), sb = split(b[j / 2]);
+            part[j] = make_float2(j & 1 ? sa.y : sa.x, (j & 1 ? sb.y : sb.x) * rs[j]);
+        }
+    }
+    // means(g): the group's means of d and d xh
+    template <class Fn> __device__ __forceinline__ void ends(const NormParams& p, int ch, f2 (&c1)[N], f2 (&c2)[N], Fn&& means) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            float u1[2], u2[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const float2 m = means((V == 1 ? ch : ch + 2 * i + k) / p.cpg);
+                const float r = rs[2 * i + k];
+                u1[k] = -r * m.x;
+                u2[k] = -r * r * m.y;
+            }
+            c1[i] = make_f2(u1[0], u1[1]);
+            c2[i] = make_f2(u2[0], u2[1]);
+        }
+    }
+    __device__ __forceinline__ void put_at(T* dx, const Pack<T, V>& v, const Pack<T, V>& w, const f2 (&c1)[N], const f2 (&c2)[N]) const {
+        Pack<T, V> o;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const f2 xm = get(v, i) + mu[i];
+            const f2 dz = get(w, i) * fn.slope(fma2(xm, za[i], zb[i]));
+            put(o, i, fma2(dz, za[i], fma2(xm, c2[i], c1[i])));
+        }
+        store_stream(dx, o);
+    }
+};
+
+// ---- three launches -----------------------------------------------------------------------------
+
+// A launch of these may begin before the one it depends on has ended: nothing it reads of that one's
+// is read before this.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+struct Range { int item, chunk, n; int64_t l0; };
+// Blocks take the chunks in order, or (the second reading) from the last.
+__device__ __forceinline__ Range range_of(const NormParams& p, bool reverse) {
+    Range s;
+    s.item = reverse ? gridDim.y - 1 - blockIdx.y : blockIdx.y;
+    s.chunk = reverse ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+    s.l0 = (int64_t)s.chunk * p.rows;
+    s.n = (int)min((int64_t)p.rows, p.positions - s.l0);
+    return s;
+}
+
+// Moments of a chunk's groups.
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant__ NormParams p) {
-    __shared__ float2 part[kThreads * V];       // [r][col][V]: mean, M2
-    const int b = blockIdx.y, chunk = blockIdx.x;
-    const int64_t l0 = (int64_t)chunk * p.rows;
-    const int n = (int)min((int64_t)p.rows, p.positions - l0);
-    const Place q = place(p);
-    const T* x = static_cast<const T*>(p.x) + b * p.xb + l0 * p.xp;
-    extern __shared__ Moments group[];          // [groups], joined over column tiles
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kThreads, 2) moments_kernel(const __grid_constant__ NormParams p) {
+    constexpr int U = 8;
+    using P = Pack<T, V>;
+    __shared__ float2 part[kThreads * V];
+    __shared__ float red[kThreads / 32];
+    extern __shared__ float2 group[];          // [groups]
+    next_may_start();
+    const Range s = range_of(p, false);
+    const Place q = place<kThreads>(p);
+    const int mine = mine_of(q, s.n);
     for (int c0 = 0; c0 < p.columns; c0 += q.width) {
         const int cols = min(q.width, p.columns - c0);
-        const bool on = q.r < q.step && q.col < cols;
-        if (on) {
-            float pivot[V], s[V], s2[V];
-            float cnt = 0.0f;
-#pragma unroll
-            for (int j = 0; j < V; j++) pivot[j] = s[j] = s2[j] = 0.0f;
-            if (q.r < n) {
-                const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(x + (int64_t)q.r * p.xp + (int64_t)(c0 + q.col) * V);
-#pragma unroll
-                for (int j = 0; j < V; j++) pivot[j] = to_float(v.v[j]);
-                cnt = (float)((n - q.r + q.step - 1) / q.step);
-            }
-#pragma unroll 4
-            for (int l = q.r + q.step; l < n; l += q.step) {
-                const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(x + (int64_t)l * p.xp + (int64_t)(c0 + q.col) * V);
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float d = to_float(v.v[j]) - pivot[j];
-                    s[j] += d;
-                    s2[j] = fmaf(d, d, s2[j]);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float m = cnt > 0.0f ? s[j] / cnt : 0.0f;
-                part[(q.r * q.width + q.col) * V + j] = make_float2(pivot[j] + m, fmaxf(fmaf(-s[j], m, s2[j]), 0.0f) + 0.0f * s[j]);
-            }
+        if (q.r < q.step && q.col < cols && mine) {
+            const T* at = static_cast<const T*>(p.x) + s.item * p.xb + (s.l0 + q.r) * p.xp + (int64_t)(c0 + q.col) * V;
+            const int64_t step = (int64_t)q.step * p.xp;
+            Sums<T, V> sums;
+            sums.start(*reinterpret_cast<const P*>(at), p.mono);
+            stream<P, U>(mine, [&](P& v) { v = *reinterpret_cast<const P*>(at); at += step; }, [&](const P& v) { sums.take(v); });
+            sums.finish(mine, p.mono, part, q.r * q.width + q.col);
         }
         __syncthreads();
-        // a warp per group of this tile: lanes join every 32nd of its (position, channel) parts
-        const int ch0 = c0 * V, ch1 = ch0 + cols * V;
-        for (int g = ch0 / p.cpg + warp; g * p.cpg < ch1; g += kThreads / 32) {
-            const int a = max(g * p.cpg, ch0) - ch0, w = min((g + 1) * p.cpg, ch1) - ch0 - a;
-            const int rows = min(q.step, n);
-            Moments m{0.0f, 0.0f, 0.0f};
-            for (int i = lane; i < rows * w; i += 32) {
-                const int r = i / w, c = a + i - r * w;
-                const float2 v = part[r * q.width * V + c];
-                join(m, Moments{(float)((n - r + q.step - 1) / q.step), v.x, v.y});
-            }
-            warp_join(m);
-            if (lane == 0) {
-                if (g * p.cpg < ch0) { Moments t = group[g]; join(t, m); m = t; }   // began in the tile before
-                group[g] = m;
-            }
-        }
-        __syncthreads();
+        block_moments<kThreads>(p, q, s.n, V, c0 * V, (c0 + cols) * V, part, group, red);
     }
-    for (int g = threadIdx.x; g < p.groups; g += kThreads)
-        p.part[((int64_t)b * p.groups + g) * p.chunks + chunk] = make_float2(group[g].mean, group[g].m2);
+    for (int g = threadIdx.x; g < p.groups; g += kThreads) p.part[((int64_t)s.item * p.groups + g) * p.chunks + s.chunk] = group[g];
 }
 
 // One warp per (item, group): its chunks' moments, joined.
 __global__ void __launch_bounds__(128) moments_join(const __grid_constant__ NormParams p) {
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
+    next_may_start();
+    after_previous();
     if (i >= (int64_t)p.batch * p.groups) return;
     Moments m{0.0f, 0.0f, 0.0f};
     for (int c = lane; c < p.chunks; c += 32) {
@@ -182,76 +410,50 @@ __global__ void __launch_bounds__(128) moments_join(const __grid_constant__ Norm
 }
 
 template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) apply_kernel(const __grid_constant__ NormParams p) {
-    const int b = blockIdx.y, chunk = blockIdx.x;
-    const int64_t l0 = (int64_t)chunk * p.rows;
-    const int n = (int)min((int64_t)p.rows, p.positions - l0);
-    const Place q = place(p);
-    if (q.r >= q.step) return;
-    constexpr bool fast = sizeof(T) == 2;
+__global__ void __launch_bounds__(kThreads, 2) apply_kernel(const __grid_constant__ NormParams p) {
+    constexpr int U = 4;
+    using P = Pack<T, V>;
+    const Range s = range_of(p, true);
+    const Place q = place<kThreads>(p);
+    after_previous();
+    const int mine = mine_of(q, s.n);
+    if (q.r >= q.step || !mine) return;
     for (int col = q.col; col < p.columns; col += q.width) {
         const int ch = col * V;
-        float mu[V], a[V], sh[V];
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            const int g = (ch + j) / p.cpg;
-            mu[j] = p.mean[(int64_t)b * p.groups + g];
-            a[j] = p.rstd[(int64_t)b * p.groups + g] * param(p.gamma, ch + j, p.param_float, 1.0f, (const T*)nullptr);
-            sh[j] = param(p.beta, ch + j, p.param_float, 0.0f, (const T*)nullptr);
-        }
-        const T* x = static_cast<const T*>(p.x) + b * p.xb + l0 * p.xp + ch;
-        T* y = static_cast<T*>(p.y) + b * p.yb + l0 * p.yp + ch;
-#pragma unroll 4
-        for (int l = q.r; l < n; l += q.step) {
-            Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(x + (int64_t)l * p.xp);
-#pragma unroll
-            for (int j = 0; j < V; j++) v.v[j] = from_float<T>(act<ACT, fast>(fmaf(to_float(v.v[j]) - mu[j], a[j], sh[j])));
-            *reinterpret_cast<Pack<T, V>*>(y + (int64_t)l * p.yp) = v;
-        }
+        Affine<T, V, ACT> f;
+        f.start(p, ch, [&](int g) { return make_float2(p.mean[(int64_t)s.item * p.groups + g], p.rstd[(int64_t)s.item * p.groups + g]); });
+        const int64_t last = s.l0 + q.r + (int64_t)(mine - 1) * q.step, sx = (int64_t)q.step * p.xp, sy = (int64_t)q.step * p.yp;
+        const T* at = static_cast<const T*>(p.x) + s.item * p.xb + last * p.xp + ch;
+        T* y = static_cast<T*>(p.y) + s.item * p.yb + last * p.yp + ch;
+        stream<P, U>(mine, [&](P& v) { v = load_stream<P>(at); at -= sx; }, [&](const P& v) { f.put_at(y, v); y -= sy; });
     }
 }
 
-// ---- backward --------------------------------------------------------------------------------
-
-// A chunk's sums of dz and dz xh per channel.
+// Backward: a chunk's sums of dz and dz xh per channel.
 template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) grad_sums_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(kThreads, 2) grad_sums_kernel(const __grid_constant__ NormParams p) {
+    constexpr int U = V == 8 ? 2 : 4, N = (V + 1) / 2;   // what the registers hold beside the channels' sums
+    using P = Pack<T, V>;
     __shared__ float2 part[kThreads * V];
-    const int b = blockIdx.y, chunk = blockIdx.x;
-    const int64_t l0 = (int64_t)chunk * p.rows;
-    const int n = (int)min((int64_t)p.rows, p.positions - l0);
-    const Place q = place(p);
-    constexpr bool fast = sizeof(T) == 2;
+    next_may_start();
+    const Range s = range_of(p, false);
+    const Place q = place<kThreads>(p);
+    const int mine = mine_of(q, s.n);
     for (int c0 = 0; c0 < p.columns; c0 += q.width) {
         const int cols = min(q.width, p.columns - c0);
         if (q.r < q.step && q.col < cols) {
             const int ch = (c0 + q.col) * V;
-            float mu[V], rs[V], ga[V], be[V], s1[V], s2[V];
+            Slope<T, V, ACT> f;
+            f.start(p, s.item, ch);
+            f2 a[N], b[N];
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                const int g = (ch + j) / p.cpg;
-                mu[j] = p.mean[(int64_t)b * p.groups + g];
-                rs[j] = p.rstd[(int64_t)b * p.groups + g];
-                ga[j] = param(p.gamma, ch + j, p.param_float, 1.0f, (const T*)nullptr);
-                be[j] = param(p.beta, ch + j, p.param_float, 0.0f, (const T*)nullptr);
-                s1[j] = s2[j] = 0.0f;
-            }
-            const T* x = static_cast<const T*>(p.x) + b * p.xb + l0 * p.xp + ch;
-            const T* dy = static_cast<const T*>(p.dy) + b * p.yb + l0 * p.yp + ch;
-#pragma unroll 2
-            for (int l = q.r; l < n; l += q.step) {
-                const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(x + (int64_t)l * p.xp);
-                const Pack<T, V> w = *reinterpret_cast<const Pack<T, V>*>(dy + (int64_t)l * p.yp);
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float xh = (to_float(v.v[j]) - mu[j]) * rs[j];
-                    const float dz = to_float(w.v[j]) * act_grad<ACT, fast>(fmaf(xh, ga[j], be[j]));
-                    s1[j] += dz;
-                    s2[j] = fmaf(dz, xh, s2[j]);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < V; j++) part[(q.r * q.width + q.col) * V + j] = make_float2(s1[j], s2[j]);
+            for (int i = 0; i < N; i++) a[i] = b[i] = make_f2(0.0f, 0.0f);
+            const T* ax = static_cast<const T*>(p.x) + s.item * p.xb + (s.l0 + q.r) * p.xp + ch;
+            const T* ad = static_cast<const T*>(p.dy) + s.item * p.yb + (s.l0 + q.r) * p.yp + ch;
+            const int64_t sx = (int64_t)q.step * p.xp, sd = (int64_t)q.step * p.yp;
+            stream<Two<P>, U>(mine, [&](Two<P>& v) { v.x = *reinterpret_cast<const P*>(ax); v.dy = *reinterpret_cast<const P*>(ad); ax += sx; ad += sd; },
+                              [&](const Two<P>& v) { f.take(v.x, v.dy, a, b); });
+            f.parts(a, b, part + (q.r * q.width + q.col) * V);
         }
         __syncthreads();
         for (int c = threadIdx.x; c < cols * V; c += kThreads) {
@@ -261,105 +463,107 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(const __grid_consta
                 t.x += v.x;
                 t.y += v.y;
             }
-            p.part[((int64_t)b * p.chunks + chunk) * p.channels + c0 * V + c] = t;
+            p.part[((int64_t)s.item * p.chunks + s.chunk) * p.channels + c0 * V + c] = t;
         }
         __syncthreads();
     }
 }
 
-// A warp per channel: every item's sums over its chunks, and their sums, dbeta and dgamma.
+// Channels side by side, 32 to a block of 32 x 8 threads: every item's sums over its chunks, and their
+// sums over the items, dbeta and dgamma.
 template <class T>
-__global__ void __launch_bounds__(128) grad_join(const __grid_constant__ NormParams p) {
-    const int c = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (c >= p.channels) return;
-    float db = 0.0f, dg = 0.0f;
+__global__ void __launch_bounds__(256) grad_join(const __grid_constant__ NormParams p) {
+    __shared__ float2 red[8][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    next_may_start();
+    after_previous();
+    float2 all = make_float2(0.0f, 0.0f);
     for (int b = 0; b < p.batch; b++) {
-        float s1 = 0.0f, s2 = 0.0f;
-        for (int k = lane; k < p.used; k += 32) {
-            const float2 v = p.part[((int64_t)b * p.chunks + k) * p.channels + c];
-            s1 += v.x;
-            s2 += v.y;
+        float2 s = make_float2(0.0f, 0.0f);
+        if (c < p.channels)
+#pragma unroll 4
+            for (int k = warp; k < p.used; k += 8) {
+                const float2 v = p.part[((int64_t)b * p.chunks + k) * p.channels + c];
+                s.x += v.x;
+                s.y += v.y;
+            }
+        red[warp][lane] = s;
+        __syncthreads();
+        if (warp == 0) {
+            for (int w = 1; w < 8; w++) { s.x += red[w][lane].x; s.y += red[w][lane].y; }
+            if (p.sums && c < p.channels) p.sums[(int64_t)b * p.channels + c] = s;
+            all.x += s.x;
+            all.y += s.y;
+        }
+        __syncthreads();
+    }
+    if (warp == 0 && c < p.channels) {
+        if (p.dbeta) set_param(p.dbeta, c, p.param_float, all.x, (const T*)nullptr);
+        if (p.dgamma) set_param(p.dgamma, c, p.param_float, all.y, (const T*)nullptr);
+    }
+}
+
+// Sums over a group's channels of gamma times their sums: s(c) -> out(g).
+template <class T, int THREADS, class S, class Out>
+__device__ __forceinline__ void group_sums(const NormParams& p, S&& s, Out&& out) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int g = warp; g < p.groups; g += THREADS / 32) {
+        float a = 0.0f, b = 0.0f;
+        for (int k = lane; k < p.cpg; k += 32) {
+            const int c = g * p.cpg + k;
+            const float2 v = s(c);
+            const float gc = param(p.gamma, c, p.param_float, 1.0f, (const T*)nullptr);
+            a = fmaf(gc, v.x, a);
+            b = fmaf(gc, v.y, b);
         }
         for (int o = 16; o > 0; o >>= 1) {
-            s1 += __shfl_xor_sync(~0u, s1, o);
-            s2 += __shfl_xor_sync(~0u, s2, o);
+            a += __shfl_xor_sync(~0u, a, o);
+            b += __shfl_xor_sync(~0u, b, o);
         }
-        if (lane == 0 && p.sums) p.sums[(int64_t)b * p.channels + c] = make_float2(s1, s2);
-        db += s1;
-        dg += s2;
-    }
-    if (lane == 0) {
-        if (p.dbeta) set_param(p.dbeta, c, p.param_float, db, (const T*)nullptr);
-        if (p.dgamma) set_param(p.dgamma, c, p.param_float, dg, (const T*)nullptr);
+        if (lane == 0) out(g, a, b);
     }
 }
 
 template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) grad_apply_kernel(const __grid_constant__ NormParams p) {
-    extern __shared__ float2 mean_of[];   // [groups]: sum(d) / m, sum(d xh) / m
-    const int b = blockIdx.y, chunk = blockIdx.x;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kThreads, 2) grad_apply_kernel(const __grid_constant__ NormParams p) {
+    constexpr int U = V == 8 ? 2 : 4, N = (V + 1) / 2;
+    using P = Pack<T, V>;
+    extern __shared__ float2 group[];   // [groups]: means of d and d xh
+    const Range s = range_of(p, true);
+    const Place q = place<kThreads>(p);
+    after_previous();
     const float m = (float)p.positions * (float)p.cpg;
-    for (int g = warp; g < p.groups; g += kThreads / 32) {
-        float a = 0.0f, c = 0.0f;
-        for (int k = lane; k < p.cpg; k += 32) {
-            const int ch = g * p.cpg + k;
-            const float2 s = p.sums[(int64_t)b * p.channels + ch];
-            const float ga = param(p.gamma, ch, p.param_float, 1.0f, (const T*)nullptr);
-            a = fmaf(ga, s.x, a);
-            c = fmaf(ga, s.y, c);
-        }
-        for (int o = 16; o > 0; o >>= 1) {
-            a += __shfl_xor_sync(~0u, a, o);
-            c += __shfl_xor_sync(~0u, c, o);
-        }
-        if (lane == 0) mean_of[g] = make_float2(a / m, c / m);
-    }
+    group_sums<T, kThreads>(p, [&](int c) { return p.sums[(int64_t)s.item * p.channels + c]; },
+                            [&](int g, float a, float b) { group[g] = make_float2(a / m, b / m); });
     __syncthreads();
-    const int64_t l0 = (int64_t)chunk * p.rows;
-    const int n = (int)min((int64_t)p.rows, p.positions - l0);
-    const Place q = place(p);
-    if (q.r >= q.step) return;
-    constexpr bool fast = sizeof(T) == 2;
+    const int mine = mine_of(q, s.n);
+    if (q.r >= q.step || !mine) return;
     for (int col = q.col; col < p.columns; col += q.width) {
         const int ch = col * V;
-        float mu[V], rs[V], ga[V], be[V];
-        float2 mo[V];
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            const int g = (ch + j) / p.cpg;
-            mu[j] = p.mean[(int64_t)b * p.groups + g];
-            rs[j] = p.rstd[(int64_t)b * p.groups + g];
-            ga[j] = param(p.gamma, ch + j, p.param_float, 1.0f, (const T*)nullptr);
-            be[j] = param(p.beta, ch + j, p.param_float, 0.0f, (const T*)nullptr);
-            mo[j] = mean_of[g];
-        }
-        const T* x = static_cast<const T*>(p.x) + b * p.xb + l0 * p.xp + ch;
-        const T* dy = static_cast<const T*>(p.dy) + b * p.yb + l0 * p.yp + ch;
-        T* dx = static_cast<T*>(p.dx) + b * p.db + l0 * p.dp + ch;
-#pragma unroll 2
-        for (int l = q.r; l < n; l += q.step) {
-            const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(x + (int64_t)l * p.xp);
-            const Pack<T, V> w = *reinterpret_cast<const Pack<T, V>*>(dy + (int64_t)l * p.yp);
-            Pack<T, V> o;
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float xh = (to_float(v.v[j]) - mu[j]) * rs[j];
-                const float d = to_float(w.v[j]) * act_grad<ACT, fast>(fmaf(xh, ga[j], be[j])) * ga[j];
-                o.v[j] = from_float<T>(rs[j] * (d - mo[j].x - xh * mo[j].y));
-            }
-            *reinterpret_cast<Pack<T, V>*>(dx + (int64_t)l * p.dp) = o;
-        }
+        Slope<T, V, ACT> f;
+        f.start(p, s.item, ch);
+        f2 c1[N], c2[N];
+        f.ends(p, ch, c1, c2, [&](int g) { return group[g]; });
+        const int64_t last = s.l0 + q.r + (int64_t)(mine - 1) * q.step;
+        const int64_t sx = (int64_t)q.step * p.xp, sd = (int64_t)q.step * p.yp, so = (int64_t)q.step * p.dp;
+        const T* ax = static_cast<const T*>(p.x) + s.item * p.xb + last * p.xp + ch;
+        const T* ad = static_cast<const T*>(p.dy) + s.item * p.yb + last * p.yp + ch;
+        T* dx = static_cast<T*>(p.dx) + s.item * p.db + last * p.dp + ch;
+        stream<Two<P>, U>(mine, [&](Two<P>& v) { v.x = load_stream<P>(ax); v.dy = load_stream<P>(ad); ax -= sx; ad -= sd; },
+                          [&](const Two<P>& v) { f.put_at(dx, v.x, v.dy, c1, c2); dx -= so; });
     }
 }
 
-// ---- one launch -------------------------------------------------------------------------------
+// ---- clusters -----------------------------------------------------------------------------------
 
 constexpr int kFused = 512;          // threads: with 1024 the registers do not hold a vector's sums
 constexpr int kFusedGroups = 2048;   // most groups
 constexpr int kClusterMost = 8;
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // The 8 bytes at the same place in another block of the cluster.
 __device__ __forceinline__ float2 peer_read(const float2* p, int rank) {
@@ -370,251 +574,85 @@ __device__ __forceinline__ float2 peer_read(const float2* p, int rank) {
     return v;
 }
 
-struct Share { int item, chunk, n; int64_t l0; };
-template <bool GRID> __device__ __forceinline__ Share share_of(const NormParams& p, int round) {
-    Share s;
-    const int slot = blockIdx.x / p.chunks;
-    s.chunk = blockIdx.x - slot * p.chunks;
-    s.item = GRID ? (slot < p.at_once ? round * p.at_once + slot : p.batch) : slot;
+__device__ __forceinline__ Range cluster_range(const NormParams& p) {
+    Range s;
+    s.item = blockIdx.x / p.chunks;
+    s.chunk = blockIdx.x - s.item * p.chunks;
     s.l0 = (int64_t)s.chunk * p.rows;
-    s.n = s.item < p.batch ? (int)min((int64_t)p.rows, p.positions - s.l0) : 0;
+    s.n = (int)max((int64_t)0, min((int64_t)p.rows, p.positions - s.l0));
     return s;
 }
 
-// Moments of the block's groups from its threads' parts: [step][row] of them, of `per` channels each,
-// mean and M2 of the rows that place r has. The mean of the means first, then the deviations from
-// it, both from the group's first part on; several warps to a group when groups are few.
-__device__ __forceinline__ void block_moments(const NormParams& p, const Place& q, int n, const float2* part, int vec, float2* group, float2* red) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kFused / 32;
-    const int per = p.mono ? vec : 1, row = p.channels / per, w = p.cpg / per;   // parts of a row, of a group in a row
-    const int rows = min(q.step, n), team = max(1, warps / p.groups);
-    const int base = n / q.step, more = n - base * q.step;       // place r has base rows, and one more below `more`
-    const int member = warp % team, lead = member * 32 + lane;
-    const int r0 = lead / w, c0 = lead - r0 * w, dr = team * 32 / w, dc = team * 32 - dr * w;
-    const float inv = 1.0f / ((float)n * (float)p.cpg);
-    for (int g0 = 0; g0 < p.groups; g0 += warps / team) {
-        const int g = g0 + warp / team;
-        const bool live = g < p.groups && warp < warps / team * team;
-        const float2* at = part + g * w;
-        const float from = live ? at[0].x : 0.0f;
-        float mean = 0.0f;
-        for (int pass = 0; pass < 2; pass++) {
-            float sum = 0.0f;
-            if (live)
-                for (int r = r0, c = c0; r < rows;) {
-                    const float2 v = at[r * row + c];
-                    const float cnt = (float)((base + (r < more)) * per), d = v.x - from - mean;
-                    sum += pass ? fmaf(cnt * d, d, v.y) : cnt * d;
-                    r += dr;
-                    if ((c += dc) >= w) { c -= w; r++; }
-                }
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-            if (team > 1) {   // then every group has its team at once: one round
-                if (lane == 0) reinterpret_cast<float*>(red)[warp] = sum;
-                __syncthreads();
-                sum = 0.0f;
-                if (live)
-                    for (int k = 0; k < team; k++) sum += reinterpret_cast<float*>(red)[warp - member + k];
-                __syncthreads();
-            }
-            if (pass == 0) mean = sum * inv;
-            else if (live && member == 0 && lane == 0) group[g] = make_float2(from + mean, sum);
-        }
-    }
-    __syncthreads();
-}
-
-template <class T, int V, int ACT, bool GRID>
-__global__ void __launch_bounds__(kFused, 1) norm_fused(const __grid_constant__ NormParams p) {
-    constexpr bool fast = sizeof(T) == 2;
-    constexpr int U = 8, N = (V + 1) / 2;       // positions in flight per thread, pairs of a vector
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(kFused, 1) norm_cluster(const __grid_constant__ NormParams p) {
+    constexpr int U = 4;                        // positions in flight per thread
     using P = Pack<T, V>;
     extern __shared__ __align__(16) uint8_t smem[];
     P* keep = reinterpret_cast<P*>(smem);       // [kept][threads]
     float2* part = reinterpret_cast<float2*>(smem + (size_t)p.kept * kFused * sizeof(P));
     float2* group = part + kFused * (p.mono ? 1 : V);   // [groups]: the block's moments
     float2* stat = group + p.groups;                    // [groups]: the item's mean and rstd
-    __shared__ float2 red[kFused / 64];
-    Place q;
-    q.width = p.columns;
-    q.step = kFused / q.width;
-    q.r = (int)p.columns_div.div(threadIdx.x);
-    q.col = threadIdx.x - q.r * q.width;
+    __shared__ float red[kFused / 32];
+    const Range s = cluster_range(p);
+    const Place q = place<kFused>(p);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ch = q.col * V;
-    const bool on = q.r < q.step;
-    const int rounds = GRID ? (p.batch + p.at_once - 1) / p.at_once : 1;
-    for (int round = 0; round < rounds; round++) {
-        const Share s = share_of<GRID>(p, round);
-        const T* x = static_cast<const T*>(p.x) + s.item * p.xb + s.l0 * p.xp + ch;
-        if (s.n > 0) {
-            if (on && q.r < s.n) {
-                // differences from the first value met, so that a mean far from zero costs no digits
-                f2 pivot[N], a[N], b[N];
-                const T* at = x + (int64_t)q.r * p.xp;
-                {
-                    const P first = *reinterpret_cast<const P*>(at);
-#pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        const float2 f = split(get(first, i)), f0 = split(get(first, 0));
-                        pivot[i] = p.mono ? make_f2(-f0.x, -f0.x) : make_f2(-f.x, -f.y);
-                        a[i] = b[i] = make_f2(0.0f, 0.0f);
-                    }
-                }
-                const int64_t step = (int64_t)q.step * p.xp;
-                const int mine = (s.n - q.r + q.step - 1) / q.step;
-                auto take = [&](const P& v) {
-#pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        const f2 d = get(v, i) + pivot[i];
-                        a[i] = a[i] + d;
-                        b[i] = fma2(d, d, b[i]);
-                    }
-                };
-                int it = 0;
-                P* k = keep + threadIdx.x;
-                for (; it + U <= min(mine, p.kept); it += U, k += U * kFused) {
-                    P v[U];
-#pragma unroll
-                    for (int u = 0; u < U; u++, at += step) v[u] = *reinterpret_cast<const P*>(at);
-#pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        k[u * kFused] = v[u];
-                        take(v[u]);
-                    }
-                }
-                for (; it < mine; it += U) {
-                    P v[U];
-#pragma unroll
-                    for (int u = 0; u < U; u++, at += step)
-                        if (it + u < mine) v[u] = *reinterpret_cast<const P*>(at);
-#pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        if (it + u >= mine) break;
-                        if (it + u < p.kept) keep[(it + u) * kFused + threadIdx.x] = v[u];
-                        take(v[u]);
-                    }
-                }
-                auto moments = [&](float sum, float sq, float n, float neg) {   // + 0 sum: a NaN stays one
-                    const float m = sum / n;
-                    return make_float2(m - neg, fmaxf(fmaf(-sum, m, sq), 0.0f) + 0.0f * sum);
-                };
-                if (V == 1) {
-                    part[q.r * q.width + q.col] = moments(split(a[0]).x, split(b[0]).x, (float)mine, split(pivot[0]).x);
-                } else if (p.mono) {
-#pragma unroll
-                    for (int i = 1; i < N; i++) { a[0] = a[0] + a[i]; b[0] = b[0] + b[i]; }
-                    const float2 sa = split(a[0]), sb = split(b[0]);
-                    part[q.r * q.width + q.col] = moments(sa.x + sa.y, sb.x + sb.y, (float)mine * V, split(pivot[0]).x);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        const float2 sa = split(a[i]), sb = split(b[i]), sp = split(pivot[i]);
-                        float2* to = part + (q.r * q.width + q.col) * V + 2 * i;
-                        to[0] = moments(sa.x, sb.x, (float)mine, sp.x);
-                        to[1] = moments(sa.y, sb.y, (float)mine, sp.y);
-                    }
-                }
-            }
-            __syncthreads();
-            block_moments(p, q, s.n, part, V, group, red);
-            if (GRID)
-                for (int g = threadIdx.x; g < p.groups; g += kFused) p.part[((int64_t)s.item * p.groups + g) * p.chunks + s.chunk] = group[g];
+    const int mine = q.r < q.step ? mine_of(q, s.n) : 0;
+    if (s.n > 0) {
+        if (mine) {
+            const T* at = static_cast<const T*>(p.x) + s.item * p.xb + (s.l0 + q.r) * p.xp + ch;
+            const int64_t step = (int64_t)q.step * p.xp;
+            Sums<T, V> sums;
+            sums.start(*reinterpret_cast<const P*>(at), p.mono);
+            P* k = keep + threadIdx.x;
+            stream<P, U>(mine, [&](P& v) { v = *reinterpret_cast<const P*>(at); at += step; }, [&](const P& v) {
+                *k = v;
+                k += kFused;
+                sums.take(v);
+            });
+            sums.finish(mine, p.mono, part, q.r * q.width + q.col);
         }
-        __syncwarp();
-        if (GRID) cg::this_grid().sync();
-        else {
-            cluster_arrive();
-            cluster_wait();
-        }
-        if (s.n > 0) {
-            for (int g = warp; g < p.groups; g += kFused / 32) {
-                Moments m{0.0f, 0.0f, 0.0f};
-                for (int c = lane; c < p.used; c += 32) {
-                    const float n = (float)min((int64_t)p.rows, p.positions - (int64_t)c * p.rows) * (float)p.cpg;
-                    const float2 v = GRID ? __ldcg(p.part + ((int64_t)s.item * p.groups + g) * p.chunks + c) : peer_read(group + g, c);
-                    join(m, Moments{n, v.x, v.y});
-                }
-                warp_join(m);
-                if (lane == 0) {
-                    const float r = 1.0f / sqrtf(m.m2 / ((float)p.positions * (float)p.cpg) + p.eps);
-                    stat[g] = make_float2(m.mean, r);
-                    if (s.chunk == 0 && p.mean) {
-                        p.mean[(int64_t)s.item * p.groups + g] = m.mean;
-                        p.rstd[(int64_t)s.item * p.groups + g] = r;
-                    }
-                }
-            }
-        }
-        __syncwarp();
-        if (!GRID) cluster_arrive();   // waited for below: no block goes while others still read its moments
         __syncthreads();
-        if (s.n > 0 && on) {
-            // z = (x - mu) a + sh. For 16-bit x as x a + (sh - mu a): what that rounds, 2^-24 of mu a, is far
-            // below the 2^-9 (2^-12) of mu a that x itself was rounded by.
-            f2 mu[N], a[N], sh[N];
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                float m[2], s1[2], s0[2];
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const int c = V == 1 ? ch : ch + 2 * i + k;
-                    const float2 st = stat[c / p.cpg];
-                    m[k] = -st.x;
-                    s1[k] = st.y * param(p.gamma, c, p.param_float, 1.0f, (const T*)nullptr);
-                    s0[k] = param(p.beta, c, p.param_float, 0.0f, (const T*)nullptr);
-                    if (fast) s0[k] = fmaf(m[k], s1[k], s0[k]);
-                }
-                mu[i] = make_f2(m[0], m[1]);
-                a[i] = make_f2(s1[0], s1[1]);
-                sh[i] = make_f2(s0[0], s0[1]);
+        block_moments<kFused>(p, q, s.n, V, 0, p.channels, part, group, red);
+    }
+    cluster_arrive();
+    cluster_wait();
+    if (s.n > 0) {
+        for (int g = warp; g < p.groups; g += kFused / 32) {
+            Moments m{0.0f, 0.0f, 0.0f};
+            for (int c = lane; c < p.used; c += 32) {
+                const float n = (float)min((int64_t)p.rows, p.positions - (int64_t)c * p.rows) * (float)p.cpg;
+                const float2 v = peer_read(group + g, c);
+                join(m, Moments{n, v.x, v.y});
             }
-            const PairAct<ACT, fast> fn;
-            const int64_t sx = (int64_t)q.step * p.xp, sy = (int64_t)q.step * p.yp;
-            auto one = [&](P v, T* y) {
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const f2 f = get(v, i);
-                    put(v, i, fn.value(fma2(fast ? f : f + mu[i], a[i], sh[i])));
+            warp_join(m);
+            if (lane == 0) {
+                const float r = 1.0f / sqrtf(m.m2 / ((float)p.positions * (float)p.cpg) + p.eps);
+                stat[g] = make_float2(m.mean, r);
+                if (s.chunk == 0 && p.mean) {
+                    p.mean[(int64_t)s.item * p.groups + g] = m.mean;
+                    p.rstd[(int64_t)s.item * p.groups + g] = r;
                 }
-                *reinterpret_cast<P*>(y) = v;
-            };
-            const int mine = q.r < s.n ? (s.n - q.r + q.step - 1) / q.step : 0;
-            // what was read last and not kept is in L2 yet: from the end
-            int it = mine - 1;
-            const T* at = x + (q.r + (int64_t)it * q.step) * p.xp;
-            T* y = static_cast<T*>(p.y) + s.item * p.yb + s.l0 * p.yp + ch + (q.r + (int64_t)it * q.step) * p.yp;
-            constexpr int W = 4;
-            for (; it >= p.kept; it -= W) {
-                P v[W];
-#pragma unroll
-                for (int u = 0; u < W; u++, at -= sx)
-                    if (it - u >= p.kept) v[u] = *reinterpret_cast<const P*>(at);
-#pragma unroll
-                for (int u = 0; u < W; u++)
-                    if (it - u >= p.kept) {
-                        one(v[u], y);
-                        y -= sy;
-                    }
             }
-            const P* k = keep + min(mine, p.kept) * kFused + threadIdx.x;
-#pragma unroll 2
-            for (it = min(mine, p.kept); it > 0; it--, y -= sy) one(*(k -= kFused), y);
-        }
-        if (GRID) __syncthreads();   // stat and the kept values are the next round's
-        else {
-            __syncwarp();
-            cluster_wait();
         }
     }
+    cluster_arrive();   // waited for below: no block goes while others still read its moments
+    __syncthreads();
+    if (mine) {
+        Affine<T, V, ACT> f;
+        f.start(p, ch, [&](int g) { return stat[g]; });
+        T* y = static_cast<T*>(p.y) + s.item * p.yb + (s.l0 + q.r) * p.yp + ch;
+        const int64_t sy = (int64_t)q.step * p.yp;
+        const P* k = keep + threadIdx.x;
+        for (int it = 0; it < mine; it++, k += kFused, y += sy) f.put_at(y, *k);
+    }
+    __syncwarp();
+    cluster_wait();
 }
 
-// Backward: the block's sums of dz and dz xh per channel, of gamma times them per group; the set's
-// blocks meet over the group sums. Channel sums go out per block for dgamma and dbeta.
-template <class T, int V, int ACT, bool GRID>
-__global__ void __launch_bounds__(kFused, 1) norm_grad_fused(const __grid_constant__ NormParams p) {
-    constexpr bool fast = sizeof(T) == 2;
-    constexpr int U = 4, N = (V + 1) / 2;
-    const PairAct<ACT, fast> fn;
+// Backward: the blocks meet over their groups' sums; channel sums go out per block for grad_join.
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(kFused, 1) norm_grad_cluster(const __grid_constant__ NormParams p) {
+    constexpr int U = 2, N = (V + 1) / 2;
     using P = Pack<T, V>;
     extern __shared__ __align__(16) uint8_t smem[];
     P* keep = reinterpret_cast<P*>(smem);       // [kept][x, dy][threads]
@@ -622,215 +660,71 @@ __global__ void __launch_bounds__(kFused, 1) norm_grad_fused(const __grid_consta
     float2* chan = part + kFused * V;           // [channels]
     float2* group = chan + p.channels;          // [groups]: the block's sums
     float2* stat = group + p.groups;            // [groups]: the item's means of d and d xh
-    Place q;
-    q.width = p.columns;
-    q.step = kFused / q.width;
-    q.r = (int)p.columns_div.div(threadIdx.x);
-    q.col = threadIdx.x - q.r * q.width;
+    next_may_start();
+    const Range s = cluster_range(p);
+    const Place q = place<kFused>(p);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ch = q.col * V;
-    const bool on = q.r < q.step;
-    const int rounds = GRID ? (p.batch + p.at_once - 1) / p.at_once : 1;
-    for (int round = 0; round < rounds; round++) {
-        const Share s = share_of<GRID>(p, round);
-        const T* x = static_cast<const T*>(p.x) + s.item * p.xb + s.l0 * p.xp + ch;
-        const T* dy = static_cast<const T*>(p.dy) + s.item * p.yb + s.l0 * p.yp + ch;
-        // z = (x - mu) za + zb; the sums are of dz and dz (x - mu), the latter scaled by rstd at the end
-        f2 mu[N], za[N], zb[N];
-        const int mine = q.r < s.n ? (s.n - q.r + q.step - 1) / q.step : 0;
-        const int64_t sx = (int64_t)q.step * p.xp, sd = (int64_t)q.step * p.yp;
-        if (s.n > 0) {
-            if (on) {
-                f2 a[N], b[N];
-                float rs[2 * N];
+    const bool on = q.r < q.step && s.n > 0;
+    const int mine = on ? mine_of(q, s.n) : 0;
+    Slope<T, V, ACT> f;
+    if (s.n > 0) {
+        if (on) {
+            f.start(p, s.item, ch);
+            f2 a[N], b[N];
 #pragma unroll
-                for (int i = 0; i < N; i++) {
-                    float m[2], s1[2], s0[2];
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const int c = V == 1 ? ch : ch + 2 * i + k;
-                        const int64_t g = (int64_t)s.item * p.groups + c / p.cpg;
-                        m[k] = -p.mean[g];
-                        rs[2 * i + k] = p.rstd[g];
-                        s1[k] = rs[2 * i + k] * param(p.gamma, c, p.param_float, 1.0f, (const T*)nullptr);
-                        s0[k] = param(p.beta, c, p.param_float, 0.0f, (const T*)nullptr);
-                    }
-                    mu[i] = make_f2(m[0], m[1]);
-                    za[i] = make_f2(s1[0], s1[1]);
-                    zb[i] = make_f2(s0[0], s0[1]);
-                    a[i] = b[i] = make_f2(0.0f, 0.0f);
-                }
-                auto take = [&](const P& v, const P& w) {
-#pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        const f2 xm = get(v, i) + mu[i];
-                        const f2 dz = get(w, i) * fn.slope(fma2(xm, za[i], zb[i]));
-                        a[i] = a[i] + dz;
-                        b[i] = fma2(dz, xm, b[i]);
-                    }
-                };
-                const T *ax = x + (int64_t)q.r * p.xp, *ad = dy + (int64_t)q.r * p.yp;
-                int it = 0;
-                P* k = keep + threadIdx.x;
-                for (; it + U <= min(mine, p.kept); it += U, k += U * 2 * kFused) {
-                    P v[U], w[U];
-#pragma unroll
-                    for (int u = 0; u < U; u++, ax += sx, ad += sd) {
-                        v[u] = *reinterpret_cast<const P*>(ax);
-                        w[u] = *reinterpret_cast<const P*>(ad);
-                    }
-#pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        k[u * 2 * kFused] = v[u];
-                        k[u * 2 * kFused + kFused] = w[u];
-                        take(v[u], w[u]);
-                    }
-                }
-                for (; it < mine; it++, ax += sx, ad += sd) {
-                    const P v = *reinterpret_cast<const P*>(ax), w = *reinterpret_cast<const P*>(ad);
-                    if (it < p.kept) {
-                        keep[it * 2 * kFused + threadIdx.x] = v;
-                        keep[it * 2 * kFused + kFused + threadIdx.x] = w;
-                    }
-                    take(v, w);
-                }
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float2 sa = split(a[j / 2]), sb = split(b[j / 2]);
-                    part[(q.r * q.width + q.col) * V + j] = make_float2(j & 1 ? sa.y : sa.x, (j & 1 ? sb.y : sb.x) * rs[j]);
-                }
-            }
-            __syncthreads();
-            for (int c = threadIdx.x; c < p.channels; c += kFused) {
-                float2 t = make_float2(0.0f, 0.0f);
-                for (int r = 0; r < q.step; r++) {
-                    const float2 v = part[r * p.channels + c];
-                    t.x += v.x;
-                    t.y += v.y;
-                }
-                chan[c] = t;
-                p.part[((int64_t)s.item * p.chunks + s.chunk) * p.channels + c] = t;
-            }
-            __syncthreads();
-            for (int g = warp; g < p.groups; g += kFused / 32) {
-                float a = 0.0f, b = 0.0f;
-                for (int k = lane; k < p.cpg; k += 32) {
-                    const int c = g * p.cpg + k;
-                    const float gc = param(p.gamma, c, p.param_float, 1.0f, (const T*)nullptr);
-                    a = fmaf(gc, chan[c].x, a);
-                    b = fmaf(gc, chan[c].y, b);
-                }
-                for (int o = 16; o > 0; o >>= 1) {
-                    a += __shfl_xor_sync(~0u, a, o);
-                    b += __shfl_xor_sync(~0u, b, o);
-                }
-                if (lane == 0) {
-                    group[g] = make_float2(a, b);
-                    if (GRID) p.sums[((int64_t)s.item * p.groups + g) * p.chunks + s.chunk] = make_float2(a, b);
-                }
-            }
+            for (int i = 0; i < N; i++) a[i] = b[i] = make_f2(0.0f, 0.0f);
+            const T* ax = static_cast<const T*>(p.x) + s.item * p.xb + (s.l0 + q.r) * p.xp + ch;
+            const T* ad = static_cast<const T*>(p.dy) + s.item * p.yb + (s.l0 + q.r) * p.yp + ch;
+            const int64_t sx = (int64_t)q.step * p.xp, sd = (int64_t)q.step * p.yp;
+            P* k = keep + threadIdx.x;
+            stream<Two<P>, U>(mine, [&](Two<P>& v) { v.x = *reinterpret_cast<const P*>(ax); v.dy = *reinterpret_cast<const P*>(ad); ax += sx; ad += sd; },
+                              [&](const Two<P>& v) {
+                                  k[0] = v.x;
+                                  k[kFused] = v.dy;
+                                  k += 2 * kFused;
+                                  f.take(v.x, v.dy, a, b);
+                              });
+            f.parts(a, b, part + (q.r * q.width + q.col) * V);
         }
-        __syncwarp();
-        if (GRID) cg::this_grid().sync();
-        else {
-            cluster_arrive();
-            cluster_wait();
-        }
-        if (s.n > 0 && p.dx) {
-            const float m = (float)p.positions * (float)p.cpg;
-            for (int g = warp; g < p.groups; g += kFused / 32) {
-                float a = 0.0f, b = 0.0f;
-                for (int c = lane; c < p.used; c += 32) {
-                    const float2 v = GRID ? __ldcg(p.sums + ((int64_t)s.item * p.groups + g) * p.chunks + c) : peer_read(group + g, c);
-                    a += v.x;
-                    b += v.y;
-                }
-                for (int o = 16; o > 0; o >>= 1) {
-                    a += __shfl_xor_sync(~0u, a, o);
-                    b += __shfl_xor_sync(~0u, b, o);
-                }
-                if (lane == 0) stat[g] = make_float2(a / m, b / m);
-            }
-        }
-        __syncwarp();
-        if (!GRID) cluster_arrive();
         __syncthreads();
-        if (s.n > 0 && p.dx && on) {
-            // dx = rstd gamma dz - (x - mu) rstd^2 mean(d xh) - rstd mean(d)
-            f2 c1[N], c2[N];
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                float u1[2], u2[2];
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const int g = (V == 1 ? ch : ch + 2 * i + k) / p.cpg;
-                    const float r = p.rstd[(int64_t)s.item * p.groups + g];
-                    u1[k] = -r * stat[g].x;
-                    u2[k] = -r * r * stat[g].y;
-                }
-                c1[i] = make_f2(u1[0], u1[1]);
-                c2[i] = make_f2(u2[0], u2[1]);
+        for (int c = threadIdx.x; c < p.channels; c += kFused) {
+            float2 t = make_float2(0.0f, 0.0f);
+            for (int r = 0; r < q.step; r++) {
+                const float2 v = part[r * p.channels + c];
+                t.x += v.x;
+                t.y += v.y;
             }
-            auto one = [&](const P& v, const P& w, T* dx) {
-                P o;
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const f2 xm = get(v, i) + mu[i];
-                    const f2 dz = get(w, i) * fn.slope(fma2(xm, za[i], zb[i]));
-                    put(o, i, fma2(dz, za[i], fma2(xm, c2[i], c1[i])));
-                }
-                *reinterpret_cast<P*>(dx) = o;
-            };
-            int it = mine - 1;
-            const int64_t last = q.r + (int64_t)it * q.step, so = (int64_t)q.step * p.dp;
-            const T *ax = x + last * p.xp, *ad = dy + last * p.yp;
-            T* dx = static_cast<T*>(p.dx) + s.item * p.db + (s.l0 + last) * p.dp + ch;
-            constexpr int W = 2;
-            for (; it >= p.kept; it -= W) {
-                P v[W], w[W];
-#pragma unroll
-                for (int u = 0; u < W; u++, ax -= sx, ad -= sd)
-                    if (it - u >= p.kept) {
-                        v[u] = *reinterpret_cast<const P*>(ax);
-                        w[u] = *reinterpret_cast<const P*>(ad);
-                    }
-#pragma unroll
-                for (int u = 0; u < W; u++)
-                    if (it - u >= p.kept) {
-                        one(v[u], w[u], dx);
-                        dx -= so;
-                    }
-            }
-            const P* k = keep + min(mine, p.kept) * 2 * kFused + threadIdx.x;
-            for (it = min(mine, p.kept); it > 0; it--, dx -= so) {
-                k -= 2 * kFused;
-                one(k[0], k[kFused], dx);
-            }
+            chan[c] = t;
+            p.part[((int64_t)s.item * p.chunks + s.chunk) * p.channels + c] = t;
         }
-        if (GRID) __syncthreads();
-        else {
-            __syncwarp();
-            cluster_wait();
-        }
+        __syncthreads();
+        group_sums<T, kFused>(p, [&](int c) { return chan[c]; }, [&](int g, float a, float b) { group[g] = make_float2(a, b); });
     }
-    if (GRID && (p.dgamma || p.dbeta)) {   // every item's parts were complete at the last meeting
-        const int all = (int)gridDim.x * (kFused / 32);
-        for (int c = blockIdx.x * (kFused / 32) + warp; c < p.channels; c += all) {
-            float a = 0.0f, b = 0.0f;
-            for (int k = lane; k < p.batch * p.chunks; k += 32) {
-                const float2 v = __ldcg(p.part + (int64_t)k * p.channels + c);
-                a += v.x;
-                b += v.y;
-            }
+    cluster_arrive();
+    cluster_wait();
+    if (s.n > 0 && p.dx) {
+        const float m = (float)p.positions * (float)p.cpg;
+        for (int g = warp; g < p.groups; g += kFused / 32) {
+            float2 v = lane < p.used ? peer_read(group + g, lane) : make_float2(0.0f, 0.0f);
             for (int o = 16; o > 0; o >>= 1) {
-                a += __shfl_xor_sync(~0u, a, o);
-                b += __shfl_xor_sync(~0u, b, o);
+                v.x += __shfl_xor_sync(~0u, v.x, o);
+                v.y += __shfl_xor_sync(~0u, v.y, o);
             }
-            if (lane == 0) {
-                if (p.dbeta) set_param(p.dbeta, c, p.param_float, a, (const T*)nullptr);
-                if (p.dgamma) set_param(p.dgamma, c, p.param_float, b, (const T*)nullptr);
-            }
+            if (lane == 0) stat[g] = make_float2(v.x / m, v.y / m);
         }
     }
+    cluster_arrive();
+    __syncthreads();
+    if (mine && p.dx) {
+        f2 c1[N], c2[N];
+        f.ends(p, ch, c1, c2, [&](int g) { return stat[g]; });
+        T* dx = static_cast<T*>(p.dx) + s.item * p.db + (s.l0 + q.r) * p.dp + ch;
+        const int64_t so = (int64_t)q.step * p.dp;
+        const P* k = keep + threadIdx.x;
+        for (int it = 0; it < mine; it++, k += 2 * kFused, dx += so) f.put_at(dx, k[0], k[kFused], c1, c2);
+    }
+    __syncwarp();
+    cluster_wait();
 }
 
 // ---- host -------------------------------------------------------------------------------------
@@ -850,8 +744,8 @@ void check_config(const stg_group_norm_config* c) {
     if (c->positions > ((int64_t)1 << 40) / c->channels) fail(STG_UNSUPPORTED, "group norm: an item of more than 2^40 elements");
 }
 
-// An item's positions are cut so that the whole call has about four blocks per SM, each with at
-// least 16 positions, and at most 1024 parts to join.
+// An item's positions are cut so that the whole call has four blocks per SM (two rounds of the two
+// that the registers allow), each with at least 16 positions, and at most 1024 parts to join.
 int chunks_of(const stg_group_norm_config& c) {
     const int64_t per_item = (148 * 4 + c.batch - 1) / std::max<int64_t>(c.batch, 1);
     const int64_t n = std::min<int64_t>({std::max<int64_t>(per_item, 1), (c.positions + 15) / 16, 1024});
@@ -861,11 +755,11 @@ int chunks_of(const stg_group_norm_config& c) {
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
-enum Path { THREE_LAUNCHES, CLUSTER, GRID };
+enum Path { THREE_LAUNCHES, CLUSTER };
 // How a call runs with vectors of `vec` channels on `sms` SMs, and the scratch it takes.
 struct NormPlan {
     Path path = THREE_LAUNCHES;
-    int chunks = 0, at_once = 1, kept = 0;
+    int chunks = 0, kept = 0;
     int64_t rows = 0;
     size_t smem = 0;
     size_t second = 0, third = 0, bytes = 0;   // offsets of the scratch's parts
@@ -883,32 +777,17 @@ NormPlan plan_of(const stg_group_norm_config& c, bool backward, int vec, int sms
     if (columns <= kFused && c.groups <= kFusedGroups && other + 8 * block_step <= most) {
         const int64_t step = kFused / columns, room = (int64_t)((most - other) / block_step);   // steps a block can keep
         const int64_t item_steps = (c.positions + step - 1) / step;
-        int64_t blocks = (item_steps + room - 1) / room;
-        if (blocks <= kClusterMost) {
-            // as many blocks as fill the GPU once, each with at least four steps
-            int64_t size = 1;
-            while (size < kClusterMost && (size < blocks || (size * 2 * c.batch <= sms && size * 8 <= item_steps))) size *= 2;
+        auto steps = [&](int64_t size) { return ((c.positions + size - 1) / size + step - 1) / step; };   // of one of `size` blocks
+        // as many blocks as fill the GPU once, each with at least four steps
+        int64_t size = 1;
+        while (size < kClusterMost && (steps(size) > room || (size * 2 * c.batch <= sms && size * 8 <= item_steps))) size *= 2;
+        if (steps(size) <= room) {
             r.path = CLUSTER;
             r.chunks = (int)size;
             r.rows = (c.positions + size - 1) / size;
-            r.kept = (int)((r.rows + step - 1) / step);
-        } else {
-            r.at_once = (int)std::max<int64_t>(1, std::min<int64_t>(c.batch, sms * room / item_steps));
-            const int64_t per = sms / r.at_once;
-            if (per * c.groups <= 32768) {   // what every block reads of the others' sums: at most 256 KB
-                r.path = GRID;
-                r.rows = (c.positions + per - 1) / per;
-                r.chunks = (int)((c.positions + r.rows - 1) / r.rows);
-                r.kept = (int)std::min<int64_t>(room, (r.rows + step - 1) / step);
-            }
-        }
-        if (r.path != THREE_LAUNCHES && r.rows <= (1 << 30)) {
+            r.kept = (int)steps(size);
             r.smem = other + (size_t)r.kept * block_step;
-            const size_t sets = (size_t)c.batch * r.chunks;
-            if (backward) {
-                r.second = up(sizeof(float2) * sets * c.channels);
-                r.bytes = r.second + (r.path == GRID ? up(sizeof(float2) * sets * c.groups) : 0);
-            } else r.bytes = r.path == GRID ? up(sizeof(float2) * sets * c.groups) : 0;
+            if (backward) r.bytes = up(sizeof(float2) * (size_t)c.batch * r.chunks * c.channels);
             return r;
         }
     }
@@ -961,29 +840,39 @@ void set_plan(NormParams& p, const NormPlan& plan, int vec, int fused) {
     p.chunks = plan.chunks;
     p.rows = (int)plan.rows;
     p.used = (int)((p.positions + plan.rows - 1) / plan.rows);
-    p.at_once = plan.at_once;
     p.kept = plan.kept;
     p.mono = p.cpg % vec == 0;
 }
-template <class K> void launch_fused(K kernel, const NormParams& p, const NormPlan& plan, int threads, cudaStream_t st) {
-    cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan.smem), "group norm kernel");
+// A launch that may begin while the one before it ends (see after_previous).
+template <class K> void launch_after(K kernel, dim3 grid, int threads, size_t smem, const NormParams& p, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
-    const int64_t blocks = plan.path == GRID ? (int64_t)plan.at_once * plan.chunks : (int64_t)p.batch * plan.chunks;
-    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = plan.smem;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (plan.path == GRID) {
-        attr[0].id = cudaLaunchAttributeCooperative;
-        attr[0].val.cooperative = 1;
-    } else {
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = plan.chunks;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    }
+    cuda_check(cudaLaunchKernelEx(&cfg, kernel, p), "group norm kernel");
+}
+template <class K> void allow_smem(K kernel, size_t smem, size_t fixed = 0) {
+    if (smem + fixed > 48 * 1024) cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "group norm kernel");
+}
+template <class K> void launch_cluster(K kernel, const NormParams& p, const NormPlan& plan, cudaStream_t st) {
+    allow_smem(kernel, plan.smem, 256);
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3((unsigned)(p.batch * plan.chunks));
+    cfg.blockDim = dim3(kFused);
+    cfg.dynamicSmemBytes = plan.smem;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = plan.chunks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     cuda_check(cudaLaunchKernelEx(&cfg, kernel, p), "group norm kernel");
 }
 bool wide_fits(const stg_group_norm_config& c, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
@@ -1042,19 +931,17 @@ STG_API stg_status stg_group_norm(stg_engine* e, const stg_group_norm_config* c,
                 set_plan(p, plan, V, kFused);
                 with_activation(c->activation, [&](auto a) {
                     constexpr int A = decltype(a)::value;
-                    if (plan.path == CLUSTER) return launch_fused(norm_fused<T, V, A, false>, p, plan, kFused, st);
-                    if (plan.path == GRID) return launch_fused(norm_fused<T, V, A, true>, p, plan, kFused, st);
+                    if (plan.path == CLUSTER) return launch_cluster(norm_cluster<T, V, A>, p, plan, st);
                     if (!p.mean) {
                         p.mean = reinterpret_cast<float*>(ws + plan.second);
                         p.rstd = reinterpret_cast<float*>(ws + plan.third);
                     }
                     const dim3 grid((unsigned)p.chunks, (unsigned)p.batch);
-                    const size_t smem = sizeof(Moments) * (size_t)p.groups;
-                    if (smem + sizeof(float2) * kThreads * V > 48 * 1024)
-                        cuda_check(cudaFuncSetAttribute(moments_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "group norm kernel");
+                    const size_t smem = sizeof(float2) * (size_t)p.groups;
+                    allow_smem(moments_kernel<T, V>, smem, sizeof(float2) * kThreads * V + 256);
                     moments_kernel<T, V><<<grid, kThreads, smem, st>>>(p);
-                    moments_join<<<(unsigned)(((int64_t)p.batch * p.groups + 3) / 4), 128, 0, st>>>(p);
-                    apply_kernel<T, V, A><<<grid, kThreads, 0, st>>>(p);
+                    launch_after(moments_join, dim3((unsigned)(((int64_t)p.batch * p.groups + 3) / 4)), 128, 0, p, st);
+                    launch_after(apply_kernel<T, V, A>, grid, kThreads, 0, p, st);
                 });
             });
         });
@@ -1100,21 +987,19 @@ STG_API stg_status stg_group_norm_backward(stg_engine* e, const stg_group_norm_c
                 set_plan(p, plan, V, kFused);
                 with_activation(c->activation, [&](auto a) {
                     constexpr int A = decltype(a)::value;
-                    const unsigned join_blocks = (unsigned)((p.channels + 3) / 4);
+                    const dim3 join_grid((unsigned)((p.channels + 31) / 32));
                     if (plan.path == CLUSTER) {
-                        launch_fused(norm_grad_fused<T, V, A, false>, p, plan, kFused, st);
-                        if (p.dgamma || p.dbeta) grad_join<T><<<join_blocks, 128, 0, st>>>(p);
+                        launch_cluster(norm_grad_cluster<T, V, A>, p, plan, st);
+                        if (p.dgamma || p.dbeta) launch_after(grad_join<T>, join_grid, 256, 0, p, st);
                         return;
                     }
-                    if (plan.path == GRID) return launch_fused(norm_grad_fused<T, V, A, true>, p, plan, kFused, st);
                     const dim3 grid((unsigned)p.chunks, (unsigned)p.batch);
                     grad_sums_kernel<T, V, A><<<grid, kThreads, 0, st>>>(p);
-                    grad_join<T><<<join_blocks, 128, 0, st>>>(p);
+                    launch_after(grad_join<T>, join_grid, 256, 0, p, st);
                     if (p.dx) {
                         const size_t smem = sizeof(float2) * (size_t)p.groups;
-                        if (smem > 48 * 1024)
-                            cuda_check(cudaFuncSetAttribute(grad_apply_kernel<T, V, A>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "group norm kernel");
-                        grad_apply_kernel<T, V, A><<<grid, kThreads, smem, st>>>(p);
+                        allow_smem(grad_apply_kernel<T, V, A>, smem);
+                        launch_after(grad_apply_kernel<T, V, A>, grid, kThreads, smem, p, st);
                     }
                 });
             });
