@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -192,21 +193,21 @@ _SIGNATURES = {
     "stg_htdemucs_spec": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p]),
     "stg_htdemucs_ispec": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_void_p,
                                        C.c_void_p]),
-    "stg_rotary_frequencies": (C.c_int32, [C.POINTER(RotaryConfig), C.POINTER(C.c_double), C.POINTER(C.c_double)]),
-    "stg_rotary": (C.c_int32, [C.c_void_p, C.POINTER(RotaryConfig), C.POINTER(RotaryTensor), C.c_int32, C.c_void_p,
+    "stg_rotary_frequencies": (C.c_int32, [C.c_void_p, C.POINTER(C.c_double), C.POINTER(C.c_double)]),
+    "stg_rotary": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p,
                                C.c_int64, C.c_void_p]),
-    "stg_group_norm_workspace": (C.c_int32, [C.POINTER(GroupNormConfig), C.c_int32, C.POINTER(C.c_size_t)]),
-    "stg_group_norm": (C.c_int32, [C.c_void_p, C.POINTER(GroupNormConfig)] + [C.c_void_p] * 7 + [C.c_size_t, C.c_void_p]),
-    "stg_group_norm_backward": (C.c_int32, [C.c_void_p, C.POINTER(GroupNormConfig)] + [C.c_void_p] * 10 +
+    "stg_group_norm_workspace": (C.c_int32, [C.c_void_p, C.c_int32, C.POINTER(C.c_size_t)]),
+    "stg_group_norm": (C.c_int32, [C.c_void_p, C.c_void_p] + [C.c_void_p] * 7 + [C.c_size_t, C.c_void_p]),
+    "stg_group_norm_backward": (C.c_int32, [C.c_void_p, C.c_void_p] + [C.c_void_p] * 10 +
                                 [C.c_size_t, C.c_void_p]),
-    "stg_gated_workspace": (C.c_int32, [C.POINTER(GatedConfig), C.c_int32, C.POINTER(C.c_size_t)]),
-    "stg_gated": (C.c_int32, [C.c_void_p, C.POINTER(GatedConfig)] + [C.c_void_p] * 7 + [C.c_size_t, C.c_void_p]),
-    "stg_gated_backward": (C.c_int32, [C.c_void_p, C.POINTER(GatedConfig)] + [C.c_void_p] * 12 +
+    "stg_gated_workspace": (C.c_int32, [C.c_void_p, C.c_int32, C.POINTER(C.c_size_t)]),
+    "stg_gated": (C.c_int32, [C.c_void_p, C.c_void_p] + [C.c_void_p] * 7 + [C.c_size_t, C.c_void_p]),
+    "stg_gated_backward": (C.c_int32, [C.c_void_p, C.c_void_p] + [C.c_void_p] * 12 +
                            [C.c_size_t, C.c_void_p]),
     "stg_engine_status": (C.c_int32, [C.c_void_p]),
     "stg_mask_head_sizes": (C.c_int32, [C.c_void_p, _I32P, _I32P, _I32P, C.POINTER(C.c_int64)]),
-    "stg_mask_head_workspace": (C.c_int32, [C.c_void_p, C.POINTER(MaskHeadConfig), C.POINTER(C.c_size_t)]),
-    "stg_mask_head": (C.c_int32, [C.c_void_p, C.POINTER(MaskHeadConfig)] + [C.c_void_p] * 5 + [C.c_size_t, C.c_void_p]),
+    "stg_mask_head_workspace": (C.c_int32, [C.c_void_p, C.c_void_p, C.POINTER(C.c_size_t)]),
+    "stg_mask_head": (C.c_int32, [C.c_void_p, C.c_void_p] + [C.c_void_p] * 5 + [C.c_size_t, C.c_void_p]),
     "stg_separate_roformer_noalloc": (C.c_int32, [C.c_int, C.POINTER(RoFormerConfig), C.c_int64, C.c_void_p,
                                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]),
 }
@@ -285,11 +286,27 @@ def _choice(table, key, what):
         raise StemsError(1, f"{what} must be one of {', '.join(table)}") from None
 
 
+# The layers' configurations as packed bytes: they cost a call a third of what the structs do.
+_ROTARY = struct.Struct("=Iiiiqqiiiidddddd")
+_ROTARY_TENSOR = struct.Struct("=QQqqqqqqq")
+_GROUP_NORM = struct.Struct("=Iiiiqqiiqqqqqqd")
+_GATED = struct.Struct("=Iiiii4xqqqqqqqq")
+_torch = None
+
+
 def _layer_tensor(t, what, device, dtype=None, shape=None):
     """A layer's tensor argument, checked; its dtype code."""
-    if not _DTYPES:
+    try:
+        if t.get_device() == device and (dtype is None or t.dtype is dtype) and (shape is None or t.shape == shape):
+            return _DTYPES[t.dtype]
+    except (AttributeError, KeyError):
+        pass
+    global _torch
+    if _torch is None:
         import torch
+        _torch = torch
         _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        return _layer_tensor(t, what, device, dtype, shape)
     if not hasattr(t, "data_ptr"):
         raise StemsError(1, f"{what}: expected a tensor")
     if t.dtype not in _DTYPES:
@@ -298,9 +315,7 @@ def _layer_tensor(t, what, device, dtype=None, shape=None):
         raise StemsError(1, f"{what}: expected dtype {dtype}, got {t.dtype}")
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise StemsError(1, f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if not t.is_cuda or t.get_device() != device:
-        raise StemsError(1, f"{what}: expected a tensor on the engine's device cuda:{device}")
-    return _DTYPES[t.dtype]
+    raise StemsError(1, f"{what}: expected a tensor on the engine's device cuda:{device}")
 
 
 def _inner(t, what):
@@ -325,12 +340,15 @@ def _run(shape, strides, alone):
 def _empty(shape, dtype, device, stream):
     """A new tensor from the pool of the stream the kernels run on: its memory's earlier users
     are then ahead of them in that stream."""
-    import torch
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
-    s = torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
-    with torch.cuda.stream(s):
-        return torch.empty(shape, dtype=dtype, device=f"cuda:{device}")
+        return _torch.empty(shape, dtype=dtype, device=device)
+    s = _torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
+    with _torch.cuda.stream(s):
+        return _torch.empty(shape, dtype=dtype, device=device)
+
+
+def _ptr_of(t):
+    return None if t is None else t.data_ptr()
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, scaling="none", factor=1.0, original_length=0.0, beta_fast=0.0,
@@ -374,6 +392,16 @@ class Engine:
         if rc != 0:
             raise StemsError(rc, f"cannot create an engine on device {device}")
         self.device = device
+        self._raw_stream = None
+
+    def _layer_stream(self, stream):
+        """The stream a layer runs on: the one given, else torch's current one of the device."""
+        if stream is not None:
+            return stream if isinstance(stream, int) else stream.cuda_stream
+        if self._raw_stream is None:
+            self._raw_stream = getattr(_torch._C, "_cuda_getCurrentRawStream", None) or (
+                lambda d: _torch.cuda.current_stream(d).cuda_stream)
+        return self._raw_stream(self.device)
 
     def close(self):
         if self._h:
@@ -531,27 +559,30 @@ class Engine:
             pairs.append((_inner(k, "k"), out_k))
         pos, pos_stride = None, 0
         if positions is not None:
-            if not hasattr(positions, "data_ptr") or str(positions.dtype) != "torch.int32":
+            if not hasattr(positions, "data_ptr") or positions.dtype is not _torch.int32:
                 raise StemsError(1, "positions: expected an int32 tensor")
-            if not positions.is_cuda or positions.get_device() != dev:
+            if positions.get_device() != dev:
                 raise StemsError(1, f"positions: expected a tensor on the engine's device cuda:{dev}")
             if tuple(positions.shape) not in ((t,), (b, t)) or (t > 1 and positions.stride(-1) != 1):
                 raise StemsError(1, "positions: expected [tokens] or [batch][tokens], the last stride 1")
             pos, pos_stride = positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0
-        tensors, results = (RotaryTensor * 2)(), []
-        for i, (x, y) in enumerate(pairs):
+        tensors, results = b"", []
+        for x, y in pairs:
             if y is None:
-                y = _empty(x.shape, x.dtype, dev, stream)
+                y = _empty(x.shape, x.dtype, q.device, stream)
             else:
                 _layer_tensor(y, "out", dev, x.dtype, x.shape)
                 _inner(y, "out")
             xs, ys = x.stride(), y.stride()
-            tensors[i] = RotaryTensor(x.data_ptr(), y.data_ptr(), x.shape[2], xs[0], xs[1], xs[2], ys[0], ys[1], ys[2])
+            tensors += _ROTARY_TENSOR.pack(x.data_ptr(), y.data_ptr(), x.shape[2], xs[0], xs[1], xs[2], ys[0], ys[1], ys[2])
             results.append(y)
-        cfg = RotaryConfig(C.sizeof(RotaryConfig), code, _choice(_LAYOUTS, layout, "layout"), int(bool(inverse)), b, t, d,
-                           rotary_dim, _choice(_SCALINGS, scaling, "scaling"), offset, base, factor, original_length,
-                           beta_fast, beta_slow, magnitude)
-        rc = lib().stg_rotary(self._h, C.byref(cfg), tensors, len(pairs), pos, pos_stride, _stream_of(stream, q))
+        try:
+            cfg = _ROTARY.pack(_ROTARY.size, code, _choice(_LAYOUTS, layout, "layout"), 1 if inverse else 0, b, t, d, rotary_dim,
+                               _choice(_SCALINGS, scaling, "scaling"), offset, base, factor, original_length, beta_fast, beta_slow,
+                               magnitude)
+        except struct.error as e:
+            raise StemsError(1, f"rotary: {e}") from None
+        rc = lib().stg_rotary(self._h, cfg, tensors, len(pairs), pos, pos_stride, self._layer_stream(stream))
         if rc != 0:
             self._check(rc, "rotary")
         return results[0] if k is None else tuple(results)
@@ -587,18 +618,21 @@ class Engine:
                 _inner(t, what)
         _, _, yb, yp = self._rows(y, "y")
         db, dp = self._rows(dx, "dx")[2:] if dx is not None else (yb, yp)
-        return GroupNormConfig(C.sizeof(GroupNormConfig), code, 0 if pcode is None else pcode,
-                               _choice(ACTIVATIONS, activation, "activation"), b, n, ch, groups, xb, xp, yb, yp, db, dp, eps)
+        try:
+            return _GROUP_NORM.pack(_GROUP_NORM.size, code, 0 if pcode is None else pcode, _choice(ACTIVATIONS, activation, "activation"),
+                                    b, n, ch, groups, xb, xp, yb, yp, db, dp, eps)
+        except struct.error as e:
+            raise StemsError(1, f"group norm: {e}") from None
 
-    def _workspace(self, fn, cfg, backward, what, stream):
+    def _workspace(self, fn, cfg, backward, what, device, stream):
+        """(pointer, bytes, the tensor that owns them) of a layer's scratch."""
         n = C.c_size_t()
-        rc = fn(C.byref(cfg), backward, C.byref(n))
+        rc = fn(cfg, backward, C.byref(n))
         if rc != 0:
             raise StemsError(rc, what)
         if not n.value:
             return None, 0, None
-        import torch
-        ws = _empty((n.value,), torch.uint8, self.device, stream)
+        ws = _empty((n.value,), _torch.uint8, device, stream)
         return ws.data_ptr(), n.value, ws
 
     def group_norm(self, x, groups, gamma=None, beta=None, activation="none", eps=1e-5, out=None, return_stats=False,
@@ -608,19 +642,19 @@ class Engine:
         will need them. gamma / beta [channels] in x's dtype or float32. out may be x."""
         dev = self.device
         _layer_tensor(x, "x", dev)
-        y = _empty(x.shape, x.dtype, dev, stream) if out is None else out
-        if out is not None:
+        at = x.device
+        if out is None:
+            y = _empty(x.shape, x.dtype, at, stream)
+        else:
             _layer_tensor(out, "out", dev, x.dtype, x.shape)
+            y = out
         cfg = self._norm_config(x, groups, gamma, beta, activation, eps, y)
-        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 0, "group_norm", stream)
+        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 0, "group_norm", at, stream)
         mean = rstd = None
         if return_stats:
-            import torch
-            mean, rstd = (_empty((x.shape[0], groups), torch.float32, dev, stream) for _ in range(2))
-        rc = lib().stg_group_norm(self._h, C.byref(cfg), x.data_ptr(), gamma.data_ptr() if gamma is not None else None,
-                                  beta.data_ptr() if beta is not None else None, y.data_ptr(),
-                                  mean.data_ptr() if return_stats else None, rstd.data_ptr() if return_stats else None,
-                                  ws, n, _stream_of(stream, x))
+            mean, rstd = (_empty((x.shape[0], groups), _torch.float32, at, stream) for _ in range(2))
+        rc = lib().stg_group_norm(self._h, cfg, x.data_ptr(), _ptr_of(gamma), _ptr_of(beta), y.data_ptr(), _ptr_of(mean), _ptr_of(rstd),
+                                  ws, n, self._layer_stream(stream))
         if rc != 0:
             self._check(rc, "group_norm")
         return (y, mean, rstd) if return_stats else y
@@ -629,20 +663,20 @@ class Engine:
                             stream=None):
         """(dx, dgamma, dbeta) of group_norm from dy and the forward pass's x, mean and rstd; the
         last two None without gamma / beta, dx None without need_dx."""
-        import torch
         dev = self.device
         _layer_tensor(x, "x", dev)
         _layer_tensor(dy, "dy", dev, x.dtype, x.shape)
         for t, what in ((mean, "mean"), (rstd, "rstd")):
-            _layer_tensor(t, what, dev, torch.float32, (x.shape[0], groups))
+            _layer_tensor(t, what, dev, _torch.float32, (x.shape[0], groups))
             if not t.is_contiguous():
                 raise StemsError(1, f"{what}: expected a contiguous tensor")
-        dx = _empty(x.shape, x.dtype, dev, stream) if need_dx else None
+        at = x.device
+        dx = _empty(x.shape, x.dtype, at, stream) if need_dx else None
         cfg = self._norm_config(x, groups, gamma, beta, activation, eps, dy, dx)
-        dgamma, dbeta = (None if t is None else _empty(t.shape, t.dtype, dev, stream) for t in (gamma, beta))
-        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 1, "group_norm_backward", stream)
-        ptrs = [None if t is None else t.data_ptr() for t in (dy, x, gamma, beta, mean, rstd, dx, dgamma, dbeta)]
-        rc = lib().stg_group_norm_backward(self._h, C.byref(cfg), *ptrs, ws, n, _stream_of(stream, x))
+        dgamma, dbeta = (None if t is None else _empty(t.shape, t.dtype, at, stream) for t in (gamma, beta))
+        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 1, "group_norm_backward", at, stream)
+        rc = lib().stg_group_norm_backward(self._h, cfg, dy.data_ptr(), x.data_ptr(), _ptr_of(gamma), _ptr_of(beta), mean.data_ptr(),
+                                           rstd.data_ptr(), _ptr_of(dx), _ptr_of(dgamma), _ptr_of(dbeta), ws, n, self._layer_stream(stream))
         if rc != 0:
             self._check(rc, "group_norm_backward")
         return dx, dgamma, dbeta
@@ -664,9 +698,8 @@ class Engine:
                 _layer_tensor(t, what, dev, x.dtype, (n,))
                 _inner(t, what)
         _layer_tensor(y, "y", dev, x.dtype, (*x.shape[:-1], n))
-        return GatedConfig(C.sizeof(GatedConfig), code, _choice(ACTIVATIONS, activation, "activation"), k, n,
-                           x.numel() // k if k else 0, self._row_stride(x, "x"), wg.stride(0), wu.stride(0),
-                           self._row_stride(y, "y"), k, k, k)
+        return _GATED.pack(_GATED.size, code, _choice(ACTIVATIONS, activation, "activation"), k, n, x.numel() // k if k else 0,
+                           self._row_stride(x, "x"), wg.stride(0), wu.stride(0), self._row_stride(y, "y"), k, k, k)
 
     @staticmethod
     def _row_stride(t, what):
@@ -685,12 +718,11 @@ class Engine:
         if out is None:
             if not hasattr(w_gate, "shape") or x.dim() < 2:
                 raise StemsError(1, "expected x [...][features] and w_gate [width][features]")
-            out = _empty((*x.shape[:-1], w_gate.shape[0]), x.dtype, dev, stream)
+            out = _empty((*x.shape[:-1], w_gate.shape[0]), x.dtype, x.device, stream)
         cfg = self._gated_config(x, w_gate, w_up, b_gate, b_up, activation, out)
-        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 0, "gated", stream)
-        rc = lib().stg_gated(self._h, C.byref(cfg), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
-                             b_gate.data_ptr() if b_gate is not None else None,
-                             b_up.data_ptr() if b_up is not None else None, out.data_ptr(), ws, n, _stream_of(stream, x))
+        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 0, "gated", x.device, stream)
+        rc = lib().stg_gated(self._h, cfg, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _ptr_of(b_gate), _ptr_of(b_up),
+                             out.data_ptr(), ws, n, self._layer_stream(stream))
         if rc != 0:
             self._check(rc, "gated")
         return out
@@ -702,12 +734,13 @@ class Engine:
         dev = self.device
         _layer_tensor(dy, "dy", dev)
         cfg = self._gated_config(x, w_gate, w_up, b_gate, b_up, activation, dy)
-        dx = _empty(x.shape, x.dtype, dev, stream) if need_dx else None
-        dws = [_empty(w.shape, w.dtype, dev, stream) if need_dw else None for w in (w_gate, w_up)]
-        dbs = [None if t is None else _empty(t.shape, t.dtype, dev, stream) for t in (b_gate, b_up)]
-        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 1, "gated_backward", stream)
-        ptrs = [None if t is None else t.data_ptr() for t in (dy, x, w_gate, w_up, b_gate, b_up, dx, *dws, *dbs)]
-        rc = lib().stg_gated_backward(self._h, C.byref(cfg), *ptrs, ws, n, _stream_of(stream, x))
+        at = x.device
+        dx = _empty(x.shape, x.dtype, at, stream) if need_dx else None
+        dws = [_empty(w.shape, w.dtype, at, stream) if need_dw else None for w in (w_gate, w_up)]
+        dbs = [None if t is None else _empty(t.shape, t.dtype, at, stream) for t in (b_gate, b_up)]
+        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 1, "gated_backward", at, stream)
+        ptrs = [_ptr_of(t) for t in (dy, x, w_gate, w_up, b_gate, b_up, dx, *dws, *dbs)]
+        rc = lib().stg_gated_backward(self._h, cfg, *ptrs, ws, n, self._layer_stream(stream))
         if rc != 0:
             self._check(rc, "gated_backward")
         return (dx, *dws, *(t for t in dbs if t is not None))
@@ -765,6 +798,7 @@ class Plan:
     def __init__(self, engine: Engine, handle):
         self.engine = engine
         self._h = handle
+        self._head_sizes = None
         info = PlanInfo()
         info.size = C.sizeof(PlanInfo)
         engine._check(lib().stg_plan_get_info(self._h, C.byref(info)), "plan_get_info")
@@ -866,9 +900,10 @@ class Plan:
         value rows before its gate rows -> float32 masks [chunks][mask floats per chunk], the
         layout back() and separate() read. out: such a tensor, or a device pointer (the network
         output a separate_network callback is given)."""
-        import torch
         dev = self.engine.device
-        s, b, t, cols = self._head_sizes = getattr(self, "_head_sizes", None) or self.mask_head_sizes()
+        if self._head_sizes is None:
+            self._head_sizes = self.mask_head_sizes()
+        s, b, t, cols = self._head_sizes
         code = _layer_tensor(hidden, "hidden", dev)
         if hidden.dim() != 5 or tuple(hidden.shape[1:4]) != (s, b, t):
             raise StemsError(1, f"hidden: expected [chunks][{s}][{b}][{t}][hidden]")
@@ -880,18 +915,18 @@ class Plan:
             if x is not None and not x.is_contiguous():
                 raise StemsError(1, f"{what}: expected a contiguous tensor")
         if out is None:
-            out = _empty((n, self.mask_floats_per_chunk), torch.float32, dev, stream)
+            out = _empty((n, self.mask_floats_per_chunk), _torch.float32, hidden.device, stream)
         elif not isinstance(out, int):
-            _layer_tensor(out, "out", dev, torch.float32)
+            _layer_tensor(out, "out", dev, _torch.float32)
             if out.numel() != n * self.mask_floats_per_chunk or not out.is_contiguous():
                 raise StemsError(1, "out: expected a contiguous [chunks][mask floats per chunk]")
         cfg = MaskHeadConfig(C.sizeof(MaskHeadConfig), code, k, n)
         need = C.c_size_t()
         self.engine._check(lib().stg_mask_head_workspace(self._h, C.byref(cfg), C.byref(need)), "mask_head")
-        ws = _empty((need.value,), torch.uint8, dev, stream) if need.value else None
-        rc = lib().stg_mask_head(self._h, C.byref(cfg), hidden.data_ptr(), weight.data_ptr(),
-                                 bias.data_ptr() if bias is not None else None, out if isinstance(out, int) else out.data_ptr(),
-                                 ws.data_ptr() if ws is not None else None, need.value, _stream_of(stream, hidden))
+        ws = _empty((need.value,), _torch.uint8, hidden.device, stream) if need.value else None
+        rc = lib().stg_mask_head(self._h, C.byref(cfg), hidden.data_ptr(), weight.data_ptr(), _ptr_of(bias),
+                                 out if isinstance(out, int) else out.data_ptr(), _ptr_of(ws), need.value,
+                                 self.engine._layer_stream(stream))
         if rc != 0:
             self.engine._check(rc, "mask_head")
         return out

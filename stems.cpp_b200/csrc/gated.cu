@@ -25,6 +25,16 @@ __device__ __forceinline__ void gate_both(int kind, float z, float& a, float& d)
     }
 }
 
+template <bool kFast> __device__ __forceinline__ float gate_value(int kind, float z) {
+    switch (kind) {
+        case STG_ACT_RELU: return act<STG_ACT_RELU, kFast>(z);
+        case STG_ACT_SILU: return act<STG_ACT_SILU, kFast>(z);
+        case STG_ACT_GELU: return act<STG_ACT_GELU, kFast>(z);
+        case STG_ACT_SIGMOID: return act<STG_ACT_SIGMOID, kFast>(z);
+        default: return z;
+    }
+}
+
 // A 128 x 16 tile of an operand on its way to shared memory, [k][128]. KMAJOR: element (i, k)
 // is at p[i * ld + k], otherwise at p[k * ld + i]. A thread takes eight neighbours in memory.
 template <class T, bool KMAJOR> struct TileLoad {
@@ -273,6 +283,90 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
     }
 }
 
+// A few rows: y for M rows at most, by streaming the weights once. A warp has O outputs, both weight
+// rows of each, and steps along the features with all lanes (V of them to an access); the rows of x
+// come from L1, where the block's warps share them. With few outputs, S warps share one and add up
+// through shared memory. Bound by reading the weights: nothing is read twice from memory.
+constexpr int kFewRows = 8;
+template <class T, int M, int V>
+__global__ void __launch_bounds__(kThreads) gated_rows(const __grid_constant__ GatedParams p) {
+    constexpr bool fast = sizeof(T) == 2;
+    constexpr int O = M > 2 ? 2 : 1, U = M > 2 ? 2 : 4;
+    using P = Pack<T, V>;
+    __shared__ float red[kThreads / 32][2 * O * M];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = p.splits, slice = warp % share;
+    const int n0 = (blockIdx.x * (kThreads / 32 / share) + warp / share) * O;
+    const T *w[2 * O], *x[M];
+#pragma unroll
+    for (int o = 0; o < O; o++) {   // an output past the last reads the last
+        const int64_t n = min(n0 + o, p.n - 1);
+        w[2 * o] = static_cast<const T*>(p.wg) + n * p.wg_row;
+        w[2 * o + 1] = static_cast<const T*>(p.wu) + n * p.wu_row;
+    }
+#pragma unroll
+    for (int m = 0; m < M; m++) x[m] = static_cast<const T*>(p.x) + min((int64_t)m, p.m - 1) * p.x_row;
+    float acc[2 * O][M];
+#pragma unroll
+    for (int i = 0; i < 2 * O; i++)
+#pragma unroll
+        for (int m = 0; m < M; m++) acc[i][m] = 0.0f;
+    auto take = [&](const P (&v)[2 * O], int k) {
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            const P xv = *reinterpret_cast<const P*>(x[m] + k);
+#pragma unroll
+            for (int i = 0; i < 2 * O; i++)
+#pragma unroll
+                for (int j = 0; j < V; j++) acc[i][m] = fmaf(to_float(v[i].v[j]), to_float(xv.v[j]), acc[i][m]);
+        }
+    };
+    const int step = 32 * V * share, whole = p.k / V * V;
+    int k = (slice * 32 + lane) * V;
+    for (; k + (U - 1) * step < whole; k += U * step) {
+        P v[U][2 * O];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < 2 * O; i++) v[u][i] = *reinterpret_cast<const P*>(w[i] + k + u * step);
+#pragma unroll
+        for (int u = 0; u < U; u++) take(v[u], k + u * step);
+    }
+    for (; k < whole; k += step) {
+        P v[2 * O];
+#pragma unroll
+        for (int i = 0; i < 2 * O; i++) v[i] = *reinterpret_cast<const P*>(w[i] + k);
+        take(v, k);
+    }
+    for (int e = whole + lane; slice == 0 && e < p.k; e += 32)   // the features past the last whole vector
+#pragma unroll
+        for (int m = 0; m < M; m++)
+#pragma unroll
+            for (int i = 0; i < 2 * O; i++) acc[i][m] = fmaf(to_float(w[i][e]), to_float(x[m][e]), acc[i][m]);
+#pragma unroll
+    for (int i = 0; i < 2 * O; i++)
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            float s = acc[i][m];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+            if (lane == 0) red[warp][i * M + m] = s;
+        }
+    __syncthreads();
+    // one thread to an output and row
+    for (int e = threadIdx.x; e < kThreads / 32 / share * O * M; e += kThreads) {
+        const int out = e / M, m = e - out * M, n = blockIdx.x * (kThreads / 32 / share) * O + out;
+        if (n >= p.n || m >= p.m) continue;
+        float g = 0.0f, u = 0.0f;
+        for (int q = 0; q < share; q++) {
+            g += red[out / O * share + q][(out % O * 2) * M + m];
+            u += red[out / O * share + q][(out % O * 2 + 1) * M + m];
+        }
+        if (p.bg) g += to_float(static_cast<const T*>(p.bg)[n]);
+        if (p.bu) u += to_float(static_cast<const T*>(p.bu)[n]);
+        static_cast<T*>(p.y)[m * p.y_row + n] = from_float<T>(gate_value<fast>(p.act, g) * u);
+    }
+}
+
 // The biases' gradients from the column sums [sums][2][n] (the first sum_blocks blocks, 32 columns
 // each) and dW from its partial sums [splits][2][n][k], both added in a fixed order.
 template <class T>
@@ -377,9 +471,9 @@ struct Copies { size_t x = 0, wg = 0, wu = 0; size_t bytes() const { return x + 
 size_t copy_bytes(int64_t rows, int64_t row, int cols) {
     return rows <= 1 || row % 8 == 0 ? 0 : up256((size_t)rows * (size_t)(ceil_div(cols, 8) * 8) * 2);
 }
-Copies copies_of(const stg_gated_config& c) {
+Copies copies_of(const stg_gated_config& c, bool backward) {
     Copies r;
-    if (c.dtype == STG_F32 || !c.rows) return r;
+    if (c.dtype == STG_F32 || !c.rows || (!backward && c.rows <= kFewRows)) return r;
     r.x = copy_bytes(c.rows, c.x_row, c.features);
     r.wg = copy_bytes(c.width, c.wg_row, c.features);
     r.wu = copy_bytes(c.width, c.wu_row, c.features);
@@ -431,7 +525,7 @@ GatedLayout backward_layout(const stg_gated_config& c) {
     l.splits = (int)std::max<int64_t>(1, ceil_div(c.rows, l.split_rows));
     l.dw = l.sums + up256(sizeof(float) * (size_t)std::max<int64_t>(ceil_div(c.rows, kGatedTileM), l.splits * ceil_div(c.features, 64)) * 2 * c.width);
     l.copies = l.dw + up256(sizeof(float) * (size_t)l.splits * 2 * c.width * c.features);
-    l.bytes = l.copies + copies_of(c).bytes();
+    l.bytes = l.copies + copies_of(c, true).bytes();
     return l;
 }
 
@@ -446,6 +540,20 @@ GatedParams params_of(const stg_gated_config& c) {
 // f16 and bf16 go to the tensor cores where the operands that are not copied start on 16 bytes.
 bool on_tensor_cores(const stg_gated_config& c, const Copies& copies, const GatedParams& p) {
     return c.dtype != STG_F32 && (copies.x || aligned(p.x, 16)) && (copies.wg || aligned(p.wg, 16)) && (copies.wu || aligned(p.wu, 16));
+}
+
+// A few rows (gated_rows): below that the tensor cores' 256-row tiles are nearly empty, and at 5461 x
+// 2048 bf16 they read the weights at 1.2 TB/s. Vectors of 16 bytes where every row starts on 16.
+template <class T, int M> void launch_rows(GatedParams& p, cudaStream_t st) {
+    constexpr int O = M > 2 ? 2 : 1, W = 16 / (int)sizeof(T);
+    // warps to an output: more while that gives fewer than eight warps per SM
+    p.splits = 1;
+    while (p.splits < kThreads / 32 && ceil_div(p.n, O) * p.splits < 148 * 8 && p.k > 32 * W * p.splits) p.splits *= 2;
+    const unsigned blocks = (unsigned)ceil_div(ceil_div(p.n, O), kThreads / 32 / p.splits);
+    const bool wide = aligned(p.x, 16) && aligned(p.wg, 16) && aligned(p.wu, 16) && (p.x_row % W == 0 || p.m == 1) &&
+                      (p.wg_row % W == 0 || p.n == 1) && (p.wu_row % W == 0 || p.n == 1);
+    if (wide) gated_rows<T, M, W><<<blocks, kThreads, 0, st>>>(p);
+    else gated_rows<T, M, 1><<<blocks, kThreads, 0, st>>>(p);
 }
 
 dim3 tile_grid(int64_t tiles, int64_t y = 1) {
@@ -463,7 +571,7 @@ STG_API stg_status stg_gated_workspace(const stg_gated_config* c, int32_t backwa
     return guard(nullptr, [&] {
         check_config(c, backward != 0);
         check(bytes && (backward == 0 || backward == 1), "gated: null buffer");
-        *bytes = !c->rows ? 0 : backward ? backward_layout(*c).bytes : copies_of(*c).bytes();
+        *bytes = !c->rows ? 0 : backward ? backward_layout(*c).bytes : copies_of(*c, false).bytes();
     });
 }
 
@@ -480,10 +588,14 @@ STG_API stg_status stg_gated(stg_engine* e, const stg_gated_config* c, const voi
         p.x = d_x; p.wg = d_wg; p.wu = d_wu; p.bg = d_bg; p.bu = d_bu; p.y = d_y;
         DeviceScope scope(e);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
-        const Copies copies = copies_of(*c);
+        const Copies copies = copies_of(*c, false);
         check(!copies.bytes() || (d_ws && aligned(d_ws, 256) && ws_bytes >= copies.bytes()), "gated: workspace is missing, unaligned or too small");
         with_dtype(c->dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
+            if (p.m == 1) return launch_rows<T, 1>(p, st);
+            if (p.m == 2) return launch_rows<T, 2>(p, st);
+            if (p.m <= 4) return launch_rows<T, 4>(p, st);
+            if (p.m <= kFewRows) return launch_rows<T, kFewRows>(p, st);
             if (on_tensor_cores(*c, copies, p)) {
                 copy_operands<T>(p, copies, p.m, p.n, static_cast<char*>(d_ws), st);
                 return launch_gated_mma(GATED_FWD, c->dtype == STG_BF16, p, 0, e->sms, st);
@@ -544,7 +656,7 @@ STG_API stg_status stg_gated_backward(stg_engine* e, const stg_gated_config* c, 
         };
         with_dtype(c->dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
-            const Copies copies = copies_of(*c);
+            const Copies copies = copies_of(*c, true);
             if (on_tensor_cores(*c, copies, p)) {
                 copy_operands<T>(p, copies, p.m, p.n, ws + lay.copies, st);
                 auto product = [&](GatedMode mode) { launch_gated_mma(mode, c->dtype == STG_BF16, p, 0, e->sms, st); };

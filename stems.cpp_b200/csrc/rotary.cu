@@ -32,7 +32,7 @@ struct RotaryParams {
     int copy_tail;
     FastDiv per_head;               // items of a head: rotated ones, then copied ones
     int rot_items, tail_items;
-    FastDiv heads_div;
+    FastDiv heads_div, half_div;
     const int32_t* pos;
     int64_t pos_batch;
     int offset;
@@ -54,83 +54,99 @@ __device__ __forceinline__ float2 cos_sin_turns(double t) {
 
 // V elements per access. LAYOUT 0: an item is a run of max(V, 2) neighbouring elements, whole
 // pairs; LAYOUT 1: V elements of the first half and their partners in the second. Tail items
-// are V elements past the rotated part.
+// are V elements past the rotated part. A thread has its next four items on their way at a time,
+// the first four while the table is made.
 template <class T, int V, int LAYOUT>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-    extern __shared__ float2 table[];
+    constexpr int U = 4;
+    constexpr int E = LAYOUT == 0 && V < 2 ? 2 : V;          // elements of an item's run
+    constexpr int R = LAYOUT == 0 ? E / V : 2;               // accesses of an item
+    using P = Pack<T, V>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    longlong2* at = reinterpret_cast<longlong2*>(smem);      // [tensor][token]: offsets into x and y
+    float2* table = reinterpret_cast<float2*>(at + 2 * p.tokens_per_block);
+    int32_t* where = reinterpret_cast<int32_t*>(table + p.tokens_per_block * p.half);   // [token]: positions
     const int64_t tok0 = (int64_t)blockIdx.x * p.tokens_per_block;
     const int n_tok = (int)min((int64_t)p.tokens_per_block, p.n - tok0);
     const int head0 = blockIdx.y * p.heads_per_block;
     const int n_heads = min(p.heads_per_block, p.heads - head0);
 
-    for (int e = threadIdx.x; e < n_tok * p.half; e += kThreads) {
-        const int tk = e / p.half, i = e - tk * p.half;
+    for (int e = threadIdx.x; e < 2 * n_tok; e += kThreads) {
+        const int k = e >= n_tok, tk = e - k * n_tok;
         const int64_t tok = tok0 + tk, b = tok / p.tokens, t = tok - b * p.tokens;
-        const int32_t pos = p.pos ? p.pos[b * p.pos_batch + t] : p.offset + (int32_t)t;
-        float2 cs = cos_sin_turns((double)pos * p.turns[i]);
+        if (!k) where[tk] = p.pos ? p.pos[b * p.pos_batch + t] : p.offset + (int32_t)t;
+        at[k * p.tokens_per_block + tk] = make_longlong2(b * p.t[k].xb + t * p.t[k].xt, b * p.t[k].yb + t * p.t[k].yt);
+    }
+    __syncthreads();
+
+    struct Item {
+        P v[R];
+        T* y;
+        const float2* cs;
+        int tail;
+    };
+    const int items = n_tok * n_heads * (int)p.per_head.d;
+    auto fetch = [&](Item& i, int it) {
+        const int hd = (int)p.per_head.div((uint32_t)it);          // token-major (token, head)
+        const int item = it - hd * (int)p.per_head.d;
+        // a block's last head range may be short: its heads count is then not the constant
+        const int tk = n_heads == (int)p.heads_div.d ? (int)p.heads_div.div((uint32_t)hd) : hd / n_heads;
+        const int h = head0 + hd - tk * n_heads, k = h >= p.heads0, hh = k ? h - p.heads0 : h;
+        const longlong2 o = at[k * p.tokens_per_block + tk];
+        i.tail = item >= p.rot_items;
+        const int run = i.tail ? p.rotary + (item - p.rot_items) * V : item * E;
+        const T* x = static_cast<const T*>(p.t[k].x) + o.x + hh * p.t[k].xh + run;
+        i.y = static_cast<T*>(p.t[k].y) + o.y + hh * p.t[k].yh + run;
+        i.cs = table + tk * p.half + (LAYOUT == 0 ? run >> 1 : run);
+        i.v[0] = *reinterpret_cast<const P*>(x);
+        if (R == 2 && !i.tail) i.v[R - 1] = *reinterpret_cast<const P*>(x + (LAYOUT == 0 ? V : p.half));
+    };
+    auto finish = [&](Item& i) {
+        if (!i.tail) {
+            if (LAYOUT == 0) {
+                float f[E];
+#pragma unroll
+                for (int j = 0; j < E; j++) f[j] = to_float(i.v[j / V].v[j % V]);
+#pragma unroll
+                for (int j = 0; j < E; j += 2) {
+                    const float2 w = i.cs[j >> 1];
+                    const float a = f[j], c = f[j + 1];
+                    i.v[j / V].v[j % V] = from_float<T>(fmaf(a, w.x, -c * w.y));
+                    i.v[(j + 1) / V].v[(j + 1) % V] = from_float<T>(fmaf(c, w.x, a * w.y));
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const float2 w = i.cs[j];
+                    const float a = to_float(i.v[0].v[j]), c = to_float(i.v[R - 1].v[j]);
+                    i.v[0].v[j] = from_float<T>(fmaf(a, w.x, -c * w.y));
+                    i.v[R - 1].v[j] = from_float<T>(fmaf(c, w.x, a * w.y));
+                }
+            }
+            if (R == 2) *reinterpret_cast<P*>(i.y + (LAYOUT == 0 ? V : p.half)) = i.v[R - 1];
+        }
+        *reinterpret_cast<P*>(i.y) = i.v[0];
+    };
+
+    Item now[U];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if ((int)threadIdx.x + u * kThreads < items) fetch(now[u], threadIdx.x + u * kThreads);
+    for (int e = threadIdx.x; e < n_tok * p.half; e += kThreads) {
+        const int tk = (int)p.half_div.div((uint32_t)e), i = e - tk * p.half;
+        float2 cs = cos_sin_turns((double)where[tk] * p.turns[i]);
         cs.x *= p.magnitude;
         cs.y *= p.magnitude;
         table[e] = cs;
     }
     __syncthreads();
-
-    using P = Pack<T, V>;
-    const int per_tok = n_heads * (int)p.per_head.d;
-    const FastDiv& heads_div = p.heads_div;
-    for (int it = threadIdx.x; it < n_tok * per_tok; it += kThreads) {
-        const int hd = (int)p.per_head.div((uint32_t)it);          // token-major (token, head)
-        const int item = it - hd * (int)p.per_head.d;
-        // a block's last head range may be short: its heads count is then not the constant
-        const int tk = n_heads == (int)heads_div.d ? (int)heads_div.div((uint32_t)hd) : hd / n_heads;
-        const int h = head0 + hd - tk * n_heads;
-        const int64_t tok = tok0 + tk;
-        const int64_t b = tok / p.tokens, t = tok - b * p.tokens;
-        const RotaryTensor& R = p.t[h >= p.heads0];
-        const int hh = h >= p.heads0 ? h - p.heads0 : h;
-        const T* x = static_cast<const T*>(R.x) + b * R.xb + t * R.xt + hh * R.xh;
-        T* y = static_cast<T*>(R.y) + b * R.yb + t * R.yt + hh * R.yh;
-        const float2* cs = table + tk * p.half;
-        if (item >= p.rot_items) {
-            const int at = p.rotary + (item - p.rot_items) * V;
-            *reinterpret_cast<P*>(y + at) = *reinterpret_cast<const P*>(x + at);
-        } else if (LAYOUT == 0) {
-            constexpr int E = V < 2 ? 2 : V;   // with one element per access, a pair is two
-            const int at = item * E;
-            T in[E], out[E];
+    for (int it = threadIdx.x; it < items; it += U * kThreads) {
 #pragma unroll
-            for (int k = 0; k < E; k += V) {
-                const P v = *reinterpret_cast<const P*>(x + at + k);
+        for (int u = 0; u < U; u++)
+            if (it + u * kThreads < items) finish(now[u]);
 #pragma unroll
-                for (int j = 0; j < V; j++) in[k + j] = v.v[j];
-            }
-#pragma unroll
-            for (int k = 0; k < E; k += 2) {
-                const float2 w = cs[(at + k) >> 1];
-                const float a = to_float(in[k]), c = to_float(in[k + 1]);
-                out[k] = from_float<T>(fmaf(a, w.x, -c * w.y));
-                out[k + 1] = from_float<T>(fmaf(c, w.x, a * w.y));
-            }
-#pragma unroll
-            for (int k = 0; k < E; k += V) {
-                P v;
-#pragma unroll
-                for (int j = 0; j < V; j++) v.v[j] = out[k + j];
-                *reinterpret_cast<P*>(y + at + k) = v;
-            }
-        } else {
-            const int at = item * V;
-            const P a = *reinterpret_cast<const P*>(x + at), c = *reinterpret_cast<const P*>(x + at + p.half);
-            P u, v;
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float2 w = cs[at + j];
-                const float fa = to_float(a.v[j]), fc = to_float(c.v[j]);
-                u.v[j] = from_float<T>(fmaf(fa, w.x, -fc * w.y));
-                v.v[j] = from_float<T>(fmaf(fc, w.x, fa * w.y));
-            }
-            *reinterpret_cast<P*>(y + at) = u;
-            *reinterpret_cast<P*>(y + at + p.half) = v;
-        }
+        for (int u = 0; u < U; u++)
+            if (it + (u + U) * kThreads < items) fetch(now[u], it + (u + U) * kThreads);
     }
 }
 
@@ -157,9 +173,10 @@ void launch(RotaryParams& p, int layout, cudaStream_t st) {
     const int parts = (p.heads + p.heads_per_block - 1) / p.heads_per_block;
     p.per_head = FastDiv((uint32_t)per_head);
     p.heads_div = FastDiv((uint32_t)p.heads_per_block);
+    p.half_div = FastDiv((uint32_t)p.half);
     if (blocks > INT32_MAX || parts > 65535) fail(STG_UNSUPPORTED, "rotary: too many tokens or heads");
     const dim3 grid((unsigned)blocks, (unsigned)parts);
-    const size_t smem = sizeof(float2) * (size_t)p.tokens_per_block * p.half;
+    const size_t smem = (size_t)p.tokens_per_block * (sizeof(float2) * p.half + 2 * sizeof(longlong2) + sizeof(int32_t));
     if (layout == 0) rotary_kernel<T, V, 0><<<grid, kThreads, smem, st>>>(p);
     else rotary_kernel<T, V, 1><<<grid, kThreads, smem, st>>>(p);
     cuda_check(cudaGetLastError(), "rotary kernel");

@@ -58,6 +58,13 @@ def test_structs_match_the_header(pkg, tmp_path):
         assert [int(o) for o in offs] == [getattr(names[n], f).offset for f, _ in names[n]._fields_], n
 
 
+def test_packed_configurations_are_the_structs(pkg):
+    for packed, struct in ((pkg._ROTARY, pkg.RotaryConfig), (pkg._ROTARY_TENSOR, pkg.RotaryTensor), (pkg._GROUP_NORM, pkg.GroupNormConfig),
+                           (pkg._GATED, pkg.GatedConfig)):
+        values = list(range(1, len(struct._fields_) + 1))
+        assert packed.pack(*values) == bytes(struct(*values))
+
+
 def test_null_engines_and_plans_are_rejected(pkg):
     L, n = pkg.lib(), C.c_size_t()
     assert L.stg_rotary(None, C.byref(rotary_cfg(pkg)), None, 1, None, 0, None) == 1
