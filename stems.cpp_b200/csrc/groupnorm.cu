@@ -79,20 +79,6 @@ template <class T> __device__ __forceinline__ void set_param(void* p, int i, boo
     else static_cast<T*>(p)[i] = from_float<T>(v);
 }
 
-// A vector's last read, and a result that is not read here: both leave L2 first.
-template <class P, class T> __device__ __forceinline__ P load_stream(const T* p) {
-    P v;
-    if constexpr (sizeof(P) == 16) {
-        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
-        v = *reinterpret_cast<const P*>(&u);
-    } else v = *reinterpret_cast<const P*>(p);
-    return v;
-}
-template <class T, class P> __device__ __forceinline__ void store_stream(T* p, const P& v) {
-    if constexpr (sizeof(P) == 16) __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
-    else *reinterpret_cast<P*>(p) = v;
-}
-
 // The thread's place in a block: column vector `col` of the current column tile and one of
 // `step` positions taken side by side.
 struct Place { int width, step, r, col; };
@@ -107,37 +93,6 @@ template <int THREADS> __device__ __forceinline__ Place place(const NormParams& 
 // Positions of n that place q has.
 __device__ __forceinline__ int mine_of(const Place& q, int n) { return q.r < n ? (n - q.r + q.step - 1) / q.step : 0; }
 
-// load() then use() n times, in that order each, with the loads U to 2U ahead.
-template <class P, int U, class Load, class Use> __device__ __forceinline__ void stream(int n, Load&& load, Use&& use) {
-    P now[U], next[U];
-    if (n >= U) {
-#pragma unroll
-        for (int u = 0; u < U; u++) load(now[u]);
-#pragma unroll 2
-        for (; n >= 2 * U; n -= U) {
-#pragma unroll
-            for (int u = 0; u < U; u++) load(next[u]);
-#pragma unroll
-            for (int u = 0; u < U; u++) use(now[u]);
-#pragma unroll
-            for (int u = 0; u < U; u++) now[u] = next[u];
-        }
-        n -= U;
-        // the rest is on its way while the last whole batch is used
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (u < n) load(next[u]);
-#pragma unroll
-        for (int u = 0; u < U; u++) use(now[u]);
-    } else {
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (u < n) load(next[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++)
-        if (u < n) use(next[u]);
-}
 template <class P> struct Two { P x, dy; };
 
 // A thread's sums of its channels.

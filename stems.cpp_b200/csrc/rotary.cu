@@ -15,7 +15,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxHalf = 256;      // rotary_dim at most 512
-constexpr int kTableEntries = 2048;   // (cos, sin) pairs a block keeps: 16 KB
+constexpr int kTableEntries = 2048;   // (cos, sin) pairs a block keeps: at most 16 KB but for a single token
 
 struct RotaryTensor {
     const void* x;
@@ -32,7 +32,7 @@ struct RotaryParams {
     int copy_tail;
     FastDiv per_head;               // items of a head: rotated ones, then copied ones
     int rot_items, tail_items;
-    FastDiv heads_div, half_div;
+    FastDiv half_div;
     const int32_t* pos;
     int64_t pos_batch;
     int offset;
@@ -54,22 +54,24 @@ __device__ __forceinline__ float2 cos_sin_turns(double t) {
 
 // V elements per access. LAYOUT 0: an item is a run of max(V, 2) neighbouring elements, whole
 // pairs; LAYOUT 1: V elements of the first half and their partners in the second. Tail items
-// are V elements past the rotated part. A thread has its next four items on their way at a time,
-// the first four while the table is made.
+// are V elements past the rotated part. A thread keeps to one place of the heads (or a few) and walks
+// the block's tokens, so that an item costs it an offset from shared memory and an addition.
 template <class T, int V, int LAYOUT>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-    constexpr int U = 4;
+__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const __grid_constant__ RotaryParams p) {
     constexpr int E = LAYOUT == 0 && V < 2 ? 2 : V;          // elements of an item's run
     constexpr int R = LAYOUT == 0 ? E / V : 2;               // accesses of an item
+    constexpr int U = 4 / R;
     using P = Pack<T, V>;
+    struct Item { P v[R]; };
     extern __shared__ __align__(16) uint8_t smem[];
     longlong2* at = reinterpret_cast<longlong2*>(smem);      // [tensor][token]: offsets into x and y
-    float2* table = reinterpret_cast<float2*>(at + 2 * p.tokens_per_block);
+    double* turns = reinterpret_cast<double*>(at + 2 * p.tokens_per_block);
+    float2* table = reinterpret_cast<float2*>(turns + p.half);
     int32_t* where = reinterpret_cast<int32_t*>(table + p.tokens_per_block * p.half);   // [token]: positions
     const int64_t tok0 = (int64_t)blockIdx.x * p.tokens_per_block;
     const int n_tok = (int)min((int64_t)p.tokens_per_block, p.n - tok0);
     const int head0 = blockIdx.y * p.heads_per_block;
-    const int n_heads = min(p.heads_per_block, p.heads - head0);
+    const int columns = min(p.heads_per_block, p.heads - head0) * (int)p.per_head.d;
 
     for (int e = threadIdx.x; e < 2 * n_tok; e += kThreads) {
         const int k = e >= n_tok, tk = e - k * n_tok;
@@ -77,76 +79,72 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
         if (!k) where[tk] = p.pos ? p.pos[b * p.pos_batch + t] : p.offset + (int32_t)t;
         at[k * p.tokens_per_block + tk] = make_longlong2(b * p.t[k].xb + t * p.t[k].xt, b * p.t[k].yb + t * p.t[k].yt);
     }
+    for (int i = threadIdx.x; i < p.half; i += kThreads) turns[i] = p.turns[i];
     __syncthreads();
-
-    struct Item {
-        P v[R];
-        T* y;
-        const float2* cs;
-        int tail;
-    };
-    const int items = n_tok * n_heads * (int)p.per_head.d;
-    auto fetch = [&](Item& i, int it) {
-        const int hd = (int)p.per_head.div((uint32_t)it);          // token-major (token, head)
-        const int item = it - hd * (int)p.per_head.d;
-        // a block's last head range may be short: its heads count is then not the constant
-        const int tk = n_heads == (int)p.heads_div.d ? (int)p.heads_div.div((uint32_t)hd) : hd / n_heads;
-        const int h = head0 + hd - tk * n_heads, k = h >= p.heads0, hh = k ? h - p.heads0 : h;
-        const longlong2 o = at[k * p.tokens_per_block + tk];
-        i.tail = item >= p.rot_items;
-        const int run = i.tail ? p.rotary + (item - p.rot_items) * V : item * E;
-        const T* x = static_cast<const T*>(p.t[k].x) + o.x + hh * p.t[k].xh + run;
-        i.y = static_cast<T*>(p.t[k].y) + o.y + hh * p.t[k].yh + run;
-        i.cs = table + tk * p.half + (LAYOUT == 0 ? run >> 1 : run);
-        i.v[0] = *reinterpret_cast<const P*>(x);
-        if (R == 2 && !i.tail) i.v[R - 1] = *reinterpret_cast<const P*>(x + (LAYOUT == 0 ? V : p.half));
-    };
-    auto finish = [&](Item& i) {
-        if (!i.tail) {
-            if (LAYOUT == 0) {
-                float f[E];
-#pragma unroll
-                for (int j = 0; j < E; j++) f[j] = to_float(i.v[j / V].v[j % V]);
-#pragma unroll
-                for (int j = 0; j < E; j += 2) {
-                    const float2 w = i.cs[j >> 1];
-                    const float a = f[j], c = f[j + 1];
-                    i.v[j / V].v[j % V] = from_float<T>(fmaf(a, w.x, -c * w.y));
-                    i.v[(j + 1) / V].v[(j + 1) % V] = from_float<T>(fmaf(c, w.x, a * w.y));
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float2 w = i.cs[j];
-                    const float a = to_float(i.v[0].v[j]), c = to_float(i.v[R - 1].v[j]);
-                    i.v[0].v[j] = from_float<T>(fmaf(a, w.x, -c * w.y));
-                    i.v[R - 1].v[j] = from_float<T>(fmaf(c, w.x, a * w.y));
-                }
-            }
-            if (R == 2) *reinterpret_cast<P*>(i.y + (LAYOUT == 0 ? V : p.half)) = i.v[R - 1];
-        }
-        *reinterpret_cast<P*>(i.y) = i.v[0];
-    };
-
-    Item now[U];
-#pragma unroll
-    for (int u = 0; u < U; u++)
-        if ((int)threadIdx.x + u * kThreads < items) fetch(now[u], threadIdx.x + u * kThreads);
     for (int e = threadIdx.x; e < n_tok * p.half; e += kThreads) {
         const int tk = (int)p.half_div.div((uint32_t)e), i = e - tk * p.half;
-        float2 cs = cos_sin_turns((double)where[tk] * p.turns[i]);
+        float2 cs = cos_sin_turns((double)where[tk] * turns[i]);
         cs.x *= p.magnitude;
         cs.y *= p.magnitude;
         table[e] = cs;
     }
     __syncthreads();
-    for (int it = threadIdx.x; it < items; it += U * kThreads) {
+
+    auto turn = [](Item& i, const float2* w) {
+        if (LAYOUT == 0) {
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            if (it + u * kThreads < items) finish(now[u]);
+            for (int j = 0; j < E; j += 2) {
+                const float2 t = w[j >> 1];
+                T &x0 = i.v[j / V].v[j % V], &x1 = i.v[(j + 1) / V].v[(j + 1) % V];
+                const float a = to_float(x0), b = to_float(x1);
+                x0 = from_float<T>(fmaf(a, t.x, -b * t.y));
+                x1 = from_float<T>(fmaf(b, t.x, a * t.y));
+            }
+        } else {
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            if (it + (u + U) * kThreads < items) fetch(now[u], it + (u + U) * kThreads);
+            for (int j = 0; j < V; j++) {
+                const float2 t = w[j];
+                const float a = to_float(i.v[0].v[j]), b = to_float(i.v[R - 1].v[j]);
+                i.v[0].v[j] = from_float<T>(fmaf(a, t.x, -b * t.y));
+                i.v[R - 1].v[j] = from_float<T>(fmaf(b, t.x, a * t.y));
+            }
+        }
+    };
+    const int width = min(columns, kThreads), step = kThreads / width, r = threadIdx.x / width;
+    if (r >= step) return;
+    for (int c = threadIdx.x - r * width; c < columns; c += width) {
+        const int hd = (int)p.per_head.div((uint32_t)c), item = c - hd * (int)p.per_head.d;
+        const int h = head0 + hd, k = h >= p.heads0, hh = k ? h - p.heads0 : h;
+        const bool tail = item >= p.rot_items;
+        const int run = tail ? p.rotary + (item - p.rot_items) * V : item * E;
+        const T* x = static_cast<const T*>(k ? p.t[1].x : p.t[0].x) + hh * (k ? p.t[1].xh : p.t[0].xh) + run;
+        T* y = static_cast<T*>(k ? p.t[1].y : p.t[0].y) + hh * (k ? p.t[1].yh : p.t[0].yh) + run;
+        const longlong2* to = at + k * p.tokens_per_block;
+        const float2* cs = table + (LAYOUT == 0 ? run >> 1 : run);
+        constexpr int other = LAYOUT == 0 ? V : 0;
+        const int second = LAYOUT == 0 ? other : p.half;
+        for (int t0 = r; t0 < n_tok; t0 += U * step) {
+            Item i[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int tk = t0 + u * step;
+                if (tk >= n_tok) break;
+                const T* q = x + to[tk].x;
+                i[u].v[0] = load_stream<P>(q);
+                if (R == 2 && !tail) i[u].v[R - 1] = load_stream<P>(q + second);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int tk = t0 + u * step;
+                if (tk >= n_tok) break;
+                T* q = y + to[tk].y;
+                if (!tail) {
+                    turn(i[u], cs + tk * p.half);
+                    if (R == 2) store_stream(q + second, i[u].v[R - 1]);
+                }
+                store_stream(q, i[u].v[0]);
+            }
+        }
     }
 }
 
@@ -156,12 +154,13 @@ void launch(RotaryParams& p, int layout, cudaStream_t st) {
     p.rot_items = (layout == 0 ? p.rotary : p.half) / e;
     p.tail_items = p.copy_tail ? (p.dim - p.rotary) / V : 0;
     const int per_head = p.rot_items + p.tail_items;
-    // tokens so that a thread has about four items and the table fits; heads split over blocks
-    // only when so few tokens would leave most of the GPU idle (then each part repeats the table)
+    // tokens so that a thread has about sixteen items, while the table fits and the GPU has two blocks
+    // per SM; heads split over blocks only when so few tokens would leave most of it idle (then
+    // each part repeats the table)
     p.heads_per_block = p.heads;
     p.tokens_per_block = 1;
-    while (p.tokens_per_block < 64 && (int64_t)p.tokens_per_block * per_head * p.heads < 4 * kThreads &&
-           2 * p.tokens_per_block * p.half <= kTableEntries)
+    while ((int64_t)p.tokens_per_block * per_head * p.heads < 16 * kThreads && 2 * p.tokens_per_block * p.half <= kTableEntries &&
+           p.n / (2 * p.tokens_per_block) >= 296)
         p.tokens_per_block *= 2;
     const int64_t blocks = (p.n + p.tokens_per_block - 1) / p.tokens_per_block;
     if (blocks < 148) {
@@ -172,11 +171,10 @@ void launch(RotaryParams& p, int layout, cudaStream_t st) {
     while ((int64_t)p.tokens_per_block * per_head * p.heads_per_block >= (1 << 30)) p.heads_per_block = (p.heads_per_block + 1) / 2;
     const int parts = (p.heads + p.heads_per_block - 1) / p.heads_per_block;
     p.per_head = FastDiv((uint32_t)per_head);
-    p.heads_div = FastDiv((uint32_t)p.heads_per_block);
     p.half_div = FastDiv((uint32_t)p.half);
     if (blocks > INT32_MAX || parts > 65535) fail(STG_UNSUPPORTED, "rotary: too many tokens or heads");
     const dim3 grid((unsigned)blocks, (unsigned)parts);
-    const size_t smem = (size_t)p.tokens_per_block * (sizeof(float2) * p.half + 2 * sizeof(longlong2) + sizeof(int32_t));
+    const size_t smem = (size_t)p.tokens_per_block * (sizeof(float2) * p.half + 2 * sizeof(longlong2) + sizeof(int32_t)) + sizeof(double) * p.half;
     if (layout == 0) rotary_kernel<T, V, 0><<<grid, kThreads, smem, st>>>(p);
     else rotary_kernel<T, V, 1><<<grid, kThreads, smem, st>>>(p);
     cuda_check(cudaGetLastError(), "rotary kernel");
