@@ -13,7 +13,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTileK = 16;
-constexpr int kPitch = 132;        // floats between two k rows of a tile
 
 __device__ __forceinline__ void gate_both(int kind, float z, float& a, float& d) {
     switch (kind) {
@@ -35,39 +34,43 @@ template <bool kFast> __device__ __forceinline__ float gate_value(int kind, floa
     }
 }
 
-// A 128 x 16 tile of an operand on its way to shared memory, [k][128]. KMAJOR: element (i, k)
-// is at p[i * ld + k], otherwise at p[k * ld + i]. A thread takes eight neighbours in memory.
-template <class T, bool KMAJOR> struct TileLoad {
-    float v[8];
+// An S x 16 tile of an operand on its way to shared memory, [k][S]. KMAJOR: element (i, k) is at
+// p[i * ld + k], otherwise at p[k * ld + i]. A thread takes its neighbours in memory.
+template <class T, bool KMAJOR, int S> struct TileLoad {
+    static constexpr int N = S / 16, PER_ROW = KMAJOR ? kTileK / N : S / N;   // elements of a thread, threads of a memory row
+    static constexpr int kPitch = S + 4;
+    float v[N];
+    // the row of the operand, within the tile, that the thread carries when KMAJOR
+    __device__ __forceinline__ static int row() { return threadIdx.x / PER_ROW; }
     __device__ __forceinline__ void fetch(const T* p, int64_t ld, int64_t i0, int64_t ni, int64_t k0, int64_t nk) {
         const int t = threadIdx.x;
-        const int64_t r = KMAJOR ? i0 + (t >> 1) : k0 + (t >> 4);
-        const int64_t c = KMAJOR ? k0 + (t & 1) * 8 : i0 + (t & 15) * 8;
+        const int64_t r = KMAJOR ? i0 : k0 + t / PER_ROW;      // KMAJOR: the caller adds row()
+        const int64_t c = (KMAJOR ? k0 : i0) + t % PER_ROW * N;
         const bool row_ok = r < (KMAJOR ? ni : nk);
         const int64_t nc = KMAJOR ? nk : ni;
         const T* q = p + r * ld + c;
-        if (row_ok && c + 8 <= nc && (reinterpret_cast<uintptr_t>(q) & 15) == 0) {
-            constexpr int W = 16 / sizeof(T);
+        constexpr int W = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+        if (row_ok && c + N <= nc && reinterpret_cast<uintptr_t>(q) % (W * sizeof(T)) == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; j += W) {
+            for (int j = 0; j < N; j += W) {
                 const Pack<T, W> w = *reinterpret_cast<const Pack<T, W>*>(q + j);
 #pragma unroll
                 for (int e = 0; e < W; e++) v[j + e] = to_float(w.v[e]);
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = row_ok && c + j < nc ? to_float(q[j]) : 0.0f;
+            for (int j = 0; j < N; j++) v[j] = row_ok && c + j < nc ? to_float(q[j]) : 0.0f;
         }
     }
-    __device__ __forceinline__ void store(float* s, int row_base = 0) const {
+    __device__ __forceinline__ void store(float* s) const {
         const int t = threadIdx.x;
         if (KMAJOR) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) s[((t & 1) * 8 + j) * kPitch + row_base + (t >> 1)] = v[j];
+            for (int j = 0; j < N; j++) s[(t % PER_ROW * N + j) * kPitch + t / PER_ROW] = v[j];
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; j += 4)
-                *reinterpret_cast<float4*>(s + (t >> 4) * kPitch + (t & 15) * 8 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            for (int j = 0; j < N; j += 4)
+                *reinterpret_cast<float4*>(s + t / PER_ROW * kPitch + t % PER_ROW * N + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         }
     }
 };
@@ -86,14 +89,18 @@ __device__ __forceinline__ float2 halves(uint64_t a) {
     return r;
 }
 
-// 128 x 128 outputs per block, 8 x 8 per thread: rows 4 ty + {0..3} and 64 + that, columns
-// 4 tx + {0..3} and 64 + that. In the dual modes the second 64 columns are the up projection of
-// the same outputs as the first, so a thread holds both factors of its outputs. Products and
-// sums are float with one rounding each (packed in pairs); K runs in order.
-template <class T, int MODE>
+// S x S outputs per block: 128 with 8 x 8 per thread (rows 4 ty + {0..3} and 64 + that, columns 4 tx +
+// {0..3} and 64 + that), or 64 with 4 x 4, for products with too few tiles for the GPU. In the dual
+// modes half of the columns are the up projection of the same outputs as the other half, placed
+// so that a thread holds both factors of its outputs: at 128 the second 64 columns, at 64 the
+// second two of each thread's four. Products and sums are float with one rounding each (packed in
+// pairs); K runs in order. Bound by the float units: 48 TFLOP/s at 48060 x 384 x 1408.
+template <class T, int MODE, int S>
 __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ GatedParams p) {
     constexpr bool DUAL = MODE == GATED_FWD || MODE == GATED_HEAD || MODE == GATED_PRE;
     constexpr bool AK = MODE != GATED_DW, BK = DUAL;   // contraction contiguous in memory
+    constexpr int G = S / 64, R = 4 * G, CP = 2 * G, kPitch = S + 4;   // rows and column pairs of a thread
+    constexpr int kTileM = S, kTileOut = DUAL ? S / 2 : S;
     __shared__ __align__(16) float As[2][kTileK * kPitch], Bs[2][kTileK * kPitch];
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 
@@ -107,9 +114,9 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
     int64_t kbeg = 0;
     if (MODE == GATED_HEAD) {
         ht = p.tiles[blockIdx.x % p.n_tiles];
-        const int64_t rest = blockIdx.x / p.n_tiles, mt = (p.frames + kGatedTileM - 1) / kGatedTileM;
+        const int64_t rest = blockIdx.x / p.n_tiles, mt = (p.frames + kTileM - 1) / kTileM;
         const int64_t cs = rest / mt;                    // chunk * stems + stem
-        m0 = (rest - cs * mt) * kGatedTileM;
+        m0 = (rest - cs * mt) * kTileM;
         n0 = ht.n0;
         ni = p.frames; nk = p.k; nj = ht.din;
         head_row = (cs * p.bands + ht.band) * p.frames;
@@ -121,18 +128,18 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
         ldb0 = ldb1 = p.k;
         head_row = cs;                                   // for the output
     } else if (DUAL) {
-        const int nt = (p.n + kGatedTileN - 1) / kGatedTileN;
-        m0 = (int64_t)(blockIdx.x / nt) * kGatedTileM;
-        n0 = (int)(blockIdx.x % nt) * kGatedTileN;
+        const int nt = (p.n + kTileOut - 1) / kTileOut;
+        m0 = (int64_t)(blockIdx.x / nt) * kTileM;
+        n0 = (int)(blockIdx.x % nt) * kTileOut;
         ni = p.m; nk = p.k; nj = p.n;
         a = static_cast<const T*>(p.x);
         b0 = static_cast<const T*>(p.wg);
         b1 = static_cast<const T*>(p.wu);
         lda = p.x_row; ldb0 = p.wg_row; ldb1 = p.wu_row;
     } else if (MODE == GATED_DX) {
-        const int nt = (p.k + 127) / 128;
-        m0 = (int64_t)(blockIdx.x / nt) * kGatedTileM;
-        n0 = (int)(blockIdx.x % nt) * 128;
+        const int nt = (p.k + S - 1) / S;
+        m0 = (int64_t)(blockIdx.x / nt) * kTileM;
+        n0 = (int)(blockIdx.x % nt) * S;
         ni = p.m; nk = p.n; nj = p.k;
         a = static_cast<const T*>(p.dg);
         a2 = static_cast<const T*>(p.du);
@@ -140,9 +147,9 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
         b1 = static_cast<const T*>(p.wu);
         lda = p.pre_row; ldb0 = p.wg_row; ldb1 = p.wu_row;
     } else {
-        const int nt = (p.k + 127) / 128;
-        m0 = (int64_t)(blockIdx.x / nt) * kGatedTileM;
-        n0 = (int)(blockIdx.x % nt) * 128;
+        const int nt = (p.k + S - 1) / S;
+        m0 = (int64_t)(blockIdx.x / nt) * kTileM;
+        n0 = (int)(blockIdx.x % nt) * S;
         const bool up = blockIdx.y & 1;
         kbeg = (int64_t)(blockIdx.y >> 1) * p.split_rows;
         ni = p.n; nk = min(p.m, kbeg + p.split_rows); nj = p.k;
@@ -151,23 +158,23 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
         lda = p.pre_row; ldb0 = ldb1 = p.x_row;
     }
 
-    uint64_t acc[8][4];
+    uint64_t acc[R][CP];
 #pragma unroll
-    for (int i = 0; i < 8; i++)
+    for (int i = 0; i < R; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = 0;
+        for (int j = 0; j < CP; j++) acc[i][j] = 0;
 
     const int64_t steps1 = (nk - kbeg + kTileK - 1) / kTileK, steps = steps1 * (MODE == GATED_DX ? 2 : 1);
-    TileLoad<T, AK> la;
-    TileLoad<T, BK> lb;
-    // the dual modes' B tile: rows 0..63 from Wg, 64..127 from Wu
+    TileLoad<T, AK, S> la;
+    TileLoad<T, BK, S> lb;
     auto fetch = [&](int64_t s) {
         const bool second = MODE == GATED_DX && s >= steps1;
         const int64_t k0 = kbeg + (second ? s - steps1 : s) * kTileK;
-        la.fetch(second ? a2 : a, lda, m0, ni, k0, nk);
+        la.fetch(second ? a2 : a, lda, m0 + (AK ? la.row() : 0), ni, k0, nk);
         if (DUAL) {
-            const bool up = threadIdx.x >= 128;   // threads 128.. carry rows 64..
-            lb.fetch(up ? b1 : b0, up ? ldb1 : ldb0, n0 - (up ? 64 : 0), nj, k0, nk);
+            const int r = lb.row();   // the tile's row the thread carries: which weight, which output
+            const bool up = S == 128 ? r >= 64 : r & 2;
+            lb.fetch(up ? b1 : b0, up ? ldb1 : ldb0, n0 + (S == 128 ? r & 63 : (r >> 2) * 2 + (r & 1)), nj, k0, nk);
         } else {
             lb.fetch(second ? b1 : b0, second ? ldb1 : ldb0, n0, nj, k0, nk);
         }
@@ -184,15 +191,20 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
         const float *pa = As[cur] + 4 * ty, *pb = Bs[cur] + 4 * tx;
 #pragma unroll
         for (int k = 0; k < kTileK; k++) {
-            const float4 a0 = *reinterpret_cast<const float4*>(pa + k * kPitch), a1 = *reinterpret_cast<const float4*>(pa + k * kPitch + 64);
-            const ulonglong2 c0 = *reinterpret_cast<const ulonglong2*>(pb + k * kPitch), c1 = *reinterpret_cast<const ulonglong2*>(pb + k * kPitch + 64);
-            const float av[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
-            const uint64_t bv[4] = {c0.x, c0.y, c1.x, c1.y};
+            float av[R];
+            uint64_t bv[CP];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int g = 0; g < G; g++) {
+                const float4 x = *reinterpret_cast<const float4*>(pa + k * kPitch + 64 * g);
+                const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(pb + k * kPitch + 64 * g);
+                av[4 * g] = x.x; av[4 * g + 1] = x.y; av[4 * g + 2] = x.z; av[4 * g + 3] = x.w;
+                bv[2 * g] = y.x; bv[2 * g + 1] = y.y;
+            }
+#pragma unroll
+            for (int i = 0; i < R; i++) {
                 const uint64_t d = twice(av[i]);
 #pragma unroll
-                for (int j = 0; j < 4; j++) fma2(acc[i][j], d, bv[j]);
+                for (int j = 0; j < CP; j++) fma2(acc[i][j], d, bv[j]);
             }
         }
         if (s + 1 < steps) {
@@ -202,11 +214,11 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
         __syncthreads();
     }
 
-    float v[8][8];
+    float v[R][2 * CP];
 #pragma unroll
-    for (int i = 0; i < 8; i++)
+    for (int i = 0; i < R; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < CP; j++) {
             const float2 h = halves(acc[i][j]);
             v[i][2 * j] = h.x;
             v[i][2 * j + 1] = h.y;
@@ -214,10 +226,11 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
     auto row_of = [&](int i) { return m0 + 4 * ty + (i & 3) + (i >> 2) * 64; };
 
     if (DUAL) {
-        float bg[4], bu[4];
+        constexpr int O = CP;   // outputs of a thread, the gate's columns before the up projection's
+        float bg[O], bu[O];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int c = n0 + 4 * tx + j;
+        for (int j = 0; j < O; j++) {
+            const int c = n0 + O * tx + j;
             bg[j] = bu[j] = 0.0f;
             if (p.bg && c < nj) {
                 bg[j] = to_float(static_cast<const T*>(p.bg)[bias0 + c]);
@@ -225,16 +238,16 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
             }
             if (MODE != GATED_HEAD && p.bu && c < nj) bu[j] = to_float(static_cast<const T*>(p.bu)[c]);
         }
-        float sg[4] = {}, su[4] = {};
+        float sg[O] = {}, su[O] = {};
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < R; i++) {
             const int64_t r = row_of(i);
             if (r >= ni) continue;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int c = n0 + 4 * tx + j;
+            for (int j = 0; j < O; j++) {
+                const int c = n0 + O * tx + j;
                 if (c >= nj) continue;
-                const float g = v[i][j] + bg[j], u = v[i][4 + j] + bu[j];
+                const float g = v[i][j] + bg[j], u = v[i][O + j] + bu[j];
                 float a, d;
                 if (MODE != GATED_HEAD) gate_both(p.act, g, a, d);
                 if (MODE == GATED_FWD) {
@@ -253,27 +266,27 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
         }
         if (MODE == GATED_PRE && p.col_sums) {
             // the 16 threads of a column group, through shared memory in a fixed order
-            float* red = As[0];   // [ty][2][64]
+            float* red = As[0];   // [ty][2][S / 2]
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                red[ty * 128 + 4 * tx + j] = sg[j];
-                red[ty * 128 + 64 + 4 * tx + j] = su[j];
+            for (int j = 0; j < O; j++) {
+                red[ty * S + O * tx + j] = sg[j];
+                red[ty * S + S / 2 + O * tx + j] = su[j];
             }
             __syncthreads();
-            if (threadIdx.x < 128) {
+            if (threadIdx.x < S) {
                 float t = 0.0f;
-                for (int r = 0; r < 16; r++) t += red[r * 128 + threadIdx.x];
-                const int c = n0 + (threadIdx.x & 63);
-                if (c < p.n) p.col_sums[((m0 / kGatedTileM) * 2 + (threadIdx.x >> 6)) * p.n + c] = t;
+                for (int r = 0; r < 16; r++) t += red[r * S + threadIdx.x];
+                const int up = threadIdx.x >= S / 2, c = n0 + threadIdx.x - up * (S / 2);
+                if (c < p.n) p.col_sums[((m0 / kTileM) * 2 + up) * p.n + c] = t;
             }
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < R; i++) {
             const int64_t r = row_of(i);
             if (r >= ni) continue;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
+            for (int j = 0; j < 2 * CP; j++) {
                 const int c = n0 + 4 * tx + (j & 3) + (j >> 2) * 64;
                 if (c >= nj) continue;
                 if (MODE == GATED_DX) static_cast<T*>(p.dx)[r * p.dx_row + c] = from_float<T>(v[i][j]);
@@ -506,6 +519,23 @@ template <class T> void copy_operands(GatedParams& p, const Copies& copies, int6
     repack<T><<<dim3(blocks, n), kThreads, 0, st>>>(r);
 }
 
+dim3 tile_grid(int64_t tiles, int64_t y = 1) {
+    if (tiles > INT32_MAX || y > 65535) fail(STG_UNSUPPORTED, "gated: too many tiles");
+    return dim3((unsigned)tiles, (unsigned)y);
+}
+
+// A product of float tiles, as 128 x 128 ones or, when those would leave a third of the SMs without a
+// second block, 64 x 64 ones. out: columns of a 128-wide tile.
+template <class T, int MODE> int launch_simt(const GatedParams& p, int64_t rows, int64_t cols, int out, int64_t y, cudaStream_t st) {
+    auto tiles = [&](int s) { return ceil_div(rows, s) * ceil_div(cols, out * s / 128); };
+    if (MODE == GATED_HEAD || tiles(128) * y >= 222) {
+        gated_simt<T, MODE, 128><<<tile_grid(MODE == GATED_HEAD ? rows : tiles(128), y), kThreads, 0, st>>>(p);
+        return 128;
+    }
+    if constexpr (MODE != GATED_HEAD) gated_simt<T, MODE, 64><<<tile_grid(tiles(64), y), kThreads, 0, st>>>(p);
+    return 64;
+}
+
 struct GatedLayout { size_t dg = 0, du = 0, sums = 0, dw = 0, copies = 0, bytes = 0; int64_t pre_row = 0; int splits = 1; int64_t split_rows = 0; };
 
 GatedLayout backward_layout(const stg_gated_config& c) {
@@ -523,7 +553,7 @@ GatedLayout backward_layout(const stg_gated_config& c) {
     l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, c.rows / 256, 64}));
     l.split_rows = std::max<int64_t>(64, ceil_div(ceil_div(c.rows, l.splits), 64) * 64);
     l.splits = (int)std::max<int64_t>(1, ceil_div(c.rows, l.split_rows));
-    l.dw = l.sums + up256(sizeof(float) * (size_t)std::max<int64_t>(ceil_div(c.rows, kGatedTileM), l.splits * ceil_div(c.features, 64)) * 2 * c.width);
+    l.dw = l.sums + up256(sizeof(float) * (size_t)std::max<int64_t>(ceil_div(c.rows, 64), l.splits * ceil_div(c.features, 64)) * 2 * c.width);
     l.copies = l.dw + up256(sizeof(float) * (size_t)l.splits * 2 * c.width * c.features);
     l.bytes = l.copies + copies_of(c, true).bytes();
     return l;
@@ -556,10 +586,6 @@ template <class T, int M> void launch_rows(GatedParams& p, cudaStream_t st) {
     else gated_rows<T, M, 1><<<blocks, kThreads, 0, st>>>(p);
 }
 
-dim3 tile_grid(int64_t tiles, int64_t y = 1) {
-    if (tiles > INT32_MAX || y > 65535) fail(STG_UNSUPPORTED, "gated: too many tiles");
-    return dim3((unsigned)tiles, (unsigned)y);
-}
 
 } // namespace
 
@@ -600,7 +626,7 @@ STG_API stg_status stg_gated(stg_engine* e, const stg_gated_config* c, const voi
                 copy_operands<T>(p, copies, p.m, p.n, static_cast<char*>(d_ws), st);
                 return launch_gated_mma(GATED_FWD, c->dtype == STG_BF16, p, 0, e->sms, st);
             }
-            gated_simt<T, GATED_FWD><<<tile_grid(ceil_div(p.m, kGatedTileM) * ceil_div(p.n, kGatedTileN)), kThreads, 0, st>>>(p);
+            launch_simt<T, GATED_FWD>(p, p.m, p.n, 64, 1, st);
         });
         cuda_check(cudaGetLastError(), "gated kernel");
     });
@@ -644,7 +670,6 @@ STG_API stg_status stg_gated_backward(stg_engine* e, const stg_gated_config* c, 
         p.dw_part = reinterpret_cast<float*>(ws + lay.dw);
         p.splits = lay.splits;
         p.split_rows = lay.split_rows;
-        const int64_t mt = ceil_div(p.m, kGatedTileM);
         auto join = [&](auto* tag, int64_t sums) {   // the partial sums of dW and of the biases' gradients
             using T = std::remove_pointer_t<decltype(tag)>;
             const bool dw = d_dwg || d_dwu;
@@ -666,10 +691,10 @@ STG_API stg_status stg_gated_backward(stg_engine* e, const stg_gated_config* c, 
                 join((T*)nullptr, gated_col_sums(p, e->sms));
                 return;
             }
-            gated_simt<T, GATED_PRE><<<tile_grid(mt * ceil_div(p.n, kGatedTileN)), kThreads, 0, st>>>(p);
-            if (d_dx) gated_simt<T, GATED_DX><<<tile_grid(mt * ceil_div(p.k, 128)), kThreads, 0, st>>>(p);
-            if (d_dwg || d_dwu) gated_simt<T, GATED_DW><<<tile_grid(ceil_div(p.n, 128) * ceil_div(p.k, 128), 2 * p.splits), kThreads, 0, st>>>(p);
-            join((T*)nullptr, mt);
+            const int pre = launch_simt<T, GATED_PRE>(p, p.m, p.n, 64, 1, st);
+            if (d_dx) launch_simt<T, GATED_DX>(p, p.m, p.k, 128, 1, st);
+            if (d_dwg || d_dwu) launch_simt<T, GATED_DW>(p, p.n, p.k, 128, 2 * p.splits, st);
+            join((T*)nullptr, ceil_div(p.m, pre));
         });
         cuda_check(cudaGetLastError(), "gated kernel");
     });
@@ -743,7 +768,6 @@ STG_API stg_status stg_mask_head(stg_plan* plan, const stg_mask_head_config* c, 
         p.n_tiles = plan->head_tiles;
         DeviceScope scope(plan->engine);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
-        const dim3 grid = tile_grid((int64_t)c->n_chunks * p.stems * ceil_div(p.frames, kGatedTileM) * p.n_tiles);
         const Copies copies = head_copies(plan, c);
         check(!copies.bytes() || (d_ws && aligned(d_ws, 256) && ws_bytes >= copies.bytes()), "mask head: workspace is missing, unaligned or too small");
         const int64_t rows = head_rows(plan, c);
@@ -756,7 +780,7 @@ STG_API stg_status stg_mask_head(stg_plan* plan, const stg_mask_head_config* c, 
                 p.n_tiles = plan->head_wide;
                 return launch_gated_mma(GATED_HEAD, c->dtype == STG_BF16, p, rows, plan->engine->sms, st);
             }
-            gated_simt<T, GATED_HEAD><<<grid, kThreads, 0, st>>>(p);
+            launch_simt<T, GATED_HEAD>(p, (int64_t)c->n_chunks * p.stems * ceil_div(p.frames, kGatedTileM) * p.n_tiles, 0, 64, 1, st);
         });
         cuda_check(cudaGetLastError(), "mask head kernel");
     });

@@ -4,8 +4,7 @@
 
 namespace stg {
 
-constexpr int kGatedTileN = kHeadTileN;   // output columns of a tile: as many gate and up columns side by side
-constexpr int kGatedTileM = 128;
+constexpr int kGatedTileM = 128;   // rows of a tile on the CUDA cores
 
 // The four products of the gated projection. Rows of x are m, outputs n, features k.
 enum GatedMode : int {
@@ -23,7 +22,7 @@ struct GatedParams {
     const void *x, *wg, *wu, *bg, *bu, *dy;
     int64_t x_row, wg_row, wu_row, y_row, dx_row;
     void *y, *dx;
-    // backward scratch: dg and du [m][pre_row] in the element type, column sums [128-row tiles, or gated_col_sums][2][n]
+    // backward scratch: dg and du [m][pre_row] in the element type, column sums [row tiles of 128 or 64, or gated_col_sums][2][n]
     void *dg, *du;
     int64_t pre_row;
     float* col_sums;
