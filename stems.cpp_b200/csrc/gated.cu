@@ -479,10 +479,10 @@ void check_config(const stg_gated_config* c, bool backward) {
 }
 
 // Which operands the tensor-core path needs a repacked copy of (bytes, 0: none): it reads by
-// TMA, whose rows are a multiple of 16 bytes apart.
+// TMA, whose rows are a multiple of 16 bytes apart and do not overlap (as a broadcast's do).
 struct Copies { size_t x = 0, wg = 0, wu = 0; size_t bytes() const { return x + wg + wu; } };
 size_t copy_bytes(int64_t rows, int64_t row, int cols) {
-    return rows <= 1 || row % 8 == 0 ? 0 : up256((size_t)rows * (size_t)(ceil_div(cols, 8) * 8) * 2);
+    return rows <= 1 || (row % 8 == 0 && row >= cols) ? 0 : up256((size_t)rows * (size_t)(ceil_div(cols, 8) * 8) * 2);
 }
 Copies copies_of(const stg_gated_config& c, bool backward) {
     Copies r;

@@ -661,7 +661,8 @@ template <class T, int MODE> void launch_act(const MmaParams& p, int sms, cudaSt
 int column_tile(int k, int64_t rest, int64_t pairs, bool sums) {
     const int most = sums ? kSumCol / 32 * 32 : 256;
     int64_t best = INT64_MAX, width = 0;
-    for (int64_t t = ceil_div(k, most); t <= ceil_div(k, 64); t++) {
+    const int64_t few = ceil_div(k, most);
+    for (int64_t t = few; t <= std::min(ceil_div(k, 64), few + 16); t++) {
         const int64_t cols = ceil_div(ceil_div(k, t), 32) * 32, cost = ceil_div(rest * ceil_div(k, cols), pairs) * (cols + 32);
         if (cost < best) { best = cost; width = cols; }
     }

@@ -193,13 +193,12 @@ __device__ __forceinline__ void block_moments(const NormParams& p, const Place& 
     __syncthreads();
 }
 
-// z = (x + mu) a + sh for a thread's channels. For 16-bit x as x a + (sh + mu a): what that rounds, 2^-24
-// of mu a, is far below the 2^-9 (2^-12) of mu a that x itself was rounded by.
+// z = (x + mu) a + sh for a thread's channels, mu the negative mean: the difference first, so that
+// values near the mean, a constant group's above all, keep their digits.
 template <class T, int V, int ACT> struct Affine {
     static constexpr int N = (V + 1) / 2;
-    static constexpr bool fast = sizeof(T) == 2;
     f2 mu[N], a[N], sh[N];
-    PairAct<ACT, fast> fn;
+    PairAct<ACT, sizeof(T) == 2> fn;
     // stat(g): mean and rstd of a group
     template <class Fn> __device__ __forceinline__ void start(const NormParams& p, int ch, Fn&& stat) {
 #pragma unroll
@@ -212,7 +211,6 @@ template <class T, int V, int ACT> struct Affine {
                 m[k] = -st.x;
                 s1[k] = st.y * param(p.gamma, c, p.param_float, 1.0f, (const T*)nullptr);
                 s0[k] = param(p.beta, c, p.param_float, 0.0f, (const T*)nullptr);
-                if (fast) s0[k] = fmaf(m[k], s1[k], s0[k]);
             }
             mu[i] = make_f2(m[0], m[1]);
             a[i] = make_f2(s1[0], s1[1]);
@@ -221,10 +219,7 @@ template <class T, int V, int ACT> struct Affine {
     }
     __device__ __forceinline__ void put_at(T* y, Pack<T, V> v) const {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const f2 f = get(v, i);
-            put(v, i, fn.value(fma2(fast ? f : f + mu[i], a[i], sh[i])));
-        }
+        for (int i = 0; i < N; i++) put(v, i, fn.value(fma2(get(v, i) + mu[i], a[i], sh[i])));
         store_stream(y, v);
     }
 };

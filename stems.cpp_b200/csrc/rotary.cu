@@ -15,7 +15,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxHalf = 256;      // rotary_dim at most 512
-constexpr int kTableEntries = 2048;   // (cos, sin) pairs a block keeps: at most 16 KB but for a single token
+constexpr size_t kSmem = 32 * 1024;   // a block's tables at most
 
 struct RotaryTensor {
     const void* x;
@@ -159,7 +159,8 @@ void launch(RotaryParams& p, int layout, cudaStream_t st) {
     // each part repeats the table)
     p.heads_per_block = p.heads;
     p.tokens_per_block = 1;
-    while ((int64_t)p.tokens_per_block * per_head * p.heads < 16 * kThreads && 2 * p.tokens_per_block * p.half <= kTableEntries &&
+    auto smem_of = [&](int tokens) { return (size_t)tokens * (sizeof(float2) * p.half + 2 * sizeof(longlong2) + sizeof(int32_t)) + sizeof(double) * p.half; };
+    while ((int64_t)p.tokens_per_block * per_head * p.heads < 16 * kThreads && smem_of(2 * p.tokens_per_block) <= kSmem &&
            p.n / (2 * p.tokens_per_block) >= 296)
         p.tokens_per_block *= 2;
     const int64_t blocks = (p.n + p.tokens_per_block - 1) / p.tokens_per_block;
@@ -174,7 +175,7 @@ void launch(RotaryParams& p, int layout, cudaStream_t st) {
     p.half_div = FastDiv((uint32_t)p.half);
     if (blocks > INT32_MAX || parts > 65535) fail(STG_UNSUPPORTED, "rotary: too many tokens or heads");
     const dim3 grid((unsigned)blocks, (unsigned)parts);
-    const size_t smem = (size_t)p.tokens_per_block * (sizeof(float2) * p.half + 2 * sizeof(longlong2) + sizeof(int32_t)) + sizeof(double) * p.half;
+    const size_t smem = smem_of(p.tokens_per_block);
     if (layout == 0) rotary_kernel<T, V, 0><<<grid, kThreads, smem, st>>>(p);
     else rotary_kernel<T, V, 1><<<grid, kThreads, smem, st>>>(p);
     cuda_check(cudaGetLastError(), "rotary kernel");

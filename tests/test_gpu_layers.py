@@ -86,6 +86,13 @@ def test_rotary_strides_and_in_place(pkg, engine, dtype, layout):
     ok(engine.rotary(shared, rotary_dim=32, layout=layout), ref.rotary(shared, pos, f, m, 32, layout))
 
 
+def test_rotary_long_and_narrow(pkg, engine):
+    """Many tokens of one narrow head: the largest blocks of tokens."""
+    x = rnd(11, 1, 1300001, 1, 2)
+    f, m = pkg.rotary_frequencies(2)
+    ok(engine.rotary(x), ref.rotary(x, torch.arange(1300001, device="cuda"), f, m, 2, "interleaved"))
+
+
 def test_rotary_empty_special_and_gradient(pkg, engine):
     for shape in ((0, 3, 2, 8), (2, 0, 2, 8), (2, 3, 0, 8)):
         assert engine.rotary(torch.empty(shape, device="cuda")).shape == shape
@@ -183,8 +190,11 @@ def test_group_norm_activations_strides_and_no_affine(engine, kind, dtype):
 def test_group_norm_far_mean_empty_and_special(pkg, engine):
     x = rnd(10, 2, 3000, 16, scale=0.01, shift=300.0)       # the mean is 30 000 deviations away
     ok(engine.group_norm(x, 2), ref.group_norm(x, 2, None, None, 1e-5, "none")[:2])
-    const = torch.full((1, 77, 8), 3.0, device="cuda")
-    assert (engine.group_norm(const, 2, eps=0.5) == 0).all()
+    for dtype, value in ((F32, 3.0), (F16, 60000.0), (BF16, 300.0)):        # a constant group is its beta, whatever its mean
+        for n in (77, 70000):
+            const = torch.full((1, n, 16), value, device="cuda", dtype=dtype)
+            be = rnd(3, 16, dtype=dtype)
+            assert torch.equal(engine.group_norm(const, 2, None, be), be.expand(1, n, 16))
     for shape in ((0, 5, 8), (2, 0, 8)):
         e = torch.empty(shape, device="cuda")
         ga = torch.ones(8, device="cuda")
@@ -248,6 +258,7 @@ GATED = [
     # rows, features, width
     (1, 1, 1), (1, 64, 64), (1, 2048, 333), (3, 40, 8), (7, 129, 65), (16, 384, 1408), (17, 256, 130), (128, 64, 64), (129, 200, 200),
     (300, 72, 1000), (1000, 384, 136), (257, 515, 301), (33, 16, 2050), (640, 1024, 64), (2000, 8, 24),
+    (40, 1, 1), (20, 3, 2), (9, 72, 16), (8, 72, 17), (2, 1000, 5), (5, 40, 3000), (300, 2200, 40),
 ]
 
 
@@ -298,6 +309,19 @@ def test_gated_activations_strides_and_one_bias(engine, dtype, kind):
         ok(a.reshape(want[i].shape), (want[i], bound[i]))
     odd = rnd(5, 70, 73, dtype=dtype)[:, 1:]                 # addresses that are not whole vectors
     ok(engine.gated(odd, wg, wu, activation=kind), ref.gated(odd, wg, wu, None, None, kind))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [3, 200])
+def test_gated_broadcast_and_overlapping_operands(engine, dtype, rows):
+    x, wg, wu, _, _ = _gated_inputs(rows, 64, 72, dtype, False)
+    one, base, dy = x[:1].expand(rows, 64), rnd(7, rows + 64, dtype=dtype), rnd(8, rows, 72, dtype=dtype)
+    windows, same = base.as_strided((rows, 64), (1, 1)), wu[:1].expand(72, 64)
+    for a, w in ((one, wu), (windows, wu), (x, same)):
+        ok(engine.gated(a, wg, w), ref.gated(a, wg, w, None, None, "silu"))
+        want, bound = ref.gated_backward(dy, a, wg, w, None, None, "silu")
+        for got, i in zip(engine.gated_backward(dy, a, wg, w), range(3)):
+            ok(got, (want[i], bound[i]))
 
 
 def test_gated_empty_special_and_refusals(pkg, engine):
