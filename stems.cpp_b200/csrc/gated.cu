@@ -164,7 +164,10 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
 #pragma unroll
         for (int j = 0; j < CP; j++) acc[i][j] = 0;
 
-    const int64_t steps1 = (nk - kbeg + kTileK - 1) / kTileK, steps = steps1 * (MODE == GATED_DX ? 2 : 1);
+    // dx runs through Wg's rows, then Wu's; its splits share out the steps of both
+    const int64_t steps1 = (nk - kbeg + kTileK - 1) / kTileK, all = steps1 * (MODE == GATED_DX ? 2 : 1);
+    const int64_t share = MODE == GATED_DX ? (all + p.dx_splits - 1) / p.dx_splits : all;
+    const int64_t first = MODE == GATED_DX ? min(all, blockIdx.y * share) : 0, steps = min(all, first + share);
     TileLoad<T, AK, S> la;
     TileLoad<T, BK, S> lb;
     auto fetch = [&](int64_t s) {
@@ -179,14 +182,14 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
             lb.fetch(second ? b1 : b0, second ? ldb1 : ldb0, n0, nj, k0, nk);
         }
     };
-    if (steps > 0) {
-        fetch(0);
+    if (first < steps) {
+        fetch(first);
         la.store(As[0]);
         lb.store(Bs[0]);
     }
     __syncthreads();
-    for (int64_t s = 0; s < steps; s++) {
-        const int cur = (int)(s & 1);
+    for (int64_t s = first; s < steps; s++) {
+        const int cur = (int)((s - first) & 1);
         if (s + 1 < steps) fetch(s + 1);
         const float *pa = As[cur] + 4 * ty, *pb = Bs[cur] + 4 * tx;
 #pragma unroll
@@ -289,8 +292,10 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
             for (int j = 0; j < 2 * CP; j++) {
                 const int c = n0 + 4 * tx + (j & 3) + (j >> 2) * 64;
                 if (c >= nj) continue;
-                if (MODE == GATED_DX) static_cast<T*>(p.dx)[r * p.dx_row + c] = from_float<T>(v[i][j]);
-                else p.dw_part[((int64_t)blockIdx.y * p.n + r) * p.k + c] = v[i][j];
+                if (MODE == GATED_DX) {
+                    if (p.dx_splits > 1) p.dx_part[(blockIdx.y * ni + r) * p.k + c] = v[i][j];
+                    else static_cast<T*>(p.dx)[r * p.dx_row + c] = from_float<T>(v[i][j]);
+                } else p.dw_part[((int64_t)blockIdx.y * p.n + r) * p.k + c] = v[i][j];
             }
         }
     }
@@ -428,6 +433,17 @@ __global__ void __launch_bounds__(kThreads) join_parts(const __grid_constant__ G
     }
 }
 
+// dx from its partial sums, added in order.
+template <class T> __global__ void __launch_bounds__(kThreads) join_dx(const __grid_constant__ GatedParams p) {
+    const int64_t total = p.m * p.k;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+        float s = 0.0f;
+        for (int q = 0; q < p.dx_splits; q++) s += p.dx_part[q * total + i];
+        const int64_t r = i / p.k;
+        static_cast<T*>(p.dx)[r * p.dx_row + i - r * p.k] = from_float<T>(s);
+    }
+}
+
 // Copies of up to three matrices of one width, their rows `pitch` elements apart, for operands
 // whose rows are no whole 16 bytes. A thread makes 16 bytes of a copy; elements past the width are 0.
 struct RepackParams {
@@ -536,7 +552,7 @@ template <class T, int MODE> int launch_simt(const GatedParams& p, int64_t rows,
     return 64;
 }
 
-struct GatedLayout { size_t dg = 0, du = 0, sums = 0, dw = 0, copies = 0, bytes = 0; int64_t pre_row = 0; int splits = 1; int64_t split_rows = 0; };
+struct GatedLayout { size_t dg = 0, du = 0, sums = 0, dw = 0, dx = 0, copies = 0, bytes = 0; int64_t pre_row = 0; int splits = 1, dx_splits = 1; int64_t split_rows = 0; };
 
 GatedLayout backward_layout(const stg_gated_config& c) {
     GatedLayout l;
@@ -551,10 +567,18 @@ GatedLayout backward_layout(const stg_gated_config& c) {
     const int64_t tiles = 2 * ceil_div(c.width, f32 ? 128 : 256) * ceil_div(c.features, f32 ? 128 : 224);
     const int64_t want = f32 ? ceil_div(2 * 148, tiles) : std::max<int64_t>(1, 74 / tiles);
     l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, c.rows / 256, 64}));
+    // float: sums in order of at most 4096 terms (and 64 parts): longer ones lose digits to a library's
+    if (f32) l.splits = (int)std::max<int64_t>(l.splits, std::min<int64_t>(64, ceil_div(c.rows, 4096)));
     l.split_rows = std::max<int64_t>(64, ceil_div(ceil_div(c.rows, l.splits), 64) * 64);
     l.splits = (int)std::max<int64_t>(1, ceil_div(c.rows, l.split_rows));
     l.dw = l.sums + up256(sizeof(float) * (size_t)std::max<int64_t>(ceil_div(c.rows, 64), l.splits * ceil_div(c.features, 64)) * 2 * c.width);
-    l.copies = l.dw + up256(sizeof(float) * (size_t)l.splits * 2 * c.width * c.features);
+    if (f32) {   // dx likewise: its sums are 2 width long, its tiles few when rows and features are
+        const int64_t tiles128 = ceil_div(c.rows, 128) * ceil_div(c.features, 128), tiles64 = ceil_div(c.rows, 64) * ceil_div(c.features, 64);
+        const int64_t more = tiles128 >= 222 ? 1 : std::min<int64_t>(ceil_div(296, tiles64), 2 * (int64_t)c.width / 256);
+        l.dx_splits = (int)std::min<int64_t>(32, std::max<int64_t>({1, more, ceil_div(2 * (int64_t)c.width, 4096)}));
+    }
+    l.dx = l.dw + up256(sizeof(float) * (size_t)l.splits * 2 * c.width * c.features);
+    l.copies = l.dx + (l.dx_splits > 1 ? up256(sizeof(float) * (size_t)l.dx_splits * c.rows * c.features) : 0);
     l.bytes = l.copies + copies_of(c, true).bytes();
     return l;
 }
@@ -669,6 +693,8 @@ STG_API stg_status stg_gated_backward(stg_engine* e, const stg_gated_config* c, 
         p.col_sums = d_dbg || d_dbu ? reinterpret_cast<float*>(ws + lay.sums) : nullptr;
         p.dw_part = reinterpret_cast<float*>(ws + lay.dw);
         p.splits = lay.splits;
+        p.dx_part = reinterpret_cast<float*>(ws + lay.dx);
+        p.dx_splits = lay.dx_splits;
         p.split_rows = lay.split_rows;
         auto join = [&](auto* tag, int64_t sums) {   // the partial sums of dW and of the biases' gradients
             using T = std::remove_pointer_t<decltype(tag)>;
@@ -692,7 +718,10 @@ STG_API stg_status stg_gated_backward(stg_engine* e, const stg_gated_config* c, 
                 return;
             }
             const int pre = launch_simt<T, GATED_PRE>(p, p.m, p.n, 64, 1, st);
-            if (d_dx) launch_simt<T, GATED_DX>(p, p.m, p.k, 128, 1, st);
+            if (d_dx) {
+                launch_simt<T, GATED_DX>(p, p.m, p.k, 128, p.dx_splits, st);
+                if (p.dx_splits > 1) join_dx<T><<<(unsigned)std::min<int64_t>(ceil_div(p.m * p.k, kThreads), 148 * 8), kThreads, 0, st>>>(p);
+            }
             if (d_dwg || d_dwu) launch_simt<T, GATED_DW>(p, p.n, p.k, 128, 2 * p.splits, st);
             join((T*)nullptr, ceil_div(p.m, pre));
         });

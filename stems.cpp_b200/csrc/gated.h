@@ -30,6 +30,9 @@ struct GatedParams {
     float* dw_part;
     int splits;
     int64_t split_rows;
+    // dx on the CUDA cores: partial sums over dx_splits ranges of the widths, [dx_splits][m][k] float, when more than one
+    float* dx_part;
+    int dx_splits;
     // mask head: tiles over the bands' columns
     const HeadTile* tiles;
     int n_tiles;                       // tiles of one stem
