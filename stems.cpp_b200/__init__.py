@@ -9,6 +9,10 @@ network is out of scope; a mask buffer stands in for its output.
 There is no CPU fallback: when the library is missing or no B200 is visible, every call
 raises. Device buffers may be torch CUDA tensors (their data_ptr and the current stream are
 used) or raw device pointers.
+
+The layers of the network between the halves (``Engine.rotary``, ``group_norm``, ``gated``, their
+backward passes, ``Plan.mask_head``) take torch tensors and run on the current stream unless given
+one; tensors made on another stream are the caller's to order, as with any torch operator.
 """
 from __future__ import annotations
 

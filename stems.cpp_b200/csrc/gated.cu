@@ -94,7 +94,8 @@ __device__ __forceinline__ float2 halves(uint64_t a) {
 // modes half of the columns are the up projection of the same outputs as the other half, placed
 // so that a thread holds both factors of its outputs: at 128 the second 64 columns, at 64 the
 // second two of each thread's four. Products and sums are float with one rounding each (packed in
-// pairs); K runs in order. Bound by the float units: 48 TFLOP/s at 48060 x 384 x 1408.
+// pairs); K runs in order. Bound by the float units: 48 TFLOP/s at 48060 x 384 x 1408; the
+// backward pass at 777 x 301 x 515 in float takes 31, 24 and 27 us and 8 us of joining.
 template <class T, int MODE, int S>
 __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ GatedParams p) {
     constexpr bool DUAL = MODE == GATED_FWD || MODE == GATED_HEAD || MODE == GATED_PRE;
@@ -304,7 +305,8 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
 // A few rows: y for M rows at most, by streaming the weights once. A warp has O outputs, both weight
 // rows of each, and steps along the features with all lanes (V of them to an access); the rows of x
 // come from L1, where the block's warps share them. With few outputs, S warps share one and add up
-// through shared memory. Bound by reading the weights: nothing is read twice from memory.
+// through shared memory. Bound by reading the weights, each once: one row at 5461 x 2048 bf16 (45 MB)
+// takes 7.4 us, 6.0 TB/s.
 constexpr int kFewRows = 8;
 template <class T, int M, int V>
 __global__ void __launch_bounds__(kThreads) gated_rows(const __grid_constant__ GatedParams p) {

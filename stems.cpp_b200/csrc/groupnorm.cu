@@ -16,6 +16,9 @@
 //     opposite order, so that what the first left in L2 is met there. A cooperative launch that
 //     kept 26 MB in the SMs' shared memory instead stood still at each item's meeting: 121 us for
 //     4 x 172032 x 96 bf16.
+// Measured: 4 x 172032 x 96 bf16 with GELU 88 us (264 MB at least; read twice, the second time half from
+// L2, 326 MB; the second reading is bound by the activation's 13 instructions a value), its backward
+// pass at 2 x 43008 x 192 f32 with SiLU 65 us (198 MB at least), one row of 336 x 48 f32 7.5 us.
 // A block's threads stand side by side along the channels (16-byte vectors, whole rows, so every
 // sector is used whatever the group size) and step down the positions. Each takes the differences
 // from the first value it meets, so that a mean far from zero costs no digits.

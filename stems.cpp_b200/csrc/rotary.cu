@@ -4,7 +4,8 @@
 // x1 cos a + x0 sin a). The work is one read and one write of the tensors; what could spoil it
 // is the sines and cosines, which every head of a token shares. A block therefore takes a few
 // tokens with all their heads, of queries and keys together, computes the tokens' table of
-// (cos, sin) once into shared memory and streams the heads past it in 16-byte vectors.
+// (cos, sin) once into shared memory and streams the heads past it in 16-byte vectors. 60 x 801
+// tokens of 8 query and 8 key heads of 64, bf16: 38 us, 5.2 TB/s.
 #include "layers.h"
 
 #include <cmath>
