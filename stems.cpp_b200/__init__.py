@@ -628,13 +628,11 @@ class Engine:
         except struct.error as e:
             raise StemsError(1, f"group norm: {e}") from None
 
-    def _workspace(self, fn, cfg, backward, what, device, stream):
-        """(pointer, bytes, the tensor that owns them) of a layer's scratch."""
+    def _workspace(self, fn, cfg, backward, device, stream):
+        """(pointer, bytes, the tensor that owns them) of a layer's scratch. A configuration that is
+        refused gets none: the call itself then refuses it, with its reason."""
         n = C.c_size_t()
-        rc = fn(cfg, backward, C.byref(n))
-        if rc != 0:
-            raise StemsError(rc, what)
-        if not n.value:
+        if fn(cfg, backward, C.byref(n)) != 0 or not n.value:
             return None, 0, None
         ws = _empty((n.value,), _torch.uint8, device, stream)
         return ws.data_ptr(), n.value, ws
@@ -653,7 +651,7 @@ class Engine:
             _layer_tensor(out, "out", dev, x.dtype, x.shape)
             y = out
         cfg = self._norm_config(x, groups, gamma, beta, activation, eps, y)
-        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 0, "group_norm", at, stream)
+        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 0, at, stream)
         mean = rstd = None
         if return_stats:
             mean, rstd = (_empty((x.shape[0], groups), _torch.float32, at, stream) for _ in range(2))
@@ -678,7 +676,7 @@ class Engine:
         dx = _empty(x.shape, x.dtype, at, stream) if need_dx else None
         cfg = self._norm_config(x, groups, gamma, beta, activation, eps, dy, dx)
         dgamma, dbeta = (None if t is None else _empty(t.shape, t.dtype, at, stream) for t in (gamma, beta))
-        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 1, "group_norm_backward", at, stream)
+        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 1, at, stream)
         rc = lib().stg_group_norm_backward(self._h, cfg, dy.data_ptr(), x.data_ptr(), _ptr_of(gamma), _ptr_of(beta), mean.data_ptr(),
                                            rstd.data_ptr(), _ptr_of(dx), _ptr_of(dgamma), _ptr_of(dbeta), ws, n, self._layer_stream(stream))
         if rc != 0:
@@ -724,7 +722,7 @@ class Engine:
                 raise StemsError(1, "expected x [...][features] and w_gate [width][features]")
             out = _empty((*x.shape[:-1], w_gate.shape[0]), x.dtype, x.device, stream)
         cfg = self._gated_config(x, w_gate, w_up, b_gate, b_up, activation, out)
-        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 0, "gated", x.device, stream)
+        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 0, x.device, stream)
         rc = lib().stg_gated(self._h, cfg, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _ptr_of(b_gate), _ptr_of(b_up),
                              out.data_ptr(), ws, n, self._layer_stream(stream))
         if rc != 0:
@@ -742,7 +740,7 @@ class Engine:
         dx = _empty(x.shape, x.dtype, at, stream) if need_dx else None
         dws = [_empty(w.shape, w.dtype, at, stream) if need_dw else None for w in (w_gate, w_up)]
         dbs = [None if t is None else _empty(t.shape, t.dtype, at, stream) for t in (b_gate, b_up)]
-        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 1, "gated_backward", at, stream)
+        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 1, at, stream)
         ptrs = [_ptr_of(t) for t in (dy, x, w_gate, w_up, b_gate, b_up, dx, *dws, *dbs)]
         rc = lib().stg_gated_backward(self._h, cfg, *ptrs, ws, n, self._layer_stream(stream))
         if rc != 0:

@@ -236,6 +236,8 @@ def test_group_norm_refusals(pkg, engine):
             call()
         assert err.value.code in (1, 2)
     import ctypes as C
+    with pytest.raises(pkg.StemsError, match="8192 channels"):      # the reason comes along
+        engine.group_norm(torch.zeros(1, 2, 8200, device="cuda"), 1)
     n = C.c_size_t()
     for positions, channels, groups in ((5, 4096, 4096), (60000, 16, 4)):     # three launches; all SMs at once
         cfg = pkg.GroupNormConfig(C.sizeof(pkg.GroupNormConfig), 0, 0, 0, 1, positions, channels, groups, 0, channels, 0, channels, 0,
