@@ -322,12 +322,6 @@ def _layer_tensor(t, what, device, dtype=None, shape=None):
     raise StemsError(1, f"{what}: expected a tensor on the engine's device cuda:{device}")
 
 
-def _inner(t, what):
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise StemsError(1, f"{what}: the last dimension must have stride 1")
-    return t
-
-
 def _run(shape, strides, alone):
     """(count, stride) of dimensions that are one run of equally spaced items; stride None when
     they are not, `alone` when there is at most one item."""
@@ -349,6 +343,15 @@ def _empty(shape, dtype, device, stream):
     s = _torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
     with _torch.cuda.stream(s):
         return _torch.empty(shape, dtype=dtype, device=device)
+
+
+def _empty_as(x, shape, stream):
+    """_empty of x's type and device; shape None: of x's shape."""
+    if stream is not None:
+        return _empty(x.shape if shape is None else shape, x.dtype, x.device, stream)
+    if shape is None:
+        return _torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+    return x.new_empty(shape)
 
 
 def _ptr_of(t):
@@ -397,6 +400,7 @@ class Engine:
             raise StemsError(rc, f"cannot create an engine on device {device}")
         self.device = device
         self._raw_stream = None
+        self._scratch = {}    # bytes of scratch by a layer's configuration
 
     def _layer_stream(self, stream):
         """The stream a layer runs on: the one given, else torch's current one of the device."""
@@ -552,64 +556,71 @@ class Engine:
         arguments gives dx."""
         dev = self.device
         code = _layer_tensor(q, "q", dev)
-        if q.dim() != 4:
+        shape = q.shape
+        if len(shape) != 4:
             raise StemsError(1, "q: expected [batch][tokens][heads][head_dim]")
-        b, t, _, d = q.shape
-        pairs = [(_inner(q, "q"), out)]
-        if k is not None:
-            _layer_tensor(k, "k", dev, q.dtype)
-            if k.dim() != 4 or k.shape[0] != b or k.shape[1] != t or k.shape[3] != d:
-                raise StemsError(1, "k: expected q's batch, tokens and head_dim")
-            pairs.append((_inner(k, "k"), out_k))
+        b, t, _, d = shape
         pos, pos_stride = None, 0
         if positions is not None:
             if not hasattr(positions, "data_ptr") or positions.dtype is not _torch.int32:
                 raise StemsError(1, "positions: expected an int32 tensor")
             if positions.get_device() != dev:
                 raise StemsError(1, f"positions: expected a tensor on the engine's device cuda:{dev}")
-            if tuple(positions.shape) not in ((t,), (b, t)) or (t > 1 and positions.stride(-1) != 1):
+            steps = positions.stride()
+            if positions.shape not in ((t,), (b, t)) or (t > 1 and steps[-1] != 1):
                 raise StemsError(1, "positions: expected [tokens] or [batch][tokens], the last stride 1")
-            pos, pos_stride = positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0
-        tensors, results = b"", []
-        for x, y in pairs:
-            if y is None:
-                y = _empty(x.shape, x.dtype, q.device, stream)
-            else:
-                _layer_tensor(y, "out", dev, x.dtype, x.shape)
-                _inner(y, "out")
-            xs, ys = x.stride(), y.stride()
-            tensors += _ROTARY_TENSOR.pack(x.data_ptr(), y.data_ptr(), x.shape[2], xs[0], xs[1], xs[2], ys[0], ys[1], ys[2])
-            results.append(y)
+            pos, pos_stride = positions.data_ptr(), steps[0] if len(steps) == 2 else 0
+        tensors, y = self._rotary_tensor(q, "q", shape, out, stream)
+        if k is not None:
+            _layer_tensor(k, "k", dev, q.dtype)
+            kshape = k.shape
+            if len(kshape) != 4 or kshape[0] != b or kshape[1] != t or kshape[3] != d:
+                raise StemsError(1, "k: expected q's batch, tokens and head_dim")
+            more, z = self._rotary_tensor(k, "k", kshape, out_k, stream)
+            tensors += more
         try:
             cfg = _ROTARY.pack(_ROTARY.size, code, _choice(_LAYOUTS, layout, "layout"), 1 if inverse else 0, b, t, d, rotary_dim,
                                _choice(_SCALINGS, scaling, "scaling"), offset, base, factor, original_length, beta_fast, beta_slow,
                                magnitude)
         except struct.error as e:
             raise StemsError(1, f"rotary: {e}") from None
-        rc = lib().stg_rotary(self._h, cfg, tensors, len(pairs), pos, pos_stride, self._layer_stream(stream))
+        rc = lib().stg_rotary(self._h, cfg, tensors, 1 if k is None else 2, pos, pos_stride, self._layer_stream(stream))
         if rc != 0:
             self._check(rc, "rotary")
-        return results[0] if k is None else tuple(results)
+        return y if k is None else (y, z)
+
+    def _rotary_tensor(self, x, what, shape, y, stream):
+        """(the packed stg_rotary_tensor, its output)."""
+        xs = x.stride()
+        if y is None:
+            y = _empty_as(x, None, stream)
+        else:
+            _layer_tensor(y, "out", self.device, x.dtype, shape)
+        ys = y.stride()
+        if shape[3] > 1 and (xs[3] != 1 or ys[3] != 1):
+            raise StemsError(1, f"{what}: the last dimension must have stride 1")
+        return _ROTARY_TENSOR.pack(x.data_ptr(), y.data_ptr(), shape[2], xs[0], xs[1], xs[2], ys[0], ys[1], ys[2]), y
 
     @staticmethod
     def _rows(t, what):
         """(batch, positions, batch stride, position stride) of [batch][...][channels], the
         middle dimensions being one run of positions."""
-        if t.dim() < 2:
+        shape, steps = t.shape, t.stride()
+        if len(shape) < 2:
             raise StemsError(1, f"{what}: expected [batch][...][channels]")
-        _inner(t, what)
-        if t.dim() == 3:
-            return t.shape[0], t.shape[1], t.stride(0), t.stride(1)
-        if t.dim() == 2:
-            return t.shape[0], 1, t.stride(0), t.shape[1]
+        if shape[-1] > 1 and steps[-1] != 1:
+            raise StemsError(1, f"{what}: the last dimension must have stride 1")
+        if len(shape) == 3:
+            return shape[0], shape[1], steps[0], steps[1]
+        if len(shape) == 2:
+            return shape[0], 1, steps[0], shape[1]
         n, step = _run(t.shape[1:-1], t.stride()[1:-1], t.shape[-1])
         if step is None:
             raise StemsError(1, f"{what}: the positions' dimensions must be one run (call contiguous())")
         return t.shape[0], n, t.stride(0), step
 
-    def _norm_config(self, x, groups, gamma, beta, activation, eps, y, dx=None):
+    def _norm_config(self, x, code, groups, gamma, beta, activation, eps, y, dx=None):
         dev = self.device
-        code = _layer_tensor(x, "x", dev)
         b, n, xb, xp = self._rows(x, "x")
         ch = x.shape[-1]
         pcode = None
@@ -619,8 +630,9 @@ class Engine:
                 if pcode is not None and pc != pcode:
                     raise StemsError(1, "gamma and beta must have one dtype")
                 pcode = pc
-                _inner(t, what)
-        _, _, yb, yp = self._rows(y, "y")
+                if ch > 1 and t.stride(0) != 1:
+                    raise StemsError(1, f"{what}: the last dimension must have stride 1")
+        yb, yp = self._rows(y, "y")[2:]
         db, dp = self._rows(dx, "dx")[2:] if dx is not None else (yb, yp)
         try:
             return _GROUP_NORM.pack(_GROUP_NORM.size, code, 0 if pcode is None else pcode, _choice(ACTIVATIONS, activation, "activation"),
@@ -628,14 +640,21 @@ class Engine:
         except struct.error as e:
             raise StemsError(1, f"group norm: {e}") from None
 
-    def _workspace(self, fn, cfg, backward, device, stream):
+    def _workspace(self, fn, cfg, backward, x, stream):
         """(pointer, bytes, the tensor that owns them) of a layer's scratch. A configuration that is
         refused gets none: the call itself then refuses it, with its reason."""
-        n = C.c_size_t()
-        if fn(cfg, backward, C.byref(n)) != 0 or not n.value:
+        need = self._scratch.get((cfg, backward))
+        if need is None:
+            n = C.c_size_t()
+            if fn(cfg, backward, C.byref(n)) != 0:
+                return None, 0, None
+            if len(self._scratch) >= 1024:
+                self._scratch.clear()
+            need = self._scratch[(cfg, backward)] = n.value
+        if not need:
             return None, 0, None
-        ws = _empty((n.value,), _torch.uint8, device, stream)
-        return ws.data_ptr(), n.value, ws
+        ws = _empty((need,), _torch.uint8, x.device, stream)
+        return ws.data_ptr(), need, ws
 
     def group_norm(self, x, groups, gamma=None, beta=None, activation="none", eps=1e-5, out=None, return_stats=False,
                    stream=None):
@@ -643,18 +662,17 @@ class Engine:
         y, or (y, mean, rstd), the statistics float32 [batch][groups], when a backward pass
         will need them. gamma / beta [channels] in x's dtype or float32. out may be x."""
         dev = self.device
-        _layer_tensor(x, "x", dev)
-        at = x.device
+        code = _layer_tensor(x, "x", dev)
         if out is None:
-            y = _empty(x.shape, x.dtype, at, stream)
+            y = _empty_as(x, None, stream)
         else:
             _layer_tensor(out, "out", dev, x.dtype, x.shape)
             y = out
-        cfg = self._norm_config(x, groups, gamma, beta, activation, eps, y)
-        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 0, at, stream)
+        cfg = self._norm_config(x, code, groups, gamma, beta, activation, eps, y)
+        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 0, x, stream)
         mean = rstd = None
         if return_stats:
-            mean, rstd = (_empty((x.shape[0], groups), _torch.float32, at, stream) for _ in range(2))
+            mean, rstd = (_empty((x.shape[0], groups), _torch.float32, x.device, stream) for _ in range(2))
         rc = lib().stg_group_norm(self._h, cfg, x.data_ptr(), _ptr_of(gamma), _ptr_of(beta), y.data_ptr(), _ptr_of(mean), _ptr_of(rstd),
                                   ws, n, self._layer_stream(stream))
         if rc != 0:
@@ -666,48 +684,54 @@ class Engine:
         """(dx, dgamma, dbeta) of group_norm from dy and the forward pass's x, mean and rstd; the
         last two None without gamma / beta, dx None without need_dx."""
         dev = self.device
-        _layer_tensor(x, "x", dev)
+        code = _layer_tensor(x, "x", dev)
         _layer_tensor(dy, "dy", dev, x.dtype, x.shape)
         for t, what in ((mean, "mean"), (rstd, "rstd")):
             _layer_tensor(t, what, dev, _torch.float32, (x.shape[0], groups))
             if not t.is_contiguous():
                 raise StemsError(1, f"{what}: expected a contiguous tensor")
-        at = x.device
-        dx = _empty(x.shape, x.dtype, at, stream) if need_dx else None
-        cfg = self._norm_config(x, groups, gamma, beta, activation, eps, dy, dx)
-        dgamma, dbeta = (None if t is None else _empty(t.shape, t.dtype, at, stream) for t in (gamma, beta))
-        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 1, at, stream)
+        dx = _empty_as(x, None, stream) if need_dx else None
+        cfg = self._norm_config(x, code, groups, gamma, beta, activation, eps, dy, dx)
+        dgamma, dbeta = (None if t is None else _empty_as(t, None, stream) for t in (gamma, beta))
+        ws, n, keep = self._workspace(lib().stg_group_norm_workspace, cfg, 1, x, stream)
         rc = lib().stg_group_norm_backward(self._h, cfg, dy.data_ptr(), x.data_ptr(), _ptr_of(gamma), _ptr_of(beta), mean.data_ptr(),
                                            rstd.data_ptr(), _ptr_of(dx), _ptr_of(dgamma), _ptr_of(dbeta), ws, n, self._layer_stream(stream))
         if rc != 0:
             self._check(rc, "group_norm_backward")
         return dx, dgamma, dbeta
 
-    def _gated_config(self, x, wg, wu, bg, bu, activation, y):
-        dev = self.device
-        code = _layer_tensor(x, "x", dev)
-        if x.dim() < 2:
-            raise StemsError(1, "x: expected [...][features]")
+    def _gated_config(self, x, code, wg, wu, bg, bu, activation, y, ywhat):
+        dev, dt = self.device, x.dtype
         k = x.shape[-1]
         if not hasattr(wg, "shape") or len(wg.shape) != 2:
             raise StemsError(1, "w_gate: expected [width][features]")
         n = wg.shape[0]
+        steps = []
         for t, what in ((wg, "w_gate"), (wu, "w_up")):
-            _layer_tensor(t, what, dev, x.dtype, (n, k))
-            _inner(t, what)
+            _layer_tensor(t, what, dev, dt, (n, k))
+            row, one = t.stride()
+            if one != 1 and k > 1:
+                raise StemsError(1, f"{what}: the last dimension must have stride 1")
+            steps.append(row)
         for t, what in ((bg, "b_gate"), (bu, "b_up")):
             if t is not None:
-                _layer_tensor(t, what, dev, x.dtype, (n,))
-                _inner(t, what)
-        _layer_tensor(y, "y", dev, x.dtype, (*x.shape[:-1], n))
+                _layer_tensor(t, what, dev, dt, (n,))
+                if n > 1 and t.stride(0) != 1:
+                    raise StemsError(1, f"{what}: the last dimension must have stride 1")
+        if y.shape[-1] != n or y.shape[:-1] != x.shape[:-1]:
+            raise StemsError(1, f"{ywhat}: expected shape {(*x.shape[:-1], n)}, got {tuple(y.shape)}")
         return _GATED.pack(_GATED.size, code, _choice(ACTIVATIONS, activation, "activation"), k, n, x.numel() // k if k else 0,
-                           self._row_stride(x, "x"), wg.stride(0), wu.stride(0), self._row_stride(y, "y"), k, k, k)
+                           self._row_stride(x, "x"), *steps, self._row_stride(y, ywhat), k, k, k)
 
     @staticmethod
     def _row_stride(t, what):
         """The one stride of the rows of [...][features]."""
-        _inner(t, what)
-        step = _run(t.shape[:-1], t.stride()[:-1], t.shape[-1])[1]
+        shape, steps = t.shape, t.stride()
+        if shape[-1] > 1 and steps[-1] != 1:
+            raise StemsError(1, f"{what}: the last dimension must have stride 1")
+        if len(shape) == 2:
+            return steps[0]
+        step = _run(shape[:-1], steps[:-1], shape[-1])[1]
         if step is None:
             raise StemsError(1, f"{what}: the rows must have one stride (call contiguous())")
         return step
@@ -716,13 +740,15 @@ class Engine:
         """act(x w_gate^T + b_gate) (x w_up^T + b_up) (stg_gated): x [...][features], weights
         [width][features], biases [width]; y [...][width]."""
         dev = self.device
-        _layer_tensor(x, "x", dev)
+        code = _layer_tensor(x, "x", dev)
+        if x.dim() < 2 or not hasattr(w_gate, "shape"):
+            raise StemsError(1, "expected x [...][features] and w_gate [width][features]")
         if out is None:
-            if not hasattr(w_gate, "shape") or x.dim() < 2:
-                raise StemsError(1, "expected x [...][features] and w_gate [width][features]")
-            out = _empty((*x.shape[:-1], w_gate.shape[0]), x.dtype, x.device, stream)
-        cfg = self._gated_config(x, w_gate, w_up, b_gate, b_up, activation, out)
-        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 0, x.device, stream)
+            out = _empty_as(x, (*x.shape[:-1], w_gate.shape[0]), stream)
+        else:
+            _layer_tensor(out, "out", dev, x.dtype)
+        cfg = self._gated_config(x, code, w_gate, w_up, b_gate, b_up, activation, out, "out")
+        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 0, x, stream)
         rc = lib().stg_gated(self._h, cfg, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _ptr_of(b_gate), _ptr_of(b_up),
                              out.data_ptr(), ws, n, self._layer_stream(stream))
         if rc != 0:
@@ -734,13 +760,15 @@ class Engine:
         """(dx, dw_gate, dw_up), then the biases' gradients for the biases given, of gated from dy
         and the forward pass's inputs. need_dx / need_dw False leave None in their places."""
         dev = self.device
-        _layer_tensor(dy, "dy", dev)
-        cfg = self._gated_config(x, w_gate, w_up, b_gate, b_up, activation, dy)
-        at = x.device
-        dx = _empty(x.shape, x.dtype, at, stream) if need_dx else None
-        dws = [_empty(w.shape, w.dtype, at, stream) if need_dw else None for w in (w_gate, w_up)]
-        dbs = [None if t is None else _empty(t.shape, t.dtype, at, stream) for t in (b_gate, b_up)]
-        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 1, at, stream)
+        code = _layer_tensor(x, "x", dev)
+        if x.dim() < 2:
+            raise StemsError(1, "x: expected [...][features]")
+        _layer_tensor(dy, "dy", dev, x.dtype)
+        cfg = self._gated_config(x, code, w_gate, w_up, b_gate, b_up, activation, dy, "dy")
+        dx = _empty_as(x, x.shape, stream) if need_dx else None
+        dws = [_empty_as(w, w.shape, stream) if need_dw else None for w in (w_gate, w_up)]
+        dbs = [None if t is None else _empty_as(t, None, stream) for t in (b_gate, b_up)]
+        ws, n, keep = self._workspace(lib().stg_gated_workspace, cfg, 1, x, stream)
         ptrs = [_ptr_of(t) for t in (dy, x, w_gate, w_up, b_gate, b_up, dx, *dws, *dbs)]
         rc = lib().stg_gated_backward(self._h, cfg, *ptrs, ws, n, self._layer_stream(stream))
         if rc != 0:
