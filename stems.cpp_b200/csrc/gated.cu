@@ -302,11 +302,11 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
     }
 }
 
-// A few rows: y for M rows at most, by streaming the weights once. A warp has O outputs, both weight
+// A few rows: y for M rows at a time, by streaming the weights once. A warp has O outputs, both weight
 // rows of each, and steps along the features with all lanes (V of them to an access); the rows of x
 // come from L1, where the block's warps share them. With few outputs, S warps share one and add up
 // through shared memory. Bound by reading the weights, each once: one row at 5461 x 2048 bf16 (45 MB)
-// takes 7.4 us, 6.0 TB/s.
+// takes 7.4 us, 6.0 TB/s. More rows than M go in groups of M.
 constexpr int kFewRows = 8;
 template <class T, int M, int V>
 __global__ void __launch_bounds__(kThreads) gated_rows(const __grid_constant__ GatedParams p) {
@@ -315,7 +315,10 @@ __global__ void __launch_bounds__(kThreads) gated_rows(const __grid_constant__ G
     using P = Pack<T, V>;
     __shared__ float red[kThreads / 32][2 * O * M];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = p.splits, slice = warp % share;
-    const int n0 = (blockIdx.x * (kThreads / 32 / share) + warp / share) * O;
+    // blocks next to one another take the same outputs for the groups of M rows: their weights come from L2
+    const int groups = (int)((p.m + M - 1) / M), block = blockIdx.x / groups;
+    const int64_t m0 = (int64_t)(blockIdx.x - block * groups) * M;
+    const int n0 = (block * (kThreads / 32 / share) + warp / share) * O;
     const T *w[2 * O], *x[M];
 #pragma unroll
     for (int o = 0; o < O; o++) {   // an output past the last reads the last
@@ -324,7 +327,7 @@ __global__ void __launch_bounds__(kThreads) gated_rows(const __grid_constant__ G
         w[2 * o + 1] = static_cast<const T*>(p.wu) + n * p.wu_row;
     }
 #pragma unroll
-    for (int m = 0; m < M; m++) x[m] = static_cast<const T*>(p.x) + min((int64_t)m, p.m - 1) * p.x_row;
+    for (int m = 0; m < M; m++) x[m] = static_cast<const T*>(p.x) + min(m0 + m, p.m - 1) * p.x_row;
     float acc[2 * O][M];
 #pragma unroll
     for (int i = 0; i < 2 * O; i++)
@@ -374,8 +377,8 @@ __global__ void __launch_bounds__(kThreads) gated_rows(const __grid_constant__ G
     __syncthreads();
     // one thread to an output and row
     for (int e = threadIdx.x; e < kThreads / 32 / share * O * M; e += kThreads) {
-        const int out = e / M, m = e - out * M, n = blockIdx.x * (kThreads / 32 / share) * O + out;
-        if (n >= p.n || m >= p.m) continue;
+        const int out = e / M, m = e - out * M, n = block * (kThreads / 32 / share) * O + out;
+        if (n >= p.n || m0 + m >= p.m) continue;
         float g = 0.0f, u = 0.0f;
         for (int q = 0; q < share; q++) {
             g += red[out / O * share + q][(out % O * 2) * M + m];
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(kThreads) gated_rows(const __grid_constant__ G
         }
         if (p.bg) g += to_float(static_cast<const T*>(p.bg)[n]);
         if (p.bu) u += to_float(static_cast<const T*>(p.bu)[n]);
-        static_cast<T*>(p.y)[m * p.y_row + n] = from_float<T>(gate_value<fast>(p.act, g) * u);
+        static_cast<T*>(p.y)[(m0 + m) * p.y_row + n] = from_float<T>(gate_value<fast>(p.act, g) * u);
     }
 }
 
@@ -604,12 +607,21 @@ template <class T, int M> void launch_rows(GatedParams& p, cudaStream_t st) {
     constexpr int O = M > 2 ? 2 : 1, W = 16 / (int)sizeof(T);
     // warps to an output: more while that gives fewer than eight warps per SM
     p.splits = 1;
-    while (p.splits < kThreads / 32 && ceil_div(p.n, O) * p.splits < 148 * 8 && p.k > 32 * W * p.splits) p.splits *= 2;
-    const unsigned blocks = (unsigned)ceil_div(ceil_div(p.n, O), kThreads / 32 / p.splits);
+    while (p.splits < kThreads / 32 && ceil_div(p.n, O) * ceil_div(p.m, M) * p.splits < 148 * 8 && p.k > 32 * W * p.splits) p.splits *= 2;
+    const unsigned blocks = (unsigned)(ceil_div(ceil_div(p.n, O), kThreads / 32 / p.splits) * ceil_div(p.m, M));
     const bool wide = aligned(p.x, 16) && aligned(p.wg, 16) && aligned(p.wu, 16) && (p.x_row % W == 0 || p.m == 1) &&
                       (p.wg_row % W == 0 || p.n == 1) && (p.wu_row % W == 0 || p.n == 1);
     if (wide) gated_rows<T, M, W><<<blocks, kThreads, 0, st>>>(p);
     else gated_rows<T, M, 1><<<blocks, kThreads, 0, st>>>(p);
+}
+
+// Off the tensor cores gated_rows also takes more rows than eight, in groups of eight, up to 32 rows or
+// while gated_simt's tiles of 64 rows x 32 outputs would leave half the SMs idle: each such tile walks
+// all features alone, 43 ns a feature. float, features x outputs, gated_rows against gated_simt in us:
+// 2048 x 5461 at 16 rows 50 and 142, at 32 88 and 143, at 64 167 and 146; 1024 x 1024 at 64 rows 21 and
+// 47, at 128 37 and 47, at 192 52 and 47; 4096 x 1000 at 128 rows 107 and 176.
+bool few_tiles(const GatedParams& p, int sms) {
+    return p.m <= 4 * kFewRows || ceil_div(p.m, 64) * ceil_div(p.n, 32) <= sms / 2;
 }
 
 
@@ -652,6 +664,7 @@ STG_API stg_status stg_gated(stg_engine* e, const stg_gated_config* c, const voi
                 copy_operands<T>(p, copies, p.m, p.n, static_cast<char*>(d_ws), st);
                 return launch_gated_mma(GATED_FWD, c->dtype == STG_BF16, p, 0, e->sms, st);
             }
+            if (few_tiles(p, e->sms)) return launch_rows<T, kFewRows>(p, st);
             launch_simt<T, GATED_FWD>(p, p.m, p.n, 64, 1, st);
         });
         cuda_check(cudaGetLastError(), "gated kernel");

@@ -261,6 +261,7 @@ GATED = [
     (1, 1, 1), (1, 64, 64), (1, 2048, 333), (3, 40, 8), (7, 129, 65), (16, 384, 1408), (17, 256, 130), (128, 64, 64), (129, 200, 200),
     (300, 72, 1000), (1000, 384, 136), (257, 515, 301), (33, 16, 2050), (640, 1024, 64), (2000, 8, 24),
     (40, 1, 1), (20, 3, 2), (9, 72, 16), (8, 72, 17), (2, 1000, 5), (5, 40, 3000), (300, 2200, 40),
+    (32, 1030, 600), (33, 260, 2400), (128, 1100, 1000), (4000, 33, 30),   # in groups of eight rows, and tiles
 ]
 
 
