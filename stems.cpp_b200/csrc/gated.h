@@ -26,7 +26,10 @@ struct GatedParams {
     void *dg, *du;
     int64_t pre_row;
     float* col_sums;
-    // dWg and dWu: partial sums over `splits` ranges of rows, [splits][2][n][k] float
+    // dWg and dWu (either may be null): written by their product when `splits` is 1, else partial sums
+    // over that many ranges of rows, [splits][2][n][k] float
+    void* dw[2];
+    int64_t dw_row[2];
     float* dw_part;
     int splits;
     int64_t split_rows;

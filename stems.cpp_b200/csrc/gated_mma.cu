@@ -445,7 +445,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_m
             auto half = [&](uint32_t (&v)[16], uint32_t (&w)[16], int c, int hh) {
                 const int lc = hh * 16, j = q.n0 + c * 32 + lc;
                 if (MODE == GATED_DW) {
-                    if (row < g.n) {
+                    if (g.splits == 1) {
+                        T* o = static_cast<T*>(g.dw[q.part]);
+                        if (row >= g.n || !o) return;
+                        o += row * g.dw_row[q.part] + j;
+                        Pack<T, 8> out[2];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) out[i / 8].v[i % 8] = from_float<T>(__uint_as_float(v[i]));
+                        if (g.dw_row[q.part] % 8 == 0 && j + 16 <= g.k && (reinterpret_cast<uintptr_t>(g.dw[q.part]) & 15) == 0) {
+                            reinterpret_cast<Pack<T, 8>*>(o)[0] = out[0];
+                            reinterpret_cast<Pack<T, 8>*>(o)[1] = out[1];
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                if (j + i < g.k) o[i] = out[i / 8].v[i % 8];
+                        }
+                    } else if (row < g.n) {
                         float* o = g.dw_part + ((int64_t)q.part * g.n + row) * g.k + j;
                         if ((g.k & 3) == 0 && j + 16 <= g.k) {
 #pragma unroll

@@ -327,6 +327,32 @@ def test_gated_broadcast_and_overlapping_operands(engine, dtype, rows):
             ok(got, (want[i], bound[i]))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [40, 1200])          # one range of rows; parts that are joined
+def test_gated_weight_gradients_in_padded_rows_and_alone(pkg, engine, dtype, rows):
+    import ctypes as C
+    k, n = 72, 200
+    x, wg, wu, bg, bu = _gated_inputs(rows, k, n, dtype)
+    dy = rnd(9, rows, n, dtype=dtype)
+    want = engine.gated_backward(dy, x, wg, wu, bg, bu)
+    bits = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    need = C.c_size_t()
+    for row, off, asked in ((72, 0, (1, 1)), (80, 0, (1, 1)), (80, 1, (1, 1)), (77, 0, (1, 1)), (80, 0, (1, 0)), (80, 8, (0, 1)), (72, 0, (0, 0))):
+        cfg = pkg.GatedConfig(C.sizeof(pkg.GatedConfig), bits, pkg.ACTIVATIONS["silu"], k, n, rows, k, k, k, n, k, row, row)
+        assert pkg.lib().stg_gated_workspace(C.byref(cfg), 1, C.byref(need)) == 0
+        ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+        dw = [torch.full((off + n * row,), 7.0, dtype=dtype, device="cuda") for _ in range(2)]
+        db = [torch.empty(n, dtype=dtype, device="cuda") for _ in range(2)]
+        ptr = [t[off:].data_ptr() if a else None for t, a in zip(dw, asked)]
+        args = [t.data_ptr() for t in (dy, x, wg, wu, bg, bu)] + [None, *ptr, *(t.data_ptr() for t in db)]
+        assert pkg.lib().stg_gated_backward(engine._h, C.byref(cfg), *args, ws.data_ptr(), need.value,
+                                            torch.cuda.current_stream().cuda_stream) == 0
+        for t, a, w, b, v in zip(dw, asked, want[1:3], db, want[3:]):
+            got = t[off:].view(n, row)
+            assert torch.equal(got[:, :k], w) if a else (t == 7).all()
+            assert (got[:, k:] == 7).all() and (t[:off] == 7).all() and torch.equal(b, v)
+
+
 def test_gated_empty_special_and_refusals(pkg, engine):
     wg, wu = rnd(1, 24, 16), rnd(2, 24, 16)
     e = torch.empty(0, 16, device="cuda")
