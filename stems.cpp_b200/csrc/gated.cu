@@ -303,18 +303,18 @@ __global__ void __launch_bounds__(kThreads) gated_simt(const __grid_constant__ G
     }
 }
 
-// A few rows: y for M rows at a time, by streaming the weights once. A warp has O outputs, both weight
+// A few rows: y, or dg and du, for M rows at a time, by streaming the weights once. A warp has O outputs, both weight
 // rows of each, and steps along the features with all lanes (V of them to an access); the rows of x
 // come from L1, where the block's warps share them. With few outputs, S warps share one and add up
 // through shared memory. Bound by reading the weights, each once: one row at 5461 x 2048 bf16 (45 MB)
 // takes 7.4 us, 6.0 TB/s. More rows than M go in groups of M.
 constexpr int kFewRows = 8;
-template <class T, int M, int V>
+template <class T, int MODE, int M, int V>
 __global__ void __launch_bounds__(kThreads) gated_rows(const __grid_constant__ GatedParams p) {
     constexpr bool fast = sizeof(T) == 2;
     constexpr int O = M > 2 ? 2 : 1, U = M > 2 ? 2 : 4;
     using P = Pack<T, V>;
-    __shared__ float red[kThreads / 32][2 * O * M];
+    __shared__ float red[kThreads / 32][2 * O * M], parts[2][MODE == GATED_PRE ? kThreads / 32 * O * M : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = p.splits, slice = warp % share;
     // blocks next to one another take the same outputs for the groups of M rows: their weights come from L2
     const int groups = (int)((p.m + M - 1) / M), block = blockIdx.x / groups;
@@ -379,6 +379,7 @@ __global__ void __launch_bounds__(kThreads) gated_rows(const __grid_constant__ G
     // one thread to an output and row
     for (int e = threadIdx.x; e < kThreads / 32 / share * O * M; e += kThreads) {
         const int out = e / M, m = e - out * M, n = block * (kThreads / 32 / share) * O + out;
+        if (MODE == GATED_PRE) parts[0][e] = parts[1][e] = 0.0f;
         if (n >= p.n || m0 + m >= p.m) continue;
         float g = 0.0f, u = 0.0f;
         for (int q = 0; q < share; q++) {
@@ -387,7 +388,25 @@ __global__ void __launch_bounds__(kThreads) gated_rows(const __grid_constant__ G
         }
         if (p.bg) g += to_float(static_cast<const T*>(p.bg)[n]);
         if (p.bu) u += to_float(static_cast<const T*>(p.bu)[n]);
-        static_cast<T*>(p.y)[(m0 + m) * p.y_row + n] = from_float<T>(gate_value<fast>(p.act, g) * u);
+        if (MODE == GATED_FWD) {
+            static_cast<T*>(p.y)[(m0 + m) * p.y_row + n] = from_float<T>(gate_value<fast>(p.act, g) * u);
+        } else {
+            float a, d;
+            gate_both(p.act, g, a, d);
+            const float dy = to_float(static_cast<const T*>(p.dy)[(m0 + m) * p.y_row + n]);
+            parts[0][e] = dy * u * d;
+            parts[1][e] = dy * a;
+            static_cast<T*>(p.dg)[(m0 + m) * p.pre_row + n] = from_float<T>(parts[0][e]);
+            static_cast<T*>(p.du)[(m0 + m) * p.pre_row + n] = from_float<T>(parts[1][e]);
+        }
+    }
+    if (MODE == GATED_PRE && p.col_sums) {   // of the group's rows, in order
+        __syncthreads();
+        const int outs = kThreads / 32 / share * O, out = threadIdx.x >> 1, up = threadIdx.x & 1, n = block * outs + out;
+        if (out >= outs || n >= p.n) return;
+        float t = 0.0f;
+        for (int m = 0; m < M; m++) t += parts[up][out * M + m];
+        p.col_sums[((m0 / M) * 2 + up) * p.n + n] = t;
     }
 }
 
@@ -558,6 +577,17 @@ template <class T, int MODE> int launch_simt(const GatedParams& p, int64_t rows,
     return 64;
 }
 
+// Off the tensor cores gated_rows also takes more rows than eight, in groups of eight, up to 32 rows or
+// while gated_simt's tiles of 64 rows x 32 outputs would leave half the SMs idle: each such tile walks
+// all features alone, 43 ns a feature. float, features x outputs, gated_rows against gated_simt in us:
+// 2048 x 5461 at 16 rows 50 and 142, at 32 88 and 143, at 64 167 and 146; 1024 x 1024 at 64 rows 21 and
+// 47, at 128 37 and 47, at 192 52 and 47; 4096 x 1000 at 128 rows 107 and 176.
+// So does the backward pass with its projections: whole, at 2048 x 5461 and 8 rows 217 us for 318, at
+// 1024 x 1024 and 32 rows 43 for 78.
+bool few_tiles(int64_t rows, int64_t width) {
+    return rows <= 4 * kFewRows || ceil_div(rows, 64) * ceil_div(width, 32) <= 148 / 2;
+}
+
 struct GatedLayout { size_t dg = 0, du = 0, sums = 0, dw = 0, dx = 0, copies = 0, bytes = 0; int64_t pre_row = 0; int splits = 1, dx_splits = 1; int64_t split_rows = 0; };
 
 GatedLayout backward_layout(const stg_gated_config& c) {
@@ -579,7 +609,7 @@ GatedLayout backward_layout(const stg_gated_config& c) {
     if (f32) l.splits = (int)std::max<int64_t>(l.splits, std::min<int64_t>(64, ceil_div(c.rows, 4096)));
     l.split_rows = std::max<int64_t>(64, ceil_div(ceil_div(c.rows, l.splits), 64) * 64);
     l.splits = (int)std::max<int64_t>(1, ceil_div(c.rows, l.split_rows));
-    l.dw = l.sums + up256(sizeof(float) * (size_t)std::max<int64_t>(ceil_div(c.rows, 64), l.splits * ceil_div(c.features, 64)) * 2 * c.width);
+    l.dw = l.sums + up256(sizeof(float) * (size_t)std::max<int64_t>(ceil_div(c.rows, few_tiles(c.rows, c.width) ? kFewRows : 64), l.splits * ceil_div(c.features, 64)) * 2 * c.width);
     if (f32) {   // dx likewise: its sums are 2 width long, its tiles few when rows and features are
         const int64_t tiles128 = ceil_div(c.rows, 128) * ceil_div(c.features, 128), tiles64 = ceil_div(c.rows, 64) * ceil_div(c.features, 64);
         const int64_t more = tiles128 >= 222 ? 1 : std::min<int64_t>(ceil_div(296, tiles64), 2 * (int64_t)c.width / 256);
@@ -606,7 +636,7 @@ bool on_tensor_cores(const stg_gated_config& c, const Copies& copies, const Gate
 
 // A few rows (gated_rows): below that the tensor cores' 256-row tiles are nearly empty, and at 5461 x
 // 2048 bf16 they read the weights at 1.2 TB/s. Vectors of 16 bytes where every row starts on 16.
-template <class T, int M> void launch_rows(GatedParams& p, cudaStream_t st) {
+template <class T, int MODE, int M> void launch_rows(GatedParams p, cudaStream_t st) {
     constexpr int O = M > 2 ? 2 : 1, W = 16 / (int)sizeof(T);
     // warps to an output: more while that gives fewer than eight warps per SM
     p.splits = 1;
@@ -614,19 +644,9 @@ template <class T, int M> void launch_rows(GatedParams& p, cudaStream_t st) {
     const unsigned blocks = (unsigned)(ceil_div(ceil_div(p.n, O), kThreads / 32 / p.splits) * ceil_div(p.m, M));
     const bool wide = aligned(p.x, 16) && aligned(p.wg, 16) && aligned(p.wu, 16) && (p.x_row % W == 0 || p.m == 1) &&
                       (p.wg_row % W == 0 || p.n == 1) && (p.wu_row % W == 0 || p.n == 1);
-    if (wide) gated_rows<T, M, W><<<blocks, kThreads, 0, st>>>(p);
-    else gated_rows<T, M, 1><<<blocks, kThreads, 0, st>>>(p);
+    if (wide) gated_rows<T, MODE, M, W><<<blocks, kThreads, 0, st>>>(p);
+    else gated_rows<T, MODE, M, 1><<<blocks, kThreads, 0, st>>>(p);
 }
-
-// Off the tensor cores gated_rows also takes more rows than eight, in groups of eight, up to 32 rows or
-// while gated_simt's tiles of 64 rows x 32 outputs would leave half the SMs idle: each such tile walks
-// all features alone, 43 ns a feature. float, features x outputs, gated_rows against gated_simt in us:
-// 2048 x 5461 at 16 rows 50 and 142, at 32 88 and 143, at 64 167 and 146; 1024 x 1024 at 64 rows 21 and
-// 47, at 128 37 and 47, at 192 52 and 47; 4096 x 1000 at 128 rows 107 and 176.
-bool few_tiles(const GatedParams& p, int sms) {
-    return p.m <= 4 * kFewRows || ceil_div(p.m, 64) * ceil_div(p.n, 32) <= sms / 2;
-}
-
 
 } // namespace
 
@@ -659,15 +679,15 @@ STG_API stg_status stg_gated(stg_engine* e, const stg_gated_config* c, const voi
         check(!copies.bytes() || (d_ws && aligned(d_ws, 256) && ws_bytes >= copies.bytes()), "gated: workspace is missing, unaligned or too small");
         with_dtype(c->dtype, [&](auto* tag) {
             using T = std::remove_pointer_t<decltype(tag)>;
-            if (p.m == 1) return launch_rows<T, 1>(p, st);
-            if (p.m == 2) return launch_rows<T, 2>(p, st);
-            if (p.m <= 4) return launch_rows<T, 4>(p, st);
-            if (p.m <= kFewRows) return launch_rows<T, kFewRows>(p, st);
+            if (p.m == 1) return launch_rows<T, GATED_FWD, 1>(p, st);
+            if (p.m == 2) return launch_rows<T, GATED_FWD, 2>(p, st);
+            if (p.m <= 4) return launch_rows<T, GATED_FWD, 4>(p, st);
+            if (p.m <= kFewRows) return launch_rows<T, GATED_FWD, kFewRows>(p, st);
             if (on_tensor_cores(*c, copies, p)) {
                 copy_operands<T>(p, copies, p.m, p.n, static_cast<char*>(d_ws), st);
                 return launch_gated_mma(GATED_FWD, c->dtype == STG_BF16, p, 0, e->sms, st);
             }
-            if (few_tiles(p, e->sms)) return launch_rows<T, kFewRows>(p, st);
+            if (few_tiles(p.m, p.n)) return launch_rows<T, GATED_FWD, kFewRows>(p, st);
             launch_simt<T, GATED_FWD>(p, p.m, p.n, 64, 1, st);
         });
         cuda_check(cudaGetLastError(), "gated kernel");
@@ -737,7 +757,9 @@ STG_API stg_status stg_gated_backward(stg_engine* e, const stg_gated_config* c, 
                 join((T*)nullptr, gated_col_sums(p, e->sms));
                 return;
             }
-            const int pre = launch_simt<T, GATED_PRE>(p, p.m, p.n, 64, 1, st);
+            int pre = kFewRows;   // rows to a column sum
+            if (few_tiles(p.m, p.n)) launch_rows<T, GATED_PRE, kFewRows>(p, st);
+            else pre = launch_simt<T, GATED_PRE>(p, p.m, p.n, 64, 1, st);
             if (d_dx) {
                 launch_simt<T, GATED_DX>(p, p.m, p.k, 128, p.dx_splits, st);
                 if (p.dx_splits > 1) join_dx<T><<<(unsigned)std::min<int64_t>(ceil_div(p.m * p.k, kThreads), 148 * 8), kThreads, 0, st>>>(p);

@@ -22,7 +22,7 @@ struct GatedParams {
     const void *x, *wg, *wu, *bg, *bu, *dy;
     int64_t x_row, wg_row, wu_row, y_row, dx_row;
     void *y, *dx;
-    // backward scratch: dg and du [m][pre_row] in the element type, column sums [row tiles of 128 or 64, or gated_col_sums][2][n]
+    // backward scratch: dg and du [m][pre_row] in the element type, column sums [row tiles of 128, 64 or 8, or gated_col_sums][2][n]
     void *dg, *du;
     int64_t pre_row;
     float* col_sums;
