@@ -59,8 +59,8 @@ __device__ __forceinline__ void join(Moments& a, const Moments& b) {
     a.m2 = a.m2 + b.m2 + d * d * a.n * w;
     a.n = n;
 }
-__device__ __forceinline__ void warp_join(Moments& a) {
-    for (int o = 16; o > 0; o >>= 1) {
+template <int LANES = 32> __device__ __forceinline__ void warp_join(Moments& a) {
+    for (int o = LANES / 2; o > 0; o >>= 1) {
         Moments b;
         b.n = __shfl_xor_sync(~0u, a.n, o);
         b.mean = __shfl_xor_sync(~0u, a.mean, o);
@@ -145,21 +145,26 @@ template <class T, int V> struct Sums {
 
 // Moments of the groups with channels in [ch0, ch1) from a block's parts of them: [step][row],
 // mean and M2 of the positions that place r has. The mean of the means first, then the deviations
-// from it, both from the group's first part on; several warps to a group when groups are few. A
-// group that began before ch0 is joined to what group[] has of it.
+// from it, both from the group's first part on. All threads are shared out to the groups at once,
+// several warps to one or, with more groups than warps, down to one lane (a warp to each in turn:
+// 542 us where this takes 37 for 2 x 16 x 4096 with 4096 groups). A group that began before ch0 is
+// joined to what group[] has of it.
 template <int THREADS>
 __device__ __forceinline__ void block_moments(const NormParams& p, const Place& q, int n, int vec, int ch0, int ch1, const float2* part, float2* group,
                                               float* red) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = THREADS / 32;
     const int per = p.mono ? vec : 1, row = q.width * vec / per, rows = min(q.step, n);
     const int base = n / q.step, more = n - base * q.step;       // place r has base positions, and one more below `more`
-    const int first = ch0 / p.cpg, count = (ch1 - 1) / p.cpg + 1 - first, team = max(1, warps / count), member = warp % team;
-    for (int g0 = 0; g0 < count; g0 += warps / team) {
-        const int g = first + g0 + warp / team;
-        const bool live = g - first < count && warp < warps / team * team;
+    const int first = ch0 / p.cpg, count = (ch1 - 1) / p.cpg + 1 - first;
+    int lanes = 32;
+    while (lanes > 1 && count * lanes > THREADS) lanes >>= 1;
+    const int team = max(1, THREADS / 32 / count), share = lanes * team, at_once = THREADS / share;
+    const int slot = threadIdx.x / share, lead = threadIdx.x - slot * share;
+    for (int g0 = 0; g0 < count; g0 += at_once) {
+        const int g = first + g0 + slot;
+        const bool live = g - first < count && slot < at_once;
         const int from_ch = max(g * p.cpg, ch0), w = live ? (min((g + 1) * p.cpg, ch1) - from_ch) / per : 1;
         const float2* at = part + (from_ch - ch0) / per;
-        const int lead = member * 32 + lane, r0 = lead / w, c0 = lead - r0 * w, dr = team * 32 / w, dc = team * 32 - dr * w;
+        const int r0 = lead / w, c0 = lead - r0 * w, dr = share / w, dc = share - dr * w;
         const float from = live ? at[0].x : 0.0f;
         float mean = 0.0f;
         for (int pass = 0; pass < 2; pass++) {
@@ -172,17 +177,17 @@ __device__ __forceinline__ void block_moments(const NormParams& p, const Place& 
                     r += dr;
                     if ((c += dc) >= w) { c -= w; r++; }
                 }
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
             if (team > 1) {   // then every group has its team at once: one round
-                if (lane == 0) red[warp] = sum;
+                if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
                 __syncthreads();
                 sum = 0.0f;
                 if (live)
-                    for (int k = 0; k < team; k++) sum += red[warp - member + k];
+                    for (int k = 0; k < team; k++) sum += red[slot * team + k];
                 __syncthreads();
             }
             if (pass == 0) mean = sum / ((float)n * (float)(w * per));
-            else if (live && member == 0 && lane == 0) {
+            else if (live && lead == 0) {
                 Moments m{(float)n * (float)(w * per), from + mean, sum};
                 if (g * p.cpg < ch0) {
                     Moments t{(float)n * (float)(ch0 - g * p.cpg), group[g].x, group[g].y};
@@ -459,21 +464,24 @@ __global__ void __launch_bounds__(256) grad_join(const __grid_constant__ NormPar
 // Sums over a group's channels of gamma times their sums: s(c) -> out(g).
 template <class T, int THREADS, class S, class Out>
 __device__ __forceinline__ void group_sums(const NormParams& p, S&& s, Out&& out) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int g = warp; g < p.groups; g += THREADS / 32) {
+    int lanes = 32;   // of a group: all threads at once, as in block_moments
+    while (lanes > 1 && p.groups * lanes > THREADS) lanes >>= 1;
+    const int lead = threadIdx.x & (lanes - 1);
+    for (int g0 = 0; g0 < p.groups; g0 += THREADS / lanes) {
+        const int g = g0 + threadIdx.x / lanes;
         float a = 0.0f, b = 0.0f;
-        for (int k = lane; k < p.cpg; k += 32) {
+        for (int k = lead; k < p.cpg && g < p.groups; k += lanes) {
             const int c = g * p.cpg + k;
             const float2 v = s(c);
             const float gc = param(p.gamma, c, p.param_float, 1.0f, (const T*)nullptr);
             a = fmaf(gc, v.x, a);
             b = fmaf(gc, v.y, b);
         }
-        for (int o = 16; o > 0; o >>= 1) {
+        for (int o = lanes / 2; o > 0; o >>= 1) {
             a += __shfl_xor_sync(~0u, a, o);
             b += __shfl_xor_sync(~0u, b, o);
         }
-        if (lane == 0) out(g, a, b);
+        if (lead == 0 && g < p.groups) out(g, a, b);
     }
 }
 
@@ -548,7 +556,7 @@ __global__ void __launch_bounds__(kFused, 1) norm_cluster(const __grid_constant_
     __shared__ float red[kFused / 32];
     const Range s = cluster_range(p);
     const Place q = place<kFused>(p);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ch = q.col * V;
+    const int ch = q.col * V;
     const int mine = q.r < q.step ? mine_of(q, s.n) : 0;
     if (s.n > 0) {
         if (mine) {
@@ -570,15 +578,15 @@ __global__ void __launch_bounds__(kFused, 1) norm_cluster(const __grid_constant_
     cluster_arrive();
     cluster_wait();
     if (s.n > 0) {
-        for (int g = warp; g < p.groups; g += kFused / 32) {
+        for (int g0 = 0; g0 < p.groups; g0 += kFused / kClusterMost) {   // a lane to a block
+            const int g = g0 + threadIdx.x / kClusterMost, c = threadIdx.x % kClusterMost;
             Moments m{0.0f, 0.0f, 0.0f};
-            for (int c = lane; c < p.used; c += 32) {
-                const float n = (float)min((int64_t)p.rows, p.positions - (int64_t)c * p.rows) * (float)p.cpg;
+            if (g < p.groups && c < p.used) {
                 const float2 v = peer_read(group + g, c);
-                join(m, Moments{n, v.x, v.y});
+                m = Moments{(float)min((int64_t)p.rows, p.positions - (int64_t)c * p.rows) * (float)p.cpg, v.x, v.y};
             }
-            warp_join(m);
-            if (lane == 0) {
+            warp_join<kClusterMost>(m);
+            if (g < p.groups && c == 0) {
                 const float r = 1.0f / sqrtf(m.m2 / ((float)p.positions * (float)p.cpg) + p.eps);
                 stat[g] = make_float2(m.mean, r);
                 if (s.chunk == 0 && p.mean) {
@@ -616,7 +624,7 @@ __global__ void __launch_bounds__(kFused, 1) norm_grad_cluster(const __grid_cons
     next_may_start();
     const Range s = cluster_range(p);
     const Place q = place<kFused>(p);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ch = q.col * V;
+    const int ch = q.col * V;
     const bool on = q.r < q.step && s.n > 0;
     const int mine = on ? mine_of(q, s.n) : 0;
     Slope<T, V, ACT> f;
@@ -657,13 +665,14 @@ __global__ void __launch_bounds__(kFused, 1) norm_grad_cluster(const __grid_cons
     cluster_wait();
     if (s.n > 0 && p.dx) {
         const float m = (float)p.positions * (float)p.cpg;
-        for (int g = warp; g < p.groups; g += kFused / 32) {
-            float2 v = lane < p.used ? peer_read(group + g, lane) : make_float2(0.0f, 0.0f);
-            for (int o = 16; o > 0; o >>= 1) {
+        for (int g0 = 0; g0 < p.groups; g0 += kFused / kClusterMost) {   // a lane to a block
+            const int g = g0 + threadIdx.x / kClusterMost, c = threadIdx.x % kClusterMost;
+            float2 v = g < p.groups && c < p.used ? peer_read(group + g, c) : make_float2(0.0f, 0.0f);
+            for (int o = kClusterMost / 2; o > 0; o >>= 1) {
                 v.x += __shfl_xor_sync(~0u, v.x, o);
                 v.y += __shfl_xor_sync(~0u, v.y, o);
             }
-            if (lane == 0) stat[g] = make_float2(v.x / m, v.y / m);
+            if (g < p.groups && c == 0) stat[g] = make_float2(v.x / m, v.y / m);
         }
     }
     cluster_arrive();

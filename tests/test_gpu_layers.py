@@ -130,6 +130,7 @@ NORM = [
     (1, 5000, 64, 2), (4, 3, 2056, 8), (1, 40, 2051, 7), (2, 3, 8192, 1), (1, 50, 8192, 8192), (5, 700, 24, 3), (1, 30011, 16, 4), (2, 9000, 192, 4),
     (65, 9, 32, 8), (1, 33, 36, 1), (7, 9, 16, 2),
     (5, 30000, 24, 2), (1, 400000, 40, 5), (3, 70001, 33, 3), (2, 20000, 520, 520),
+    (3, 100, 1000, 1000), (2, 50, 384, 128), (1, 257, 1030, 103), (2, 16, 4096, 4096), (2, 20, 4104, 1026),      # more groups than warps
 ]
 
 
