@@ -85,10 +85,10 @@ template <class T> __device__ __forceinline__ void set_param(void* p, int i, boo
 // The thread's place in a block: column vector `col` of the current column tile and one of
 // `step` positions taken side by side.
 struct Place { int width, step, r, col; };
-template <int THREADS> __device__ __forceinline__ Place place(const NormParams& p) {
+__device__ __forceinline__ Place place(const NormParams& p, int threads) {
     Place q;
     q.width = (int)p.columns_div.d;
-    q.step = THREADS / q.width;
+    q.step = threads / q.width;
     q.r = (int)p.columns_div.div(threadIdx.x);
     q.col = threadIdx.x - q.r * q.width;
     return q;
@@ -149,15 +149,14 @@ template <class T, int V> struct Sums {
 // several warps to one or, with more groups than warps, down to one lane (a warp to each in turn:
 // 542 us where this takes 37 for 2 x 16 x 4096 with 4096 groups). A group that began before ch0 is
 // joined to what group[] has of it.
-template <int THREADS>
-__device__ __forceinline__ void block_moments(const NormParams& p, const Place& q, int n, int vec, int ch0, int ch1, const float2* part, float2* group,
+__device__ __forceinline__ void block_moments(const NormParams& p, int threads, const Place& q, int n, int vec, int ch0, int ch1, const float2* part, float2* group,
                                               float* red) {
     const int per = p.mono ? vec : 1, row = q.width * vec / per, rows = min(q.step, n);
     const int base = n / q.step, more = n - base * q.step;       // place r has base positions, and one more below `more`
     const int first = ch0 / p.cpg, count = (ch1 - 1) / p.cpg + 1 - first;
     int lanes = 32;
-    while (lanes > 1 && count * lanes > THREADS) lanes >>= 1;
-    const int team = max(1, THREADS / 32 / count), share = lanes * team, at_once = THREADS / share;
+    while (lanes > 1 && count * lanes > threads) lanes >>= 1;
+    const int team = max(1, threads / 32 / count), share = lanes * team, at_once = threads / share;
     const int slot = threadIdx.x / share, lead = threadIdx.x - slot * share;
     for (int g0 = 0; g0 < count; g0 += at_once) {
         const int g = first + g0 + slot;
@@ -329,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 2) moments_kernel(const __grid_const
     extern __shared__ float2 group[];          // [groups]
     next_may_start();
     const Range s = range_of(p, false);
-    const Place q = place<kThreads>(p);
+    const Place q = place(p, kThreads);
     const int mine = mine_of(q, s.n);
     for (int c0 = 0; c0 < p.columns; c0 += q.width) {
         const int cols = min(q.width, p.columns - c0);
@@ -342,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 2) moments_kernel(const __grid_const
             sums.finish(mine, p.mono, part, q.r * q.width + q.col);
         }
         __syncthreads();
-        block_moments<kThreads>(p, q, s.n, V, c0 * V, (c0 + cols) * V, part, group, red);
+        block_moments(p, kThreads, q, s.n, V, c0 * V, (c0 + cols) * V, part, group, red);
     }
     for (int g = threadIdx.x; g < p.groups; g += kThreads) p.part[((int64_t)s.item * p.groups + g) * p.chunks + s.chunk] = group[g];
 }
@@ -372,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 2) apply_kernel(const __grid_constan
     constexpr int U = 4;
     using P = Pack<T, V>;
     const Range s = range_of(p, true);
-    const Place q = place<kThreads>(p);
+    const Place q = place(p, kThreads);
     after_previous();
     const int mine = mine_of(q, s.n);
     if (q.r >= q.step || !mine) return;
@@ -395,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 2) grad_sums_kernel(const __grid_con
     __shared__ float2 part[kThreads * V];
     next_may_start();
     const Range s = range_of(p, false);
-    const Place q = place<kThreads>(p);
+    const Place q = place(p, kThreads);
     const int mine = mine_of(q, s.n);
     for (int c0 = 0; c0 < p.columns; c0 += q.width) {
         const int cols = min(q.width, p.columns - c0);
@@ -496,12 +495,12 @@ __global__ void __launch_bounds__(1024) items_join(const __grid_constant__ NormP
 }
 
 // Sums over a group's channels of gamma times their sums: s(c) -> out(g).
-template <class T, int THREADS, class S, class Out>
-__device__ __forceinline__ void group_sums(const NormParams& p, S&& s, Out&& out) {
+template <class T, class S, class Out>
+__device__ __forceinline__ void group_sums(const NormParams& p, int threads, S&& s, Out&& out) {
     int lanes = 32;   // of a group: all threads at once, as in block_moments
-    while (lanes > 1 && p.groups * lanes > THREADS) lanes >>= 1;
+    while (lanes > 1 && p.groups * lanes > threads) lanes >>= 1;
     const int lead = threadIdx.x & (lanes - 1);
-    for (int g0 = 0; g0 < p.groups; g0 += THREADS / lanes) {
+    for (int g0 = 0; g0 < p.groups; g0 += threads / lanes) {
         const int g = g0 + threadIdx.x / lanes;
         float a = 0.0f, b = 0.0f;
         for (int k = lead; k < p.cpg && g < p.groups; k += lanes) {
@@ -525,10 +524,10 @@ __global__ void __launch_bounds__(kThreads, 2) grad_apply_kernel(const __grid_co
     using P = Pack<T, V>;
     extern __shared__ float2 group[];   // [groups]: means of d and d xh
     const Range s = range_of(p, true);
-    const Place q = place<kThreads>(p);
+    const Place q = place(p, kThreads);
     after_previous();
     const float m = (float)p.positions * (float)p.cpg;
-    group_sums<T, kThreads>(p, [&](int c) { return p.sums[(int64_t)s.item * p.channels + c]; },
+    group_sums<T>(p, kThreads, [&](int c) { return p.sums[(int64_t)s.item * p.channels + c]; },
                             [&](int g, float a, float b) { group[g] = make_float2(a / m, b / m); });
     __syncthreads();
     const int mine = mine_of(q, s.n);
@@ -583,13 +582,14 @@ __global__ void __launch_bounds__(kFused, 1) norm_cluster(const __grid_constant_
     constexpr int U = 4;                        // positions in flight per thread
     using P = Pack<T, V>;
     extern __shared__ __align__(16) uint8_t smem[];
+    const int threads = blockDim.x;             // kFused at most
     P* keep = reinterpret_cast<P*>(smem);       // [kept][threads]
-    float2* part = reinterpret_cast<float2*>(smem + (size_t)p.kept * kFused * sizeof(P));
-    float2* group = part + kFused * (p.mono ? 1 : V);   // [groups]: the block's moments
+    float2* part = reinterpret_cast<float2*>(smem + (size_t)p.kept * threads * sizeof(P));
+    float2* group = part + threads * (p.mono ? 1 : V);   // [groups]: the block's moments
     float2* stat = group + p.groups;                    // [groups]: the item's mean and rstd
     __shared__ float red[kFused / 32];
     const Range s = cluster_range(p);
-    const Place q = place<kFused>(p);
+    const Place q = place(p, threads);
     const int ch = q.col * V;
     const int mine = q.r < q.step ? mine_of(q, s.n) : 0;
     if (s.n > 0) {
@@ -601,18 +601,18 @@ __global__ void __launch_bounds__(kFused, 1) norm_cluster(const __grid_constant_
             P* k = keep + threadIdx.x;
             stream<P, U>(mine, [&](P& v) { v = *reinterpret_cast<const P*>(at); at += step; }, [&](const P& v) {
                 *k = v;
-                k += kFused;
+                k += threads;
                 sums.take(v);
             });
             sums.finish(mine, p.mono, part, q.r * q.width + q.col);
         }
         __syncthreads();
-        block_moments<kFused>(p, q, s.n, V, 0, p.channels, part, group, red);
+        block_moments(p, threads, q, s.n, V, 0, p.channels, part, group, red);
     }
     cluster_arrive();
     cluster_wait();
     if (s.n > 0) {
-        for (int g0 = 0; g0 < p.groups; g0 += kFused / kClusterMost) {   // a lane to a block
+        for (int g0 = 0; g0 < p.groups; g0 += threads / kClusterMost) {   // a lane to a block
             const int g = g0 + threadIdx.x / kClusterMost, c = threadIdx.x % kClusterMost;
             Moments m{0.0f, 0.0f, 0.0f};
             if (g < p.groups && c < p.used) {
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(kFused, 1) norm_cluster(const __grid_constant_
         T* y = static_cast<T*>(p.y) + s.item * p.yb + (s.l0 + q.r) * p.yp + ch;
         const int64_t sy = (int64_t)q.step * p.yp;
         const P* k = keep + threadIdx.x;
-        for (int it = 0; it < mine; it++, k += kFused, y += sy) f.put_at(y, *k);
+        for (int it = 0; it < mine; it++, k += threads, y += sy) f.put_at(y, *k);
     }
     __syncwarp();
     cluster_wait();
@@ -650,14 +650,15 @@ __global__ void __launch_bounds__(kFused, 1) norm_grad_cluster(const __grid_cons
     constexpr int U = 2, N = (V + 1) / 2;
     using P = Pack<T, V>;
     extern __shared__ __align__(16) uint8_t smem[];
+    const int threads = blockDim.x;             // kFused at most
     P* keep = reinterpret_cast<P*>(smem);       // [kept][x, dy][threads]
-    float2* part = reinterpret_cast<float2*>(smem + (size_t)p.kept * 2 * kFused * sizeof(P));   // [step][channels]
-    float2* chan = part + kFused * V;           // [channels]
+    float2* part = reinterpret_cast<float2*>(smem + (size_t)p.kept * 2 * threads * sizeof(P));   // [step][channels]
+    float2* chan = part + threads * V;           // [channels]
     float2* group = chan + p.channels;          // [groups]: the block's sums
     float2* stat = group + p.groups;            // [groups]: the item's means of d and d xh
     next_may_start();
     const Range s = cluster_range(p);
-    const Place q = place<kFused>(p);
+    const Place q = place(p, threads);
     const int ch = q.col * V;
     const bool on = q.r < q.step && s.n > 0;
     const int mine = on ? mine_of(q, s.n) : 0;
@@ -675,14 +676,14 @@ __global__ void __launch_bounds__(kFused, 1) norm_grad_cluster(const __grid_cons
             stream<Two<P>, U>(mine, [&](Two<P>& v) { v.x = *reinterpret_cast<const P*>(ax); v.dy = *reinterpret_cast<const P*>(ad); ax += sx; ad += sd; },
                               [&](const Two<P>& v) {
                                   k[0] = v.x;
-                                  k[kFused] = v.dy;
-                                  k += 2 * kFused;
+                                  k[threads] = v.dy;
+                                  k += 2 * threads;
                                   f.take(v.x, v.dy, a, b);
                               });
             f.parts(a, b, part + (q.r * q.width + q.col) * V);
         }
         __syncthreads();
-        for (int c = threadIdx.x; c < p.channels; c += kFused) {
+        for (int c = threadIdx.x; c < p.channels; c += threads) {
             float2 t = make_float2(0.0f, 0.0f);
             for (int r = 0; r < q.step; r++) {
                 const float2 v = part[r * p.channels + c];
@@ -693,15 +694,15 @@ __global__ void __launch_bounds__(kFused, 1) norm_grad_cluster(const __grid_cons
             p.part[((int64_t)s.item * p.chunks + s.chunk) * p.channels + c] = t;
         }
         __syncthreads();
-        group_sums<T, kFused>(p, [&](int c) { return chan[c]; }, [&](int g, float a, float b) { group[g] = make_float2(a, b); });
+        group_sums<T>(p, threads, [&](int c) { return chan[c]; }, [&](int g, float a, float b) { group[g] = make_float2(a, b); });
     } else {
-        for (int c = threadIdx.x; c < p.channels; c += kFused) p.part[((int64_t)s.item * p.chunks + s.chunk) * p.channels + c] = make_float2(0.0f, 0.0f);
+        for (int c = threadIdx.x; c < p.channels; c += threads) p.part[((int64_t)s.item * p.chunks + s.chunk) * p.channels + c] = make_float2(0.0f, 0.0f);
     }
     cluster_arrive();
     cluster_wait();
     if (s.n > 0 && p.dx) {
         const float m = (float)p.positions * (float)p.cpg;
-        for (int g0 = 0; g0 < p.groups; g0 += kFused / kClusterMost) {   // a lane to a block
+        for (int g0 = 0; g0 < p.groups; g0 += threads / kClusterMost) {   // a lane to a block
             const int g = g0 + threadIdx.x / kClusterMost, c = threadIdx.x % kClusterMost;
             float2 v = g < p.groups && c < p.used ? peer_read(group + g, c) : make_float2(0.0f, 0.0f);
             for (int o = kClusterMost / 2; o > 0; o >>= 1) {
@@ -719,7 +720,7 @@ __global__ void __launch_bounds__(kFused, 1) norm_grad_cluster(const __grid_cons
         T* dx = static_cast<T*>(p.dx) + s.item * p.db + (s.l0 + q.r) * p.dp + ch;
         const int64_t so = (int64_t)q.step * p.dp;
         const P* k = keep + threadIdx.x;
-        for (int it = 0; it < mine; it++, k += 2 * kFused, dx += so) f.put_at(dx, k[0], k[kFused], c1, c2);
+        for (int it = 0; it < mine; it++, k += 2 * threads, dx += so) f.put_at(dx, k[0], k[threads], c1, c2);
     }
     __syncwarp();
     cluster_wait();
@@ -759,7 +760,7 @@ enum Path { THREE_LAUNCHES, CLUSTER };
 // How a call runs with vectors of `vec` channels on `sms` SMs, and the scratch it takes.
 struct NormPlan {
     Path path = THREE_LAUNCHES;
-    int chunks = 0, kept = 0;
+    int chunks = 0, kept = 0, threads = 0;      // threads: a cluster's blocks
     int64_t rows = 0;
     size_t smem = 0;
     size_t second = 0, third = 0, bytes = 0;   // offsets of the scratch's parts
@@ -768,14 +769,19 @@ NormPlan plan_of(const stg_group_norm_config& c, bool backward, int vec, int sms
     NormPlan r;
     if (!c.batch || !c.positions) return r;
     const int columns = c.channels / vec, cpg = c.channels / c.groups;
-    const size_t vb = (size_t)vec * elem_size(c.dtype) * (backward ? 2 : 1), block_step = vb * kFused;
+    // Items that a smaller block reads in eight steps, more of them than SMs: such blocks, of which an SM
+    // holds several (3000 x 7 x 75 f32: 21 us, 97 with kFused threads each).
+    int threads = kFused;
+    while (threads > 128 && columns <= threads / 2 && c.positions <= 8 * (threads / 2 / columns) && c.batch > sms) threads /= 2;
+    r.threads = threads;
+    const size_t vb = (size_t)vec * elem_size(c.dtype) * (backward ? 2 : 1), block_step = vb * threads;
     const bool mono = cpg % vec == 0;
     // shared memory besides the kept values: the threads' parts, channel and group sums
-    const size_t other = backward ? sizeof(float2) * ((size_t)kFused * vec + c.channels + 2 * (size_t)c.groups)
-                                  : sizeof(float2) * ((size_t)kFused * (mono ? 1 : vec) + 2 * (size_t)c.groups);
+    const size_t other = backward ? sizeof(float2) * ((size_t)threads * vec + c.channels + 2 * (size_t)c.groups)
+                                  : sizeof(float2) * ((size_t)threads * (mono ? 1 : vec) + 2 * (size_t)c.groups);
     const size_t most = 225 * 1024;
-    if (columns <= kFused && c.groups <= kFusedGroups && other + 8 * block_step <= most) {
-        const int64_t step = kFused / columns, room = (int64_t)((most - other) / block_step);   // steps a block can keep
+    if (columns <= threads && c.groups <= kFusedGroups && other + 8 * block_step <= most) {
+        const int64_t step = threads / columns, room = (int64_t)((most - other) / block_step);   // steps a block can keep
         const int64_t item_steps = (c.positions + step - 1) / step;
         auto steps = [&](int64_t size) { return ((c.positions + size - 1) / size + step - 1) / step; };   // of one of `size` blocks
         // as many blocks as fill the GPU once, each with at least four steps
@@ -834,9 +840,9 @@ template <class T, class Fn> void with_width(bool wide, Fn&& fn) {
     if (wide) fn(std::integral_constant<int, 16 / (int)sizeof(T)>{});
     else fn(std::integral_constant<int, 1>{});
 }
-void set_plan(NormParams& p, const NormPlan& plan, int vec, int fused) {
+void set_plan(NormParams& p, const NormPlan& plan, int vec) {
     p.columns = p.channels / vec;
-    p.columns_div = FastDiv((uint32_t)std::min(p.columns, plan.path == THREE_LAUNCHES ? kThreads : fused));
+    p.columns_div = FastDiv((uint32_t)std::min(p.columns, plan.path == THREE_LAUNCHES ? kThreads : plan.threads));
     p.chunks = plan.chunks;
     p.rows = (int)plan.rows;
     p.used = (int)((p.positions + plan.rows - 1) / plan.rows);
@@ -876,7 +882,7 @@ template <class K> void launch_cluster(K kernel, const NormParams& p, const Norm
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
     cfg.gridDim = dim3((unsigned)(p.batch * plan.chunks));
-    cfg.blockDim = dim3(kFused);
+    cfg.blockDim = dim3(plan.threads);
     cfg.dynamicSmemBytes = plan.smem;
     cfg.stream = st;
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -939,7 +945,7 @@ STG_API stg_status stg_group_norm(stg_engine* e, const stg_group_norm_config* c,
             using T = std::remove_pointer_t<decltype(tag)>;
             with_width<T>(wide, [&](auto v) {
                 constexpr int V = decltype(v)::value;
-                set_plan(p, plan, V, kFused);
+                set_plan(p, plan, V);
                 with_activation(c->activation, [&](auto a) {
                     constexpr int A = decltype(a)::value;
                     if (plan.path == CLUSTER) return launch_cluster(norm_cluster<T, V, A>, p, plan, st);
@@ -995,7 +1001,7 @@ STG_API stg_status stg_group_norm_backward(stg_engine* e, const stg_group_norm_c
             using T = std::remove_pointer_t<decltype(tag)>;
             with_width<T>(wide, [&](auto v) {
                 constexpr int V = decltype(v)::value;
-                set_plan(p, plan, V, kFused);
+                set_plan(p, plan, V);
                 with_activation(c->activation, [&](auto a) {
                     constexpr int A = decltype(a)::value;
                     const unsigned columns = (unsigned)((p.channels + 31) / 32);
