@@ -770,9 +770,9 @@ NormPlan plan_of(const stg_group_norm_config& c, bool backward, int vec, int sms
     if (!c.batch || !c.positions) return r;
     const int columns = c.channels / vec, cpg = c.channels / c.groups;
     // Items that a smaller block reads in eight steps, more of them than SMs: such blocks, of which an SM
-    // holds several (3000 x 7 x 75 f32: 21 us, 97 with kFused threads each).
+    // holds several (9000 x 16 x 16 f32: 35 us, 281 with kFused threads each; 3000 x 7 x 75 21 and 97).
     int threads = kFused;
-    while (threads > 128 && columns <= threads / 2 && c.positions <= 8 * (threads / 2 / columns) && c.batch > sms) threads /= 2;
+    while (threads > 32 && columns <= threads / 2 && c.positions <= 8 * (threads / 2 / columns) && c.batch > sms) threads /= 2;
     r.threads = threads;
     const size_t vb = (size_t)vec * elem_size(c.dtype) * (backward ? 2 : 1), block_step = vb * threads;
     const bool mono = cpg % vec == 0;

@@ -131,6 +131,7 @@ NORM = [
     (65, 9, 32, 8), (1, 33, 36, 1), (7, 9, 16, 2),
     (5, 30000, 24, 2), (1, 400000, 40, 5), (3, 70001, 33, 3), (2, 20000, 520, 520),
     (3, 100, 1000, 1000), (2, 50, 384, 128), (1, 257, 1030, 103), (2, 16, 4096, 4096), (2, 20, 4104, 1026),      # more groups than warps
+    (700, 5, 24, 3), (600, 16, 16, 1), (1200, 3, 75, 25), (300, 7, 96, 96), (20, 12, 4104, 8),     # many small items
 ]
 
 
