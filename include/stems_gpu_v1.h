@@ -481,7 +481,7 @@ enum { STG_ACT_NONE = 0, STG_ACT_RELU = 1, STG_ACT_SILU = 2, STG_ACT_GELU = 3, S
  *   scaling 1 linear   f_i / s
  *   scaling 2 NTK      base s^(rotary_dim / (rotary_dim - 2)) in place of base
  *   scaling 3 YaRN     (1 - g_i) f_i + g_i f_i / s and m = 0.1 ln(s) + 1, where g_i rises from 0 to 1
- *                      between i = max(floor(j(beta_fast)), 0) and min(ceil(j(beta_slow)), rotary_dim / 2 - 1)
+ *                      between i = max(floor(j(beta_fast)), 0) and min(ceil(j(beta_slow)), rotary_dim - 1)
  *                      (at least 0.001 apart), j(r) = rotary_dim ln(original_length / (2 pi r)) / (2 ln base)
  * Angles are reduced in double, so far positions keep their phase. */
 typedef struct {

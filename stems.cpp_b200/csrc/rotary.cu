@@ -228,7 +228,8 @@ double frequencies(const stg_rotary_config& c, double* f) {
         const double fast = none ? 32.0 : c.beta_fast, slow = none ? 1.0 : c.beta_slow;
         auto dim_of = [&](double turns) { return r * std::log(c.original_length / (turns * 2.0 * M_PI)) / (2.0 * std::log(base)); };
         const double lo = std::max(std::floor(dim_of(fast)), 0.0);
-        const double hi = std::min(std::ceil(dim_of(slow)), (double)(half - 1));
+        // the ramp may end past the last pair (half - 1): then every pair turns more than `slow` times
+        const double hi = std::min(std::ceil(dim_of(slow)), (double)(r - 1));
         for (int i = 0; i < half; i++) {
             const double g = std::min(std::max((i - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
             f[i] = (1.0 - g) * f[i] + g * f[i] / s;
