@@ -566,9 +566,9 @@ typedef struct {
     uint32_t size;
     int32_t dtype;
     int32_t activation;
-    int32_t features;          /* at least 1 */
-    int32_t width;             /* at least 1 */
-    int64_t rows;              /* rows, width and features below 2^31 each; rows 0 allowed */
+    int32_t features;          /* 1 .. 2^31 - 2^16 */
+    int32_t width;             /* 1 .. 2^31 - 2^16 */
+    int64_t rows;              /* below 2^31; 0 allowed; no matrix may have more than 2^50 elements */
     int64_t x_row, wg_row, wu_row, y_row;   /* row strides; y_row is dy's in the backward pass */
     int64_t dx_row, dwg_row, dwu_row;       /* row strides of the gradients (backward pass only) */
 } stg_gated_config;
@@ -600,7 +600,7 @@ STG_API stg_status stg_engine_status(stg_engine* engine);
 typedef struct {
     uint32_t size;
     int32_t dtype;             /* h, weight and bias */
-    int32_t hidden;            /* at least 1 */
+    int32_t hidden;            /* 1 .. 2^31 - 2^16 */
     int32_t n_chunks;
 } stg_mask_head_config;
 /* S, n_bands, T and sum_b din_b of a RoFormer plan: the sizes of the mask head's buffers. */

@@ -509,12 +509,24 @@ __global__ void __launch_bounds__(kThreads) repack(const __grid_constant__ Repac
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// The kernels' 32-bit positions along features and outputs reach a tile, or gated_rows' steps, past the last one.
+constexpr int kMostSpan = INT32_MAX - 65535;
+void check_span(int n, const char* what) {
+    if (n > kMostSpan) fail(STG_UNSUPPORTED, std::string(what) + " above 2^31 - 2^16");
+}
+
 void check_config(const stg_gated_config* c, bool backward) {
     check_sized(c, "gated");
     check(valid_dtype(c->dtype), "gated: unknown dtype");
     check(valid_activation(c->activation), "gated: unknown activation");
     check(c->features >= 1 && c->width >= 1 && c->rows >= 0, "gated: features and width must be at least 1, rows at least 0");
     if (c->rows > INT32_MAX) fail(STG_UNSUPPORTED, "gated: too many rows");
+    check_span(c->features, "gated: features");
+    check_span(c->width, "gated: width");
+    // operands broadcast by strides of 0 make such sizes possible: the scratch's bytes must not pass 64 bits
+    const int64_t most = 1ll << 50, rows = std::max<int64_t>(c->rows, 1);
+    if (c->width > most / rows || c->features > most / rows || c->features > most / c->width)
+        fail(STG_UNSUPPORTED, "gated: a matrix of more than 2^50 elements");
     check(c->x_row >= 0 && c->wg_row >= 0 && c->wu_row >= 0 && c->y_row >= 0, "gated: negative stride");
     check((c->y_row >= c->width || c->rows <= 1) || backward, "gated: the output's rows overlap");
 }
@@ -784,6 +796,7 @@ static void check_head(const stg_plan* p, const stg_mask_head_config* c) {
     check(p->H.arch == ARCH_ROFORMER && !p->H.band_din.empty(), "mask head: not a RoFormer plan");
     check(valid_dtype(c->dtype), "mask head: unknown dtype");
     check(c->hidden >= 1 && c->n_chunks >= 0, "mask head: hidden must be at least 1, n_chunks at least 0");
+    check_span(c->hidden, "mask head: hidden");
 }
 
 static int64_t head_rows(const stg_plan* p, const stg_mask_head_config* c) {

@@ -1,6 +1,8 @@
 """The layers' contracts that need no GPU: YaRN's ramp at lengths where its upper end lies past
-the last pair."""
+the last pair, sizes that the gated projection's kernels cannot reach."""
 from __future__ import annotations
+
+import ctypes as C
 
 import numpy as np
 import pytest
@@ -19,3 +21,22 @@ def test_yarn_ramp_past_the_last_pair(pkg, r, length, base, pairs, tail):
     np.testing.assert_allclose(f[-len(tail):], tail, rtol=1e-12)
     share = np.clip((np.arange(r // 2) - pairs[0]) / (pairs[1] - pairs[0]), 0, 1)
     np.testing.assert_allclose(f, base ** (-2 * np.arange(r // 2) / r) * (1 - share * 7 / 8), rtol=1e-12)
+
+
+@pytest.mark.parametrize("sizes, code", [
+    (dict(features=2 ** 31 - 2 ** 16), 0), (dict(features=2 ** 31 - 2 ** 16 + 1), 2), (dict(features=2 ** 31 - 1), 2),
+    (dict(width=2 ** 31 - 2 ** 16), 0), (dict(width=2 ** 31 - 1), 2), (dict(rows=2 ** 31 - 1, features=8, width=8), 0),
+    # a broadcast dy, x or weight makes these calls possible; their scratch would not fit 64 bits
+    (dict(rows=2 ** 31 - 1, width=2 ** 30), 2), (dict(rows=2 ** 31 - 1, features=2 ** 30), 2), (dict(width=2 ** 30, features=2 ** 30), 2),
+    (dict(rows=2 ** 24, width=2 ** 26, features=2 ** 24), 0)])
+def test_gated_sizes_past_the_kernels_reach_are_refused(pkg, sizes, code):
+    """Positions along the features and the outputs are 32 bits wide in the kernels and run up to a
+    tile past the end; the scratch's bytes are 64 bits wide."""
+    for dtype in (0, 1, 2):
+        c = dict(dict(rows=10, features=64, width=96), **sizes)
+        k, n = c["features"], c["width"]
+        cfg = pkg.GatedConfig(C.sizeof(pkg.GatedConfig), dtype, 2, k, n, c["rows"], 0, 0, 0, 0, k, k, k)
+        need = C.c_size_t(12345)
+        assert pkg.lib().stg_gated_workspace(C.byref(cfg), 1, C.byref(need)) == code
+        # dg and du alone are rows x width each
+        assert need.value >= 2 * c["rows"] * n * (2 if dtype else 4) if code == 0 else need.value == 12345
