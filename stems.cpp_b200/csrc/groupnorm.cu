@@ -553,6 +553,7 @@ __global__ void __launch_bounds__(kThreads, 2) grad_apply_kernel(const __grid_co
 constexpr int kFused = 512;          // threads: with 1024 the registers do not hold a vector's sums
 constexpr int kFusedGroups = 2048;   // most groups
 constexpr int kClusterMost = 8;
+constexpr size_t kClusterSmem = 225 * 1024;   // dynamic shared memory of a block
 
 __device__ __forceinline__ void cluster_arrive() {
     __syncwarp();
@@ -779,7 +780,7 @@ NormPlan plan_of(const stg_group_norm_config& c, bool backward, int vec, int sms
     // shared memory besides the kept values: the threads' parts, channel and group sums
     const size_t other = backward ? sizeof(float2) * ((size_t)threads * vec + c.channels + 2 * (size_t)c.groups)
                                   : sizeof(float2) * ((size_t)threads * (mono ? 1 : vec) + 2 * (size_t)c.groups);
-    const size_t most = 225 * 1024;
+    const size_t most = kClusterSmem;
     if (columns <= threads && c.groups <= kFusedGroups && other + 8 * block_step <= most) {
         const int64_t step = threads / columns, room = (int64_t)((most - other) / block_step);   // steps a block can keep
         const int64_t item_steps = (c.positions + step - 1) / step;
@@ -874,11 +875,13 @@ template <class T> void join_items(const NormParams& p, const float2* from, int6
     if (runs > 1) launch_after(items_join<T>, dim3(columns), 1024, 0, st, p, (const float2*)p.part, p.part, runs, kJoinRun, runs);
     else launch_after(items_join<T>, dim3(columns), 1024, 0, st, p, from, p.part, count, (int64_t)1, count);
 }
-template <class K> void allow_smem(K kernel, size_t smem, size_t fixed = 0) {
-    if (smem + fixed > 48 * 1024) cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "group norm kernel");
+// The limit belongs to the function on the device, not to the call: it is only ever set to the kernel's `most`, so
+// that another host thread's smaller call cannot lower it between this one's setting and its launch.
+template <class K> void allow_smem(K kernel, size_t smem, size_t most, size_t fixed = 0) {
+    if (smem + fixed > 48 * 1024) cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most), "group norm kernel");
 }
 template <class K> void launch_cluster(K kernel, const NormParams& p, const NormPlan& plan, cudaStream_t st) {
-    allow_smem(kernel, plan.smem, 256);
+    allow_smem(kernel, plan.smem, kClusterSmem, 256);
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
     cfg.gridDim = dim3((unsigned)(p.batch * plan.chunks));
@@ -955,7 +958,7 @@ STG_API stg_status stg_group_norm(stg_engine* e, const stg_group_norm_config* c,
                     }
                     const dim3 grid((unsigned)p.chunks, (unsigned)p.batch);
                     const size_t smem = sizeof(float2) * (size_t)p.groups;
-                    allow_smem(moments_kernel<T, V>, smem, sizeof(float2) * kThreads * V + 256);
+                    allow_smem(moments_kernel<T, V>, smem, sizeof(float2) * kMaxChannels, sizeof(float2) * kThreads * V + 256);
                     moments_kernel<T, V><<<grid, kThreads, smem, st>>>(p);
                     launch_after(moments_join, dim3((unsigned)(((int64_t)p.batch * p.groups + 3) / 4)), 128, 0, st, p);
                     launch_after(apply_kernel<T, V, A>, grid, kThreads, 0, st, p);
@@ -1017,7 +1020,7 @@ STG_API stg_status stg_group_norm_backward(stg_engine* e, const stg_group_norm_c
                     if (each) join_items<T>(p, p.sums, p.batch, st);
                     if (p.dx) {
                         const size_t smem = sizeof(float2) * (size_t)p.groups;
-                        allow_smem(grad_apply_kernel<T, V, A>, smem);
+                        allow_smem(grad_apply_kernel<T, V, A>, smem, sizeof(float2) * kMaxChannels);
                         launch_after(grad_apply_kernel<T, V, A>, grid, kThreads, smem, st, p);
                     }
                 });
