@@ -535,7 +535,7 @@ typedef struct {
     int32_t groups;            /* divides channels */
     int64_t x_batch, x_position;   /* strides of x */
     int64_t y_batch, y_position;   /* strides of y; of dy in the backward pass */
-    int64_t dx_batch, dx_position; /* strides of dx (backward pass only) */
+    int64_t dx_batch, dx_position; /* strides of dx (backward pass only, and there only with dx) */
     double eps;                /* >= 0 */
 } stg_group_norm_config;
 /* backward: 0 the bytes of stg_group_norm's workspace, 1 of stg_group_norm_backward's. Host only. */

@@ -979,7 +979,7 @@ STG_API stg_status stg_group_norm_backward(stg_engine* e, const stg_group_norm_c
         check(aligned(d_gamma, ps) && aligned(d_beta, ps) && aligned(d_dgamma, ps) && aligned(d_dbeta, ps) && aligned(d_mean, 4) &&
                   aligned(d_rstd, 4) && aligned(d_x, es) && aligned(d_dy, es) && aligned(d_dx, es),
               "group norm: a buffer is not aligned to its elements");
-        check_output_strides(c->dx_batch, c->dx_position, *c);
+        if (d_dx) check_output_strides(c->dx_batch, c->dx_position, *c);
         DeviceScope scope(e);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
         if (!c->batch || !c->positions) {   // sums over nothing
@@ -989,7 +989,8 @@ STG_API stg_status stg_group_norm_backward(stg_engine* e, const stg_group_norm_c
         }
         check(d_x && d_dy && d_mean && d_rstd, "group norm: null buffer");
         if (!d_dx && !d_dgamma && !d_dbeta) return;
-        const bool wide = wide_fits(*c, {d_x, d_dy, d_dx}, {c->x_batch, c->x_position, c->y_batch, c->y_position, c->dx_batch, c->dx_position});
+        const bool wide = wide_fits(*c, {d_x, d_dy}, {c->x_batch, c->x_position, c->y_batch, c->y_position}) &&
+                          (!d_dx || wide_fits(*c, {d_dx}, {c->dx_batch, c->dx_position}));
         const NormPlan plan = plan_of(*c, true, wide ? 16 / (int)es : 1, std::min(e->sms, kSms));
         check(d_ws && aligned(d_ws, 256) && ws_bytes >= plan.bytes, "group norm: workspace is missing, unaligned or too small");
         NormParams p = params_of(*c);

@@ -61,3 +61,31 @@ def test_two_engines_in_two_threads(pkg, large, small, backward):
     for t in threads:
         t.join()
     assert not faults, (len(faults), faults[0])
+
+
+@pytest.mark.parametrize("shape", [(2, 40, 24, 3), (3, 5, 4104, 1026), (2, 30000, 24, 2)])      # a cluster; three launches; the same, large
+def test_group_norm_parameter_gradients_alone(pkg, engine, shape):
+    """Without dx its strides say nothing: a broadcast dy is fine, and so are strides of 0."""
+    b, n, ch, groups = shape
+    x, dy, ga = rnd(1, b, n, ch), rnd(2, ch).expand(b, n, ch), rnd(3, ch)
+    _, mean, rstd = engine.group_norm(x, groups, ga, ga, activation="silu", return_stats=True)
+    want = engine.group_norm_backward(dy, x, groups, ga, ga, mean, rstd, activation="silu")
+    got = engine.group_norm_backward(dy, x, groups, ga, ga, mean, rstd, activation="silu", need_dx=False)
+    assert got[0] is None and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    need, L = C.c_size_t(), pkg.lib()
+    for dx_strides in ((0, 0), (1, 1)):      # of which the second would allow scalar accesses only
+        cfg = pkg.GroupNormConfig(C.sizeof(pkg.GroupNormConfig), 0, 0, pkg.ACTIVATIONS["silu"], b, n, ch, groups, n * ch, ch, 0, 0, *dx_strides, 1e-5)
+        assert L.stg_group_norm_workspace(C.byref(cfg), 1, C.byref(need)) == 0
+        ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+        grads = [torch.full((ch,), 7.0, device="cuda") for _ in range(2)]
+        ins = [t.data_ptr() for t in (dy, x, ga, ga, mean, rstd)]
+        stream = torch.cuda.current_stream().cuda_stream
+        for asked in ((1, 1), (1, 0), (0, 1)):
+            for g in grads:
+                g.fill_(7.0)
+            outs = [g.data_ptr() if a else None for g, a in zip(grads, asked)]
+            assert L.stg_group_norm_backward(engine._h, C.byref(cfg), *ins, None, *outs, ws.data_ptr(), need.value, stream) == 0, engine.last_error()
+            for g, a, w in zip(grads, asked, want[1:]):
+                assert torch.equal(g, w) if a else (g == 7).all()
+        dx = torch.empty_like(x)             # with dx they count
+        assert L.stg_group_norm_backward(engine._h, C.byref(cfg), *ins, dx.data_ptr(), None, None, ws.data_ptr(), need.value, stream) == 1
