@@ -766,6 +766,7 @@ void launch_gated_mma(GatedMode mode, bool bf16, const GatedParams& g, int64_t h
 
 int gated_gave_up() {
     unsigned int v = 0;
+    cuda_check(cudaDeviceSynchronize(), "gated status");   // the copy alone does not wait for streams that do not block
     cuda_check(cudaMemcpyFromSymbol(&v, g_gave_up, sizeof(v)), "gated status");
     return (int)v;
 }

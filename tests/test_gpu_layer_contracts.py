@@ -89,3 +89,14 @@ def test_group_norm_parameter_gradients_alone(pkg, engine, shape):
                 assert torch.equal(g, w) if a else (g == 7).all()
         dx = torch.empty_like(x)             # with dx they count
         assert L.stg_group_norm_backward(engine._h, C.byref(cfg), *ins, dx.data_ptr(), None, None, ws.data_ptr(), need.value, stream) == 1
+
+
+def test_status_waits_for_every_stream(engine):
+    """torch's streams do not block the default one, on which the flag is read."""
+    engine.status()
+    stream, done = torch.cuda.Stream(), torch.cuda.Event()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(200_000_000)
+        done.record()
+    engine.status()
+    assert done.query()
