@@ -340,7 +340,9 @@ def _empty(shape, dtype, device, stream):
     are then ahead of them in that stream."""
     if stream is None:
         return _torch.empty(shape, dtype=dtype, device=device)
-    s = _torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
+    s = stream
+    if isinstance(stream, int):   # handle 0 is the default stream, but ExternalStream(0) is one of torch's pool
+        s = _torch.cuda.ExternalStream(stream, device=device) if stream else _torch.cuda.default_stream(device)
     with _torch.cuda.stream(s):
         return _torch.empty(shape, dtype=dtype, device=device)
 

@@ -100,3 +100,20 @@ def test_status_waits_for_every_stream(engine):
         done.record()
     engine.status()
     assert done.query()
+
+
+def _segment_stream(t):
+    at = t.data_ptr()
+    return next(s["stream"] for s in torch.cuda.memory_snapshot() if s["address"] <= at < s["address"] + s["total_size"])
+
+
+def test_results_come_from_the_streams_own_pool(engine):
+    """Memory of another stream's pool could still be in use there: handle 0 is the default stream."""
+    x, w = rnd(1, 1, 30000, 64), rnd(2, 64, 64)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for stream, pool in ((0, 0), (torch.cuda.default_stream(), 0), (None, side.cuda_stream), (side, side.cuda_stream), (side.cuda_stream, side.cuda_stream)):
+            for y in (engine.group_norm(x, 4, stream=stream), engine.gated(x, w, w, stream=stream), engine.rotary(x[None], stream=stream)):
+                assert _segment_stream(y) == pool
+    torch.cuda.synchronize()
