@@ -13,6 +13,7 @@ used) or raw device pointers.
 The layers of the network between the halves (``Engine.rotary``, ``group_norm``, ``gated``, their
 backward passes, ``Plan.mask_head``) take torch tensors and run on the current stream unless given
 one; tensors made on another stream are the caller's to order, as with any torch operator.
+They are not autograd functions: while gradients are recorded, tensors that require one are refused.
 """
 from __future__ import annotations
 
@@ -300,12 +301,16 @@ _torch = None
 
 def _layer_tensor(t, what, device, dtype=None, shape=None):
     """A layer's tensor argument, checked; its dtype code."""
+    global _torch
     try:
         if t.get_device() == device and (dtype is None or t.dtype is dtype) and (shape is None or t.shape == shape):
-            return _DTYPES[t.dtype]
+            code = _DTYPES[t.dtype]
+            if t.requires_grad and _torch.is_grad_enabled():   # the result would be cut off from its graph, silently
+                raise StemsError(1, f"{what} requires a gradient: the layers record none. Call them under torch.no_grad(), or in a "
+                                    "torch.autograd.Function whose backward() calls the *_backward methods")
+            return code
     except (AttributeError, KeyError):
         pass
-    global _torch
     if _torch is None:
         import torch
         _torch = torch

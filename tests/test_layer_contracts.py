@@ -1,11 +1,12 @@
 """The layers' contracts that need no GPU: YaRN's ramp at lengths where its upper end lies past
-the last pair, sizes that the gated projection's kernels cannot reach."""
+the last pair, sizes that the gated projection's kernels cannot reach, tensors that require gradients."""
 from __future__ import annotations
 
 import ctypes as C
 
 import numpy as np
 import pytest
+import torch
 
 
 @pytest.mark.parametrize("r, length, base, pairs, tail", [
@@ -40,3 +41,25 @@ def test_gated_sizes_past_the_kernels_reach_are_refused(pkg, sizes, code):
         assert pkg.lib().stg_gated_workspace(C.byref(cfg), 1, C.byref(need)) == code
         # dg and du alone are rows x width each
         assert need.value >= 2 * c["rows"] * n * (2 if dtype else 4) if code == 0 else need.value == 12345
+
+
+def test_tensors_that_require_gradients_are_refused_while_they_are_recorded(pkg):
+    """The layers record no graph; without the refusal their results would be cut off from it silently."""
+    e = pkg.Engine.__new__(pkg.Engine)
+    e._h, e.device, e._raw_stream, e._scratch = C.c_void_p(), -1, lambda device: 0, {}      # of CPU tensors' device
+    e.last_error = lambda: "no engine"
+    x, w, v = torch.zeros(4, 8), torch.zeros(8, 8), torch.zeros(8)
+    stats = torch.zeros(4, 2)
+    xg = x.clone().requires_grad_()
+    for call, args in ((e.gated, (x, w, w, v, v)), (e.gated_backward, (x, x, w, w, v, v)), (e.group_norm, (x, 2, v, v)),
+                       (e.group_norm_backward, (x, x, 2, v, v, stats, stats)), (e.rotary, (x.view(1, 2, 2, 8), x.view(1, 2, 2, 8)))):
+        for i, a in enumerate(args):
+            if a is stats or not torch.is_tensor(a):
+                continue
+            some = [b if j != i else b.clone().requires_grad_() for j, b in enumerate(args)]
+            with pytest.raises(pkg.StemsError, match="requires a gradient"):
+                call(*some)
+            with torch.no_grad(), pytest.raises(pkg.StemsError, match="no engine"):   # this one reached the library
+                call(*some)
+    with pytest.raises(pkg.StemsError, match="requires a gradient"):
+        e.group_norm(x, 2, out=xg * 1)
