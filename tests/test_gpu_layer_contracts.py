@@ -117,3 +117,27 @@ def test_results_come_from_the_streams_own_pool(engine):
             for y in (engine.group_norm(x, 4, stream=stream), engine.gated(x, w, w, stream=stream), engine.rotary(x[None], stream=stream)):
                 assert _segment_stream(y) == pool
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_mask_heads_sigmoid_is_a_floats(pkg, engine, dtype):
+    """The masks are float whatever the inputs' type: sigmoid to 16 half units of the last place over
+    [-60, 60], with projections that are exact (one feature of 1, the others 0). The parts, in
+    2^-24: power of two and reciprocal 2^-22 each (4 + 4), what the exponent's correction leaves 1,
+    the sum 1, the value's product 1."""
+    sizes, freqs = pkg.bands.bs_bands()
+    plan = engine.plan_roformer(441 * 11, sizes, freqs, chunk=441 * 11, num_overlap=1)
+    din = [int(s) * 4 for s in sizes]
+    _, bands, frames, cols = plan.mask_head_sizes()
+    hidden, weight = torch.zeros(1, 1, bands, frames, 8, device="cuda", dtype=dtype), torch.zeros(1, 2 * cols, 8, device="cuda", dtype=dtype)
+    hidden[..., 0] = 1
+    want, at = [], 0
+    for d in din:
+        weight[0, at:at + d, 0] = 1
+        z = ((torch.arange(d, device="cuda") % 121 - 60) * 0.99609375).to(dtype)
+        weight[0, at + d:at + 2 * d, 0] = z
+        want.append(torch.sigmoid(z.double()).expand(frames, d).reshape(-1))
+        at += 2 * d
+    want = torch.cat(want)
+    got = plan.mask_head(hidden, weight).double().flatten()
+    assert float(((got - want).abs() / want).max()) <= 16 * 2.0 ** -24
