@@ -61,9 +61,11 @@ template <class Fn> void with_dtype(int dtype, Fn&& fn) {
     else fn((__nv_bfloat16*)nullptr);
 }
 
-// load() then use() n times, in that order each, with the loads U to 2U ahead. (Group norm's moments of
+struct Nothing { __device__ __forceinline__ void operator()() const {} };
+// load() then use() n times, in that order each, with the loads U to 2U ahead; batch() after every U uses. (Group norm's moments of
 // 132 MB take 34 us this way, 39 with four plain loads at a time and twice the warps.)
-template <class P, int U, class Load, class Use> __device__ __forceinline__ void stream(int n, Load&& load, Use&& use) {
+template <class P, int U, class Load, class Use, class Batch = Nothing>
+__device__ __forceinline__ void stream(int n, Load&& load, Use&& use, Batch&& batch = Batch{}) {
     P now[U], next[U];
     if (n >= U) {
 #pragma unroll
@@ -74,6 +76,7 @@ template <class P, int U, class Load, class Use> __device__ __forceinline__ void
             for (int u = 0; u < U; u++) load(next[u]);
 #pragma unroll
             for (int u = 0; u < U; u++) use(now[u]);
+            batch();
 #pragma unroll
             for (int u = 0; u < U; u++) now[u] = next[u];
         }
@@ -84,6 +87,7 @@ template <class P, int U, class Load, class Use> __device__ __forceinline__ void
             if (u < n) load(next[u]);
 #pragma unroll
         for (int u = 0; u < U; u++) use(now[u]);
+        batch();
     } else {
 #pragma unroll
         for (int u = 0; u < U; u++)

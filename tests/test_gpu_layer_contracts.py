@@ -141,3 +141,26 @@ def test_mask_heads_sigmoid_is_a_floats(pkg, engine, dtype):
     want = torch.cat(want)
     got = plan.mask_head(hidden, weight).double().flatten()
     assert float(((got - want).abs() / want).max()) <= 16 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("k", [30.0, 1000.0, 100000.0])
+@pytest.mark.parametrize("shape", [(296, 1 << 20, 1, 1), (300, 40000, 64, 2), (4, 172032, 24, 8), (3, 5000, 48, 4)])
+def test_group_norm_statistics_behind_an_outlier(engine, shape, k):
+    """The first position k deviations from the rest costs the statistics no digits. A thread adds up n
+    squares in order, n roundings of their sum; the pivot's turns and the joining of the parts
+    count 128 more: the variance is good to (n + 128) 2^-24, rstd to half of that and its own 8
+    roundings, the mean to as much of the deviation it is off by at most."""
+    b, n, ch, groups = shape
+    x = torch.randn(shape[:3], generator=torch.Generator(device="cuda").manual_seed(5), device="cuda")
+    x[:, 0] = k
+    _, mean, rstd = engine.group_norm(x, groups, return_stats=True)
+    chunks = max(1, -(-296 // b))
+    wide = 4 if ch % 4 == 0 else 1
+    terms = -(-n // chunks) // (256 // (ch // wide)) + 1            # of a thread
+    for i in (0, b // 2, b - 1):
+        d = x[i].double().reshape(n, groups, -1)
+        mu = d.mean((0, 2))
+        var = (d - mu[:, None]).square().mean((0, 2))
+        want = 1 / torch.sqrt(var + 1e-5)
+        assert float(((rstd[i] - want).abs() / want).max()) <= ((terms * wide + 128) / 2 + 8) * 2.0 ** -24
+        assert float(((mean[i] - mu).abs() * want).max()) <= (terms * wide + 128) * 2.0 ** -24
