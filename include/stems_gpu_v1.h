@@ -467,7 +467,8 @@ STG_API stg_status stg_htdemucs_ispec(stg_engine* engine, const float* d_spec, i
  * NULL buffers, sizes and strides that make no sense, pointers that are not aligned to their
  * element, and a workspace that is too small; STG_UNSUPPORTED for sizes past the stated limits. */
 
-/* Element types. Arithmetic is in float whatever the type; results are rounded once. */
+/* Element types. Arithmetic is in float whatever the type; results are rounded once (but see
+ * stg_gated_backward, whose products pass 16-bit gradients between them). */
 enum { STG_F32 = 0, STG_F16 = 1, STG_BF16 = 2 };
 /* Activations: z, max(z, 0), z sigmoid(z), z (1 + erf(z / sqrt 2)) / 2, sigmoid(z). ReLU's
  * derivative at 0 is 0. */
@@ -579,8 +580,12 @@ STG_API stg_status stg_gated(stg_engine* engine, const stg_gated_config* config,
                              void* d_y, void* d_workspace, size_t workspace_bytes, void* stream);
 /* Gradients from dy and the forward pass's inputs (the projections are computed again): dx,
  * dWg, dWu, dbg, dbu in the layouts of what they are the gradients of. Any may be NULL. The
- * projections' own gradients pass between the products in `dtype`. With rows 0 the weights'
- * gradients are zeros. */
+ * projections' own gradients pass between the products in `dtype`, the type that the tensor
+ * cores read: in f16 one beyond 65504 becomes infinite and one below 2^-25 zero, so dy is scaled as
+ * in any f16 training. With rows 0 the weights' gradients are zeros. The workspace holds those
+ * gradients (2 rows x width), the parts of dW (2 width x features floats each, up to 64: until
+ * the tiles fill the GPU, in f32 also one per 4096 rows) and in f32 the parts of dx (rows x features
+ * floats each, up to 32: one per 4096 of its 2 width terms): 48060 x 2048 x 5461 in f32 takes 4.4 GB. */
 STG_API stg_status stg_gated_backward(stg_engine* engine, const stg_gated_config* config, const void* d_dy,
                                       const void* d_x, const void* d_wg, const void* d_wu, const void* d_bg,
                                       const void* d_bu, void* d_dx, void* d_dwg, void* d_dwu, void* d_dbg,

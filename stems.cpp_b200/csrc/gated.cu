@@ -577,8 +577,12 @@ dim3 tile_grid(int64_t tiles, int64_t y = 1) {
     return dim3((unsigned)tiles, (unsigned)y);
 }
 
-// A product of float tiles, as 128 x 128 ones or, when those would leave a third of the SMs without a
-// second block, 64 x 64 ones. out: columns of a 128-wide tile.
+// A product of float tiles, as 128 x 128 ones or, when those number fewer than one and a half per SM, 64 x 64
+// ones, of which an SM holds three or four where it holds two of the large ones (one in dx and the mask head, whose f32
+// kernels have 132 and 134 registers). f32, 64 and 128 wide in us: y of 384 x 1408 at 1000 rows (176 large tiles)
+// 71 and 77, at 1300 (242) 96 and 78; dx there at 4000 rows (96) 285 and 271; dW at 1300 rows (330) 84 and 64, at
+// 777 x 301 x 515 (90) 27 and 88. Not the better one everywhere below the border: y of 1024 x 1024 at 1000 rows (128) 146 and 111.
+// out: columns of a 128-wide tile.
 template <class T, int MODE> int launch_simt(const GatedParams& p, int64_t rows, int64_t cols, int out, int64_t y, cudaStream_t st) {
     auto tiles = [&](int s) { return ceil_div(rows, s) * ceil_div(cols, out * s / 128); };
     if (MODE == GATED_HEAD || tiles(128) * y >= 222) {
@@ -609,15 +613,18 @@ GatedLayout backward_layout(const stg_gated_config& c) {
     l.du = up256((size_t)c.rows * l.pre_row * es);
     l.sums = l.du + up256((size_t)c.rows * l.pre_row * es);
     // dW has 2 width x features outputs and a sum over all rows: rows are split until the tiles
-    // fill the GPU, while a part keeps at least 256 rows
+    // fill the GPU, while a part keeps at least 256 rows, into at most 64 parts
     // (f32: 128 x 128 tiles, two blocks per SM; else pairs of SMs and their 256 x 224 tiles).
+    // bf16, product and joining in us with parts of at least 64, 256 and 1024 rows: 2000 x 64 x 64 10.4, 10.0 and
+    // 11.6; 2000 x 384 x 136 16.2, 12.7 and 12.9; 777 x 301 x 515 23.8, 18.8 and 17.0; f32 there 29 and 31.
     // With one part the product writes dW itself: the backward pass at 5461 x 2048 bf16 and 256 rows
     // takes 109 us, with float sums (89 MB) and a kernel that converts them 184.
     const bool f32 = c.dtype == STG_F32;
     const int64_t tiles = 2 * ceil_div(c.width, f32 ? 128 : 256) * ceil_div(c.features, f32 ? 128 : 224);
     const int64_t want = f32 ? ceil_div(2 * 148, tiles) : std::max<int64_t>(1, 74 / tiles);
     l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, c.rows / 256, 64}));
-    // float: sums in order of at most 4096 terms (and 64 parts): longer ones lose digits to a library's
+    // float: sums in order of at most 4096 terms, while 64 parts (in dx 32) are enough for that: longer ones lose
+    // digits to a library's
     if (f32) l.splits = (int)std::max<int64_t>(l.splits, std::min<int64_t>(64, ceil_div(c.rows, 4096)));
     l.split_rows = std::max<int64_t>(64, ceil_div(ceil_div(c.rows, l.splits), 64) * 64);
     l.splits = (int)std::max<int64_t>(1, ceil_div(c.rows, l.split_rows));

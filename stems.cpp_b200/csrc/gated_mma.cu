@@ -18,10 +18,13 @@
 //
 // Measured (bf16, kernel time): gated 48060 x K x 1408 at K 1536 254 us, 1.64 PFLOP/s (97 % of the
 // measured cuBLAS rate), at 768 132 us, at 384 86 us, 1.21 PFLOP/s: there a tile is six slices and the
-// epilogue of 128 x 128 outputs per block is what bounds it (60 us with the products left out). The
-// backward products at 24030 x 384 x 1408: dg and du 66 us (the epilogue reads dy too), dx 56 and dW 56 us
-// (the loads: L2 to shared memory at about 64 bytes a cycle and SM). The mask head of 60 mel
-// bands x 801 frames at hidden 1536 66 us: 220 MB at least, the loads again.
+// epilogue of 128 x 128 outputs per block is what bounds it (60 us with the products left out; the tensor cores
+// are active in 64 % of the cycles). The backward products at 24030 x 384 x 1408: dg and du 65 us (the
+// epilogue reads dy too; tensor cores active in 41 %), dx 56 and dW 56 us (52 and 56 %): the SMs take in 50 and
+// 46 bytes a cycle of operands, dx 24 KB per slice and block for its 128-column tiles (282 in four rounds of
+// 74 pairs), dW 32 KB for its 192-column ones (72 in one round), of which a block loads boxes of 128 columns for
+// its 96. The mask head of 60 mel bands x 801 frames at hidden 1536 67 us (220 MB at least; 45 %): one
+// accumulator set, so a tile's epilogue runs alone, in 5.3 rounds of tiles.
 #include "gated.h"
 
 #include <cuda.h>
@@ -506,6 +509,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_m
                         o[i / 2] = pack2<T>(act<ACT, true>(__uint_as_float(v[i])) * __uint_as_float(w[i]),
                                             act<ACT, true>(__uint_as_float(v[i + 1])) * __uint_as_float(w[i + 1]));
                 } else if (MODE == GATED_PRE) {
+                    // rounded to the type: the next products' operands have 16 bits (dx and dW are 2.4e-3
+                    // off for it in bf16, 1.7e-3 by their own rounding alone)
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
                         float dg[2], du[2];
@@ -712,7 +717,8 @@ void launch_gated_mma(GatedMode mode, bool bf16, const GatedParams& g, int64_t h
         encode(&p.a[0], bf16, g.x, head_rows, g.k, g.x_row, kDepth, 128);
         encode(&p.b[0], bf16, g.wg, g.stems * 2 * g.band_cols, g.k, g.wg_row, kDepth, 32);
     } else if (mode == GATED_FWD || mode == GATED_PRE) {
-        // 128 outputs to a tile; 64 when that would leave SMs without a tile
+        // 128 outputs to a tile; 64 when that would leave SMs without a tile (384 x 1408 bf16, 64 and 128: 256
+        // rows 6.6 and 8.2 us, 1500 8.4 and 8.7, 3000 12.1 and 11.1)
         const int n = mt * ceil_div(g.n, 128) < pairs ? 64 : 128;
         p.cols = 2 * n;
         tiles_n = ceil_div(g.n, n);

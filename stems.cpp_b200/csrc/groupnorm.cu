@@ -17,8 +17,10 @@
 //     kept 26 MB in the SMs' shared memory instead stood still at each item's meeting: 121 us for
 //     4 x 172032 x 96 bf16.
 // Measured: 4 x 172032 x 96 bf16 with GELU 88 us (264 MB at least; read twice, the second time half from
-// L2, 326 MB; the second reading is bound by the activation's 13 instructions a value), its backward
-// pass at 2 x 43008 x 192 f32 with SiLU 65 us (198 MB at least), one row of 336 x 48 f32 7.5 us.
+// L2, 326 MB): moments 30 us at 4.7 TB/s, the second reading 58 us, which issues in 52 % of its cycles
+// (14 instructions a value, mostly the activation's) and waits about evenly for the arithmetic and
+// for loads in the rest, with 14 warps per SM. Its backward pass at 2 x 43008 x 192 f32 with SiLU 64 us
+// (198 MB at least; both readings at 4.7 TB/s and 40 % issue, waiting for loads), one row of 336 x 48 f32 7.7 us.
 // A block's threads stand side by side along the channels (16-byte vectors, whole rows, so every
 // sector is used whatever the group size) and step down the positions. Each takes the differences
 // from a pivot near its mean (Sums), so that neither a mean far from zero nor an outlier costs digits.
@@ -175,7 +177,7 @@ template <class T, int V, int U> struct Sums {
 // mean and M2 of the positions that place r has. The mean of the means first, then the deviations
 // from it, both from the group's first part on. All threads are shared out to the groups at once,
 // several warps to one or, with more groups than warps, down to one lane (a warp to each in turn:
-// 542 us where this takes 37 for 2 x 16 x 4096 with 4096 groups). A group that began before ch0 is
+// 542 us where this takes 43 for 2 x 16 x 4096 with 4096 groups). A group that began before ch0 is
 // joined to what group[] has of it.
 __device__ __forceinline__ void block_moments(const NormParams& p, int threads, const Place& q, int n, int vec, int ch0, int ch1, const float2* part, float2* group,
                                               float* red) {
@@ -493,8 +495,8 @@ __global__ void __launch_bounds__(256) grad_join(const __grid_constant__ NormPar
 
 // The same over `count` rows of channel sums in one list, `every` rows apart, `run` of them to a grid
 // row: their sum goes to the first one's place in `to` (which may be `from`), or, with one grid row,
-// to dbeta and dgamma. The loads of a warp do not wait for each other: 3000 x 7 x 75 f32 takes
-// 84 us backward, 1391 when the items were added up one after the other.
+// to dbeta and dgamma. The loads of a warp do not wait for each other: the backward pass of 3000 x 7 x 75
+// f32 takes 23 us, 1391 when the items were added up one after the other.
 template <class T>
 __global__ void __launch_bounds__(1024) items_join(const __grid_constant__ NormParams p, const float2* from, float2* to, int64_t count, int64_t every,
                                                    int64_t run) {
@@ -774,12 +776,12 @@ void check_config(const stg_group_norm_config* c) {
 }
 
 // An item's positions are cut so that the whole call has two blocks per SM, what the registers
-// allow at a time, each with at least 16 positions, and at most 1024 parts to join: a block's joining
-// at its end reads nothing, so few long blocks beat more short ones (moments of 132 MB: 30 us with
-// two per SM, 34 with four, 43 with eight).
+// allow at a time, each with at least 16 positions: a block's joining at its end reads nothing, so few
+// long blocks beat more short ones (moments of 132 MB: 30 us with two per SM, 34 with four, 43 with
+// eight).
 int chunks_of(const stg_group_norm_config& c) {
     const int64_t per_item = (148 * 2 + c.batch - 1) / std::max<int64_t>(c.batch, 1);
-    const int64_t n = std::min<int64_t>({std::max<int64_t>(per_item, 1), (c.positions + 15) / 16, 1024});
+    const int64_t n = std::min<int64_t>({std::max<int64_t>(per_item, 1), (c.positions + 15) / 16});
     const int64_t rows = (c.positions + n - 1) / std::max<int64_t>(n, 1);
     return (int)((c.positions + rows - 1) / std::max<int64_t>(rows, 1));
 }
@@ -800,7 +802,7 @@ NormPlan plan_of(const stg_group_norm_config& c, bool backward, int vec, int sms
     if (!c.batch || !c.positions) return r;
     const int columns = c.channels / vec, cpg = c.channels / c.groups;
     // Items that a smaller block reads in eight steps, more of them than SMs: such blocks, of which an SM
-    // holds several (9000 x 16 x 16 f32: 35 us, 281 with kFused threads each; 3000 x 7 x 75 21 and 97).
+    // holds several (9000 x 16 x 16 f32: 35 us, 281 with kFused threads each; 3000 x 7 x 75 20 and 97).
     int threads = kFused;
     while (threads > 32 && columns <= threads / 2 && c.positions <= 8 * (threads / 2 / columns) && c.batch > sms) threads /= 2;
     r.threads = threads;
@@ -893,9 +895,15 @@ template <class K, class... More> void launch_after(K kernel, dim3 grid, int thr
     cfg.numAttrs = 1;
     cuda_check(cudaLaunchKernelEx(&cfg, kernel, p, more...), "group norm kernel");
 }
-// dbeta and dgamma from `count` rows of channel sums; many rows first in runs, into p.part.
-constexpr int kItemsInTurn = 16;   // up to here grad_join adds items up as it goes, one launch less
+// Up to here grad_join adds the items up as it goes, one launch less; past it a grid row has an item each and
+// items_join adds them up. N x 3000 x 384 f32, whole backward pass, in turn and each: 24 items 127 and 110 us,
+// 64 315 and 285; but also 16 85 and 74, 4 21 and 17.
+constexpr int kItemsInTurn = 16;
+// Rows of channel sums of one run; more rows are joined in runs first, into p.part (a launch more). N x 7 x 75 f32, whole
+// backward pass, in runs of 512, of 128 and in one: 600 items 9.4, 9.0 and 9.6 us, 3000 23, 22 and 32; 60000 x 4 x 16
+// 212, 215 and 396.
 constexpr int64_t kJoinRun = 512;
+// dbeta and dgamma from `count` rows of channel sums.
 template <class T> void join_items(const NormParams& p, const float2* from, int64_t count, cudaStream_t st) {
     if (!p.dgamma && !p.dbeta) return;
     const unsigned columns = (unsigned)((p.channels + 31) / 32);
