@@ -43,7 +43,8 @@ struct RotaryParams {
 
 // cos and sin of 2 pi t, t in turns. The fraction r in [-1/2, 1/2] is exact in double; it goes to
 // float as a leading part and a rest, and the rest's effect is added to first order, so the
-// result is good to about one unit of the last place at any position.
+// result is good to about one unit of the last place, and past positions of 2^28 to what the product
+// p f_i loses in double (2^-52 of it: 5e-7 at 2^31).
 __device__ __forceinline__ float2 cos_sin_turns(double t) {
     const double r = 2.0 * (t - rint(t));   // half turns
     const float hi = (float)r;

@@ -164,3 +164,48 @@ def test_group_norm_statistics_behind_an_outlier(engine, shape, k):
         want = 1 / torch.sqrt(var + 1e-5)
         assert float(((rstd[i] - want).abs() / want).max()) <= ((terms * wide + 128) / 2 + 8) * 2.0 ** -24
         assert float(((mean[i] - mu).abs() * want).max()) <= (terms * wide + 128) * 2.0 ** -24
+
+
+def _large_calls(engine):
+    bf = torch.bfloat16
+    x, dx, many, dmany = rnd(1, 2, 30000, 24), rnd(2, 2, 30000, 24), rnd(3, 20, 3000, 96, dtype=bf), rnd(4, 20, 3000, 96, dtype=bf)
+    ga, gb = rnd(5, 24), rnd(6, 96)
+    stats, more = engine.group_norm(x, 3, ga, ga, return_stats=True)[1:], engine.group_norm(many, 8, gb, gb, return_stats=True)[1:]
+    h, dh, w, v = rnd(7, 3000, 200, dtype=bf), rnd(8, 3000, 300, dtype=bf), rnd(9, 300, 200, dtype=bf, scale=0.07), rnd(10, 300, 200, dtype=bf, scale=0.07)
+    odd = rnd(11, 3000, 203, dtype=bf)[:, 2:202]                  # rows that are copied first
+    return {
+        "norm": lambda: [engine.group_norm(x, 3, ga, ga, activation="gelu")],
+        "norm_back": lambda: list(engine.group_norm_backward(dx, x, 3, ga, ga, *stats, activation="silu")),
+        "norm_back_many": lambda: list(engine.group_norm_backward(dmany, many, 8, gb, gb, *more, activation="silu")),
+        "gated": lambda: [engine.gated(odd, w, v, gb.new_ones(300).to(bf))],
+        "gated_back": lambda: list(engine.gated_backward(dh, h, w, v, gb.new_ones(300).to(bf))),
+    }
+
+
+@pytest.mark.parametrize("name", ["norm", "norm_back", "norm_back_many", "gated", "gated_back"])
+def test_calls_of_several_launches_in_graphs_and_overlapping(engine, name):
+    """Launches that begin before the one before them has ended, and scratch between them: captured
+    twice in a row, replayed on two streams at once, and eager calls side by side."""
+    call = _large_calls(engine)[name]
+    want = call()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = [call(), call()]
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    outs = [o for _, both in graphs for o in both]
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(call())
+    torch.cuda.synchronize()
+    for out in outs:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
