@@ -491,7 +491,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gated_m
                     // through shared memory, so that a row's 16 floats are stored side by side
                     float* sm = reinterpret_cast<float*>(stage);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) sm[lane * 17 + i] = __uint_as_float(v[i]) * sigmoid<false>(__uint_as_float(w[i]));
+                    for (int i = 0; i < 16; i += 2) {
+                        const float2 m = split(make_f2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])) *
+                                               sigmoid(make_f2(__uint_as_float(w[i]), __uint_as_float(w[i + 1]))));
+                        sm[lane * 17 + i] = m.x;
+                        sm[lane * 17 + i + 1] = m.y;
+                    }
                     __syncwarp();
                     const int rows = (int)max((int64_t)0, min((int64_t)32, g.frames - row0)), col = j + (lane & 15);
                     float* o = g.masks + (q.cs * g.band_cols + q.h.off) * g.frames + row0 * q.h.din + col;
